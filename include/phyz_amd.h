@@ -347,6 +347,111 @@ int phz_train_update(phz_train* t, const uint32_t* const* order, const uint64_t*
 int phz_train_time_update(phz_train* t, const uint32_t* const* order, const uint64_t* order_lens, uint64_t n_order,
                           const phz_ppo_cfg* cfg, phz_update_stats* out, double* ms_kernels, uint64_t* minibatches);
 
+/* ── Operators of sequence policies, on device tensors: a gated linear
+ * recurrence over rollouts, a linear layer with its epilogue, both with their
+ * gradients, and the orthogonalised (Muon) update of weight matrices. The
+ * reference has none of these; a policy with memory, or wider than the fused
+ * three-layer nets above, is built from them.
+ *
+ * Conventions of this section
+ *   - Tensors are device memory of the handle's GPU, given as views
+ *     (phz_tensor). NULL stands for an absent optional tensor.
+ *   - A call enqueues its work on `stream` (a hipStream_t; NULL is the default
+ *     stream) and returns without waiting. It reads and writes nothing after
+ *     that stream's earlier work or before its later work.
+ *   - Outputs may not overlap inputs, except where a call says so. Views that
+ *     interleave without sharing elements (two halves of one buffer's rows)
+ *     do not overlap.
+ *   - Workspace belongs to the handle, one block per stream, grown on demand.
+ *     A call that would have to grow it while its stream is being captured is
+ *     refused: run the call once before the capture, or phz_ops_reserve. A
+ *     captured graph uses the block of the stream it was captured on.
+ *   - A handle is not thread-safe. Results do not depend on timing: the same
+ *     call on the same inputs gives the same bits. ── */
+typedef struct phz_ops phz_ops;
+
+enum { PHZ_BF16 = 2, PHZ_U8 = 3 }; /* further phz_tensor dtypes, beside PHZ_F32 */
+
+/* A view of up to three dimensions; sizes and strides in elements. */
+typedef struct {
+  void* data;
+  int64_t size[3];
+  int64_t stride[3];
+  int32_t dtype; /* PHZ_F32, PHZ_BF16 or PHZ_U8 */
+  int32_t ndim;  /* 1..3; the entries beyond it are ignored */
+} phz_tensor;
+
+/* device_ordinal -1 makes a host-only handle: calls check their arguments and
+ * then fail. */
+int phz_ops_create(int device_ordinal, phz_ops** out);
+void phz_ops_destroy(phz_ops* ops);
+/* The last error's message; with NULL, the last failed create's. */
+const char* phz_ops_last_error(const phz_ops* ops);
+/* Grows the workspace of `stream` to at least `bytes`. */
+int phz_ops_reserve(phz_ops* ops, void* stream, uint64_t bytes);
+/* Workspace bytes that the handle holds, over all streams. */
+uint64_t phz_ops_workspace_bytes(const phz_ops* ops);
+
+/* How a recurrence reads its gate z:
+ * SIGMOID  c = sigmoid(z), h_t = c h_{t-1} + (1 - c) x_t
+ * DECAY    c = z,          h_t = c h_{t-1} + x_t            */
+enum { PHZ_GATE_SIGMOID = 0, PHZ_GATE_DECAY = 1 };
+
+/* The recurrence over z, x [steps][worlds][width] (f32 or bf16, any strides of
+ * the first two axes, the last one dense), into h of the same shape and type.
+ * h0 [worlds][width] f32: the state before the first step (NULL: zeros).
+ * reset [steps][worlds] u8: where nonzero, an episode begins at that step and
+ * h_{t-1} counts as 0, whatever it holds. h_last [worlds][width] f32 (or NULL)
+ * receives the state after the last step. The state is held in f32. */
+int phz_gated_scan(phz_ops* ops, void* stream, int form, const phz_tensor* z, const phz_tensor* x, const phz_tensor* h0,
+                   const phz_tensor* reset, const phz_tensor* h, const phz_tensor* h_last);
+/* Its gradients: dh, dh_last (f32, or NULL) are the loss's gradients for h and
+ * h_last, h the states that the forward pass stored. dz, dx like z; dh0
+ * [worlds][width] f32 or NULL. */
+int phz_gated_scan_backward(phz_ops* ops, void* stream, int form, const phz_tensor* dh, const phz_tensor* dh_last,
+                            const phz_tensor* z, const phz_tensor* x, const phz_tensor* h, const phz_tensor* h0,
+                            const phz_tensor* reset, const phz_tensor* dz, const phz_tensor* dx, const phz_tensor* dh0);
+/* One step: z, x [worlds][width], reset [worlds] or NULL; h [worlds][width]
+ * f32 is read and replaced. */
+int phz_gated_step(phz_ops* ops, void* stream, int form, const phz_tensor* z, const phz_tensor* x,
+                   const phz_tensor* reset, const phz_tensor* h);
+
+/* Activations of phz_linear. GELU is its tanh form,
+ * 0.5 p (1 + tanh(sqrt(2/pi) (p + 0.044715 p^3))). */
+enum { PHZ_ACT_NONE = 0, PHZ_ACT_TANH = 1, PHZ_ACT_RELU = 2, PHZ_ACT_SILU = 3, PHZ_ACT_GELU = 4 };
+
+/* y = act(x W^T + bias) + residual for x [rows][n_in], w [n_out][n_in], bias
+ * [n_out] or NULL, residual [rows][n_out] or NULL, all of one type (f32 or
+ * bf16), rows dense. pre (or NULL) receives x W^T + bias, what the backward
+ * pass needs. y may be the same view as residual. Sums are f32. */
+int phz_linear(phz_ops* ops, void* stream, int act, const phz_tensor* x, const phz_tensor* w, const phz_tensor* bias,
+               const phz_tensor* residual, const phz_tensor* pre, const phz_tensor* y);
+/* Its gradients for dz = dy act'(pre): dx = dz W, dw = dz^T x, db = the sum of
+ * dz over rows; each of dx, dw, db may be NULL. The residual's gradient is dy.
+ * pre may be NULL for PHZ_ACT_NONE. In bf16, dz is rounded to bf16 before the
+ * products, as the matrix cores take it. */
+int phz_linear_backward(phz_ops* ops, void* stream, int act, const phz_tensor* dy, const phz_tensor* x,
+                        const phz_tensor* w, const phz_tensor* pre, const phz_tensor* dx, const phz_tensor* dw,
+                        const phz_tensor* db);
+
+/* Newton-Schulz coefficients and Muon's settings. */
+typedef struct {
+  double a, b, c; /* X <- a X + (b A + c A^2) X with A = X X^T */
+  double eps;     /* X starts as g / (|g|_F + eps) */
+  double lr, momentum, weight_decay; /* phz_muon_step only */
+  int32_t steps;
+  int32_t nesterov;
+} phz_muon_cfg;
+
+/* o = `steps` Newton-Schulz steps on each [rows][cols] matrix of g (2 or 3
+ * dimensions; f32 or bf16, rows dense), in o's type, which is g's. */
+int phz_orthogonalize(phz_ops* ops, void* stream, const phz_muon_cfg* cfg, const phz_tensor* g, const phz_tensor* o);
+/* m <- momentum m + g; u = g + momentum m (nesterov) or m;
+ * w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u).
+ * w and m are f32, g f32 or bf16. */
+int phz_muon_step(phz_ops* ops, void* stream, const phz_muon_cfg* cfg, const phz_tensor* w, const phz_tensor* g,
+                  const phz_tensor* m);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,9 @@ i64p = C.POINTER(C.c_int64)
 SIM = C.c_void_p
 
 TRAIN = C.c_void_p
+OPS = C.c_void_p
+TENSOR = C.c_void_p  # address of a phz_tensor
+STREAM = C.c_void_p
 
 
 class NetDims(C.Structure):
@@ -39,6 +42,11 @@ class PpoCfg(C.Structure):
 class UpdateStats(C.Structure):
     _fields_ = [("policy_loss", C.c_double), ("value_loss", C.c_double), ("kl", C.c_double),
                 ("grad_steps", C.c_uint64), ("stopped_early", C.c_int32)]
+
+
+class MuonCfg(C.Structure):
+    _fields_ = [("a", C.c_double), ("b", C.c_double), ("c", C.c_double), ("eps", C.c_double), ("lr", C.c_double),
+                ("momentum", C.c_double), ("weight_decay", C.c_double), ("steps", C.c_int32), ("nesterov", C.c_int32)]
 
 
 fp = C.POINTER(C.c_float)
@@ -122,6 +130,18 @@ SIGNATURES = {
                                    C.POINTER(UpdateStats)]),
     "phz_train_time_update": (C.c_int, [TRAIN, C.POINTER(u32p), u64p, C.c_uint64, C.POINTER(PpoCfg),
                                         C.POINTER(UpdateStats), dp, u64p]),
+    "phz_ops_create": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
+    "phz_ops_destroy": (None, [OPS]),
+    "phz_ops_last_error": (C.c_char_p, [OPS]),
+    "phz_ops_reserve": (C.c_int, [OPS, STREAM, C.c_uint64]),
+    "phz_ops_workspace_bytes": (C.c_uint64, [OPS]),
+    "phz_gated_scan": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 6),
+    "phz_gated_scan_backward": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 10),
+    "phz_gated_step": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 4),
+    "phz_linear": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 6),
+    "phz_linear_backward": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 7),
+    "phz_orthogonalize": (C.c_int, [OPS, STREAM, C.POINTER(MuonCfg), TENSOR, TENSOR]),
+    "phz_muon_step": (C.c_int, [OPS, STREAM, C.POINTER(MuonCfg), TENSOR, TENSOR, TENSOR]),
 }
 
 

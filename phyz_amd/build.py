@@ -6,8 +6,9 @@
    (csrc/phz_device_src.inc, csrc/phz_control_src.inc) so the library can hand
    them to hiprtc with each model's constants.
 2. Compile the host library (csrc/phz_host.cpp), the ahead-of-time layout
-   kernels (csrc/phz_io.hip) and the PPO update pass (csrc/phz_train.hip) for
-   gfx950 and link them with hiprtc.
+   kernels (csrc/phz_io.hip), the PPO update pass (csrc/phz_train.hip) and the
+   operators of sequence policies (csrc/phz_ops.hip, phz_scan.hip,
+   phz_linear.hip, phz_muon.hip) for gfx950 and link them with hiprtc.
 
 Packed FP32 instructions are disabled in every device compile.
 """
@@ -17,11 +18,13 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libphyz_amd.so")
 ARCH = "gfx950"
+KERNELS = ["phz_io", "phz_train", "phz_ops", "phz_scan", "phz_linear", "phz_muon"]  # csrc/*.hip, ahead of time
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
@@ -62,17 +65,16 @@ def build(verbose: bool = False) -> str:
     cc = hipcc()
     bdir = os.path.join(HERE, "_build")
     os.makedirs(bdir, exist_ok=True)
-    io_obj = os.path.join(bdir, "phz_io.o")
-    host_obj = os.path.join(bdir, "phz_host.o")
-    train_obj = os.path.join(bdir, "phz_train.o")
-    _run([cc, "-x", "hip", f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", *NO_PACKED_FP32, "-c",
-          os.path.join(CSRC, "phz_io.hip"), "-o", io_obj], verbose)
-    _run([cc, "-x", "hip", f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", *NO_PACKED_FP32, "-c",
-          os.path.join(CSRC, "phz_train.hip"), "-o", train_obj], verbose)
-    _run([cc, "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-c",
-          os.path.join(CSRC, "phz_host.cpp"), "-o", host_obj], verbose)
+    obj = lambda name: os.path.join(bdir, name + ".o")  # noqa: E731
+    jobs = [[cc, "-x", "hip", f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", *NO_PACKED_FP32, "-c",
+             os.path.join(CSRC, name + ".hip"), "-o", obj(name)] for name in KERNELS]
+    jobs.append([cc, "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-c",
+                 os.path.join(CSRC, "phz_host.cpp"), "-o", obj("phz_host")])
+    with ThreadPoolExecutor(4) as pool:
+        for done in [pool.submit(_run, j, verbose) for j in jobs]:
+            done.result()
     tmp = LIB + ".tmp"
-    _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", io_obj, train_obj, host_obj, "-o", tmp,
+    _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(obj, KERNELS), obj("phz_host"), "-o", tmp,
           "-L/opt/rocm/lib", "-lhiprtc", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib"], verbose)
     os.replace(tmp, LIB)
     return LIB

@@ -1,0 +1,221 @@
+// phz_ops.hip — the handle of the sequence operators: create and destroy, the
+// per-stream workspaces, and the checks that every operator makes of its
+// tensors before it launches anything.
+#include "phz_ops.h"
+
+#include <string.h>
+
+#include <algorithm>
+
+using namespace phzop;
+
+namespace {
+
+thread_local std::string g_ops_create_error;
+
+}  // namespace
+
+char* phz_ops::workspace(hipStream_t stream, uint64_t bytes) {
+  bytes = std::max<uint64_t>((bytes + 255) & ~255ull, 256);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (!hip_ok(hipStreamIsCapturing(stream, &status), "hipStreamIsCapturing")) return nullptr;
+  const bool capturing = status != hipStreamCaptureStatusNone;
+  Block* b = nullptr;
+  for (auto& x : blocks)
+    if (x.stream == (void*)stream) b = &x;
+  if (!b || b->bytes < bytes) {
+    if (capturing) {
+      err = fmt("the stream is being captured and its workspace would have to grow to %llu bytes: run the call once "
+                "before, or phz_ops_reserve",
+                (unsigned long long)bytes);
+      return nullptr;
+    }
+    // Half as much again as asked, so that growing sizes do not allocate on
+    // every call.
+    uint64_t want = bytes + bytes / 2;
+    void* p = nullptr;
+    if (hipMalloc(&p, want) != hipSuccess) {
+      (void)hipGetLastError();
+      want = bytes;
+      if (!hip_ok(hipMalloc(&p, want), "workspace")) {
+        (void)hipGetLastError();
+        return nullptr;
+      }
+    }
+    if (b) {
+      // hipFree waits for the device, so work in flight has ended; a captured
+      // graph may run again, and keeps its block.
+      if (captured) retired.push_back(*b);
+      else (void)hipFree(b->data);
+      b->data = p;
+      b->bytes = want;
+    } else {
+      blocks.push_back(Block{(void*)stream, p, want});
+      b = &blocks.back();
+    }
+  }
+  captured = captured || capturing;
+  return (char*)b->data;
+}
+
+namespace phzop {
+
+bool check(phz_ops* o, const char* name, const phz_tensor* t, const Want& want) {
+  if (!t) return o->err = fmt("%s is missing", name), false;
+  if (t->ndim != want.ndim) return o->err = fmt("%s has %d dimensions, expected %d", name, t->ndim, want.ndim), false;
+  if (t->dtype != want.dtype)
+    return o->err = fmt("%s is %s, expected %s", name, dtype_name(t->dtype), dtype_name(want.dtype)), false;
+  for (int i = 0; i < want.ndim; i++) {
+    if (t->size[i] < 0) return o->err = fmt("%s has a negative size", name), false;
+    if (want.size[i] >= 0 && t->size[i] != want.size[i])
+      return o->err = fmt("%s has %lld elements along axis %d, expected %lld", name, (long long)t->size[i], i,
+                          (long long)want.size[i]),
+             false;
+  }
+  if (empty(t)) return true;
+  if (!t->data) return o->err = fmt("%s has no data", name), false;
+  int64_t extent = 1;
+  for (int i = 0; i < want.ndim; i++) {
+    if (t->stride[i] < 0 || t->stride[i] > (1ll << 48) || t->size[i] > (1ll << 40))
+      return o->err = fmt("%s has a negative or absurd stride or size along axis %d", name, i), false;
+    if (want.output && t->size[i] > 1 && t->stride[i] == 0)
+      return o->err = fmt("%s is broadcast along axis %d: an output's elements have to be its own", name, i), false;
+    if (t->size[i] > 1 && __builtin_add_overflow(extent, (t->size[i] - 1) * (__int128)t->stride[i] > (1ll << 56)
+                                                             ? (1ll << 62)
+                                                             : (t->size[i] - 1) * t->stride[i],
+                                                 &extent))
+      return o->err = fmt("%s is too large", name), false;
+  }
+  if (extent > (1ll << 56)) return o->err = fmt("%s is too large", name), false;
+  if (want.output) {
+    // Axes from the smallest stride up: each has to step over all of those below.
+    int axis[3], n = 0;
+    for (int i = 0; i < want.ndim; i++)
+      if (t->size[i] > 1) axis[n++] = i;
+    std::sort(axis, axis + n, [&](int a, int b) { return t->stride[a] < t->stride[b]; });
+    int64_t below = 1;
+    for (int k = 0; k < n; k++) {
+      if (t->stride[axis[k]] < below) return o->err = fmt("%s overlaps itself along axis %d", name, axis[k]), false;
+      below += (t->size[axis[k]] - 1) * t->stride[axis[k]];
+    }
+  }
+  if (want.dense && t->size[want.ndim - 1] > 1 && t->stride[want.ndim - 1] != 1)
+    return o->err = fmt("%s: the last axis has to be dense (stride %lld)", name, (long long)t->stride[want.ndim - 1]),
+           false;
+  if ((uintptr_t)t->data % (uintptr_t)elem_bytes(t->dtype))
+    return o->err = fmt("%s is not aligned to its elements", name), false;
+  return true;
+}
+
+namespace {
+
+void span(const phz_tensor* t, uintptr_t* lo, uintptr_t* hi) {
+  int64_t n = 1;
+  for (int i = 0; i < t->ndim; i++) n += (t->size[i] - 1) * t->stride[i];
+  *lo = (uintptr_t)t->data;
+  *hi = *lo + (uintptr_t)(n * elem_bytes(t->dtype));
+}
+
+}  // namespace
+
+bool apart(phz_ops* o, const char* an, const phz_tensor* a, const char* bn, const phz_tensor* b) {
+  if (!a || !b || empty(a) || empty(b)) return true;
+  uintptr_t al, ah, bl, bh;
+  span(a, &al, &ah);
+  span(b, &bl, &bh);
+  if (ah <= bl || bh <= al) return true;
+  // Interleaved views: rows of the same steps, whose dense parts lie beside
+  // each other within the smallest step.
+  if (a->ndim == b->ndim && a->ndim > 1 && a->dtype == b->dtype) {
+    const int last = a->ndim - 1;
+    const int64_t e = elem_bytes(a->dtype);
+    int64_t step = 0;
+    bool same = (a->size[last] <= 1 || a->stride[last] == 1) && (b->size[last] <= 1 || b->stride[last] == 1);
+    for (int i = 0; i < last && same; i++) {
+      if (a->size[i] <= 1 && b->size[i] <= 1) continue;
+      same = a->stride[i] == b->stride[i] && a->stride[i] > 0;
+      if (same) step = step ? std::min(step, a->stride[i]) : a->stride[i];
+    }
+    for (int i = 0; i < last && same && step; i++)
+      if ((a->size[i] > 1 || b->size[i] > 1) && a->stride[i] % step) same = false;
+    if (same && step) {
+      const int64_t delta = (int64_t)(bl - al), pitch = step * e;
+      const int64_t off = ((delta % pitch) + pitch) % pitch;
+      if (off >= a->size[last] * e && pitch - off >= b->size[last] * e) return true;
+    }
+  }
+  o->err = fmt("%s overlaps %s", an, bn);
+  return false;
+}
+
+}  // namespace phzop
+
+extern "C" {
+
+int phz_ops_create(int device_ordinal, phz_ops** out) {
+  try {
+    g_ops_create_error.clear();
+    if (!out) return g_ops_create_error = "null output pointer", 1;
+    *out = nullptr;
+    if (device_ordinal == -1) {
+      *out = new phz_ops();
+      return 0;
+    }
+    int count = 0;
+    if (hipGetDeviceCount(&count) != hipSuccess || count == 0) return g_ops_create_error = "no HIP device available", 1;
+    if (device_ordinal < 0 || device_ordinal >= count)
+      return g_ops_create_error = fmt("device ordinal %d out of range (%d devices)", device_ordinal, count), 1;
+    auto* o = new phz_ops();
+    o->device = device_ordinal;
+    DeviceGuard g(o);
+    int cus = 0;
+    bool ok = g.ok && o->hip_ok(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device_ordinal),
+                                "compute units");
+    ok = ok && o->hip_ok(hipMalloc(&o->zeros, 256), "zeros") && o->hip_ok(hipMemset(o->zeros, 0, 256), "zeros") &&
+         o->hip_ok(hipDeviceSynchronize(), "create");
+    if (!ok) {
+      g_ops_create_error = o->err;
+      if (o->zeros) (void)hipFree(o->zeros);
+      delete o;
+      return 1;
+    }
+    o->cus = cus;
+    *out = o;
+    return 0;
+  } catch (const std::exception& e) {
+    g_ops_create_error = e.what();
+    return 1;
+  }
+}
+
+void phz_ops_destroy(phz_ops* o) {
+  if (!o) return;
+  if (o->device >= 0) {
+    DeviceGuard g(o);
+    for (auto& b : o->blocks) (void)hipFree(b.data);
+    for (auto& b : o->retired) (void)hipFree(b.data);
+    if (o->zeros) (void)hipFree(o->zeros);
+  }
+  delete o;
+}
+
+const char* phz_ops_last_error(const phz_ops* o) { return o ? o->err.c_str() : g_ops_create_error.c_str(); }
+
+int phz_ops_reserve(phz_ops* o, void* stream, uint64_t bytes) {
+  return guarded(o, [&] {
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    DeviceGuard g(o);
+    return g.ok && o->workspace((hipStream_t)stream, bytes) ? 0 : 1;
+  });
+}
+
+uint64_t phz_ops_workspace_bytes(const phz_ops* o) {
+  uint64_t n = 0;
+  if (o) {
+    for (auto& b : o->blocks) n += b.bytes;
+    for (auto& b : o->retired) n += b.bytes;
+  }
+  return n;
+}
+
+}  // extern "C"

@@ -1,0 +1,569 @@
+// phz_scan.hip — the gated linear recurrence over rollouts, forward and
+// backward, and its single step.
+//
+//   forward   h_t = c_t h_{t-1} + u_t                       t = 0 .. T-1
+//   backward  e_t = dh_t + k_{t+1},  k_t = c_t e_t           t = T-1 .. 0
+//             dx_t = (1 - c_t) e_t,  dz_t = e_t (h_{t-1} - x_t) c_t (1 - c_t)
+//             (decay: dx_t = e_t, dz_t = e_t h_{t-1}),  dh0 = k_0
+//
+// with c = sigmoid(z), u = (1 - c) x or c = z, u = x, and h_{t-1} := 0 where an
+// episode begins. Both directions are one affine recurrence per channel,
+// s <- c s + v, over the steps in processing order; a span of steps composes to
+// s <- A s + H with A the product of its c. The layout of the work follows:
+//
+//   lane    VEC neighbouring channels of one world; the state in f32 registers
+//   wave    64 lanes, U steps loaded ahead of the ones being computed
+//   group   NW waves take NW consecutive runs of U steps of the same channels
+//           (a slab): each wave composes its run from registers, the runs'
+//           (A, H) meet in LDS, and each wave then runs its steps from the
+//           state that the earlier ones leave. The data is read once.
+//   chunk   where the channels do not fill the chip, the steps are split in S
+//           chunks over the grid: one pass composes each chunk, the second
+//           starts each chunk from its predecessors' (A, H), folded in order.
+//           That pass visits the chunks in the opposite order, so what the
+//           first one read last is still in the memory-side cache.
+//
+// Every composition has a fixed order, so results do not depend on timing.
+#include "phz_ops.h"
+
+#include <algorithm>
+
+using namespace phzop;
+
+namespace {
+
+constexpr int kWaveLanes = 64;
+
+struct ScanArgs {
+  const void *z, *x, *h, *dh;   // h and dh: backward only
+  void *o1, *o2;                // h | dz, dx
+  const float* start;           // h0 | dh_last, or null
+  const float* h0;              // backward: the state before the first step, or null
+  float* end;                   // h_last | dh0, or null
+  const uint8_t* reset;
+  int64_t z_t, z_b, x_t, x_b, h_t, h_b, dh_t, dh_b, o1_t, o1_b, o2_t, o2_b, r_t, r_b, start_b, h0_b, end_b;
+  int64_t lanes;                // worlds * groups
+  int32_t steps, width, groups; // groups: lanes that cover one world's width
+  int32_t chunk, chunks;        // steps per chunk
+  float* agg;                   // [chunks][2][lanes][VEC]: each chunk's A, then H
+};
+
+// A span in which an episode begins keeps nothing of the state before it, be
+// that infinite or NaN: its A is this NaN, and stands for "forget", which a
+// product that underflows to 0 does not. (A gate that is NaN makes H NaN, so
+// no other NaN in A matters.)
+constexpr uint32_t kForget = 0x7fc5a5a5u;
+__device__ __forceinline__ bool forgets(float a) { return __builtin_bit_cast(uint32_t, a) == kForget; }
+__device__ __forceinline__ float compose(float a, float s, float h) { return forgets(a) ? h : fmaf(a, s, h); }
+
+// One step's affine map and outputs. `s` is h (forward) or k (backward).
+template <int FORM>
+struct Step;
+
+template <>
+struct Step<PHZ_GATE_SIGMOID> {
+  // The gate as its smaller side c with z's sign (signed_gate):
+  // h' = h + c (x - h) where the gate keeps, x + c (h - x) where it writes, so
+  // a gate at rest leaves the state exactly as it is.
+  static __device__ __forceinline__ float gate(float z) { return signed_gate(z); }
+  static __device__ __forceinline__ float keep(float q) { return __float_as_int(q) < 0 ? fabsf(q) : 1.0f - fabsf(q); }
+  static __device__ __forceinline__ float write(float q) { return __float_as_int(q) < 0 ? 1.0f - fabsf(q) : fabsf(q); }
+  static __device__ __forceinline__ float next(float h, float q, float x) {
+    const bool w = __float_as_int(q) < 0;
+    const float base = w ? x : h, other = w ? h : x;
+    return fmaf(fabsf(q), other - base, base);
+  }
+  static __device__ __forceinline__ float dz(float e, float hp, float x, float q) {
+    const float c = fabsf(q);
+    return e * (hp - x) * (c * (1.0f - c));
+  }
+};
+
+template <>
+struct Step<PHZ_GATE_DECAY> {
+  static __device__ __forceinline__ float gate(float z) { return z; }
+  static __device__ __forceinline__ float keep(float q) { return q; }
+  static __device__ __forceinline__ float write(float) { return 1.0f; }
+  static __device__ __forceinline__ float next(float h, float q, float x) { return fmaf(q, h, x); }
+  static __device__ __forceinline__ float dz(float e, float hp, float, float) { return e * hp; }
+};
+
+template <class E, int VEC>
+__device__ __forceinline__ Pack<E, VEC> load(const void* base, int64_t at) {
+  return *(const Pack<E, VEC>*)((const E*)base + at);
+}
+template <class E, int VEC>
+__device__ __forceinline__ void store(void* base, int64_t at, const float* v) {
+  Pack<E, VEC> p;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) p.v[i] = from_f32<E>(v[i]);
+  *(Pack<E, VEC>*)((E*)base + at) = p;
+}
+
+// A run of U steps as loaded. Backward: a = dh and hp = h_{t-1}; the decay
+// form's gradients do not need x.
+template <class E, int VEC, int U, bool BACK, bool NEED_X>
+struct Run {
+  Pack<E, VEC> z[U], x[NEED_X ? U : 1], a[BACK ? U : 1], hp[BACK ? U : 1];
+  uint32_t reset;  // bit u: an episode begins at this step
+};
+
+template <class E, int FORM, bool BACK, int VEC, int NW, int U, bool AGG>
+__global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p) {
+  using S = Step<FORM>;
+  // What a chunk's map needs: forward z, x; backward z and dh only.
+  constexpr bool kNeedX = BACK ? (FORM == PHZ_GATE_SIGMOID && !AGG) : true;
+  constexpr bool kNeedH = BACK && !AGG;
+  using R = Run<E, VEC, U, BACK, kNeedX>;
+  // Double-buffered, so one barrier a slab is enough.
+  __shared__ float lds[NW > 1 ? 2 * NW * 2 * VEC * kWaveLanes : 1];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int64_t id = (int64_t)blockIdx.x * kWaveLanes + lane;
+  const bool live = id < p.lanes;
+  const int64_t idc = live ? id : p.lanes - 1;  // idle lanes follow the last one, and store nothing
+  const int64_t b = idc / p.groups;
+  // The last group of a world starts early where VEC does not divide the
+  // width: its first channels are computed twice, to the same bits.
+  const int d = min((int)(idc - b * p.groups) * VEC, p.width - VEC);
+  const int chunk = p.chunks == 1 ? 0 : AGG ? (int)blockIdx.y : p.chunks - 1 - (int)blockIdx.y;
+  const int first = chunk * p.chunk, last = min(p.steps, first + p.chunk);
+
+  const E* z = (const E*)p.z + b * p.z_b + d;
+  const E* x = kNeedX ? (const E*)p.x + b * p.x_b + d : nullptr;
+  const E* dh = BACK ? (const E*)p.dh + b * p.dh_b + d : nullptr;
+  const E* h = kNeedH ? (const E*)p.h + b * p.h_b + d : nullptr;
+  const uint8_t* rs = p.reset ? p.reset + b * p.r_b : nullptr;
+
+  float s[VEC], prod[VEC];
+  bool forgot = false;  // the chunk so far (AGG)
+#pragma unroll
+  for (int v = 0; v < VEC; v++) s[v] = 0.0f, prod[v] = 1.0f;
+  if (!AGG) {
+    if (p.start) {
+#pragma unroll
+      for (int v = 0; v < VEC; v++) s[v] = p.start[b * p.start_b + d + v];
+    }
+    // The state that the earlier chunks leave.
+    for (int j = 0; j < chunk; j++) {
+      const float* a = p.agg + ((int64_t)j * 2 * p.lanes + idc) * VEC;
+      const Pack<float, VEC> A = load<float, VEC>(a, 0), H = load<float, VEC>(a, p.lanes * VEC);
+#pragma unroll
+      for (int v = 0; v < VEC; v++) s[v] = compose(A.v[v], s[v], H.v[v]);
+    }
+  }
+
+  auto step_of = [&](int i) { return (int64_t)(BACK ? p.steps - 1 - i : i); };
+  auto fetch = [&](R& r, int base) {
+    r.reset = 0;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = base + u;
+      if (i < last) {
+        const int64_t t = step_of(i);
+        r.z[u] = load<E, VEC>(z, t * p.z_t);
+        if (kNeedX) r.x[u] = load<E, VEC>(x, t * p.x_t);
+        if (BACK) r.a[u] = load<E, VEC>(dh, t * p.dh_t);
+        if (kNeedH && t > 0) r.hp[u] = load<E, VEC>(h, (t - 1) * p.h_t);
+        if (rs) r.reset |= (rs[t * p.r_t] ? 1u : 0u) << u;
+      }
+    }
+  };
+
+  const int stride = NW * U;
+  R cur, nxt;
+  int base = first + wave * U;
+  fetch(cur, base);
+  int buf = 0;
+  for (int slab = first; slab < last; slab += stride, base += stride) {
+    if (slab + stride < last) fetch(nxt, base + stride);
+    float q[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) q[u][v] = S::gate(to_f32(cur.z[u].v[v]));
+
+    // One step of the affine recurrence: forward to h_t, backward to k_t.
+    auto advance = [&](float st, int u, int v, bool rst) {
+      if (BACK) return rst ? 0.0f : S::keep(q[u][v]) * (to_f32(cur.a[u].v[v]) + st);
+      return S::next(rst ? 0.0f : st, q[u][v], to_f32(cur.x[kNeedX ? u : 0].v[v]));
+    };
+
+    if (AGG || NW > 1) {
+      // Compose this wave's run (onto the chunk's so far, where a wave works alone).
+      float A[VEC], H[VEC];
+      bool forget = false;
+#pragma unroll
+      for (int v = 0; v < VEC; v++) A[v] = NW > 1 ? 1.0f : prod[v], H[v] = NW > 1 ? 0.0f : s[v];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (base + u < last) {
+          const bool rst = (cur.reset >> u) & 1u;
+#pragma unroll
+          for (int v = 0; v < VEC; v++) {
+            H[v] = advance(H[v], u, v, rst);
+            A[v] *= S::keep(q[u][v]);
+          }
+          forget = forget || rst;
+        }
+      if (NW > 1) {
+        float* mine = lds + buf * (NW * 2 * VEC * kWaveLanes);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          mine[(wave * 2 * kWaveLanes + lane) * VEC + v] = forget ? __builtin_bit_cast(float, kForget) : A[v];
+          mine[((wave * 2 + 1) * kWaveLanes + lane) * VEC + v] = H[v];
+        }
+        __syncthreads();
+        // Fold every run of the slab in order; keep the state before this
+        // wave's own.
+        float before[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) before[v] = s[v];
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+          if (w == wave) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) before[v] = s[v];
+          }
+#pragma unroll
+          for (int v = 0; v < VEC; v++) {
+            const float a = mine[(w * 2 * kWaveLanes + lane) * VEC + v];
+            const float g = mine[((w * 2 + 1) * kWaveLanes + lane) * VEC + v];
+            s[v] = compose(a, s[v], g);
+            if (AGG) {
+              forgot = forgot || forgets(a);
+              prod[v] *= a;
+            }
+          }
+        }
+        if (!AGG) {
+          // The outputs, from the state before the run; s stays the slab's end.
+#pragma unroll
+          for (int u = 0; u < U; u++)
+            if (base + u < last) {
+              const int64_t t = step_of(base + u);
+              const bool rst = (cur.reset >> u) & 1u;
+              if (BACK) {
+                float dz[VEC], dx[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                  const float e = to_f32(cur.a[u].v[v]) + before[v];
+                  float hp = 0.0f;
+                  if (!rst) {
+                    if (t > 0) hp = to_f32(cur.hp[kNeedH ? u : 0].v[v]);
+                    else if (p.h0) hp = p.h0[b * p.h0_b + d + v];
+                  }
+                  dz[v] = S::dz(e, hp, kNeedX ? to_f32(cur.x[kNeedX ? u : 0].v[v]) : 0.0f, q[u][v]);
+                  dx[v] = S::write(q[u][v]) * e;
+                  before[v] = rst ? 0.0f : S::keep(q[u][v]) * e;
+                }
+                if (live) {
+                  store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, dz);
+                  store<E, VEC>(p.o2, b * p.o2_b + d + t * p.o2_t, dx);
+                }
+              } else {
+#pragma unroll
+                for (int v = 0; v < VEC; v++) before[v] = advance(before[v], u, v, rst);
+                if (live) store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, before);
+              }
+            }
+        }
+        buf ^= 1;
+      } else {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) prod[v] = A[v], s[v] = H[v];
+        forgot = forgot || forget;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (base + u < last) {
+          const int64_t t = step_of(base + u);
+          const bool rst = (cur.reset >> u) & 1u;
+          if (BACK) {
+            float dz[VEC], dx[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+              const float e = to_f32(cur.a[u].v[v]) + s[v];
+              float hp = 0.0f;
+              if (!rst) {
+                if (t > 0) hp = to_f32(cur.hp[kNeedH ? u : 0].v[v]);
+                else if (p.h0) hp = p.h0[b * p.h0_b + d + v];
+              }
+              dz[v] = S::dz(e, hp, kNeedX ? to_f32(cur.x[kNeedX ? u : 0].v[v]) : 0.0f, q[u][v]);
+              dx[v] = S::write(q[u][v]) * e;
+              s[v] = rst ? 0.0f : S::keep(q[u][v]) * e;
+            }
+            if (live) {
+              store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, dz);
+              store<E, VEC>(p.o2, b * p.o2_b + d + t * p.o2_t, dx);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) s[v] = advance(s[v], u, v, rst);
+            if (live) store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, s);
+          }
+        }
+    }
+    cur = nxt;
+  }
+
+  if (AGG) {
+    if (live && wave == 0) {
+      float* a = p.agg + ((int64_t)chunk * 2 * p.lanes + id) * VEC;
+#pragma unroll
+      for (int v = 0; v < VEC; v++) a[v] = forgot ? __builtin_bit_cast(float, kForget) : prod[v], a[p.lanes * VEC + v] = s[v];
+    }
+  } else if (p.end && chunk == p.chunks - 1 && live && wave == 0) {
+#pragma unroll
+    for (int v = 0; v < VEC; v++) p.end[b * p.end_b + d + v] = s[v];
+  }
+}
+
+template <class E, int FORM, bool BACK, int VEC>
+void launch(const ScanArgs& p, int nw, hipStream_t stream) {
+  constexpr int U = BACK ? 4 : 8;
+  const dim3 grid((unsigned)ceil_div(p.lanes, kWaveLanes), (unsigned)p.chunks);
+  if (p.chunks > 1) {
+    const dim3 front(grid.x, p.chunks - 1);  // nobody starts from the last chunk
+    if (nw == 1)
+      hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 1, U, true>), front, dim3(64), 0, stream, p);
+    else
+      hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 8, U, true>), front, dim3(512), 0, stream, p);
+  }
+  if (nw == 1)
+    hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 1, U, false>), grid, dim3(64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 8, U, false>), grid, dim3(512), 0, stream, p);
+}
+
+template <class E>
+void launch_any(const ScanArgs& p, int form, bool back, int vec, int nw, hipStream_t stream) {
+  auto go = [&](auto f, auto bk) {
+    if (vec == 4) launch<E, decltype(f)::value, decltype(bk)::value, 4>(p, nw, stream);
+    else launch<E, decltype(f)::value, decltype(bk)::value, 1>(p, nw, stream);
+  };
+  using Sg = std::integral_constant<int, PHZ_GATE_SIGMOID>;
+  using Dc = std::integral_constant<int, PHZ_GATE_DECAY>;
+  if (form == PHZ_GATE_SIGMOID) back ? go(Sg{}, std::true_type{}) : go(Sg{}, std::false_type{});
+  else back ? go(Dc{}, std::true_type{}) : go(Dc{}, std::false_type{});
+}
+
+// What is left where there are no steps: the last state is the first one.
+__global__ void copy_rows(const float* src, int64_t src_b, float* dst, int64_t dst_b, int64_t rows, int32_t width) {
+  const int64_t n = rows * width;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / width, c = i - r * width;
+    dst[r * dst_b + c] = src ? src[r * src_b + c] : 0.0f;
+  }
+}
+
+// One step for every channel, the state replaced in place. Bound by launch
+// latency below about a million channels, by memory above.
+template <class E, int FORM, int VEC>
+__global__ __launch_bounds__(256) void gated_step_kernel(const void* z, int64_t z_b, const void* x, int64_t x_b,
+                                                         const uint8_t* reset, int64_t r_b, float* h, int64_t h_b,
+                                                         int64_t lanes, int32_t groups, int32_t width) {
+  using S = Step<FORM>;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < lanes; id += (int64_t)gridDim.x * 256) {
+    const int64_t b = id / groups;
+    const int d = (int)(id - b * groups) * VEC;
+    const bool rst = reset && reset[b * r_b];
+    float* hs = h + b * h_b + d;
+    if (d + VEC <= width) {
+      const auto zv = load<E, VEC>(z, b * z_b + d), xv = load<E, VEC>(x, b * x_b + d);
+      auto hv = load<float, VEC>(hs, 0);
+#pragma unroll
+      for (int v = 0; v < VEC; v++)
+        hv.v[v] = S::next(rst ? 0.0f : hv.v[v], S::gate(to_f32(zv.v[v])), to_f32(xv.v[v]));
+      *(Pack<float, VEC>*)hs = hv;
+    } else {
+      for (int v = 0; d + v < width; v++)
+        hs[v] = S::next(rst ? 0.0f : hs[v], S::gate(to_f32(((const E*)z)[b * z_b + d + v])),
+                        to_f32(((const E*)x)[b * x_b + d + v]));
+    }
+  }
+}
+
+// How the steps and channels are spread. Lanes of four channels, two waves a
+// SIMD wanted (8 a compute unit).
+struct Plan {
+  int vec, nw, chunk, chunks;
+  int64_t groups, lanes;
+};
+
+Plan plan(const phz_ops* o, int64_t steps, int64_t worlds, int64_t width, bool back) {
+  Plan p;
+  p.vec = width >= 4 ? 4 : 1;
+  p.groups = ceil_div(width, p.vec);
+  p.lanes = worlds * p.groups;
+  const int64_t waves = ceil_div(p.lanes, kWaveLanes), want = 8ll * o->cus;
+  const int u = back ? 4 : 8;
+  p.nw = waves >= want / 2 || steps <= 2 * u ? 1 : 8;
+  const int64_t slab = (int64_t)p.nw * u;
+  int64_t chunks = std::min<int64_t>(ceil_div(want, waves * p.nw), steps / (4 * slab));
+  chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
+  p.chunk = (int)(ceil_div(ceil_div(steps, chunks), slab) * slab);
+  p.chunks = (int)std::max<int64_t>(1, ceil_div(steps, p.chunk));
+  return p;
+}
+
+bool check_form(phz_ops* o, int form) {
+  if (form == PHZ_GATE_SIGMOID || form == PHZ_GATE_DECAY) return true;
+  o->err = "unknown gate form";
+  return false;
+}
+
+bool check_type(phz_ops* o, const char* name, const phz_tensor* t) {
+  if (!t) return o->err = fmt("%s is missing", name), false;
+  if (t->dtype == PHZ_F32 || t->dtype == PHZ_BF16) return true;
+  o->err = fmt("%s is %s, expected f32 or bf16", name, dtype_name(t->dtype));
+  return false;
+}
+
+bool check_limits(phz_ops* o, int64_t steps, int64_t worlds, int64_t width) {
+  if (steps > 0x7fff0000ll || width > 0x7fff0000ll || worlds > 0x7fff0000ll)
+    return o->err = "steps, worlds and width have to be below 2^31", false;
+  if (worlds * ((width + 3) / 4) > 64ll * 0x7fff0000ll) return o->err = "too many channels", false;
+  return true;
+}
+
+int scan(phz_ops* o, hipStream_t stream, int form, bool back, ScanArgs a, int dtype, int64_t steps, int64_t worlds,
+         int64_t width) {
+  if (worlds == 0 || width == 0) return 0;
+  DeviceGuard g(o);
+  if (!g.ok) return 1;
+  if (steps == 0) {
+    if (a.end) {
+      const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(worlds * width, 256), 4096);
+      hipLaunchKernelGGL(copy_rows, dim3(blocks), dim3(256), 0, stream, a.start, a.start_b, a.end, a.end_b, worlds,
+                         (int32_t)width);
+    }
+    return launched(o, "gated scan") ? 0 : 1;
+  }
+  const Plan p = plan(o, steps, worlds, width, back);
+  a.steps = (int32_t)steps;
+  a.width = (int32_t)width;
+  a.groups = (int32_t)p.groups;
+  a.lanes = p.lanes;
+  a.chunk = p.chunk;
+  a.chunks = p.chunks;
+  if (p.chunks > 1) {
+    a.agg = (float*)o->workspace(stream, (uint64_t)p.chunks * 2 * p.lanes * p.vec * sizeof(float));
+    if (!a.agg) return 1;
+  }
+  if (dtype == PHZ_F32) launch_any<float>(a, form, back, p.vec, p.nw, stream);
+  else launch_any<bf16>(a, form, back, p.vec, p.nw, stream);
+  return launched(o, "gated scan") ? 0 : 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+int phz_gated_scan(phz_ops* o, void* stream, int form, const phz_tensor* z, const phz_tensor* x, const phz_tensor* h0,
+                   const phz_tensor* reset, const phz_tensor* h, const phz_tensor* h_last) {
+  return guarded(o, [&] {
+    if (!check_form(o, form) || !check_type(o, "z", z)) return 1;
+    const Want in{3, {-1, -1, -1}, z->dtype, true, false};
+    if (!check(o, "z", z, in)) return 1;
+    const int64_t T = z->size[0], B = z->size[1], D = z->size[2];
+    const Want like{3, {T, B, D}, z->dtype, true, false}, out{3, {T, B, D}, z->dtype, true, true};
+    const Want row{2, {B, D, 0}, PHZ_F32, true, false}, row_out{2, {B, D, 0}, PHZ_F32, true, true};
+    const Want mask{2, {T, B, 0}, PHZ_U8, false, false};
+    if (!check(o, "x", x, like) || !check(o, "h", h, out) || (h0 && !check(o, "h0", h0, row)) ||
+        (reset && !check(o, "reset", reset, mask)) || (h_last && !check(o, "h_last", h_last, row_out)) ||
+        !check_limits(o, T, B, D))
+      return 1;
+    for (const phz_tensor* t : {h, h_last}) {
+      const char* name = t == h ? "h" : "h_last";
+      if (!apart(o, name, t, "z", z) || !apart(o, name, t, "x", x) || !apart(o, name, t, "h0", h0) ||
+          !apart(o, name, t, "reset", reset))
+        return 1;
+    }
+    if (!apart(o, "h", h, "h_last", h_last)) return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    ScanArgs a{};
+    a.z = z->data, a.z_t = z->stride[0], a.z_b = z->stride[1];
+    a.x = x->data, a.x_t = x->stride[0], a.x_b = x->stride[1];
+    a.o1 = h->data, a.o1_t = h->stride[0], a.o1_b = h->stride[1];
+    if (h0) a.start = (const float*)h0->data, a.start_b = h0->stride[0];
+    if (h_last) a.end = (float*)h_last->data, a.end_b = h_last->stride[0];
+    if (reset) a.reset = (const uint8_t*)reset->data, a.r_t = reset->stride[0], a.r_b = reset->stride[1];
+    return scan(o, (hipStream_t)stream, form, false, a, z->dtype, T, B, D);
+  });
+}
+
+int phz_gated_scan_backward(phz_ops* o, void* stream, int form, const phz_tensor* dh, const phz_tensor* dh_last,
+                            const phz_tensor* z, const phz_tensor* x, const phz_tensor* h, const phz_tensor* h0,
+                            const phz_tensor* reset, const phz_tensor* dz, const phz_tensor* dx, const phz_tensor* dh0) {
+  return guarded(o, [&] {
+    if (!check_form(o, form) || !check_type(o, "z", z)) return 1;
+    const Want in{3, {-1, -1, -1}, z->dtype, true, false};
+    if (!check(o, "z", z, in)) return 1;
+    const int64_t T = z->size[0], B = z->size[1], D = z->size[2];
+    const Want like{3, {T, B, D}, z->dtype, true, false}, out{3, {T, B, D}, z->dtype, true, true};
+    const Want row{2, {B, D, 0}, PHZ_F32, true, false}, row_out{2, {B, D, 0}, PHZ_F32, true, true};
+    const Want mask{2, {T, B, 0}, PHZ_U8, false, false};
+    if (!check(o, "x", x, like) || !check(o, "h", h, like) || !check(o, "dh", dh, like) || !check(o, "dz", dz, out) ||
+        !check(o, "dx", dx, out) || (h0 && !check(o, "h0", h0, row)) || (dh_last && !check(o, "dh_last", dh_last, row)) ||
+        (reset && !check(o, "reset", reset, mask)) || (dh0 && !check(o, "dh0", dh0, row_out)) ||
+        !check_limits(o, T, B, D))
+      return 1;
+    const struct { const char* name; const phz_tensor* t; } outs[] = {{"dz", dz}, {"dx", dx}, {"dh0", dh0}},
+        ins[] = {{"dh", dh}, {"dh_last", dh_last}, {"z", z}, {"x", x}, {"h", h}, {"h0", h0}, {"reset", reset}};
+    for (auto& u : outs)
+      for (auto& v : ins)
+        if (!apart(o, u.name, u.t, v.name, v.t)) return 1;
+    if (!apart(o, "dz", dz, "dx", dx) || !apart(o, "dz", dz, "dh0", dh0) || !apart(o, "dx", dx, "dh0", dh0)) return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    ScanArgs a{};
+    a.z = z->data, a.z_t = z->stride[0], a.z_b = z->stride[1];
+    a.x = x->data, a.x_t = x->stride[0], a.x_b = x->stride[1];
+    a.h = h->data, a.h_t = h->stride[0], a.h_b = h->stride[1];
+    a.dh = dh->data, a.dh_t = dh->stride[0], a.dh_b = dh->stride[1];
+    a.o1 = dz->data, a.o1_t = dz->stride[0], a.o1_b = dz->stride[1];
+    a.o2 = dx->data, a.o2_t = dx->stride[0], a.o2_b = dx->stride[1];
+    if (dh_last) a.start = (const float*)dh_last->data, a.start_b = dh_last->stride[0];
+    if (h0) a.h0 = (const float*)h0->data, a.h0_b = h0->stride[0];
+    if (dh0) a.end = (float*)dh0->data, a.end_b = dh0->stride[0];
+    if (reset) a.reset = (const uint8_t*)reset->data, a.r_t = reset->stride[0], a.r_b = reset->stride[1];
+    return scan(o, (hipStream_t)stream, form, true, a, z->dtype, T, B, D);
+  });
+}
+
+int phz_gated_step(phz_ops* o, void* stream, int form, const phz_tensor* z, const phz_tensor* x,
+                   const phz_tensor* reset, const phz_tensor* h) {
+  return guarded(o, [&] {
+    if (!check_form(o, form) || !check_type(o, "z", z)) return 1;
+    if (!check(o, "z", z, Want{2, {-1, -1, 0}, z->dtype, true, false})) return 1;
+    const int64_t B = z->size[0], D = z->size[1];
+    if (!check(o, "x", x, Want{2, {B, D, 0}, z->dtype, true, false}) ||
+        (reset && !check(o, "reset", reset, Want{1, {B, 0, 0}, PHZ_U8, false, false})) ||
+        !check(o, "h", h, Want{2, {B, D, 0}, PHZ_F32, true, true}) || !check_limits(o, 1, B, D) ||
+        !apart(o, "h", h, "z", z) || !apart(o, "h", h, "x", x) || !apart(o, "h", h, "reset", reset))
+      return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    if (B == 0 || D == 0) return 0;
+    DeviceGuard g(o);
+    if (!g.ok) return 1;
+    constexpr int VEC = 4;
+    const int64_t groups = ceil_div(D, VEC), lanes = B * groups;
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(lanes, 256), 1 << 20);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, z->data, z->stride[0], x->data,
+                         x->stride[0], reset ? (const uint8_t*)reset->data : nullptr, reset ? reset->stride[0] : 0,
+                         (float*)h->data, h->stride[0], lanes, (int32_t)groups, (int32_t)D);
+    };
+    if (z->dtype == PHZ_F32)
+      form == PHZ_GATE_SIGMOID ? go(gated_step_kernel<float, PHZ_GATE_SIGMOID, VEC>)
+                               : go(gated_step_kernel<float, PHZ_GATE_DECAY, VEC>);
+    else
+      form == PHZ_GATE_SIGMOID ? go(gated_step_kernel<bf16, PHZ_GATE_SIGMOID, VEC>)
+                               : go(gated_step_kernel<bf16, PHZ_GATE_DECAY, VEC>);
+    return launched(o, "gated step") ? 0 : 1;
+  });
+}
+
+}  // extern "C"
