@@ -65,12 +65,24 @@ struct LinearOut {
   E *pre, *y;
   int64_t residual_row, pre_row, y_row, bias_step;
   int act;
-  __device__ __forceinline__ void operator()(int, int, int i, int j, float p) const {
-    if (bias) p += to_f32(bias[j * bias_step]);
-    if (pre) pre[i * pre_row + j] = from_f32<E>(p);
-    p = act_of(act, p);
-    if (residual) p += to_f32(residual[i * residual_row + j]);
-    y[i * y_row + j] = from_f32<E>(p);
+  template <int N>
+  __device__ __forceinline__ void put(int, int, int i, int j, const float* sums) const {
+    float p[N];
+    Pack<E, N> r, out;
+    if (residual) r = *(const Pack<E, N>*)(residual + i * residual_row + j);
+#pragma unroll
+    for (int c = 0; c < N; c++) p[c] = bias ? sums[c] + to_f32(bias[(j + c) * bias_step]) : sums[c];
+    if (pre) {
+#pragma unroll
+      for (int c = 0; c < N; c++) out.v[c] = from_f32<E>(p[c]);
+      *(Pack<E, N>*)(pre + i * pre_row + j) = out;
+    }
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+      p[c] = act_of(act, p[c]);
+      out.v[c] = from_f32<E>(residual ? p[c] + to_f32(r.v[c]) : p[c]);
+    }
+    *(Pack<E, N>*)(y + i * y_row + j) = out;
   }
 };
 
@@ -78,14 +90,26 @@ template <class E>
 struct PlainOut {
   E* y;
   int64_t row;
-  __device__ __forceinline__ void operator()(int, int, int i, int j, float p) const { y[i * row + j] = from_f32<E>(p); }
+  template <int N>
+  __device__ __forceinline__ void put(int, int, int i, int j, const float* sums) const {
+    Pack<E, N> out;
+#pragma unroll
+    for (int c = 0; c < N; c++) out.v[c] = from_f32<E>(sums[c]);
+    *(Pack<E, N>*)(y + i * row + j) = out;
+  }
 };
 
 // Sums of one split of the contraction, joined by join_splits.
 struct SplitOut {
   float* part;
   int64_t row, split;
-  __device__ __forceinline__ void operator()(int, int s, int i, int j, float p) const { part[s * split + i * row + j] = p; }
+  template <int N>
+  __device__ __forceinline__ void put(int, int s, int i, int j, const float* sums) const {
+    Pack<float, N> out;
+#pragma unroll
+    for (int c = 0; c < N; c++) out.v[c] = sums[c];
+    *(Pack<float, N>*)(part + s * split + i * row + j) = out;
+  }
 };
 
 // y[i][j] = the splits' sums, added in order.

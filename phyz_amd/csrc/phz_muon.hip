@@ -5,7 +5,7 @@
 //
 // on whichever side is shorter: for tall matrices A = X^T X and
 // X <- a X + X (b A + c A^2), so nothing is transposed.
-#include "phz_gemm.h"
+#include "phz_gemm_fast.h"
 
 #include <math.h>
 
@@ -15,111 +15,309 @@ using namespace phzop;
 
 namespace {
 
-constexpr int kNormBlocks = 64;  // partial sums of squares per matrix
-
 struct View {
   void* data;
   int64_t batch, row;
 };
 
-// The matrix to orthogonalise into X (f32, dense) and partial sums of its
-// squares, in f64: gradients whose squares leave f32's range have a norm too.
-// With a momentum, m <- mu m + g comes first and the matrix is g + mu m or m.
-template <class E>
-__global__ __launch_bounds__(256) void gather_kernel(View g, View m, float mu, int nesterov, float* x, double* part,
-                                                     int32_t rows, int32_t cols) {
-  const int q = blockIdx.y;
-  const int64_t n = (int64_t)rows * cols;
-  double sum = 0.0;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)kNormBlocks * 256) {
-    const int64_t i = t / cols, j = t - i * cols;
-    float v = to_f32(((const E*)g.data)[q * g.batch + i * g.row + j]);
-    if (m.data) {
-      float* mp = (float*)m.data + q * m.batch + i * m.row + j;
-      const float mn = fmaf(mu, *mp, v);
-      *mp = mn;
-      v = nesterov ? fmaf(mu, mn, v) : mn;
-    }
-    x[q * n + t] = v;
-    sum += (double)v * v;
-  }
+// Blocks that share a matrix's sum of squares; each leaves one partial.
+int norm_blocks(int64_t elements) { return (int)std::max<int64_t>(1, std::min<int64_t>(512, elements / 4096)); }
+
+__device__ __forceinline__ double block_sum(double v) {
   __shared__ double s[256];
-  s[threadIdx.x] = sum;
+  s[threadIdx.x] = v;
   __syncthreads();
   for (int k = 128; k; k >>= 1) {
     if (threadIdx.x < k) s[threadIdx.x] += s[threadIdx.x + k];
     __syncthreads();
   }
-  if (threadIdx.x == 0) part[q * kNormBlocks + blockIdx.x] = s[0];
+  return s[0];
 }
 
-__global__ __launch_bounds__(256) void scale_kernel(float* x, const double* part, double eps, int64_t n) {
+// Eight neighbouring elements of a row (fewer at its end: zeros).
+template <class E>
+__device__ __forceinline__ void load8(const View& t, int q, int64_t i, int j, int cols, float* v) {
+  const E* p = (const E*)t.data + q * t.batch + i * t.row + j;
+  if (j + 8 <= cols) {
+    const Pack<E, 8> w = *(const Pack<E, 8>*)p;
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = to_f32(w.v[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = j + c < cols ? to_f32(p[c]) : 0.0f;
+  }
+}
+
+// The matrix: g, or with a momentum m (already updated) what Muon
+// orthogonalises.
+template <class E>
+struct Source {
+  View g, m;
+  float mu;
+  int nesterov;
+  __device__ __forceinline__ void at(int q, int64_t i, int j, int cols, float* v) const {
+    if (!m.data) return load8<E>(g, q, i, j, cols, v);
+    load8<float>(m, q, i, j, cols, v);
+    if (nesterov) {
+      float d[8];
+      load8<E>(g, q, i, j, cols, d);
+#pragma unroll
+      for (int c = 0; c < 8; c++) v[c] = fmaf(mu, v[c], d[c]);
+    }
+  }
+};
+
+// m <- mu m + g, and partial sums of the matrix's squares in f64: gradients
+// whose squares leave f32's range have a norm too.
+template <class E>
+__global__ __launch_bounds__(256) void norm_kernel(Source<E> s, double* part, int32_t rows, int32_t cols) {
   const int q = blockIdx.y;
+  const uint32_t per = (cols + 7) / 8, n = (uint32_t)rows * per;  // eights
   double sum = 0.0;
-  for (int i = 0; i < kNormBlocks; i++) sum += part[q * kNormBlocks + i];
-  const double inv = 1.0 / (sqrt(sum) + eps);
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256)
-    x[q * n + t] = (float)(x[q * n + t] * inv);
+  for (uint32_t t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
+    const uint32_t i = t / per;
+    const int j = (t - i * per) * 8;
+    float v[8];
+    if (s.m.data) {
+      float d[8];
+      load8<float>(s.m, q, i, j, cols, v);
+      load8<E>(s.g, q, i, j, cols, d);
+#pragma unroll
+      for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
+      float* mp = (float*)s.m.data + q * s.m.batch + i * s.m.row + j;
+      if (j + 8 <= cols) {
+        Pack<float, 8> w;
+#pragma unroll
+        for (int c = 0; c < 8; c++) w.v[c] = v[c];
+        *(Pack<float, 8>*)mp = w;
+      } else {
+        for (int c = 0; j + c < cols; c++) mp[c] = v[c];
+      }
+      if (s.nesterov) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
+      }
+    } else {
+      load8<E>(s.g, q, i, j, cols, v);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; c++) sum = fma((double)v[c], (double)v[c], sum);
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) part[(int64_t)q * gridDim.x + blockIdx.x] = sum;
 }
 
-// C = alpha * product + beta * D
+// X as planes of f16: the value times `scale` as hi + lo (or hi alone), rows of
+// `ld` (a multiple of eight), zeros past the matrix's columns.
+struct Planes {
+  half_t* data;
+  int64_t plane, row, batch;  // elements
+};
+
+template <int P>
+__device__ __forceinline__ void put_planes(const Planes& p, int64_t at, const float* v) {
+  Pack<half_t, 8> hi, lo;
+#pragma unroll
+  for (int c = 0; c < 8; c++) {
+    hi.v[c] = from_f32<half_t>(v[c]);
+    if (P == 2) lo.v[c] = from_f32<half_t>(v[c] - to_f32(hi.v[c]));
+  }
+  *(Pack<half_t, 8>*)(p.data + at) = hi;
+  if (P == 2) *(Pack<half_t, 8>*)(p.data + p.plane + at) = lo;
+}
+template <int P>
+__device__ __forceinline__ void get_planes(const Planes& p, int64_t at, float* v) {
+  const Pack<half_t, 8> hi = *(const Pack<half_t, 8>*)(p.data + at);
+  Pack<half_t, 8> lo{};
+  if (P == 2) lo = *(const Pack<half_t, 8>*)(p.data + p.plane + at);
+#pragma unroll
+  for (int c = 0; c < 8; c++) v[c] = P == 2 ? to_f32(hi.v[c]) + to_f32(lo.v[c]) : to_f32(hi.v[c]);
+}
+
+__device__ __forceinline__ double inverse_norm(const double* part, int parts, int q, double eps) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) sum += part[(int64_t)q * parts + i];
+  return 1.0 / (sqrt(block_sum(sum)) + eps);
+}
+
+// X = the matrix over its norm, as two planes, or in f32 where xf is given.
+template <class E>
+__global__ __launch_bounds__(256) void scale_kernel(Source<E> s, const double* part, int parts, double eps, float scale,
+                                                    Planes x, float* xf, int32_t rows, int32_t cols) {
+  const int q = blockIdx.y;
+  const double inv = inverse_norm(part, parts, q, eps) * scale;
+  const uint32_t per = (cols + 7) / 8, n = (uint32_t)rows * per;
+  for (uint32_t t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
+    const uint32_t i = t / per;
+    const int j = (t - i * per) * 8;
+    float v[8];
+    s.at(q, i, j, cols, v);
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = (float)(v[c] * inv);
+    if (xf) {
+#pragma unroll
+      for (int c = 0; c < 8; c++)
+        if (j + c < cols) xf[((int64_t)q * rows + i) * cols + j + c] = v[c];
+    } else {
+      put_planes<2>(x, q * x.batch + i * x.row + j, v);
+    }
+  }
+}
+
+// y = alpha sum + beta d, as PY planes; d has PD.
+template <int PY, int PD>
+struct PlanesOut {
+  Planes y, d;
+  float alpha, beta;
+  int32_t cols;  // columns that exist: zeros beyond
+  template <int N>
+  __device__ __forceinline__ void put(int q, int, int i, int j, const float* sums) const {
+    static_assert(N == 8 || N == 1, "");
+    if (N != 8) return;  // rows are whole eights
+    float v[8], o[8];
+    if (d.data) get_planes<PD>(d, q * d.batch + i * d.row + j, o);
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      v[c] = j + c < cols ? (d.data ? fmaf(alpha, sums[c], beta * o[c]) : alpha * sums[c]) : 0.0f;
+    put_planes<PY>(y, q * y.batch + i * y.row + j, v);
+  }
+};
+
+// The last X' as o, or into the weights: w <- keep w - step X'.
+template <class O>
+struct Result {
+  O* o;
+  int64_t row, batch;
+  float keep, step;
+  int update;
+  __device__ __forceinline__ void put(int q, int64_t i, int64_t j, float v) const {
+    O* at = o + q * batch + i * row + j;
+    *at = from_f32<O>(update ? fmaf(-step, v, keep * to_f32(*at)) : v);
+  }
+  template <int N>
+  __device__ __forceinline__ void put_many(int q, int64_t i, int64_t j, const float* v) const {
+    Pack<O, N>* at = (Pack<O, N>*)(o + q * batch + i * row + j);
+    Pack<O, N> w;
+    if (update) w = *at;
+#pragma unroll
+    for (int c = 0; c < N; c++) w.v[c] = from_f32<O>(update ? fmaf(-step, v[c], keep * to_f32(w.v[c])) : v[c]);
+    *at = w;
+  }
+};
+
+// alpha sum + beta X into the result.
+template <class O>
+struct LastOut {
+  Planes x;
+  float alpha, beta;
+  int32_t cols;
+  Result<O> out;
+  template <int N>
+  __device__ __forceinline__ void put(int q, int, int i, int j, const float* sums) const {
+    if (N != 8) return;
+    float v[8];
+    get_planes<2>(x, q * x.batch + i * x.row + j, v);
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = fmaf(alpha, sums[c], beta * v[c]);
+    if (j + 8 <= cols) out.template put_many<8>(q, i, j, v);
+    else
+      for (int c = 0; c < 8 && j + c < cols; c++) out.put(q, i, j + c, v[c]);
+  }
+};
+
+// C = alpha product + beta D in f32 (any coefficients; see newton_schulz_any).
 struct Axpby {
   float *y;
   const float* d;
   float alpha, beta;
   int64_t row, batch;
-  __device__ __forceinline__ void operator()(int q, int, int i, int j, float p) const {
+  template <int N>
+  __device__ __forceinline__ void put(int q, int, int i, int j, const float* p) const {
     const int64_t at = q * batch + i * row + j;
-    y[at] = fmaf(alpha, p, d ? beta * d[at] : 0.0f);
+    y[at] = fmaf(alpha, p[0], d ? beta * d[at] : 0.0f);
   }
 };
 
-// The last step's X' as o, or into the weights: w <- keep w - step X'.
-template <class E>
-struct LastOut {
+template <class O>
+struct LastAny {
   const float* x;
   float a;
   int64_t row, batch;
-  E* o;
-  int64_t o_row, o_batch;
-  float keep, step;
-  int update;
-  __device__ __forceinline__ void operator()(int q, int, int i, int j, float p) const {
-    const float v = fmaf(a, x[q * batch + i * row + j], p);
-    E* at = o + q * o_batch + i * o_row + j;
-    *at = from_f32<E>(update ? fmaf(-step, v, keep * to_f32(*at)) : v);
+  Result<O> out;
+  template <int N>
+  __device__ __forceinline__ void put(int q, int, int i, int j, const float* p) const {
+    out.put(q, i, j, fmaf(a, x[q * batch + i * row + j], p[0]));
   }
 };
 
-template <class E>
-__global__ __launch_bounds__(256) void finish_kernel(LastOut<E> out, int32_t rows, int32_t cols) {
+template <class O>
+__global__ __launch_bounds__(256) void finish_kernel(LastAny<O> out, int32_t rows, int32_t cols) {
   const int64_t n = (int64_t)rows * cols;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256)
-    out(blockIdx.y, 0, (int)(t / cols), (int)(t % cols), 0.0f);
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const float zero = 0.0f;
+    out.template put<1>(blockIdx.y, 0, (int)(t / cols), (int)(t % cols), &zero);
+  }
 }
 
+// The largest |p(s)| for s in [0, top], p odd: p(s) = a s + b s^3 + c s^5, at
+// the ends or where p' = 0, a quadratic in s^2.
+double quintic_top(double a, double b, double c, double top) {
+  auto p = [&](double s) { return fabs(s * (a + s * s * (b + s * s * c))); };
+  double best = p(top);
+  auto at = [&](double t) {
+    if (t > 0 && t < top * top) best = std::max(best, p(sqrt(t)));
+  };
+  if (c == 0.0) {
+    if (b != 0.0) at(-a / (3 * b));
+  } else if (9 * b * b >= 20 * a * c) {
+    const double d = sqrt(9 * b * b - 20 * a * c);
+    at((-3 * b + d) / (10 * c));
+    at((-3 * b - d) / (10 * c));
+  }
+  return best;
+}
+
+// What the iterates' singular values stay below, and so every element: of X,
+// of A, and of b A + c A^2.
+struct Bounds {
+  double x, a, p;
+};
+Bounds bounds(const phz_muon_cfg& g) {
+  Bounds m{1.0, 1.0, 0.0};
+  double top = 1.0;
+  for (int k = 0; k < g.steps; k++) {
+    const double t = top * top;
+    m.a = std::max(m.a, t);
+    m.p = std::max(m.p, fabs(t * (g.b + g.c * t)));
+    if (g.c != 0.0 && -g.b / (2 * g.c) > 0 && -g.b / (2 * g.c) < t) m.p = std::max(m.p, g.b * g.b / fabs(4 * g.c));
+    top = quintic_top(g.a, g.b, g.c, top) * 1.001;
+    m.x = std::max(m.x, top);
+    if (!(m.x < 1e30)) break;
+  }
+  return m;
+}
+
+// Any coefficients: products of f32 operands at any size (phz_gemm.h).
 template <class G, class O>
-int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t batch, int32_t rows, int32_t cols,
-                  View g, View m, LastOut<O> last) {
+int newton_schulz_any(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t batch, int32_t rows,
+                      int32_t cols, const Source<G>& src, const Result<O>& out) {
   const int64_t n = (int64_t)rows * cols, s = std::min(rows, cols);
-  const uint64_t part_bytes = ((uint64_t)batch * kNormBlocks * 8 + 255) & ~255ull;
-  const uint64_t bytes = part_bytes + (uint64_t)batch * (2 * n + 2 * s * s) * 4;
-  char* ws = o->workspace(stream, bytes);
+  const int parts = norm_blocks(n);
+  const uint64_t part_bytes = ((uint64_t)batch * parts * 8 + 255) & ~255ull;
+  char* ws = o->workspace(stream, part_bytes + (uint64_t)batch * (2 * n + 2 * s * s) * 4);
   if (!ws) return 1;
   double* part = (double*)ws;
   float* x = (float*)(ws + part_bytes);
   float *y = x + batch * n, *a = y + batch * n, *p = a + batch * s * s;
-  hipLaunchKernelGGL(gather_kernel<G>, dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, stream, g, m,
-                     (float)cfg.momentum, cfg.nesterov, x, part, rows, cols);
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, 256), 4096);
-  hipLaunchKernelGGL(scale_kernel, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, x, part, cfg.eps, n);
+  hipLaunchKernelGGL(norm_kernel<G>, dim3(parts, (unsigned)batch), dim3(256), 0, stream, src, part, rows, cols);
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, 2048), 2048);
+  hipLaunchKernelGGL(scale_kernel<G>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, src, part, parts, cfg.eps,
+                     1.0f, Planes{}, x, rows, cols);
   const bool wide = rows <= cols;
   const int32_t si = (int32_t)s, l = std::max(rows, cols);
-  last.row = cols, last.batch = n;
-  if (cfg.steps == 0) {
-    last.x = x, last.a = 1.0f;
-    hipLaunchKernelGGL(finish_kernel<O>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, last, rows, cols);
-  }
+  if (cfg.steps == 0)
+    hipLaunchKernelGGL(finish_kernel<O>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream,
+                       LastAny<O>{x, 1.0f, cols, n, out}, rows, cols);
   for (int k = 0; k < cfg.steps; k++) {
     const Operand xo{x, cols, n}, ao{a, s, s * s}, po{p, s, s * s};
     const Axpby gram{a, nullptr, 1.0f, 0.0f, s, s * s};
@@ -134,13 +332,89 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64
       if (wide) launch_gemm_any<float, true, false>(o, stream, po, xo, xs, (int)batch, next);
       else launch_gemm_any<float, true, true>(o, stream, xo, po, xs, (int)batch, next);
     } else {
-      last.x = x, last.a = (float)cfg.a;
+      const LastAny<O> last{x, (float)cfg.a, cols, n, out};
       if (wide) launch_gemm_any<float, true, false>(o, stream, po, xo, xs, (int)batch, last);
       else launch_gemm_any<float, true, true>(o, stream, xo, po, xs, (int)batch, last);
     }
     std::swap(x, y);
   }
   return launched(o, "orthogonalize") ? 0 : 1;
+}
+
+FastArgs product(const Planes& a, const Planes& b, int32_t m, int32_t n, int32_t k, int32_t a_rows, int32_t b_rows) {
+  FastArgs f{};
+  f.a = (const char*)a.data, f.b = (const char*)b.data;
+  f.a_row = a.row * 2, f.b_row = b.row * 2, f.a_batch = a.batch * 2, f.b_batch = b.batch * 2;
+  f.a_plane = (uint32_t)(a.plane * 2), f.b_plane = (uint32_t)(b.plane * 2);
+  f.m = m, f.n = n, f.k = k, f.a_rows = a_rows, f.b_rows = b_rows;
+  f.k_split = (k + 63) / 64 * 64, f.splits = 1;
+  return f;
+}
+
+// The iterates as f16 planes. X starts at norm 1 and its singular values stay
+// below a bound that the coefficients give, so a power of two puts every
+// element in f16's range: no element leaves it, and what falls below its
+// smallest is 2^-39 of what the bound allows.
+//
+// P = 2, for f32 gradients: every operand is hi + lo, 22 bits. P = 1, for bf16
+// ones: products take hi alone, 11 bits to the gradient's 8, but X is carried
+// as hi + lo through a X. Its rounding to 11 bits would be noise in every
+// direction, which the steps raise along with the small singular values (3.3e-3
+// of the result at 1024 x 4096 with a few directions ten times the rest,
+// against 1.7e-3 for rounding the result alone); that of A and of the products
+// only moves the directions that are large.
+template <class G, class O, int P>
+int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const Bounds& top, int64_t batch,
+                  int32_t rows, int32_t cols, const Source<G>& src, const Result<O>& out) {
+  const bool wide = rows <= cols;
+  const int32_t s = std::min(rows, cols), l = std::max(rows, cols), s8 = (s + 7) & ~7, c8 = (cols + 7) & ~7;
+  const int parts = norm_blocks((int64_t)rows * cols);
+  const uint64_t part_bytes = ((uint64_t)batch * parts * 8 + 255) & ~255ull;
+  // A matrix's planes lie together, each from a multiple of 256 bytes.
+  const int64_t xn = ((int64_t)rows * c8 + 127) & ~127ll, an = ((int64_t)s * s8 + 127) & ~127ll;
+  char* ws = o->workspace(stream, part_bytes + (uint64_t)batch * (4 * xn + 2 * P * an) * 2);
+  if (!ws) return 1;
+  double* part = (double*)ws;
+  half_t* h = (half_t*)(ws + part_bytes);
+  Planes x{h, xn, c8, 2 * xn}, y{h + 2 * batch * xn, xn, c8, 2 * xn};
+  const Planes a{h + 4 * batch * xn, an, s8, P * an}, p{h + (4 * xn + P * an) * batch, an, s8, P * an};
+  auto scale = [](double bound) { return exp2(floor(log2(32768.0 / bound))); };
+  const double sx = scale(top.x), sa = scale(top.a), sp = scale(top.p > 0 ? top.p : 1.0);
+  hipLaunchKernelGGL(norm_kernel<G>, dim3(parts, (unsigned)batch), dim3(256), 0, stream, src, part, rows, cols);
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 2048), 2048);
+  hipLaunchKernelGGL(scale_kernel<G>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, src, part, parts, cfg.eps,
+                     (float)sx, x, nullptr, rows, cols);
+  for (int k = 0; k < cfg.steps; k++) {
+    const PlanesOut<P, P> gram{a, Planes{}, (float)(sa / (sx * sx)), 0.0f, s};
+    if (wide) launch_gemm_fast<half_t, P, true, true>(o, stream, product(x, x, s, s8, c8, s, s), (int)batch, gram);
+    else launch_gemm_fast<half_t, P, false, false>(o, stream, product(x, x, s, s8, l, s8, s8), (int)batch, gram);
+    const PlanesOut<P, P> poly{p, a, (float)(cfg.c * sp / (sa * sa)), (float)(cfg.b * sp / sa), s};
+    launch_gemm_fast<half_t, P, true, true>(o, stream, product(a, a, s, s8, s8, s, s), (int)batch, poly);
+    const FastArgs f = wide ? product(p, x, rows, c8, s, s, c8) : product(x, p, rows, c8, s8, rows, s);
+    if (k + 1 < cfg.steps) {
+      const PlanesOut<2, 2> next{y, x, (float)(1.0 / sp), (float)cfg.a, cols};
+      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, next);
+      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, next);
+    } else {
+      const LastOut<O> last{x, (float)(1.0 / (sp * sx)), (float)(cfg.a / sx), cols, out};
+      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, last);
+      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, last);
+    }
+    std::swap(x, y);
+  }
+  return launched(o, "orthogonalize") ? 0 : 1;
+}
+
+template <class G, class O>
+int orthogonal(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t batch, int64_t rows, int64_t cols,
+               View g, View m, const Result<O>& out) {
+  const Source<G> src{g, m, (float)cfg.momentum, cfg.nesterov};
+  const Bounds top = bounds(cfg);
+  // Coefficients that let the iterates grow past f16 (or no step at all).
+  if (cfg.steps == 0 || !(top.x <= 64) || !(top.a <= 4096) || !(top.p <= 4096))
+    return newton_schulz_any<G, O>(o, stream, cfg, batch, (int32_t)rows, (int32_t)cols, src, out);
+  constexpr int P = sizeof(O) == 2 ? 1 : 2;
+  return newton_schulz<G, O, P>(o, stream, cfg, top, batch, (int32_t)rows, (int32_t)cols, src, out);
 }
 
 bool check_cfg(phz_ops* o, const phz_muon_cfg* c, bool step) {
@@ -194,17 +468,11 @@ int phz_orthogonalize(phz_ops* o, void* stream, const phz_muon_cfg* cfg, const p
     DeviceGuard guard(o);
     if (!guard.ok) return 1;
     const View ov = view(out);
-    phz_muon_cfg c = *cfg;
-    if (g->dtype == PHZ_F32) {
-      LastOut<float> last{};
-      last.o = (float*)ov.data, last.o_row = ov.row, last.o_batch = ov.batch;
-      return newton_schulz<float, float>(o, (hipStream_t)stream, c, s.batch, (int32_t)s.rows, (int32_t)s.cols, view(g),
-                                         View{}, last);
-    }
-    LastOut<bf16> last{};
-    last.o = (bf16*)ov.data, last.o_row = ov.row, last.o_batch = ov.batch;
-    return newton_schulz<bf16, bf16>(o, (hipStream_t)stream, c, s.batch, (int32_t)s.rows, (int32_t)s.cols, view(g),
-                                     View{}, last);
+    if (g->dtype == PHZ_F32)
+      return orthogonal<float, float>(o, (hipStream_t)stream, *cfg, s.batch, s.rows, s.cols, view(g), View{},
+                                      Result<float>{(float*)ov.data, ov.row, ov.batch, 0.0f, 0.0f, 0});
+    return orthogonal<bf16, bf16>(o, (hipStream_t)stream, *cfg, s.batch, s.rows, s.cols, view(g), View{},
+                                  Result<bf16>{(bf16*)ov.data, ov.row, ov.batch, 0.0f, 0.0f, 0});
   });
 }
 
@@ -225,16 +493,12 @@ int phz_muon_step(phz_ops* o, void* stream, const phz_muon_cfg* cfg, const phz_t
     DeviceGuard guard(o);
     if (!guard.ok) return 1;
     const View wv = view(w);
-    LastOut<float> last{};
-    last.o = (float*)wv.data, last.o_row = wv.row, last.o_batch = wv.batch;
-    last.update = 1;
-    last.keep = (float)(1.0 - cfg->lr * cfg->weight_decay);
-    last.step = (float)(cfg->lr * sqrt(std::max(1.0, (double)s.rows / (double)s.cols)));
+    const double shape = sqrt(std::max(1.0, (double)s.rows / (double)s.cols));
+    const Result<float> out{(float*)wv.data, wv.row, wv.batch, (float)(1.0 - cfg->lr * cfg->weight_decay),
+                            (float)(cfg->lr * shape), 1};
     return g->dtype == PHZ_F32
-               ? newton_schulz<float, float>(o, (hipStream_t)stream, *cfg, s.batch, (int32_t)s.rows, (int32_t)s.cols,
-                                             view(g), view(m), last)
-               : newton_schulz<bf16, float>(o, (hipStream_t)stream, *cfg, s.batch, (int32_t)s.rows, (int32_t)s.cols,
-                                            view(g), view(m), last);
+               ? orthogonal<float, float>(o, (hipStream_t)stream, *cfg, s.batch, s.rows, s.cols, view(g), view(m), out)
+               : orthogonal<bf16, float>(o, (hipStream_t)stream, *cfg, s.batch, s.rows, s.cols, view(g), view(m), out);
   });
 }
 
