@@ -129,7 +129,7 @@ struct Stage {
 
 // Any size and layout: a workgroup of four waves per BM x BN tile, registers
 // holding the next k tile while the matrix cores work on the one in LDS.
-// `epi.put<N>(q, split, i, j, sums)` takes N neighbouring elements of a row.
+// `epi.put1(q, split, i, j, sum)` takes each element.
 template <class E, bool AK, bool BKD, int BM, int BN, class Epi>
 __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape s, Epi epi) {
   constexpr int P = Cut<E>::pieces, BK = Cut<E>::tile_k, LD = BK + 8;
@@ -240,10 +240,7 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int row = m0 + wm + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-          if (row < s.m) {
-            const float v = acc[i][j][r];
-            epi.template put<1>(q, split, row, col, &v);
-          }
+          if (row < s.m) epi.put1(q, split, row, col, acc[i][j][r]);
         }
       }
     }

@@ -8,6 +8,8 @@
 // operands dense along rows), a multiple of eight elements long or padded with
 // zeros to one.
 #pragma once
+#include <algorithm>
+
 #include "phz_gemm.h"
 
 namespace phzop {
@@ -127,6 +129,11 @@ struct FastTile {
   }
 };
 
+// An epilogue has
+//   Held, fetch(q, i, j, held)         what it reads for eight elements, ahead
+//   put8(q, split, i, j, sums, held)   eight neighbouring sums of row i
+//   put1(q, split, i, j, sum)          one, at a ragged end
+//
 // A tile BM x BN, contraction BK a stage, NS stages of LDS, MW x NW waves, and
 // NG such groups of waves: each takes every NG-th stage of the contraction, and
 // their sums are added in order at the end. One group where the tiles fill the
@@ -198,15 +205,15 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
   for (int t = 0; t < NS - 1; t++)
     if (t < steps) load(base + t * kStage);
   int now = 0;
-  for (int t = 0; t < steps; t++) {
-    // This wave's loads of this stage have landed (those of later stages may be
-    // in flight; a group's last ones may be fewer, then all of them are waited
-    // for) and its reads of the last one are done; past the barrier that holds
-    // for every wave, and the last stage may be overwritten.
+  // Waits for stage t: this wave's loads of it have landed (those of later
+  // stages may be in flight; a group's last ones may be fewer, then all of them
+  // are waited for) and its reads of the last one are done; past the barrier
+  // that holds for every wave, and the last stage may be overwritten.
+  auto arrive = [&](int t) {
     if (t + NS - 1 + (NG > 1) <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * kLoads) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + NS - 1 < steps) load(base + (now == 0 ? (NS - 1) * kStage : now - kStage));
-    if (NG > 1 && t * NG + group >= total) continue;  // no stage is left for this group
+  };
+  auto compute = [&] {
     const char* l = lds + group * kOne + now;
     now = now == (NS - 1) * kStage ? 0 : now + kStage;
 #pragma unroll
@@ -230,19 +237,40 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
           acc[i][j] = Mfma<T>::run(fa[0][i], fb[0][j], acc[i][j]);
         }
     }
+  };
+  for (int t = 0; t + 1 < steps; t++) {
+    arrive(t);
+    if (t + NS - 1 < steps) load(base + (now == 0 ? (NS - 1) * kStage : now - kStage));
+    compute();
   }
+
+  // What the epilogue reads is under way during the last stage: each lane's
+  // eight columns of the first 32 rows of its wave's part.
+  constexpr int kLanes = WN / 8, kRows = 64 / kLanes;  // lanes along a row, rows at once
+  constexpr int kShare = 32 / NG;  // rows that a group puts out; where they are fewer than kRows, lanes idle
+  constexpr int kPuts = kShare < kRows ? 1 : kShare / kRows;
+  const int col = n0 + wn + (lane % kLanes) * 8;
+  const bool mine = kShare >= kRows || lane / kLanes < kShare;
+  auto row_of = [&](int i, int r) { return m0 + wm + i * 32 + group * kShare + r * kRows + lane / kLanes; };
+  typename Epi::Held held[2][kPuts];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int r = 0; r < kPuts; r++)
+      if (mine && row_of(i, r) < p.m && col + 8 <= p.n) epi.fetch(q, row_of(i, r), col, held[i & 1][r]);
+  };
+  arrive(steps - 1);
+  fetch(0);
+  if (NG == 1 || (steps - 1) * NG + group < total) compute();  // a group may have no last stage
 
   // Out through LDS, 32 rows of a wave's part at a time, so that each lane
   // holds eight neighbouring columns: wide loads and stores, whole lines. The
   // groups' sums meet here, and each group puts out its share of the rows.
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   float* out = (float*)lds + wave * 32 * kOutRow;
-  constexpr int kGroup = NWAVE * 32 * kOutRow;       // floats between groups
-  constexpr int kLanes = WN / 8, kRows = 64 / kLanes;  // lanes along a row, rows at once
-  constexpr int kShare = 32 / NG;  // rows that a group puts out; where they are fewer than kRows, lanes idle
-  const int col = n0 + wn + (lane % kLanes) * 8;
+  constexpr int kGroup = NWAVE * 32 * kOutRow;  // floats between groups
 #pragma unroll
   for (int i = 0; i < TM; i++) {
+    if (i + 1 < TM) fetch(i + 1);
 #pragma unroll
     for (int j = 0; j < TN; j++)
 #pragma unroll
@@ -251,65 +279,153 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
     if (NG > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r0 = 0; r0 < kShare; r0 += kRows) {
-      if (kShare < kRows && lane / kLanes >= kShare) break;
-      const int r = group * kShare + r0 + lane / kLanes, row = m0 + wm + i * 32 + r;
+    for (int r = 0; r < kPuts; r++) {
+      const int row = row_of(i, r);
+      if (!mine || row >= p.m) continue;
       float v[8];
-      const float* s = out + r * kOutRow + (lane % kLanes) * 8;
+      const float* s = out + (group * kShare + r * kRows + lane / kLanes) * kOutRow + (lane % kLanes) * 8;
       *(f32x4*)v = *(const f32x4*)s;
       *(f32x4*)(v + 4) = *(const f32x4*)(s + 4);
 #pragma unroll
       for (int g = 1; g < NG; g++)
 #pragma unroll
         for (int c = 0; c < 8; c++) v[c] += s[g * kGroup + c];
-      if (row < p.m) {
-        if (col + 8 <= p.n) epi.template put<8>(q, split, row, col, v);
-        else
-          for (int c = 0; c < 8 && col + c < p.n; c++) epi.template put<1>(q, split, row, col + c, v + c);
-      }
+      if (col + 8 <= p.n) epi.put8(q, split, row, col, v, held[i & 1][r]);
+      else
+        for (int c = 0; c < 8 && col + c < p.n; c++) epi.put1(q, split, row, col + c, v[c]);
     }
     if (NG > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
   }
 }
 
-// The four tiles and when each is taken, for `tiles` of its size over all
-// batches and splits (one MI355X, bf16, us; torch's library beside them):
+// ── which tile, and over how many splits of the contraction ─────────────────
+
+typedef Tile<256, 256, 64, 2, 2, 4> TileBig;
+typedef Tile<128, 128, 64, 2, 2, 2, 2> TileMid;
+typedef Tile<64, 64, 64, 4, 2, 2, 2> TileDeep;   // one a compute unit
+typedef Tile<64, 64, 64, 2, 2, 2, 2> TileSmall;  // two
+
+struct FastPlan {
+  int tile;  // 0 big, 1 mid, 2 deep, 3 small
+  int32_t splits, k_split;
+  uint64_t part_bytes;  // workspace for the splits' sums
+};
+
+// The least of an estimate: rounds of workgroups over the chip, times the
+// stages of a workgroup's contraction at the tile's measured time, and for a
+// split contraction the sums' way through memory. One MI355X, bf16, us:
 //
-//                         256x256  128x128  128x128g2  64x64g2  64x64g2  library
-//                         8 waves  2 a CU   1 a CU     1 a CU   2 a CU
-//   8192 x 8192 x 8192    903      1023     .          .        .        860
-//   4096 x 4096 x 1024    36.7     38.3     .          .        .        29.8
-//   2048 x 2048 x 2048    51.6     26.9     23.9       42.9     30.3     21.9
-//   1024 x 4096 x 1024    28.1     15.0     14.2       25.4     18.4     14.0
-//   1500 x 1000 x 3000    78.1     40.8     36.8       31.3     26.6     26.6
-//   1024 x 1024 x 4096    91.2     44.1     36.5       21.1     26.3     19.3
-//   512 x 512 x 2048      47.4     21.9     19.2       10.9     10.8     7.4
-//   4096 x 256 x 256      11.0     6.2      6.1        4.4      4.3      6.1
+//                         256x256  128x128  64x64 deep  64x64 small  library
+//   8192 x 8192 x 8192    903      1023     .           .            860
+//   4096 x 4096 x 1024    36.7     38.3     .           .            29.8
+//   2048 x 2048 x 2048    51.6     23.9     42.9        30.3         21.9
+//   1024 x 4096 x 1024    28.1     14.2     25.4        18.4         14.0
+//   1500 x 1000 x 3000    78.1     36.8     31.3        26.6         26.6
+//   1024 x 1024 x 4096    91.2     36.5     21.1        26.3         19.3
+//   512 x 512 x 2048      47.4     19.2     10.9        10.8         7.4
+//   4096 x 256 x 256      11.0     6.1      4.4         4.3          6.1
 //
 // Large tiles read LDS and L2 least for each product and win where there are
 // enough of them; below, what counts is that every compute unit has one.
-typedef Tile<256, 256, 64, 2, 2, 4> TileBig;
-typedef Tile<128, 128, 64, 2, 2, 2, 2> TileMid;
-typedef Tile<64, 64, 64, 4, 2, 2, 2> TileDeep;
-typedef Tile<64, 64, 64, 2, 2, 2, 2> TileSmall;
+inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool may_split) {
+  struct Kind { int bm, bn, per_cu; double stage; };
+  // Time of a stage of 64 (of 32 twice, for two planes) with the chip full.
+  const Kind kinds[4] = {{256, 256, 1, 1.7}, {128, 128, 1, 0.65}, {64, 64, 1, 0.29}, {64, 64, 2, 0.43}};
+  const int64_t sk = 64 / planes, stages = std::max<int64_t>(1, ceil_div(k, sk));
+  FastPlan best{};
+  double least = 1e30;
+  for (int t = 0; t < 4; t++) {
+    const int64_t tiles = ceil_div(m, kinds[t].bm) * ceil_div(n, kinds[t].bn) * batch;
+    for (int64_t splits = 1; splits <= (may_split ? 64 : 1); splits *= 2) {
+      if (splits > 1 && stages < 8 * splits) break;
+      const int64_t rounds = ceil_div(tiles * splits, (int64_t)o->cus * kinds[t].per_cu);
+      double us = rounds * (3.0 + ceil_div(stages, splits) * kinds[t].stage);
+      if (splits > 1) us += 4.0 + (2.0 * splits + 1) * m * n * batch * 4 / 4e6;
+      if (us < least) {
+        least = us;
+        best.tile = t;
+        best.splits = (int32_t)splits;
+      }
+    }
+  }
+  const int64_t per = ceil_div(ceil_div(k, best.splits), 64) * 64;
+  best.k_split = (int32_t)std::max<int64_t>(64, per);
+  best.splits = (int32_t)std::max<int64_t>(1, ceil_div(k, best.k_split));
+  best.part_bytes = best.splits > 1 ? (uint64_t)best.splits * batch * m * ((n + 7) / 8 * 8) * 4 : 0;
+  return best;
+}
 
+// Sums of one split, joined by join_kernel.
+struct PartOut {
+  float* part;
+  int64_t row, batch, split;
+  struct Held {};
+  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held&) const {
+    float* at = part + s * split + q * batch + i * row + j;
+    *(f32x4*)at = *(const f32x4*)sums;
+    *(f32x4*)(at + 4) = *(const f32x4*)(sums + 4);
+  }
+  __device__ __forceinline__ void put1(int q, int s, int i, int j, float sum) const {
+    part[s * split + q * batch + i * row + j] = sum;
+  }
+};
+
+// The splits' sums, added in order, to the epilogue.
+template <class Epi>
+__global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_t m, int32_t n, Epi epi) {
+  const uint32_t per = (n + 7) / 8;
+  const int q = blockIdx.y;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)m * per; t += (int64_t)gridDim.x * 256) {
+    const int i = (int)(t / per), j = (int)(t - (int64_t)i * per) * 8;
+    const float* at = p.part + q * p.batch + i * p.row + j;
+    typename Epi::Held held;
+    if (j + 8 <= n) epi.fetch(q, i, j, held);
+    float v[8];
+    *(f32x4*)v = *(const f32x4*)at;
+    *(f32x4*)(v + 4) = *(const f32x4*)(at + 4);
+    for (int s = 1; s < splits; s++) {
+      const f32x4 lo = *(const f32x4*)(at + s * p.split), hi = *(const f32x4*)(at + s * p.split + 4);
+#pragma unroll
+      for (int c = 0; c < 4; c++) v[c] += lo[c], v[4 + c] += hi[c];
+    }
+    if (j + 8 <= n) epi.put8(q, 0, i, j, v, held);
+    else
+      for (int c = 0; c < 8 && j + c < n; c++) epi.put1(q, 0, i, j + c, v[c]);
+  }
+}
+
+// `part`: plan.part_bytes of workspace.
 template <class T, int PL, bool AK, bool BKD, class Epi>
-void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batch, const Epi& epi) {
+void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batch, const FastPlan& plan, float* part,
+                      const Epi& epi) {
   p.zeros = (const char*)o->zeros;
-  const int64_t z = (int64_t)batch * p.splits;
-  auto tiles = [&](int bm, int bn) { return ceil_div(p.m, bm) * ceil_div(p.n, bn) * z; };
+  p.splits = plan.splits;
+  p.k_split = plan.k_split;
+  const PartOut sums{part, (p.n + 7) / 8 * 8, (int64_t)p.m * ((p.n + 7) / 8 * 8),
+                     (int64_t)batch * p.m * ((p.n + 7) / 8 * 8)};
   auto go = [&](auto shape) {
     using S = decltype(shape);
     p.tiles_m = (int32_t)ceil_div(p.m, S::BM);
     p.tiles_n = (int32_t)ceil_div(p.n, S::BN);
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch, (unsigned)p.splits);
-    hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, Epi>), grid, dim3(S::kThreads), 0, stream, p, epi);
+    if (p.splits == 1)
+      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, Epi>), grid, dim3(S::kThreads), 0, stream, p, epi);
+    else
+      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, PartOut>), grid, dim3(S::kThreads), 0, stream, p, sums);
   };
-  if (tiles(256, 256) >= o->cus) go(TileBig{});
-  else if (tiles(128, 128) >= o->cus * 3 / 4) go(TileMid{});
-  else if (tiles(64, 64) <= o->cus) go(TileDeep{});
-  else go(TileSmall{});
+  switch (plan.tile) {
+    case 0: go(TileBig{}); break;
+    case 1: go(TileMid{}); break;
+    case 2: go(TileDeep{}); break;
+    default: go(TileSmall{});
+  }
+  if (p.splits > 1) {
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 256), 4096);
+    hipLaunchKernelGGL(join_kernel<Epi>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, sums, p.splits, p.m, p.n,
+                       epi);
+  }
 }
 
 }  // namespace phzop

@@ -1,7 +1,7 @@
 // phz_linear.hip — the linear layer with its epilogue, y = act(x W^T + b) + r,
 // and its gradients dx = dz W, dw = dz^T x, db = sum of dz over rows, for
 // dz = dy act'(pre).
-#include "phz_gemm.h"
+#include "phz_gemm_fast.h"
 
 #include <algorithm>
 
@@ -13,23 +13,36 @@ namespace {
 
 // tanh as ocml's (2 ulp): its 1 - t cancels near 0 in any form made of one
 // exponential, and f32 callers see that.
-__device__ __forceinline__ float gate_of(float p) {  // sigmoid(p)
-  const float q = signed_gate(p);
-  return __float_as_int(q) < 0 ? fabsf(q) : 1.0f - fabsf(q);
-}
+// sigmoid(p), to a few ulp of itself at either end.
+__device__ __forceinline__ float gate_of(float p) { return __builtin_amdgcn_rcpf(1.0f + __expf(-p)); }
 
 constexpr float kGeluA = 0.79788456080286536f, kGeluB = 0.044715f;  // sqrt(2 / pi)
 
-__device__ __forceinline__ float act_of(int act, float p) {
+// The activation in place; the choice is outside the loop.
+template <int N>
+__device__ __forceinline__ void act_of(int act, float* p) {
   switch (act) {
-    case PHZ_ACT_TANH: return tanhf(p);
-    case PHZ_ACT_RELU: return p < 0.0f ? 0.0f : p;  // NaN stays
-    // p sigmoid(p); -inf has the limit 0, not the product's NaN.
-    case PHZ_ACT_SILU: return p == -__builtin_inff() ? 0.0f : p * gate_of(p);
-    // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+    case PHZ_ACT_TANH:
+#pragma unroll
+      for (int c = 0; c < N; c++) p[c] = tanhf(p[c]);
+      break;
+    case PHZ_ACT_RELU:
+#pragma unroll
+      for (int c = 0; c < N; c++) p[c] = p[c] < 0.0f ? 0.0f : p[c];  // NaN stays
+      break;
+    case PHZ_ACT_SILU:
+      // p sigmoid(p); -inf has the limit 0, not the product's NaN.
+#pragma unroll
+      for (int c = 0; c < N; c++) p[c] = p[c] == -__builtin_inff() ? 0.0f : p[c] * gate_of(p[c]);
+      break;
     case PHZ_ACT_GELU:
-      return p == -__builtin_inff() ? 0.0f : p * gate_of(2.0f * kGeluA * p * fmaf(kGeluB * p, p, 1.0f));
-    default: return p;
+      // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+#pragma unroll
+      for (int c = 0; c < N; c++)
+        p[c] = p[c] == -__builtin_inff() ? 0.0f
+                                         : p[c] * gate_of(p[c] * fmaf(2.0f * kGeluA * kGeluB * p[c], p[c], 2.0f * kGeluA));
+      break;
+    default: break;
   }
 }
 
@@ -65,24 +78,44 @@ struct LinearOut {
   E *pre, *y;
   int64_t residual_row, pre_row, y_row, bias_step;
   int act;
-  template <int N>
-  __device__ __forceinline__ void put(int, int, int i, int j, const float* sums) const {
-    float p[N];
-    Pack<E, N> r, out;
-    if (residual) r = *(const Pack<E, N>*)(residual + i * residual_row + j);
+  struct Held {
+    Pack<E, 8> residual;
+  };
+  __device__ __forceinline__ void fetch(int, int i, int j, Held& h) const {
+    if (residual) h.residual = *(const Pack<E, 8>*)(residual + i * residual_row + j);
+  }
+  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held& h) const {
+    float p[8];
+    Pack<E, 8> out;
 #pragma unroll
-    for (int c = 0; c < N; c++) p[c] = bias ? sums[c] + to_f32(bias[(j + c) * bias_step]) : sums[c];
+    for (int c = 0; c < 8; c++) p[c] = sums[c];
+    if (bias) {
+      Pack<E, 8> b;
+      if (bias_step == 1) {
+        b = *(const Pack<E, 8>*)(bias + j);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; c++) b.v[c] = bias[(j + c) * bias_step];
+      }
+#pragma unroll
+      for (int c = 0; c < 8; c++) p[c] += to_f32(b.v[c]);
+    }
     if (pre) {
 #pragma unroll
-      for (int c = 0; c < N; c++) out.v[c] = from_f32<E>(p[c]);
-      *(Pack<E, N>*)(pre + i * pre_row + j) = out;
+      for (int c = 0; c < 8; c++) out.v[c] = from_f32<E>(p[c]);
+      *(Pack<E, 8>*)(pre + i * pre_row + j) = out;
     }
+    act_of<8>(act, p);
 #pragma unroll
-    for (int c = 0; c < N; c++) {
-      p[c] = act_of(act, p[c]);
-      out.v[c] = from_f32<E>(residual ? p[c] + to_f32(r.v[c]) : p[c]);
-    }
-    *(Pack<E, N>*)(y + i * y_row + j) = out;
+    for (int c = 0; c < 8; c++) out.v[c] = from_f32<E>(residual ? p[c] + to_f32(h.residual.v[c]) : p[c]);
+    *(Pack<E, 8>*)(y + i * y_row + j) = out;
+  }
+  __device__ __forceinline__ void put1(int, int, int i, int j, float p) const {
+    if (bias) p += to_f32(bias[j * bias_step]);
+    if (pre) pre[i * pre_row + j] = from_f32<E>(p);
+    act_of<1>(act, &p);
+    if (residual) p += to_f32(residual[i * residual_row + j]);
+    y[i * y_row + j] = from_f32<E>(p);
   }
 };
 
@@ -90,27 +123,143 @@ template <class E>
 struct PlainOut {
   E* y;
   int64_t row;
-  template <int N>
-  __device__ __forceinline__ void put(int, int, int i, int j, const float* sums) const {
-    Pack<E, N> out;
+  struct Held {};
+  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
+  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held&) const {
+    Pack<E, 8> out;
 #pragma unroll
-    for (int c = 0; c < N; c++) out.v[c] = from_f32<E>(sums[c]);
-    *(Pack<E, N>*)(y + i * row + j) = out;
+    for (int c = 0; c < 8; c++) out.v[c] = from_f32<E>(sums[c]);
+    *(Pack<E, 8>*)(y + i * row + j) = out;
   }
+  __device__ __forceinline__ void put1(int, int, int i, int j, float p) const { y[i * row + j] = from_f32<E>(p); }
 };
 
 // Sums of one split of the contraction, joined by join_splits.
 struct SplitOut {
   float* part;
   int64_t row, split;
-  template <int N>
-  __device__ __forceinline__ void put(int, int s, int i, int j, const float* sums) const {
-    Pack<float, N> out;
-#pragma unroll
-    for (int c = 0; c < N; c++) out.v[c] = sums[c];
-    *(Pack<float, N>*)(part + s * split + i * row + j) = out;
+  __device__ __forceinline__ void put1(int, int s, int i, int j, float p) const { part[s * split + i * row + j] = p; }
+};
+
+// ── few rows ────────────────────────────────────────────────────────────────
+//
+// Up to 32 rows (a policy acting, a serving batch): the weights are read once
+// and everything else is small, so the floor is their way from memory. A
+// workgroup takes 16 TN outputs, its eight waves every eighth run of 128 bytes
+// of each weight row, straight into the matrix cores' fragments: lane l holds
+// the 16 bytes of row l % 16 at l / 16, and so does it of the inputs' row l %
+// 16; which k an instruction pairs is the same on both sides and does not
+// matter to the sum. The waves' sums meet in LDS in order. f32 takes the f32
+// matrix instructions: exact products, and still below the weights' time.
+// 16 x 2048 -> 8192 bf16: 8.2 us of 7.2 for 33.6 MB at a large copy's rate.
+
+template <class E> struct Small;
+template <> struct Small<bf16> {
+  static constexpr int kPer = 8;
+  static __device__ __forceinline__ f32x4 run(const Pack<bf16, 8>& a, const Pack<bf16, 8>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
+template <> struct Small<float> {
+  static constexpr int kPer = 4;
+  static __device__ __forceinline__ f32x4 run(const Pack<float, 4>& a, const Pack<float, 4>& b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+constexpr int kSmallRows = 32, kSmallWaves = 8;
+
+template <class E, int TM, int TN, class Epi>
+__global__ __launch_bounds__(kSmallWaves * 64) void few_rows(const E* x, int64_t x_row, const E* w, int64_t w_row,
+                                                             int32_t m, int32_t n, int32_t k, Epi epi) {
+  constexpr int PER = Small<E>::kPer, U = 2;  // U loads of 64 bytes a row make a line
+  typedef Pack<E, PER> Frag;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, at = (lane >> 4) * PER;
+  const int n0 = blockIdx.x * 16 * TN;
+  const E* wp[TN];
+#pragma unroll
+  for (int j = 0; j < TN; j++) wp[j] = w + min(n0 + j * 16 + r, n - 1) * w_row + at;
+  const E* xp[TM];
+#pragma unroll
+  for (int i = 0; i < TM; i++) xp[i] = x + min(i * 16 + r, m - 1) * x_row + at;
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kRun = 4 * PER * U;
+  int k0 = wave * kRun;
+#pragma unroll 2
+  for (; k0 + kRun <= k; k0 += kSmallWaves * kRun) {
+    Frag fw[U][TN], fx[U][TM];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+      for (int j = 0; j < TN; j++) fw[u][j] = *(const Frag*)(wp[j] + k0 + u * 4 * PER);
+#pragma unroll
+      for (int i = 0; i < TM; i++) fx[u][i] = *(const Frag*)(xp[i] + k0 + u * 4 * PER);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = Small<E>::run(fw[u][j], fx[u][i], acc[i][j]);
+  }
+  if (k0 < k) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      Frag fw[TN], fx[TM];
+      const int left = k - (k0 + u * 4 * PER + at);  // of this lane's elements
+#pragma unroll
+      for (int c = 0; c < PER; c++) {
+#pragma unroll
+        for (int j = 0; j < TN; j++) fw[j].v[c] = c < left ? wp[j][k0 + u * 4 * PER + c] : E{};
+#pragma unroll
+        for (int i = 0; i < TM; i++) fx[i].v[c] = c < left ? xp[i][k0 + u * 4 * PER + c] : E{};
+      }
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = Small<E>::run(fw[j], fx[i], acc[i][j]);
+    }
+  }
+  // Rows past m repeat the last one; their sums are not stored.
+  // [wave][input row][output], outputs one apart: row (lane / 16) 4 + r of the
+  // accumulator is an output, column lane % 16 an input row.
+  constexpr int kRow = 16 * TN + 1;
+  __shared__ float sums[kSmallWaves][16 * TM][kRow];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) sums[wave][i * 16 + r][j * 16 + (lane >> 4) * 4 + c] = acc[i][j][c];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 16 * TM * 16 * TN; t += kSmallWaves * 64) {
+    const int i = t / (16 * TN), j = t % (16 * TN);
+    float v = sums[0][i][j];
+#pragma unroll
+    for (int g = 1; g < kSmallWaves; g++) v += sums[g][i][j];
+    if (i < m && n0 + j < n) epi.put1(0, 0, i, n0 + j, v);
+  }
+}
+
+template <class E, class Epi>
+void launch_few_rows(const phz_ops* o, hipStream_t stream, const phz_tensor* x, const phz_tensor* w, Epi epi) {
+  const int32_t m = (int32_t)x->size[0], k = (int32_t)x->size[1], n = (int32_t)w->size[0];
+  auto go = [&](auto kernel, int per) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, per)), dim3(kSmallWaves * 64), 0, stream, (const E*)x->data,
+                       x->stride[0], (const E*)w->data, w->stride[0], m, n, k, epi);
+  };
+  // 32 outputs a workgroup where that still is one for every compute unit.
+  const bool wide = ceil_div(n, 32) >= o->cus;
+  if (m <= 16) wide ? go(few_rows<E, 1, 2, Epi>, 32) : go(few_rows<E, 1, 1, Epi>, 16);
+  else wide ? go(few_rows<E, 2, 2, Epi>, 32) : go(few_rows<E, 2, 1, Epi>, 16);
+}
 
 // y[i][j] = the splits' sums, added in order.
 template <class E>
@@ -124,34 +273,94 @@ __global__ __launch_bounds__(256) void join_splits(const float* part, int splits
   }
 }
 
-constexpr int kDzRows = 64;
-
-// dz = dy act'(pre) (where there is an activation) and the sums of dz over
-// each block of kDzRows rows, which column_sums adds up in order.
+// dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
+// rows of `dz_row` with zeros past n, and the sums of dz over each block's rows,
+// which column_sums adds up in order. A thread takes eight columns and every
+// eighth row of its block.
 template <class E>
 __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_row, const E* pre, int64_t pre_row,
-                                               E* dz, int64_t dz_row, float* sums, int32_t m, int32_t n) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
-  const int i0 = blockIdx.y * kDzRows, i1 = min(m, i0 + kDzRows);
-  float total = 0.0f;
-#pragma unroll 8
-  for (int i = i0; i < i1; i++) {
-    float d = to_f32(dy[i * dy_row + j]);
-    if (act != PHZ_ACT_NONE) d *= act_grad(act, to_f32(pre[i * pre_row + j]));
-    total += d;
-    if (dz) dz[i * dz_row + j] = from_f32<E>(d);
+                                               E* dz, int64_t dz_row, float* sums, int32_t m, int32_t n, int32_t rows) {
+  const int j = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, lane = threadIdx.x >> 5;
+  const int64_t i0 = (int64_t)blockIdx.y * rows, i1 = min((int64_t)m, i0 + rows);
+  float total[8];
+#pragma unroll
+  for (int c = 0; c < 8; c++) total[c] = 0.0f;
+  if (j + 8 <= n) {
+#pragma unroll 4
+    for (int64_t i = i0 + lane; i < i1; i += 8) {
+      const Pack<E, 8> d = *(const Pack<E, 8>*)(dy + i * dy_row + j);
+      Pack<E, 8> p, out;
+      if (act != PHZ_ACT_NONE) p = *(const Pack<E, 8>*)(pre + i * pre_row + j);
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        float v = to_f32(d.v[c]);
+        if (act != PHZ_ACT_NONE) v *= act_grad(act, to_f32(p.v[c]));
+        total[c] += v;
+        out.v[c] = from_f32<E>(v);
+      }
+      if (dz) *(Pack<E, 8>*)(dz + i * dz_row + j) = out;
+    }
+  } else if (j < n) {
+    for (int64_t i = i0 + lane; i < i1; i += 8) {
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        float v = 0.0f;
+        if (j + c < n) {
+          v = to_f32(dy[i * dy_row + j + c]);
+          if (act != PHZ_ACT_NONE) v *= act_grad(act, to_f32(pre[i * pre_row + j + c]));
+          total[c] += v;
+        }
+        if (dz && j + c < dz_row) dz[i * dz_row + j + c] = from_f32<E>(v);
+      }
+    }
   }
-  if (sums) sums[(int64_t)blockIdx.y * n + j] = total;
+  if (!sums) return;
+  __shared__ float s[8][256];
+#pragma unroll
+  for (int c = 0; c < 8; c++) s[lane][(threadIdx.x & 31) * 8 + c] = total[c];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < n) {
+    float v = 0.0f;
+#pragma unroll
+    for (int l = 0; l < 8; l++) v += s[l][threadIdx.x];
+    sums[(int64_t)blockIdx.y * n + col] = v;
+  }
 }
 
+// Eight threads a column, each every eighth block's sum.
 template <class E>
 __global__ __launch_bounds__(256) void column_sums(const float* sums, int32_t blocks, int32_t n, E* db, int64_t step) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
+  __shared__ float s[8][32];
+  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5, j = blockIdx.x * 32 + c;
   float v = 0.0f;
-  for (int i = 0; i < blocks; i++) v += sums[(int64_t)i * n + j];
-  db[j * step] = from_f32<E>(v);
+  if (j < n) {
+#pragma unroll 8
+    for (int i = lane; i < blocks; i += 8) v += sums[(int64_t)i * n + j];
+  }
+  s[lane][c] = v;
+  __syncthreads();
+  if (lane == 0 && j < n) {
+#pragma unroll
+    for (int l = 1; l < 8; l++) v += s[l][c];
+    db[j * step] = from_f32<E>(v);
+  }
+}
+
+// Rows of n elements into rows of `to_row`, zeros between.
+template <class E>
+__global__ __launch_bounds__(256) void pack_rows(const E* from, int64_t from_row, E* to, int64_t to_row, int32_t m,
+                                                 int32_t n) {
+  const int64_t per = to_row / 8;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < m * per; t += (int64_t)gridDim.x * 256) {
+    const int64_t i = t / per, j = (t - i * per) * 8;
+    const E* p = from + i * from_row + j;
+    Pack<E, 8> v{};
+    if (j + 8 <= n) v = *(const Pack<E, 8>*)p;
+    else
+      for (int c = 0; c < 8 && j + c < n; c++) v.v[c] = p[c];
+    *(Pack<E, 8>*)(to + i * to_row + j) = v;
+  }
 }
 
 template <class E>
@@ -182,18 +391,88 @@ bool check_limits(phz_ops* o, int64_t m, int64_t n, int64_t k) {
   return true;
 }
 
+// Workspace of one call, handed out in pieces of whole 256 bytes: first counted,
+// then taken.
+struct Carve {
+  char* base = nullptr;
+  uint64_t used = 0;
+  template <class T> T* take(uint64_t bytes) {
+    T* p = (T*)(base ? base + used : nullptr);
+    used += (bytes + 255) & ~255ull;
+    return p;
+  }
+};
+
+// Whether rows of bf16 can go to LDS as they lie: whole 16 bytes, and a tile's
+// rows within 32-bit offsets.
+bool lies_well(const void* data, int64_t row, int64_t cols) {
+  return (uintptr_t)data % 16 == 0 && row % 8 == 0 && cols % 8 == 0 && row <= 1 << 22;
+}
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+void pack(hipStream_t stream, const bf16* from, int64_t from_row, bf16* to, int64_t m, int64_t n) {
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(m * (pad8(n) / 8), 256), 8192);
+  hipLaunchKernelGGL(pack_rows<bf16>, dim3(blocks), dim3(256), 0, stream, from, from_row, to, pad8(n), (int32_t)m,
+                     (int32_t)n);
+}
+
+FastArgs operands(const void* a, int64_t a_row, const void* b, int64_t b_row, int64_t m, int64_t n, int64_t k,
+                  int64_t a_rows, int64_t b_rows) {
+  FastArgs f{};
+  f.a = (const char*)a, f.b = (const char*)b, f.a_row = a_row * 2, f.b_row = b_row * 2;
+  f.m = (int32_t)m, f.n = (int32_t)n, f.k = (int32_t)k, f.a_rows = (int32_t)a_rows, f.b_rows = (int32_t)b_rows;
+  return f;
+}
+
+// bf16 products go through gemm_fast where rows are whole eights, operands that
+// do not lie well being copied first, and, with ragged rows, from this many
+// multiply-adds on: gemm_any takes 10 us for as many, the copies of both
+// operands as long. The choice is by sizes alone, so a view's strides do not
+// change the result's bits.
+constexpr int64_t kPackFrom = 1ll << 30;
+
 template <class E>
 int linear(phz_ops* o, hipStream_t stream, int act, const phz_tensor* x, const phz_tensor* w, const phz_tensor* bias,
            const phz_tensor* residual, const phz_tensor* pre, const phz_tensor* y) {
-  const int32_t m = (int32_t)x->size[0], k = (int32_t)x->size[1], n = (int32_t)w->size[0];
+  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
   LinearOut<E> out{};
   if (bias) out.bias = (const E*)bias->data, out.bias_step = bias->stride[0];
   if (residual) out.residual = (const E*)residual->data, out.residual_row = residual->stride[0];
   if (pre) out.pre = (E*)pre->data, out.pre_row = pre->stride[0];
   out.y = (E*)y->data, out.y_row = y->stride[0];
   out.act = act;
+  if (m <= kSmallRows) {
+    launch_few_rows<E>(o, stream, x, w, out);
+    return launched(o, "linear") ? 0 : 1;
+  }
+  if constexpr (sizeof(E) == 2) {
+    const bool x_well = lies_well(x->data, x->stride[0], k), w_well = lies_well(w->data, w->stride[0], k);
+    if (k > 0 && (k % 8 == 0 || m * n * k >= kPackFrom)) {
+      const FastPlan plan = plan_fast(o, m, n, pad8(k), 1, 1, true);
+      Carve c;
+      const bf16 *xd = (const bf16*)x->data, *wd = (const bf16*)w->data;
+      int64_t x_row = x->stride[0], w_row = w->stride[0];
+      bf16 *xp = nullptr, *wp = nullptr;
+      float* part = nullptr;
+      for (int pass = 0; pass < 2; pass++) {
+        c.used = 0;
+        if (!x_well) xp = c.take<bf16>(m * pad8(k) * 2);
+        if (!w_well) wp = c.take<bf16>(n * pad8(k) * 2);
+        part = c.take<float>(plan.part_bytes);
+        if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
+      }
+      if (xp) pack(stream, xd, x_row, xp, m, k), xd = xp, x_row = pad8(k);
+      if (wp) pack(stream, wd, w_row, wp, n, k), wd = wp, w_row = pad8(k);
+      launch_gemm_fast<bf16, 1, true, true>(o, stream, operands(xd, x_row, wd, w_row, m, n, pad8(k), m, n), 1, plan, part,
+                                            out);
+      return launched(o, "linear") ? 0 : 1;
+    }
+  }
   const Operand a{x->data, x->stride[0], 0}, b{w->data, w->stride[0], 0};
-  launch_gemm_any<E, true, true>(o, stream, a, b, GemmShape{m, n, k, std::max(k, 1), 1}, 1, out);
+  launch_gemm_any<E, true, true>(o, stream, a, b,
+                                 GemmShape{(int32_t)m, (int32_t)n, (int32_t)k, (int32_t)std::max<int64_t>(k, 1), 1}, 1,
+                                 out);
   return launched(o, "linear") ? 0 : 1;
 }
 
@@ -201,53 +480,84 @@ template <class E>
 int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* dy, const phz_tensor* x,
                     const phz_tensor* w, const phz_tensor* pre, const phz_tensor* dx, const phz_tensor* dw,
                     const phz_tensor* db) {
-  const int32_t m = (int32_t)x->size[0], k = (int32_t)x->size[1], n = (int32_t)w->size[0];
-  const bool products = (dx || dw) && m > 0;
-  // The contraction of dw runs over rows: split where its few tiles would not
-  // fill the chip.
-  const int64_t tiles = ceil_div(n, 64) * ceil_div(k, 64);
-  const int bk = Cut<E>::tile_k;
-  int64_t splits = dw ? std::min<int64_t>(ceil_div(2 * o->cus, tiles), ceil_div(m, 4 * bk)) : 1;
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
-  const int32_t k_split = (int32_t)std::max<int64_t>(bk, ceil_div(ceil_div(m, splits), bk) * bk);
-  splits = std::max<int64_t>(1, ceil_div(m, k_split));
-  const int64_t dz_row = (n + 7) / 8 * 8, blocks = ceil_div(m, kDzRows);
-  const uint64_t dz_bytes = act != PHZ_ACT_NONE && products ? ((uint64_t)m * dz_row * sizeof(E) + 255) & ~255ull : 0;
-  const uint64_t sum_bytes = db ? ((uint64_t)blocks * n * 4 + 255) & ~255ull : 0;
-  const uint64_t part_bytes = dw && splits > 1 ? (uint64_t)splits * n * k * 4 : 0;
-  char* ws = nullptr;
-  if (dz_bytes + sum_bytes + part_bytes && !(ws = o->workspace(stream, dz_bytes + sum_bytes + part_bytes))) return 1;
-  E* dz = dz_bytes ? (E*)ws : nullptr;
-  float* sums = sum_bytes ? (float*)(ws + dz_bytes) : nullptr;
-  float* part = (float*)(ws + dz_bytes + sum_bytes);
-  if (dz || db) {
-    if (blocks)
-      hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, 256), (unsigned)blocks), dim3(256), 0, stream, act,
-                         (const E*)dy->data, dy->stride[0], pre ? (const E*)pre->data : nullptr,
-                         pre ? pre->stride[0] : 0, dz, dz_row, sums, m, n);
-    if (db)
-      hipLaunchKernelGGL(column_sums<E>, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, stream, sums, (int32_t)blocks, n,
-                         (E*)db->data, db->stride[0]);
+  const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
+  const bool need_dx = dx && m > 0 && k > 0, need_dw = dw && k > 0 && m > 0;
+  const E *dyd = (const E*)dy->data, *xd = (const E*)x->data, *wd = (const E*)w->data;
+  int64_t x_row = x->stride[0], w_row = w->stride[0];
+  const int64_t n8 = pad8(n), k8 = pad8(k);
+
+  // bf16 products that are large enough, or lie well, go through gemm_fast.
+  bool fast = false, x_well = true, w_well = true, dy_well = false;
+  FastPlan dx_plan{}, dw_plan{};
+  int32_t splits = 1, k_split = (int32_t)std::max<int64_t>(m, 1);
+  if constexpr (sizeof(E) == 2) {
+    x_well = lies_well(xd, x_row, k), w_well = lies_well(wd, w_row, k), dy_well = lies_well(dyd, dy->stride[0], n);
+    fast = (k % 8 == 0 && n % 8 == 0) || m * n * k >= kPackFrom;
+    if (fast && need_dx) dx_plan = plan_fast(o, m, k, n8, 1, 1, true);
+    if (fast && need_dw) dw_plan = plan_fast(o, n, k, m, 1, 1, true);
   }
-  const Operand d{dz ? dz : dy->data, dz ? dz_row : dy->stride[0], 0};
-  if (dx && m > 0 && k > 0)
-    launch_gemm_any<E, true, false>(o, stream, d, Operand{w->data, w->stride[0], 0}, GemmShape{m, k, n, std::max(n, 1), 1},
-                                    1, PlainOut<E>{(E*)dx->data, dx->stride[0]});
-  if (dw && n > 0 && k > 0) {
-    const Operand xo{x->data, x->stride[0], 0};
-    if (m == 0) {
-      hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], k, (int64_t)n * k);
-    } else if (splits == 1) {
-      launch_gemm_any<E, false, false>(o, stream, d, xo, GemmShape{n, k, m, k_split, 1}, 1,
-                                       PlainOut<E>{(E*)dw->data, dw->stride[0]});
+  if (!fast && need_dw) {
+    // The contraction of dw runs over rows: split where its few tiles would
+    // not fill the chip.
+    const int64_t bk = Cut<E>::tile_k;
+    const int64_t want = std::min<int64_t>(ceil_div(2 * o->cus, ceil_div(n, 64) * ceil_div(k, 64)), ceil_div(m, 4 * bk));
+    k_split = (int32_t)(ceil_div(ceil_div(m, std::max<int64_t>(1, std::min<int64_t>(want, 256))), bk) * bk);
+    splits = (int32_t)ceil_div(m, k_split);
+  }
+  const bool copy_dz = (need_dx || need_dw) && (act != PHZ_ACT_NONE || (fast && !dy_well));
+  // Blocks of rows whose sums of dz are added up in the end, at most 256.
+  const int64_t rows = std::max<int64_t>(32, ceil_div(ceil_div(m, 256), 8) * 8), blocks = ceil_div(m, rows);
+
+  Carve c;
+  E *dz = nullptr, *xp = nullptr, *wp = nullptr;
+  float *sums = nullptr, *part = nullptr;
+  for (int pass = 0; pass < 2; pass++) {
+    c.used = 0;
+    if (copy_dz) dz = c.take<E>(m * n8 * sizeof(E));
+    if (db) sums = c.take<float>(blocks * n * 4);
+    if (fast && need_dw && !x_well) xp = c.take<E>(m * k8 * sizeof(E));
+    if (fast && need_dx && !w_well) wp = c.take<E>(n * k8 * sizeof(E));
+    part = c.take<float>(std::max({dx_plan.part_bytes, dw_plan.part_bytes, splits > 1 ? (uint64_t)splits * n * k * 4 : 0}));
+    if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
+  }
+  if (copy_dz || db) {
+    if (m > 0)
+      hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, 256), (unsigned)blocks), dim3(256), 0, stream, act, dyd,
+                         dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0, dz, n8, sums,
+                         (int32_t)m, (int32_t)n, (int32_t)rows);
+    if (db)
+      hipLaunchKernelGGL(column_sums<E>, dim3((unsigned)ceil_div(n, 32)), dim3(256), 0, stream, sums, (int32_t)blocks,
+                         (int32_t)n, (E*)db->data, db->stride[0]);
+  }
+  const E* d = copy_dz ? dz : dyd;
+  const int64_t d_row = copy_dz ? n8 : dy->stride[0];
+  if constexpr (sizeof(E) == 2) {
+    if (xp) pack(stream, xd, x_row, xp, m, k), xd = xp, x_row = k8;
+    if (wp) pack(stream, wd, w_row, wp, n, k), wd = wp, w_row = k8;
+    if (fast && need_dx)
+      launch_gemm_fast<bf16, 1, true, false>(o, stream, operands(d, d_row, wd, w_row, m, k, n, m, k8), 1, dx_plan, part,
+                                             PlainOut<E>{(E*)dx->data, dx->stride[0]});
+    if (fast && need_dw)
+      launch_gemm_fast<bf16, 1, false, false>(o, stream, operands(d, d_row, xd, x_row, n, k, m, n8, k8), 1, dw_plan, part,
+                                              PlainOut<E>{(E*)dw->data, dw->stride[0]});
+  }
+  const int32_t mi = (int32_t)m, ni = (int32_t)n, ki = (int32_t)k;
+  const Operand dop{d, d_row, 0}, xo{xd, x_row, 0}, wo{wd, w_row, 0};
+  if (need_dx && !fast)
+    launch_gemm_any<E, true, false>(o, stream, dop, wo, GemmShape{mi, ki, ni, ni, 1}, 1,
+                                    PlainOut<E>{(E*)dx->data, dx->stride[0]});
+  if (need_dw && !fast) {
+    const GemmShape shape{ni, ki, mi, k_split, splits};
+    if (splits == 1) {
+      launch_gemm_any<E, false, false>(o, stream, dop, xo, shape, 1, PlainOut<E>{(E*)dw->data, dw->stride[0]});
     } else {
-      launch_gemm_any<E, false, false>(o, stream, d, xo, GemmShape{n, k, m, k_split, (int32_t)splits}, 1,
-                                       SplitOut{part, k, (int64_t)n * k});
-      const int64_t total = (int64_t)n * k;
-      hipLaunchKernelGGL(join_splits<E>, dim3((unsigned)std::min<int64_t>(ceil_div(total, 256), 8192)), dim3(256), 0,
-                         stream, part, (int)splits, total, (E*)dw->data, dw->stride[0], k, total);
+      launch_gemm_any<E, false, false>(o, stream, dop, xo, shape, 1, SplitOut{part, k, n * k});
+      hipLaunchKernelGGL(join_splits<E>, dim3((unsigned)std::min<int64_t>(ceil_div(n * k, 256), 8192)), dim3(256), 0,
+                         stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k);
     }
   }
+  if (dw && k > 0 && m == 0)
+    hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], ki, n * k);
   return launched(o, "linear backward") ? 0 : 1;
 }
 

@@ -126,13 +126,14 @@ __device__ __forceinline__ void put_planes(const Planes& p, int64_t at, const fl
   if (P == 2) *(Pack<half_t, 8>*)(p.data + p.plane + at) = lo;
 }
 template <int P>
-__device__ __forceinline__ void get_planes(const Planes& p, int64_t at, float* v) {
-  const Pack<half_t, 8> hi = *(const Pack<half_t, 8>*)(p.data + at);
-  Pack<half_t, 8> lo{};
-  if (P == 2) lo = *(const Pack<half_t, 8>*)(p.data + p.plane + at);
-#pragma unroll
-  for (int c = 0; c < 8; c++) v[c] = P == 2 ? to_f32(hi.v[c]) + to_f32(lo.v[c]) : to_f32(hi.v[c]);
-}
+struct PlaneEight {
+  Pack<half_t, 8> hi, lo;
+  __device__ __forceinline__ void get(const Planes& p, int64_t at) {
+    hi = *(const Pack<half_t, 8>*)(p.data + at);
+    if (P == 2) lo = *(const Pack<half_t, 8>*)(p.data + p.plane + at);
+  }
+  __device__ __forceinline__ float value(int c) const { return P == 2 ? to_f32(hi.v[c]) + to_f32(lo.v[c]) : to_f32(hi.v[c]); }
+};
 
 __device__ __forceinline__ double inverse_norm(const double* part, int parts, int q, double eps) {
   double sum = 0.0;
@@ -170,17 +171,18 @@ struct PlanesOut {
   Planes y, d;
   float alpha, beta;
   int32_t cols;  // columns that exist: zeros beyond
-  template <int N>
-  __device__ __forceinline__ void put(int q, int, int i, int j, const float* sums) const {
-    static_assert(N == 8 || N == 1, "");
-    if (N != 8) return;  // rows are whole eights
-    float v[8], o[8];
-    if (d.data) get_planes<PD>(d, q * d.batch + i * d.row + j, o);
+  typedef PlaneEight<PD> Held;
+  __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const {
+    if (d.data) h.get(d, q * d.batch + i * d.row + j);
+  }
+  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h) const {
+    float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++)
-      v[c] = j + c < cols ? (d.data ? fmaf(alpha, sums[c], beta * o[c]) : alpha * sums[c]) : 0.0f;
+      v[c] = j + c < cols ? (d.data ? fmaf(alpha, sums[c], beta * h.value(c)) : alpha * sums[c]) : 0.0f;
     put_planes<PY>(y, q * y.batch + i * y.row + j, v);
   }
+  __device__ __forceinline__ void put1(int, int, int, int, float) const {}  // rows are whole eights
 };
 
 // The last X' as o, or into the weights: w <- keep w - step X'.
@@ -194,14 +196,11 @@ struct Result {
     O* at = o + q * batch + i * row + j;
     *at = from_f32<O>(update ? fmaf(-step, v, keep * to_f32(*at)) : v);
   }
-  template <int N>
-  __device__ __forceinline__ void put_many(int q, int64_t i, int64_t j, const float* v) const {
-    Pack<O, N>* at = (Pack<O, N>*)(o + q * batch + i * row + j);
-    Pack<O, N> w;
-    if (update) w = *at;
+  __device__ __forceinline__ void put8(int q, int64_t i, int64_t j, const float* v, const Pack<O, 8>& before) const {
+    Pack<O, 8> w;
 #pragma unroll
-    for (int c = 0; c < N; c++) w.v[c] = from_f32<O>(update ? fmaf(-step, v[c], keep * to_f32(w.v[c])) : v[c]);
-    *at = w;
+    for (int c = 0; c < 8; c++) w.v[c] = from_f32<O>(update ? fmaf(-step, v[c], keep * to_f32(before.v[c])) : v[c]);
+    *(Pack<O, 8>*)(o + q * batch + i * row + j) = w;
   }
 };
 
@@ -212,17 +211,23 @@ struct LastOut {
   float alpha, beta;
   int32_t cols;
   Result<O> out;
-  template <int N>
-  __device__ __forceinline__ void put(int q, int, int i, int j, const float* sums) const {
-    if (N != 8) return;
+  struct Held {
+    PlaneEight<2> x;
+    Pack<O, 8> before;
+  };
+  __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const {
+    h.x.get(x, q * x.batch + i * x.row + j);
+    if (out.update && j + 8 <= cols) h.before = *(const Pack<O, 8>*)(out.o + q * out.batch + i * out.row + j);
+  }
+  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h) const {
     float v[8];
-    get_planes<2>(x, q * x.batch + i * x.row + j, v);
 #pragma unroll
-    for (int c = 0; c < 8; c++) v[c] = fmaf(alpha, sums[c], beta * v[c]);
-    if (j + 8 <= cols) out.template put_many<8>(q, i, j, v);
+    for (int c = 0; c < 8; c++) v[c] = fmaf(alpha, sums[c], beta * h.x.value(c));
+    if (j + 8 <= cols) out.put8(q, i, j, v, h.before);
     else
       for (int c = 0; c < 8 && j + c < cols; c++) out.put(q, i, j + c, v[c]);
   }
+  __device__ __forceinline__ void put1(int, int, int, int, float) const {}  // rows are whole eights
 };
 
 // C = alpha product + beta D in f32 (any coefficients; see newton_schulz_any).
@@ -231,10 +236,9 @@ struct Axpby {
   const float* d;
   float alpha, beta;
   int64_t row, batch;
-  template <int N>
-  __device__ __forceinline__ void put(int q, int, int i, int j, const float* p) const {
+  __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
     const int64_t at = q * batch + i * row + j;
-    y[at] = fmaf(alpha, p[0], d ? beta * d[at] : 0.0f);
+    y[at] = fmaf(alpha, p, d ? beta * d[at] : 0.0f);
   }
 };
 
@@ -244,19 +248,16 @@ struct LastAny {
   float a;
   int64_t row, batch;
   Result<O> out;
-  template <int N>
-  __device__ __forceinline__ void put(int q, int, int i, int j, const float* p) const {
-    out.put(q, i, j, fmaf(a, x[q * batch + i * row + j], p[0]));
+  __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
+    out.put(q, i, j, fmaf(a, x[q * batch + i * row + j], p));
   }
 };
 
 template <class O>
 __global__ __launch_bounds__(256) void finish_kernel(LastAny<O> out, int32_t rows, int32_t cols) {
   const int64_t n = (int64_t)rows * cols;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-    const float zero = 0.0f;
-    out.template put<1>(blockIdx.y, 0, (int)(t / cols), (int)(t % cols), &zero);
-  }
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256)
+    out.put1(blockIdx.y, 0, (int)(t / cols), (int)(t % cols), 0.0f);
 }
 
 // The largest |p(s)| for s in [0, top], p odd: p(s) = a s + b s^3 + c s^5, at
@@ -347,7 +348,6 @@ FastArgs product(const Planes& a, const Planes& b, int32_t m, int32_t n, int32_t
   f.a_row = a.row * 2, f.b_row = b.row * 2, f.a_batch = a.batch * 2, f.b_batch = b.batch * 2;
   f.a_plane = (uint32_t)(a.plane * 2), f.b_plane = (uint32_t)(b.plane * 2);
   f.m = m, f.n = n, f.k = k, f.a_rows = a_rows, f.b_rows = b_rows;
-  f.k_split = (k + 63) / 64 * 64, f.splits = 1;
   return f;
 }
 
@@ -372,10 +372,15 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
   const uint64_t part_bytes = ((uint64_t)batch * parts * 8 + 255) & ~255ull;
   // A matrix's planes lie together, each from a multiple of 256 bytes.
   const int64_t xn = ((int64_t)rows * c8 + 127) & ~127ll, an = ((int64_t)s * s8 + 127) & ~127ll;
-  char* ws = o->workspace(stream, part_bytes + (uint64_t)batch * (4 * xn + 2 * P * an) * 2);
+  // The Gram product is long and has few tiles: it may be split.
+  const FastPlan gplan = plan_fast(o, s, s8, wide ? c8 : l, batch, P, true), pplan = plan_fast(o, s, s8, s8, batch, P, true),
+                 xplan = plan_fast(o, rows, c8, s, batch, P, false);
+  const uint64_t split_bytes = (std::max(gplan.part_bytes, pplan.part_bytes) + 255) & ~255ull;
+  char* ws = o->workspace(stream, part_bytes + split_bytes + (uint64_t)batch * (4 * xn + 2 * P * an) * 2);
   if (!ws) return 1;
   double* part = (double*)ws;
-  half_t* h = (half_t*)(ws + part_bytes);
+  float* sums = (float*)(ws + part_bytes);
+  half_t* h = (half_t*)(ws + part_bytes + split_bytes);
   Planes x{h, xn, c8, 2 * xn}, y{h + 2 * batch * xn, xn, c8, 2 * xn};
   const Planes a{h + 4 * batch * xn, an, s8, P * an}, p{h + (4 * xn + P * an) * batch, an, s8, P * an};
   auto scale = [](double bound) { return exp2(floor(log2(32768.0 / bound))); };
@@ -386,19 +391,21 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
                      (float)sx, x, nullptr, rows, cols);
   for (int k = 0; k < cfg.steps; k++) {
     const PlanesOut<P, P> gram{a, Planes{}, (float)(sa / (sx * sx)), 0.0f, s};
-    if (wide) launch_gemm_fast<half_t, P, true, true>(o, stream, product(x, x, s, s8, c8, s, s), (int)batch, gram);
-    else launch_gemm_fast<half_t, P, false, false>(o, stream, product(x, x, s, s8, l, s8, s8), (int)batch, gram);
+    if (wide) launch_gemm_fast<half_t, P, true, true>(o, stream, product(x, x, s, s8, c8, s, s), (int)batch, gplan, sums,
+                                                           gram);
+    else launch_gemm_fast<half_t, P, false, false>(o, stream, product(x, x, s, s8, l, s8, s8), (int)batch, gplan, sums,
+                                                     gram);
     const PlanesOut<P, P> poly{p, a, (float)(cfg.c * sp / (sa * sa)), (float)(cfg.b * sp / sa), s};
-    launch_gemm_fast<half_t, P, true, true>(o, stream, product(a, a, s, s8, s8, s, s), (int)batch, poly);
+    launch_gemm_fast<half_t, P, true, true>(o, stream, product(a, a, s, s8, s8, s, s), (int)batch, pplan, sums, poly);
     const FastArgs f = wide ? product(p, x, rows, c8, s, s, c8) : product(x, p, rows, c8, s8, rows, s);
     if (k + 1 < cfg.steps) {
       const PlanesOut<2, 2> next{y, x, (float)(1.0 / sp), (float)cfg.a, cols};
-      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, next);
-      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, next);
+      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, xplan, nullptr, next);
+      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, xplan, nullptr, next);
     } else {
       const LastOut<O> last{x, (float)(1.0 / (sp * sx)), (float)(cfg.a / sx), cols, out};
-      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, last);
-      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, last);
+      if (wide) launch_gemm_fast<half_t, P, true, false>(o, stream, f, (int)batch, xplan, nullptr, last);
+      else launch_gemm_fast<half_t, P, true, true>(o, stream, f, (int)batch, xplan, nullptr, last);
     }
     std::swap(x, y);
   }

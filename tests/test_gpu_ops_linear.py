@@ -50,6 +50,43 @@ def test_forward_and_backward(ops, shape, dtype):
         R.within(a, b, c, name)
 
 
+#: Large enough for every tile, for split contractions and for operands that
+#: are copied first, on and off the tiles' sizes.
+LARGE = [(4096, 4096, 64, "silu"), (3001, 1024, 2056, "none"), (257, 4104, 520, "tanh"), (9000, 131, 1003, "gelu"),
+         (70000, 64, 72, "relu"), (2100, 1001, 2049, "none")]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large(ops, shape, dtype):
+    m, k, n, act = shape
+    d = data(m, k, n, dtype, seed=4)
+    y, pre = ops.linear(d["x"], d["w"], bias=d["bias"], act=act, residual=d["residual"], save_pre=True)
+    wy, wp, by, bp = R.linear(d["x"], d["w"], d["bias"], d["residual"], act, dtype)
+    R.within(y, wy, by, "y")
+    R.within(pre, wp, bp, "pre")
+    p = d["pre"] if act != "none" else None
+    got = ops.linear_backward(d["dy"], d["x"], d["w"], pre=p, act=act)
+    want, bounds = R.linear_backward(d["dy"], d["x"], d["w"], p, act, dtype)
+    for name, a, b, c in zip(("dx", "dw", "db"), got, want, bounds):
+        R.within(a, b, c, name)
+    for a, b in zip(got, ops.linear_backward(d["dy"], d["x"], d["w"], pre=p, act=act)):
+        assert torch.equal(a, b)
+
+
+def test_rows_far_apart(ops):
+    """Rows 32 MiB apart: a tile's rows leave 32-bit offsets."""
+    m, k, n = 300, 64, 48
+    big = torch.zeros((m - 1) * (1 << 24) + k, dtype=BF16, device="cuda")
+    x = torch.as_strided(big, (m, k), (1 << 24, 1))
+    x.copy_(torch.randn(m, k, device="cuda"))
+    w = torch.randn(n, k, device="cuda").to(BF16)
+    assert torch.equal(ops.linear(x, w), ops.linear(x.contiguous(), w))
+    dy = torch.randn(m, n, device="cuda").to(BF16)
+    for a, b in zip(ops.linear_backward(dy, x, w), ops.linear_backward(dy, x.contiguous(), w)):
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-2)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("act", ACTS)
 def test_activations(ops, act, dtype):
