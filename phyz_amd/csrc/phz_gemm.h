@@ -5,12 +5,10 @@
 // on the matrix cores, each operand dense along k or along its rows, at any
 // size, stride and alignment.
 //
-// bf16 operands go to the matrix cores as they are. f32 operands are cut into
-// three bf16 pieces, x = h + m + l, by truncation: 8 bits of the significand
-// each, 24 in all, so the cut is exact. Of the nine products of pieces the six
-// largest are taken (hh, hm, mh, mm, hl, lh); what is left out is below 2^-23
-// of |a||b|. Six products of the bf16 rate are 2.7 times the rate of the f32
-// matrix instructions. Sums are f32.
+// bf16 operands take the bf16 matrix instructions, f32 operands the f32 ones,
+// whose products are exact: the path for small sizes, any layout and any value.
+// Sums are f32. (Large f32 products are faster cut in bf16 pieces, see cut3 and
+// phz_gemm_fast.h: the f32 instructions have a sixteenth of the bf16 rate.)
 #pragma once
 #include "phz_ops.h"
 
@@ -34,10 +32,18 @@ struct GemmShape {
   int32_t splits;
 };
 
-template <class E> struct Cut;
-template <> struct Cut<bf16> { static constexpr int pieces = 1, tile_k = 64; };
-template <> struct Cut<float> { static constexpr int pieces = 3, tile_k = 32; };
+// Contraction per tile, and elements between a tile's rows in LDS: four or
+// eight more than it, so that the 16-byte reads of 16 consecutive rows fall
+// into all 64 banks.
+template <class E> struct Any;
+template <> struct Any<bf16> { static constexpr int tile_k = 64, ld = 72; };
+template <> struct Any<float> { static constexpr int tile_k = 32, ld = 36; };
 
+// x = h + m + l in bf16 pieces by truncation: 8 bits of the significand each,
+// 24 in all, so the cut is exact. Of the nine products of two numbers' pieces
+// the six largest are taken (hh, hm, mh, mm, hl, lh); what is left out is below
+// 2^-22 of |a||b|. Six products of the bf16 rate are 2.7 times the rate of the
+// f32 matrix instructions.
 // The three pieces of x. Where x is not finite, all of it is in the first.
 __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t& l) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
@@ -53,16 +59,14 @@ __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t
 }
 
 // Moves one operand's tile of ROWS rows by tile_k through registers into LDS,
-// laid out [piece][row][k] with 16 bytes between rows, which spreads the 16-byte
-// reads of consecutive rows over the banks. A chunk is eight k of one row
-// (dense along k), or of R rows (dense along rows: then a wave's loads are
-// contiguous along rows, and the transpose is done in registers).
+// laid out [row][k]. A chunk is eight k of one row (dense along k), or of R
+// rows (dense along rows: then a wave's loads are contiguous along rows, and
+// the transpose is done in registers).
 template <class E, bool ALONG_K, int ROWS>
 struct Stage {
-  static constexpr int P = Cut<E>::pieces, BK = Cut<E>::tile_k, LD = BK + 8, KC = BK / 8;
+  static constexpr int BK = Any<E>::tile_k, LD = Any<E>::ld, KC = BK / 8;
   static constexpr int R = ALONG_K ? 1 : (int)(4 / sizeof(E));
   static constexpr int kChunks = ROWS / R * KC, N = kChunks / 256;
-  static constexpr int kLds = P * ROWS * LD;
   static_assert(kChunks % 256 == 0, "whole chunks for every thread");
   E v[N][R][8];
 
@@ -102,43 +106,52 @@ struct Stage {
       }
     }
   }
-  __device__ __forceinline__ void store(uint16_t* lds) const {
+  __device__ __forceinline__ void store(E* lds) const {
 #pragma unroll
     for (int i = 0; i < N; i++) {
       int row, k;
       place(threadIdx.x + i * 256, row, k);
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        uint16_t w[P][8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          if constexpr (P == 1) w[0][j] = v[i][r][j].bits;
-          else cut3(v[i][r][j], w[0][j], w[1][j], w[2][j]);
-        }
-#pragma unroll
-        for (int p = 0; p < P; p++) {
+        E* to = lds + (row + r) * LD + k;
+        if constexpr (sizeof(E) == 2) {
           u32x4 q;
 #pragma unroll
-          for (int j = 0; j < 4; j++) q[j] = (uint32_t)w[p][2 * j] | (uint32_t)w[p][2 * j + 1] << 16;
-          *(u32x4*)(lds + (p * ROWS + row + r) * LD + k) = q;
+          for (int j = 0; j < 4; j++) q[j] = (uint32_t)v[i][r][2 * j].bits | (uint32_t)v[i][r][2 * j + 1].bits << 16;
+          *(u32x4*)to = q;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) *(f32x4*)(to + j) = f32x4{v[i][r][j], v[i][r][j + 1], v[i][r][j + 2], v[i][r][j + 3]};
         }
       }
     }
   }
 };
 
+// What a lane takes of 32 rows in one 16-byte read, and the products of it:
+// bf16, 16 of k in one instruction; f32, eight of k in four, where an
+// instruction pairs the k of lanes below 32 with that four further on. Both
+// operands pair alike, so the sum is the same.
+__device__ __forceinline__ f32x16 multiply(const bf16* a, const bf16* b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)a, *(const bf16x8*)b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 multiply(const float* a, const float* b, f32x16 c) {
+  const f32x4 x = *(const f32x4*)a, y = *(const f32x4*)b;
+#pragma unroll
+  for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+  return c;
+}
+
 // Any size and layout: a workgroup of four waves per BM x BN tile, registers
 // holding the next k tile while the matrix cores work on the one in LDS.
 // `epi.put1(q, split, i, j, sum)` takes each element.
 template <class E, bool AK, bool BKD, int BM, int BN, class Epi>
 __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape s, Epi epi) {
-  constexpr int P = Cut<E>::pieces, BK = Cut<E>::tile_k, LD = BK + 8;
+  constexpr int BK = Any<E>::tile_k, LD = Any<E>::ld, PER = 16 / sizeof(E);
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
   using SA = Stage<E, AK, BM>;
   using SB = Stage<E, BKD, BN>;
-  __shared__ uint16_t lds[SA::kLds + SB::kLds];
-  uint16_t* la = lds;
-  uint16_t* lb = lds + SA::kLds;
+  __shared__ __attribute__((aligned(16))) E la[BM * LD], lb[BN * LD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
   const int q = blockIdx.z / s.splits, split = blockIdx.z - q * s.splits;
@@ -146,87 +159,35 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
   const E* pa = (const E*)a.data + q * a.batch;
   const E* pb = (const E*)b.data + q * b.batch;
   const int wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
-  const int fr = lane & 31, fk = (lane >> 5) * 8;
+  const int fr = lane & 31, fk = (lane >> 5) * PER;
 
   f32x16 acc[TM][TN];
-  bool again = false;
-  // A second pass only where f32 sums came out infinite or NaN: an infinite
-  // element times the zero pieces of a finite one is NaN, so those elements
-  // are taken from the first pieces alone, whose infinities are the inputs'.
-  for (;;) {
-    f32x16 sum[TM][TN];
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+  for (int i = 0; i < TM; i++)
 #pragma unroll
-      for (int j = 0; j < TN; j++)
+    for (int j = 0; j < TN; j++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) sum[i][j][r] = 0.0f;
-    SA sa;
-    SB sb;
-    sa.load(pa, a.row, m0, s.m, k0, k_end);
-    sb.load(pb, b.row, n0, s.n, k0, k_end);
-    for (int k = k0; k < k_end; k += BK) {
-      __syncthreads();
-      sa.store(la);
-      sb.store(lb);
-      __syncthreads();
-      if (k + BK < k_end) {
-        sa.load(pa, a.row, m0, s.m, k + BK, k_end);
-        sb.load(pb, b.row, n0, s.n, k + BK, k_end);
-      }
-#pragma unroll
-      for (int kk = 0; kk < BK; kk += 16) {
-        bf16x8 fa[P][TM], fb[P][TN];
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-#pragma unroll
-          for (int i = 0; i < TM; i++) fa[p][i] = *(const bf16x8*)(la + (p * BM + wm + i * 32 + fr) * LD + kk + fk);
-#pragma unroll
-          for (int j = 0; j < TN; j++) fb[p][j] = *(const bf16x8*)(lb + (p * BN + wn + j * 32 + fr) * LD + kk + fk);
-        }
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-          for (int j = 0; j < TN; j++) {
-            f32x16 c = sum[i][j];
-            if constexpr (P == 3) {
-              if (!again) {
-                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[2][i], fb[0][j], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[0][i], fb[2][j], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[1][i], fb[1][j], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[1][i], fb[0][j], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[0][i], fb[1][j], c, 0, 0, 0);
-              }
-            }
-            sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[0][i], fb[0][j], c, 0, 0, 0);
-          }
-      }
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+  SA sa;
+  SB sb;
+  sa.load(pa, a.row, m0, s.m, k0, k_end);
+  sb.load(pb, b.row, n0, s.n, k0, k_end);
+  for (int k = k0; k < k_end; k += BK) {
+    __syncthreads();
+    sa.store(la);
+    sb.store(lb);
+    __syncthreads();
+    if (k + BK < k_end) {
+      sa.load(pa, a.row, m0, s.m, k + BK, k_end);
+      sb.load(pb, b.row, n0, s.n, k + BK, k_end);
     }
-    if constexpr (P == 1) {
 #pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = sum[i][j];
-      break;
-    } else {
-      bool odd = false;
+    for (int kk = 0; kk < BK; kk += 2 * PER)
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const bool bad = !(fabsf(sum[i][j][r]) < __builtin_inff());
-            if (!again) {
-              acc[i][j][r] = sum[i][j][r];
-              odd = odd || bad;
-            } else if (bad) {
-              acc[i][j][r] = sum[i][j][r];
-            }
-          }
-      if (again || !__syncthreads_or(odd)) break;
-      again = true;
-    }
+          acc[i][j] = multiply(la + (wm + i * 32 + fr) * LD + kk + fk, lb + (wn + j * 32 + fr) * LD + kk + fk, acc[i][j]);
   }
 
   // Accumulator layout: register r of a lane is row (r / 4) 8 + (lane / 32) 4 +
@@ -247,11 +208,11 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
 }
 
 // Launches gemm_any with the tile that fills the chip: 128 x 128 where those
-// are two for every compute unit, 64 x 64 below.
+// are two for every compute unit and not mostly beyond the edge, 64 x 64 below.
 template <class E, bool AK, bool BKD, class Epi>
 void launch_gemm_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b, GemmShape s, int batch, Epi epi) {
   const int64_t z = (int64_t)batch * s.splits;
-  if (ceil_div(s.m, 128) * ceil_div(s.n, 128) * z >= 2ll * o->cus)
+  if (s.m > 64 && s.n > 64 && ceil_div(s.m, 128) * ceil_div(s.n, 128) * z >= 2ll * o->cus)
     hipLaunchKernelGGL((gemm_any<E, AK, BKD, 128, 128, Epi>), dim3(ceil_div(s.n, 128), ceil_div(s.m, 128), z),
                        dim3(256), 0, stream, a, b, s, epi);
   else

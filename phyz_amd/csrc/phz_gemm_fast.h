@@ -1,12 +1,15 @@
-// phz_gemm_fast.h — the matrix product for large aligned operands of 16 bits:
+// phz_gemm_fast.h — the matrix product for aligned operands:
 //
 //   C[i][j] = sum_k A(i, k) B(j, k)
 //
-// Operands are one plane of 16-bit elements, or two: A = hi + lo, f32 data cut
-// in f16, whose product is taken as lo hi + hi lo + hi hi (lo lo is below what
-// f32 sums hold). Rows are 16-byte aligned and, along k (or along rows, for
-// operands dense along rows), a multiple of eight elements long or padded with
-// zeros to one.
+// Operands are one plane of 16-bit elements, f32 (through the f32 matrix
+// instructions: exact products at a sixteenth of the rate), or a sum of planes:
+//   two    A = hi + lo, f32 data cut in f16: lo hi + hi lo + hi hi (lo lo is
+//          below what f32 sums hold), for data of a known range;
+//   three  A = h + m + l, f32 data cut in bf16 without loss (cut3): six of the
+//          nine products, as in phz_gemm.h, for any data.
+// Rows are 16-byte aligned and, along k (or along rows, for
+// operands dense along rows), whole 16 bytes long or padded with zeros to them.
 #pragma once
 #include <algorithm>
 
@@ -24,13 +27,25 @@ template <> __device__ __forceinline__ half_t from_f32<half_t>(float v) {
   return half_t{__builtin_bit_cast(uint16_t, (_Float16)v)};
 }
 
+// Products of two fragments of 16 bytes a lane: kStep of k.
 template <class T> struct Mfma;
+template <> struct Mfma<float> {
+  static constexpr int kStep = 8;  // as multiply() in phz_gemm.h
+  static __device__ __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  }
+};
 template <> struct Mfma<bf16> {
+  static constexpr int kStep = 16;
   static __device__ __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 template <> struct Mfma<half_t> {
+  static constexpr int kStep = 16;
   static __device__ __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -39,9 +54,9 @@ template <> struct Mfma<half_t> {
 struct FastArgs {
   const char *a, *b, *zeros;
   int64_t a_row, b_row, a_batch, b_batch;  // bytes
-  uint32_t a_plane, b_plane;               // bytes from hi to lo
+  uint32_t a_plane, b_plane;               // bytes from a plane to the next
   int32_t m, n, k;
-  int32_t a_rows, b_rows;   // rows that exist (dense along rows: a multiple of eight)
+  int32_t a_rows, b_rows;   // rows that exist (dense along rows: whole 16 bytes)
   int32_t k_split, splits;  // contraction per split, a multiple of 64
   int32_t tiles_m, tiles_n;
 };
@@ -69,36 +84,40 @@ __device__ __forceinline__ void dma16(uint32_t lds, const char* at) {
 // so the four rows of a block fall into all banks (with rows of 128 bytes, two
 // of them a bank row, g ^ (k / 2 % 2)). Measured (counters): no
 // bank conflicts in either.
-// With two planes the tile holds SK = BK / 2 of k twice: hi's, then lo's.
-template <bool ALONG_K, int ROWS, int BK, int NW, int PL>
+// With two planes the tile holds SK = 32 of k twice: hi's, then lo's. With
+// three it is three tiles of 32 of k.
+template <class T, bool ALONG_K, int ROWS, int SLOTS, int NW, int PL>
 struct FastTile {
-  static constexpr int SK = BK / PL;
-  static constexpr int kBytes = ROWS * BK * 2;
+  static constexpr int ES = sizeof(T), EL = 16 / ES;  // bytes of an element, elements of 16 bytes
+  static constexpr int kParts = PL == 3 ? 3 : 1, BK = SLOTS / kParts, SK = SLOTS / PL;
+  static constexpr int kPart = ROWS * BK * ES, kBytes = kParts * kPart;
   static constexpr int kPerWave = kBytes / 1024 / NW;  // 1 KB loads of each wave
-  static constexpr int kChunks = ALONG_K ? BK / 8 : ROWS / 8, kRows = 64 / kChunks;  // 16-byte chunks of a row, rows of a load
+  static constexpr int kChunks = (ALONG_K ? BK : ROWS) / EL, kRows = 64 / kChunks;  // 16-byte chunks of a row, rows of a load
   static_assert(kPerWave * NW * 1024 == kBytes, "whole loads for every wave");
   uint32_t off[kPerWave];
   int32_t kk[kPerWave];  // first k of the lane's 16 bytes within the tile
 
   // What the row r's (k's) chunks are permuted by.
   static __device__ __forceinline__ int order(int r) {
-    if (ALONG_K) return BK == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
+    if (ALONG_K) return BK * ES == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
+    if (ES == 4) return 0;  // read an element a lane: no two share a bank
     return (ROWS == 64 ? (r >> 1) & 1 : r & 3) << 2;
   }
 
   __device__ __forceinline__ void init(int wave, int lane, int row0, int rows, int64_t row_bytes, uint32_t plane) {
 #pragma unroll
     for (int i = 0; i < kPerWave; i++) {
-      const int r = (wave * kPerWave + i) * kRows + lane / kChunks;
+      const int at = wave * kPerWave + i, part = at / (kPart / 1024);
+      const int r = at % (kPart / 1024) * kRows + lane / kChunks;
       if (ALONG_K) {
         const int c = (lane % kChunks) ^ order(r);
         // Rows past the end repeat the last one: their sums are not stored.
-        kk[i] = c * 8 % SK;
-        off[i] = (uint32_t)((min(row0 + r, rows - 1) - row0) * row_bytes) + kk[i] * 2 + (c * 8 / SK) * plane;
+        kk[i] = c * EL % SK;
+        off[i] = (uint32_t)((min(row0 + r, rows - 1) - row0) * row_bytes) + kk[i] * ES + (part + c * EL / SK) * plane;
       } else {
         const int c = (lane % kChunks) ^ order(r);
         kk[i] = r % SK;
-        off[i] = (uint32_t)(kk[i] * row_bytes) + (min(row0 + c * 8, rows - 8) - row0) * 2 + (r / SK) * plane;
+        off[i] = (uint32_t)(kk[i] * row_bytes) + (min(row0 + c * EL, rows - EL) - row0) * ES + (part + r / SK) * plane;
       }
     }
   }
@@ -113,11 +132,19 @@ struct FastTile {
         dma16(lds + (wave * kPerWave + i) * 1024, kk[i] < left ? base + off[i] : zeros);
     }
   }
-  // The fragment of rows row + lane % 32, the tile's k from k + 8 (lane / 32).
-  static __device__ __forceinline__ s16x8 read(const char* l, int lane, int row, int k) {
+  // The fragment of rows row + lane % 32, plane h: EL of k from kk + EL (lane / 32).
+  static __device__ __forceinline__ s16x8 read(const char* l, int lane, int row, int h, int kk) {
+    const int k = kParts == 1 ? h * SK + kk : kk;
+    if (kParts > 1) l += h * kPart;
     if constexpr (ALONG_K) {
-      const int r = row + (lane & 31), c = ((k >> 3) + (lane >> 5)) ^ order(r);
-      return *(const s16x8*)(l + r * (BK * 2) + c * 16);
+      const int r = row + (lane & 31), c = (k / EL + (lane >> 5)) ^ order(r);
+      return *(const s16x8*)(l + r * (BK * ES) + c * 16);
+    }
+    if constexpr (ES == 4) {
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = *(const float*)(l + ((k + (lane >> 5) * 4 + j) * ROWS + row + (lane & 31)) * 4);
+      return __builtin_bit_cast(s16x8, v);
     }
     const int p = lane & 15;
     const int at = (k + (lane >> 5) * 8 + (p >> 2)) * (ROWS * 2) +
@@ -134,7 +161,7 @@ struct FastTile {
 //   put8(q, split, i, j, sums, held)   eight neighbouring sums of row i
 //   put1(q, split, i, j, sum)          one, at a ragged end
 //
-// A tile BM x BN, contraction BK a stage, NS stages of LDS, MW x NW waves, and
+// A tile BM x BN, BK slots of contraction a stage (SK = BK / planes of k), NS stages of LDS, MW x NW waves, and
 // NG such groups of waves: each takes every NG-th stage of the contraction, and
 // their sums are added in order at the end. One group where the tiles fill the
 // chip; several where they do not, so that a compute unit has other waves to
@@ -150,8 +177,8 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
   constexpr int BM = Shape::BM, BN = Shape::BN, BK = Shape::BK, NS = Shape::NS, NG = Shape::NG;
   constexpr int NWAVE = Shape::MW * Shape::NW;
   constexpr int WM = BM / Shape::MW, WN = BN / Shape::NW, TM = WM / 32, TN = WN / 32, SK = BK / PL;
-  using TA = FastTile<AK, BM, BK, NWAVE, PL>;
-  using TB = FastTile<BKD, BN, BK, NWAVE, PL>;
+  using TA = FastTile<T, AK, BM, BK, NWAVE, PL>;
+  using TB = FastTile<T, BKD, BN, BK, NWAVE, PL>;
   constexpr int kOne = TA::kBytes + TB::kBytes, kStage = NG * kOne, kLoads = TA::kPerWave + TB::kPerWave;
   constexpr int kOutRow = WN + 4;  // floats of one staged output row
   constexpr int kOut = NG * NWAVE * 32 * kOutRow * 4;
@@ -178,9 +205,10 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
   TB tb;
   ta.init(wave, lane, m0, p.a_rows, p.a_row, p.a_plane);
   tb.init(wave, lane, n0, p.b_rows, p.b_row, p.b_plane);
-  const int64_t a_step = AK ? 2 : p.a_row, b_step = BKD ? 2 : p.b_row;
-  const char* ga = p.a + q * p.a_batch + (AK ? m0 * p.a_row : (int64_t)m0 * 2);
-  const char* gb = p.b + q * p.b_batch + (BKD ? n0 * p.b_row : (int64_t)n0 * 2);
+  constexpr int ES = sizeof(T);
+  const int64_t a_step = AK ? ES : p.a_row, b_step = BKD ? ES : p.b_row;
+  const char* ga = p.a + q * p.a_batch + (AK ? m0 * p.a_row : (int64_t)m0 * ES);
+  const char* gb = p.b + q * p.b_batch + (BKD ? n0 * p.b_row : (int64_t)n0 * ES);
 
   // The groups take the stages in turn.
   const int total = (k1 - k0 + SK - 1) / SK, steps = (total + NG - 1) / NG;
@@ -217,20 +245,25 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
     const char* l = lds + group * kOne + now;
     now = now == (NS - 1) * kStage ? 0 : now + kStage;
 #pragma unroll
-    for (int kk = 0; kk < SK; kk += 16) {
+    for (int kk = 0; kk < SK; kk += Mfma<T>::kStep) {
       s16x8 fa[PL][TM], fb[PL][TN];
 #pragma unroll
       for (int h = 0; h < PL; h++) {
 #pragma unroll
-        for (int i = 0; i < TM; i++) fa[h][i] = TA::read(l, lane, wm + i * 32, h * SK + kk);
+        for (int i = 0; i < TM; i++) fa[h][i] = TA::read(l, lane, wm + i * 32, h, kk);
 #pragma unroll
-        for (int j = 0; j < TN; j++) fb[h][j] = TB::read(l + TA::kBytes, lane, wn + j * 32, h * SK + kk);
+        for (int j = 0; j < TN; j++) fb[h][j] = TB::read(l + TA::kBytes, lane, wn + j * 32, h, kk);
       }
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++) {
-          if constexpr (PL == 2) {
+          if constexpr (PL == 3) {
+            acc[i][j] = Mfma<T>::run(fa[2][i], fb[0][j], acc[i][j]);
+            acc[i][j] = Mfma<T>::run(fa[0][i], fb[2][j], acc[i][j]);
+            acc[i][j] = Mfma<T>::run(fa[1][i], fb[1][j], acc[i][j]);
+          }
+          if constexpr (PL >= 2) {
             acc[i][j] = Mfma<T>::run(fa[1][i], fb[0][j], acc[i][j]);
             acc[i][j] = Mfma<T>::run(fa[0][i], fb[1][j], acc[i][j]);
           }
@@ -301,10 +334,24 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
 
 // ── which tile, and over how many splits of the contraction ─────────────────
 
-typedef Tile<256, 256, 64, 2, 2, 4> TileBig;
-typedef Tile<128, 128, 64, 2, 2, 2, 2> TileMid;
-typedef Tile<64, 64, 64, 4, 2, 2, 2> TileDeep;   // one a compute unit
-typedef Tile<64, 64, 64, 2, 2, 2, 2> TileSmall;  // two
+template <class T, int PL> struct Tiles {
+  typedef Tile<256, 256, 64, 2, 2, 4> Big;
+  typedef Tile<128, 128, 64, 2, 2, 2, 2> Mid;
+  typedef Tile<64, 64, 64, 4, 2, 2, 2> Deep;   // one a compute unit
+  typedef Tile<64, 64, 64, 2, 2, 2, 2> Small;  // two
+};
+template <> struct Tiles<bf16, 3> {
+  typedef Tile<256, 128, 96, 2, 4, 2> Big;
+  typedef Tile<128, 128, 96, 3, 2, 2> Mid;
+  typedef Tile<64, 64, 96, 3, 2, 2, 2> Deep;
+  typedef Tile<64, 64, 96, 3, 2, 2> Small;
+};
+template <> struct Tiles<float, 1> {
+  typedef Tile<64, 64, 32, 2, 2, 2, 2> Deep;
+  typedef Tile<64, 64, 32, 2, 2, 2> Small;  // four
+};
+
+enum { PLANES_F32 = 0 };  // plan_fast's name for f32 operands as they are
 
 struct FastPlan {
   int tile;  // 0 big, 1 mid, 2 deep, 3 small
@@ -327,15 +374,21 @@ struct FastPlan {
 //   4096 x 256 x 256      11.0     6.1      4.4         4.3          6.1
 //
 // Large tiles read LDS and L2 least for each product and win where there are
-// enough of them; below, what counts is that every compute unit has one.
+// enough of them; below, what counts is that every compute unit has one. f32
+// products are bound by their instructions and take small tiles throughout
+// (4096 x 2048 x 2048: 64x64 four a CU 265, 128x128 273; 1024 x 1024 x 1024:
+// 64x64g2 21, 128x128 66).
 inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool may_split) {
   struct Kind { int bm, bn, per_cu; double stage; };
-  // Time of a stage of 64 (of 32 twice, for two planes) with the chip full.
-  const Kind kinds[4] = {{256, 256, 1, 1.7}, {128, 128, 1, 0.65}, {64, 64, 1, 0.29}, {64, 64, 2, 0.43}};
-  const int64_t sk = 64 / planes, stages = std::max<int64_t>(1, ceil_div(k, sk));
+  // Time of a stage of 64 (of 32 for two and three planes) with the chip full.
+  const Kind one[4] = {{256, 256, 1, 1.7}, {128, 128, 1, 0.65}, {64, 64, 1, 0.29}, {64, 64, 2, 0.43}};
+  const Kind three[4] = {{256, 128, 1, 2.8}, {128, 128, 1, 1.5}, {64, 64, 1, 0.45}, {64, 64, 2, 0.8}};
+  const Kind f32[4] = {{}, {}, {64, 64, 1, 0.57}, {64, 64, 4, 2.0}};
+  const Kind* kinds = planes == 3 ? three : planes == PLANES_F32 ? f32 : one;
+  const int64_t sk = planes == 1 ? 64 : 32, stages = std::max<int64_t>(1, ceil_div(k, sk));
   FastPlan best{};
   double least = 1e30;
-  for (int t = 0; t < 4; t++) {
+  for (int t = planes == PLANES_F32 ? 2 : 0; t < 4; t++) {
     const int64_t tiles = ceil_div(m, kinds[t].bm) * ceil_div(n, kinds[t].bn) * batch;
     for (int64_t splits = 1; splits <= (may_split ? 64 : 1); splits *= 2) {
       if (splits > 1 && stages < 8 * splits) break;
@@ -415,12 +468,12 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
     else
       hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, PartOut>), grid, dim3(S::kThreads), 0, stream, p, sums);
   };
-  switch (plan.tile) {
-    case 0: go(TileBig{}); break;
-    case 1: go(TileMid{}); break;
-    case 2: go(TileDeep{}); break;
-    default: go(TileSmall{});
+  if constexpr (sizeof(T) == 2) {
+    if (plan.tile == 0) go(typename Tiles<T, PL>::Big{});
+    if (plan.tile == 1) go(typename Tiles<T, PL>::Mid{});
   }
+  if (plan.tile == 2) go(typename Tiles<T, PL>::Deep{});
+  if (plan.tile == 3) go(typename Tiles<T, PL>::Small{});
   if (p.splits > 1) {
     const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 256), 4096);
     hipLaunchKernelGGL(join_kernel<Epi>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, sums, p.splits, p.m, p.n,

@@ -134,6 +134,41 @@ struct PlainOut {
   __device__ __forceinline__ void put1(int, int, int i, int j, float p) const { y[i * row + j] = from_f32<E>(p); }
 };
 
+// For f32 operands cut in three planes: a sum that is not finite is taken again
+// from the operands themselves, one element at a time. An infinite element
+// times the zero pieces of a finite one would have made it NaN.
+template <class Epi>
+struct Repair {
+  Epi to;
+  const bf16 *a, *b;
+  int64_t a_i, a_k, a_plane, b_j, b_k, b_plane;  // elements
+  int32_t k;
+  typedef typename Epi::Held Held;
+  __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const { to.fetch(q, i, j, h); }
+  __device__ __noinline__ float again(int i, int j) const {
+    float sum = 0.0f;
+    for (int t = 0; t < k; t++) {
+      const bf16 *x = a + i * a_i + t * a_k, *y = b + j * b_j + t * b_k;
+      sum = fmaf(to_f32(x[0]) + (to_f32(x[a_plane]) + to_f32(x[2 * a_plane])),
+                 to_f32(y[0]) + (to_f32(y[b_plane]) + to_f32(y[2 * b_plane])), sum);
+    }
+    return sum;
+  }
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held& h) const {
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+      v[c] = sums[c];
+      if (!(fabsf(v[c]) < __builtin_inff())) v[c] = again(i, j + c);
+    }
+    to.put8(q, s, i, j, v, h);
+  }
+  __device__ __forceinline__ void put1(int q, int s, int i, int j, float v) const {
+    if (!(fabsf(v) < __builtin_inff())) v = again(i, j);
+    to.put1(q, s, i, j, v);
+  }
+};
+
 // Sums of one split of the contraction, joined by join_splits.
 struct SplitOut {
   float* part;
@@ -261,35 +296,63 @@ void launch_few_rows(const phz_ops* o, hipStream_t stream, const phz_tensor* x, 
   else wide ? go(few_rows<E, 2, 2, Epi>, 32) : go(few_rows<E, 2, 1, Epi>, 16);
 }
 
-// y[i][j] = the splits' sums, added in order.
+// y[i][j] = the splits' sums, added in a fixed order: eight threads an element,
+// each every eighth split.
 template <class E>
 __global__ __launch_bounds__(256) void join_splits(const float* part, int splits, int64_t split, E* y, int64_t row,
                                                    int32_t n, int64_t total) {
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    float v = part[t];
-    for (int s = 1; s < splits; s++) v += part[s * split + t];
-    const int64_t i = t / n;
-    y[i * row + (t - i * n)] = from_f32<E>(v);
+  __shared__ float s[8][32];
+  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  for (int64_t t0 = (int64_t)blockIdx.x * 32; t0 < total; t0 += (int64_t)gridDim.x * 32) {
+    const int64_t t = t0 + c;
+    float v = 0.0f;
+    if (t < total) {
+#pragma unroll 8
+      for (int k = lane; k < splits; k += 8) v += part[k * split + t];
+    }
+    s[lane][c] = v;
+    __syncthreads();
+    if (lane == 0 && t < total) {
+#pragma unroll
+      for (int l = 1; l < 8; l++) v += s[l][c];
+      const int64_t i = t / n;
+      y[i * row + (t - i * n)] = from_f32<E>(v);
+    }
+    __syncthreads();
   }
 }
 
+// Eight f32 as three planes of bf16.
+__device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v) {
+  Pack<bf16, 8> h, m, l;
+#pragma unroll
+  for (int c = 0; c < 8; c++) cut3(v[c], h.v[c].bits, m.v[c].bits, l.v[c].bits);
+  *(Pack<bf16, 8>*)to = h;
+  *(Pack<bf16, 8>*)(to + plane) = m;
+  *(Pack<bf16, 8>*)(to + 2 * plane) = l;
+}
+
 // dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
-// rows of `dz_row` with zeros past n, and the sums of dz over each block's rows,
-// which column_sums adds up in order. A thread takes eight columns and every
-// eighth row of its block.
+// rows of `dz_row` with zeros past n, or cut into three planes of such rows, and the sums of dz over each block's rows,
+// which column_sums adds up in order. A thread takes eight columns; `across`
+// (a power of two, at most 32) of them lie along a row, the others take rows in
+// turn.
 template <class E>
 __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_row, const E* pre, int64_t pre_row,
-                                               E* dz, int64_t dz_row, float* sums, int32_t m, int32_t n, int32_t rows) {
-  const int j = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, lane = threadIdx.x >> 5;
+                                               E* dz, bf16* cut, int64_t plane, int64_t dz_row, float* sums, int32_t m,
+                                               int32_t n, int32_t rows, int32_t across) {
+  const int lanes = 256 / across, at = threadIdx.x & (across - 1), lane = threadIdx.x / across;
+  const int j = (blockIdx.x * across + at) * 8;
   const int64_t i0 = (int64_t)blockIdx.y * rows, i1 = min((int64_t)m, i0 + rows);
   float total[8];
 #pragma unroll
   for (int c = 0; c < 8; c++) total[c] = 0.0f;
   if (j + 8 <= n) {
 #pragma unroll 4
-    for (int64_t i = i0 + lane; i < i1; i += 8) {
+    for (int64_t i = i0 + lane; i < i1; i += lanes) {
       const Pack<E, 8> d = *(const Pack<E, 8>*)(dy + i * dy_row + j);
       Pack<E, 8> p, out;
+      float all[8];
       if (act != PHZ_ACT_NONE) p = *(const Pack<E, 8>*)(pre + i * pre_row + j);
 #pragma unroll
       for (int c = 0; c < 8; c++) {
@@ -297,11 +360,14 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
         if (act != PHZ_ACT_NONE) v *= act_grad(act, to_f32(p.v[c]));
         total[c] += v;
         out.v[c] = from_f32<E>(v);
+        all[c] = v;
       }
       if (dz) *(Pack<E, 8>*)(dz + i * dz_row + j) = out;
+      if (cut) put_cut(cut + i * dz_row + j, plane, all);
     }
   } else if (j < n) {
-    for (int64_t i = i0 + lane; i < i1; i += 8) {
+    for (int64_t i = i0 + lane; i < i1; i += lanes) {
+      float all[8];
 #pragma unroll
       for (int c = 0; c < 8; c++) {
         float v = 0.0f;
@@ -310,21 +376,24 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
           if (act != PHZ_ACT_NONE) v *= act_grad(act, to_f32(pre[i * pre_row + j + c]));
           total[c] += v;
         }
-        if (dz && j + c < dz_row) dz[i * dz_row + j + c] = from_f32<E>(v);
+        all[c] = v;
+        if (dz) dz[i * dz_row + j + c] = from_f32<E>(v);  // dz_row is whole eights
       }
+      if (cut) put_cut(cut + i * dz_row + j, plane, all);
     }
   }
   if (!sums) return;
-  __shared__ float s[8][256];
+  __shared__ float s[256][9];  // [lane][eight of columns][column], one apart
 #pragma unroll
-  for (int c = 0; c < 8; c++) s[lane][(threadIdx.x & 31) * 8 + c] = total[c];
+  for (int c = 0; c < 8; c++) s[threadIdx.x][c] = total[c];
   __syncthreads();
-  const int col = blockIdx.x * 256 + threadIdx.x;
-  if (col < n) {
-    float v = 0.0f;
-#pragma unroll
-    for (int l = 0; l < 8; l++) v += s[l][threadIdx.x];
-    sums[(int64_t)blockIdx.y * n + col] = v;
+  for (int t = threadIdx.x; t < across * 8; t += 256) {
+    const int col = blockIdx.x * across * 8 + t;
+    if (col < n) {
+      float v = 0.0f;
+      for (int l = 0; l < lanes; l++) v += s[l * across + t / 8][t % 8];
+      sums[(int64_t)blockIdx.y * n + col] = v;
+    }
   }
 }
 
@@ -347,10 +416,11 @@ __global__ __launch_bounds__(256) void column_sums(const float* sums, int32_t bl
   }
 }
 
-// Rows of n elements into rows of `to_row`, zeros between.
+// Rows of n elements into rows of `to_row`, zeros between: as they are, or f32
+// cut into three planes.
 template <class E>
-__global__ __launch_bounds__(256) void pack_rows(const E* from, int64_t from_row, E* to, int64_t to_row, int32_t m,
-                                                 int32_t n) {
+__global__ __launch_bounds__(256) void pack_rows(const E* from, int64_t from_row, E* to, bf16* cut, int64_t to_row,
+                                                 int64_t plane, int32_t m, int32_t n) {
   const int64_t per = to_row / 8;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < m * per; t += (int64_t)gridDim.x * 256) {
     const int64_t i = t / per, j = (t - i * per) * 8;
@@ -359,7 +429,9 @@ __global__ __launch_bounds__(256) void pack_rows(const E* from, int64_t from_row
     if (j + 8 <= n) v = *(const Pack<E, 8>*)p;
     else
       for (int c = 0; c < 8 && j + c < n; c++) v.v[c] = p[c];
-    *(Pack<E, 8>*)(to + i * to_row + j) = v;
+    if (to) *(Pack<E, 8>*)(to + i * to_row + j) = v;
+    if constexpr (sizeof(E) == 4)
+      if (cut) put_cut(cut + i * to_row + j, plane, v.v);
   }
 }
 
@@ -403,34 +475,79 @@ struct Carve {
   }
 };
 
-// Whether rows of bf16 can go to LDS as they lie: whole 16 bytes, and a tile's
-// rows within 32-bit offsets.
-bool lies_well(const void* data, int64_t row, int64_t cols) {
-  return (uintptr_t)data % 16 == 0 && row % 8 == 0 && cols % 8 == 0 && row <= 1 << 22;
-}
-
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
-void pack(hipStream_t stream, const bf16* from, int64_t from_row, bf16* to, int64_t m, int64_t n) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(m * (pad8(n) / 8), 256), 8192);
-  hipLaunchKernelGGL(pack_rows<bf16>, dim3(blocks), dim3(256), 0, stream, from, from_row, to, pad8(n), (int32_t)m,
-                     (int32_t)n);
+// How a product's operands go to gemm_fast: as they are, copied into whole
+// eights where they do not lie well (rows of whole 16 bytes, and a tile's rows
+// within 32-bit offsets); or, f32, cut in three planes.
+enum Way { AS_IS, CUT, ANY };  // ANY: gemm_any
+
+// By sizes alone, so a view's strides do not change the result's bits. `whole`:
+// the sizes along dense axes are whole 16 bytes, so that usually nothing needs
+// a copy; from `copy_from` multiply-adds on the copies pay all the same. f32
+// goes to bf16 pieces from 2^33 multiply-adds on, where their rate pays for the
+// cuts (us, f32 instructions / pieces: 2048 x 1024 -> 1024 43 / 50, 4096 x 1024
+// -> 1024 80 / 71, 8192 x 1024 -> 1024 140 / 110).
+template <class E>
+Way way_of(int64_t m, int64_t n, int64_t k, bool whole) {
+  constexpr int64_t copy_from = 1ll << 30;
+  const int64_t work = m * n * k;
+  if (sizeof(E) == 4 && work >= 1ll << 33 && m * pad8(k) < 1ll << 29 && m * pad8(n) < 1ll << 29 && n * pad8(k) < 1ll << 29)
+    return CUT;  // planes keep their distance within the 32 bits of a tile's offsets
+  return whole || work >= copy_from ? AS_IS : ANY;
 }
 
-FastArgs operands(const void* a, int64_t a_row, const void* b, int64_t b_row, int64_t m, int64_t n, int64_t k,
-                  int64_t a_rows, int64_t b_rows) {
+template <class E>
+struct Lain {
+  const E* from;
+  int64_t from_row, rows, cols;
+  Way way;
+  bool well;
+  char* copy = nullptr;
+  Lain(const phz_tensor* t, Way w)
+      : from((const E*)t->data), from_row(t->stride[0]), rows(t->size[0]), cols(t->size[1]), way(w) {
+    constexpr int64_t el = 16 / sizeof(E);
+    well = way == ANY || (way == AS_IS && (uintptr_t)from % 16 == 0 && from_row % el == 0 && cols % el == 0 &&
+                          from_row <= 1 << 22);
+  }
+  int64_t plane() const { return way == CUT ? (rows * pad8(cols) + 127) / 128 * 128 : 0; }  // elements
+  uint64_t bytes() const { return way == CUT ? 3 * plane() * 2 : rows * pad8(cols) * sizeof(E); }
+  const void* data() const { return well ? (const void*)from : copy; }
+  int64_t row() const { return well ? from_row : pad8(cols); }
+  int64_t whole_cols() const { return well ? cols : pad8(cols); }
+  void lay(hipStream_t stream) const {
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows * (pad8(cols) / 8), 256), 8192);
+    if (!well)
+      hipLaunchKernelGGL(pack_rows<E>, dim3(blocks), dim3(256), 0, stream, from, from_row, (E*)(way == CUT ? nullptr : copy),
+                         (bf16*)(way == CUT ? copy : nullptr), pad8(cols), plane(), (int32_t)rows, (int32_t)cols);
+  }
+};
+
+template <class E>
+FastPlan plan(const phz_ops* o, Way way, int64_t m, int64_t n, int64_t k) {
+  return plan_fast(o, m, n, k, 1, way == CUT ? 3 : sizeof(E) == 4 ? (int)PLANES_F32 : 1, true);
+}
+
+// The product of two operands, C of m x n, contraction k; AK, BK: dense along
+// it. Epilogues of cut products are repaired where sums are not finite.
+template <class E, bool AK, bool BK, class Epi>
+void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<E>& b, int64_t m, int64_t n, int64_t k,
+             const FastPlan& plan, float* part, const Epi& epi) {
+  const int64_t e = a.way == CUT ? 2 : sizeof(E);
   FastArgs f{};
-  f.a = (const char*)a, f.b = (const char*)b, f.a_row = a_row * 2, f.b_row = b_row * 2;
-  f.m = (int32_t)m, f.n = (int32_t)n, f.k = (int32_t)k, f.a_rows = (int32_t)a_rows, f.b_rows = (int32_t)b_rows;
-  return f;
+  f.a = (const char*)a.data(), f.b = (const char*)b.data(), f.a_row = a.row() * e, f.b_row = b.row() * e;
+  f.a_plane = (uint32_t)(a.plane() * 2), f.b_plane = (uint32_t)(b.plane() * 2);
+  f.m = (int32_t)m, f.n = (int32_t)n, f.k = (int32_t)k;
+  f.a_rows = (int32_t)(AK ? a.rows : a.whole_cols()), f.b_rows = (int32_t)(BK ? b.rows : b.whole_cols());
+  if constexpr (sizeof(E) == 4) {
+    if (a.way == CUT) {
+      const Repair<Epi> safe{epi, (const bf16*)a.data(), (const bf16*)b.data(), AK ? a.row() : 1, AK ? 1 : a.row(),
+                             a.plane(), BK ? b.row() : 1, BK ? 1 : b.row(), b.plane(), (int32_t)k};
+      return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, safe);
+    }
+  }
+  launch_gemm_fast<E, 1, AK, BK>(o, stream, f, 1, plan, part, epi);
 }
-
-// bf16 products go through gemm_fast where rows are whole eights, operands that
-// do not lie well being copied first, and, with ragged rows, from this many
-// multiply-adds on: gemm_any takes 10 us for as many, the copies of both
-// operands as long. The choice is by sizes alone, so a view's strides do not
-// change the result's bits.
-constexpr int64_t kPackFrom = 1ll << 30;
 
 template <class E>
 int linear(phz_ops* o, hipStream_t stream, int act, const phz_tensor* x, const phz_tensor* w, const phz_tensor* bias,
@@ -446,33 +563,27 @@ int linear(phz_ops* o, hipStream_t stream, int act, const phz_tensor* x, const p
     launch_few_rows<E>(o, stream, x, w, out);
     return launched(o, "linear") ? 0 : 1;
   }
-  if constexpr (sizeof(E) == 2) {
-    const bool x_well = lies_well(x->data, x->stride[0], k), w_well = lies_well(w->data, w->stride[0], k);
-    if (k > 0 && (k % 8 == 0 || m * n * k >= kPackFrom)) {
-      const FastPlan plan = plan_fast(o, m, n, pad8(k), 1, 1, true);
-      Carve c;
-      const bf16 *xd = (const bf16*)x->data, *wd = (const bf16*)w->data;
-      int64_t x_row = x->stride[0], w_row = w->stride[0];
-      bf16 *xp = nullptr, *wp = nullptr;
-      float* part = nullptr;
-      for (int pass = 0; pass < 2; pass++) {
-        c.used = 0;
-        if (!x_well) xp = c.take<bf16>(m * pad8(k) * 2);
-        if (!w_well) wp = c.take<bf16>(n * pad8(k) * 2);
-        part = c.take<float>(plan.part_bytes);
-        if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
-      }
-      if (xp) pack(stream, xd, x_row, xp, m, k), xd = xp, x_row = pad8(k);
-      if (wp) pack(stream, wd, w_row, wp, n, k), wd = wp, w_row = pad8(k);
-      launch_gemm_fast<bf16, 1, true, true>(o, stream, operands(xd, x_row, wd, w_row, m, n, pad8(k), m, n), 1, plan, part,
-                                            out);
-      return launched(o, "linear") ? 0 : 1;
+  const Way way = k == 0 ? ANY : way_of<E>(m, n, k, k % (16 / sizeof(E)) == 0);
+  if (way != ANY) {
+    Lain<E> a(x, way), b(w, way);
+    const FastPlan how = plan<E>(o, way, m, n, pad8(k));
+    Carve c;
+    float* part = nullptr;
+    for (int pass = 0; pass < 2; pass++) {
+      c.used = 0;
+      if (!a.well) a.copy = c.take<char>(a.bytes());
+      if (!b.well) b.copy = c.take<char>(b.bytes());
+      part = c.take<float>(how.part_bytes);
+      if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
     }
+    a.lay(stream);
+    b.lay(stream);
+    product<E, true, true>(o, stream, a, b, m, n, k, how, part, out);
+  } else {
+    launch_gemm_any<E, true, true>(o, stream, Operand{x->data, x->stride[0], 0}, Operand{w->data, w->stride[0], 0},
+                                   GemmShape{(int32_t)m, (int32_t)n, (int32_t)k, (int32_t)std::max<int64_t>(k, 1), 1}, 1,
+                                   out);
   }
-  const Operand a{x->data, x->stride[0], 0}, b{w->data, w->stride[0], 0};
-  launch_gemm_any<E, true, true>(o, stream, a, b,
-                                 GemmShape{(int32_t)m, (int32_t)n, (int32_t)k, (int32_t)std::max<int64_t>(k, 1), 1}, 1,
-                                 out);
   return launched(o, "linear") ? 0 : 1;
 }
 
@@ -482,82 +593,77 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
                     const phz_tensor* db) {
   const int64_t m = x->size[0], k = x->size[1], n = w->size[0];
   const bool need_dx = dx && m > 0 && k > 0, need_dw = dw && k > 0 && m > 0;
-  const E *dyd = (const E*)dy->data, *xd = (const E*)x->data, *wd = (const E*)w->data;
-  int64_t x_row = x->stride[0], w_row = w->stride[0];
-  const int64_t n8 = pad8(n), k8 = pad8(k);
-
-  // bf16 products that are large enough, or lie well, go through gemm_fast.
-  bool fast = false, x_well = true, w_well = true, dy_well = false;
+  constexpr int64_t el = 16 / sizeof(E);
+  const Way way = way_of<E>(m, n, k, k % el == 0 && n % el == 0);
+  const bool fast = way != ANY;
+  Lain<E> d(dy, way), xo(x, way), wo(w, way);
+  if (act != PHZ_ACT_NONE) d.well = false;  // dz is made here
   FastPlan dx_plan{}, dw_plan{};
+  if (fast && need_dx) dx_plan = plan<E>(o, way, m, k, pad8(n));
+  if (fast && need_dw) dw_plan = plan<E>(o, way, n, k, m);
   int32_t splits = 1, k_split = (int32_t)std::max<int64_t>(m, 1);
-  if constexpr (sizeof(E) == 2) {
-    x_well = lies_well(xd, x_row, k), w_well = lies_well(wd, w_row, k), dy_well = lies_well(dyd, dy->stride[0], n);
-    fast = (k % 8 == 0 && n % 8 == 0) || m * n * k >= kPackFrom;
-    if (fast && need_dx) dx_plan = plan_fast(o, m, k, n8, 1, 1, true);
-    if (fast && need_dw) dw_plan = plan_fast(o, n, k, m, 1, 1, true);
-  }
   if (!fast && need_dw) {
     // The contraction of dw runs over rows: split where its few tiles would
     // not fill the chip.
-    const int64_t bk = Cut<E>::tile_k;
+    const int64_t bk = Any<E>::tile_k;
     const int64_t want = std::min<int64_t>(ceil_div(2 * o->cus, ceil_div(n, 64) * ceil_div(k, 64)), ceil_div(m, 4 * bk));
     k_split = (int32_t)(ceil_div(ceil_div(m, std::max<int64_t>(1, std::min<int64_t>(want, 256))), bk) * bk);
     splits = (int32_t)ceil_div(m, k_split);
   }
-  const bool copy_dz = (need_dx || need_dw) && (act != PHZ_ACT_NONE || (fast && !dy_well));
+  const bool lay_d = (need_dx || need_dw) && (fast ? !d.well : act != PHZ_ACT_NONE);
   // Blocks of rows whose sums of dz are added up in the end, at most 256.
   const int64_t rows = std::max<int64_t>(32, ceil_div(ceil_div(m, 256), 8) * 8), blocks = ceil_div(m, rows);
 
   Carve c;
-  E *dz = nullptr, *xp = nullptr, *wp = nullptr;
   float *sums = nullptr, *part = nullptr;
   for (int pass = 0; pass < 2; pass++) {
     c.used = 0;
-    if (copy_dz) dz = c.take<E>(m * n8 * sizeof(E));
+    if (lay_d) d.copy = c.take<char>(d.bytes());
     if (db) sums = c.take<float>(blocks * n * 4);
-    if (fast && need_dw && !x_well) xp = c.take<E>(m * k8 * sizeof(E));
-    if (fast && need_dx && !w_well) wp = c.take<E>(n * k8 * sizeof(E));
+    if (fast && need_dw && !xo.well) xo.copy = c.take<char>(xo.bytes());
+    if (fast && need_dx && !wo.well) wo.copy = c.take<char>(wo.bytes());
     part = c.take<float>(std::max({dx_plan.part_bytes, dw_plan.part_bytes, splits > 1 ? (uint64_t)splits * n * k * 4 : 0}));
     if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
   }
-  if (copy_dz || db) {
-    if (m > 0)
-      hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, 256), (unsigned)blocks), dim3(256), 0, stream, act, dyd,
-                         dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0, dz, n8, sums,
-                         (int32_t)m, (int32_t)n, (int32_t)rows);
-    if (db)
-      hipLaunchKernelGGL(column_sums<E>, dim3((unsigned)ceil_div(n, 32)), dim3(256), 0, stream, sums, (int32_t)blocks,
-                         (int32_t)n, (E*)db->data, db->stride[0]);
+  if (m > 0 && (lay_d || db)) {
+    int across = 32;
+    while (across > 1 && across * 4 >= n) across /= 2;
+    hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, across * 8), (unsigned)blocks), dim3(256), 0, stream, act,
+                       (const E*)dy->data, dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0,
+                       (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(), pad8(n), sums, (int32_t)m, (int32_t)n, (int32_t)rows, across);
   }
-  const E* d = copy_dz ? dz : dyd;
-  const int64_t d_row = copy_dz ? n8 : dy->stride[0];
-  if constexpr (sizeof(E) == 2) {
-    if (xp) pack(stream, xd, x_row, xp, m, k), xd = xp, x_row = k8;
-    if (wp) pack(stream, wd, w_row, wp, n, k), wd = wp, w_row = k8;
-    if (fast && need_dx)
-      launch_gemm_fast<bf16, 1, true, false>(o, stream, operands(d, d_row, wd, w_row, m, k, n, m, k8), 1, dx_plan, part,
-                                             PlainOut<E>{(E*)dx->data, dx->stride[0]});
-    if (fast && need_dw)
-      launch_gemm_fast<bf16, 1, false, false>(o, stream, operands(d, d_row, xd, x_row, n, k, m, n8, k8), 1, dw_plan, part,
-                                              PlainOut<E>{(E*)dw->data, dw->stride[0]});
-  }
-  const int32_t mi = (int32_t)m, ni = (int32_t)n, ki = (int32_t)k;
-  const Operand dop{d, d_row, 0}, xo{xd, x_row, 0}, wo{wd, w_row, 0};
-  if (need_dx && !fast)
-    launch_gemm_any<E, true, false>(o, stream, dop, wo, GemmShape{mi, ki, ni, ni, 1}, 1,
-                                    PlainOut<E>{(E*)dx->data, dx->stride[0]});
-  if (need_dw && !fast) {
-    const GemmShape shape{ni, ki, mi, k_split, splits};
-    if (splits == 1) {
-      launch_gemm_any<E, false, false>(o, stream, dop, xo, shape, 1, PlainOut<E>{(E*)dw->data, dw->stride[0]});
-    } else {
-      launch_gemm_any<E, false, false>(o, stream, dop, xo, shape, 1, SplitOut{part, k, n * k});
-      hipLaunchKernelGGL(join_splits<E>, dim3((unsigned)std::min<int64_t>(ceil_div(n * k, 256), 8192)), dim3(256), 0,
-                         stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k);
+  if (db)
+    hipLaunchKernelGGL(column_sums<E>, dim3((unsigned)ceil_div(n, 32)), dim3(256), 0, stream, sums, (int32_t)blocks,
+                       (int32_t)n, (E*)db->data, db->stride[0]);
+  if (fast) {
+    if (need_dx) {
+      wo.lay(stream);
+      product<E, true, false>(o, stream, d, wo, m, k, n, dx_plan, part, PlainOut<E>{(E*)dx->data, dx->stride[0]});
+    }
+    if (need_dw) {
+      xo.lay(stream);
+      product<E, false, false>(o, stream, d, xo, n, k, m, dw_plan, part, PlainOut<E>{(E*)dw->data, dw->stride[0]});
+    }
+  } else {
+    const int32_t mi = (int32_t)m, ni = (int32_t)n, ki = (int32_t)k;
+    const Operand dop{d.copy ? d.copy : dy->data, d.copy ? pad8(n) : dy->stride[0], 0}, xa{x->data, x->stride[0], 0},
+        wa{w->data, w->stride[0], 0};
+    if (need_dx)
+      launch_gemm_any<E, true, false>(o, stream, dop, wa, GemmShape{mi, ki, ni, ni, 1}, 1,
+                                      PlainOut<E>{(E*)dx->data, dx->stride[0]});
+    if (need_dw) {
+      const GemmShape shape{ni, ki, mi, k_split, splits};
+      if (splits == 1) {
+        launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, PlainOut<E>{(E*)dw->data, dw->stride[0]});
+      } else {
+        launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, SplitOut{part, k, n * k});
+        hipLaunchKernelGGL(join_splits<E>, dim3((unsigned)std::min<int64_t>(ceil_div(n * k, 32), 8192)), dim3(256), 0,
+                           stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k);
+      }
     }
   }
   if (dw && k > 0 && m == 0)
-    hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], ki, n * k);
+    hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], (int32_t)k, n * k);
   return launched(o, "linear backward") ? 0 : 1;
 }
 

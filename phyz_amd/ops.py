@@ -37,8 +37,17 @@ ACTS = {"none": 0, "tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 _DTYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.uint8: 3, torch.bool: 3}
-_TENSOR = struct.Struct("=q3q3qii")
+_TENSOR = struct.Struct("=q3q3qii")  # phz_tensor, 64 bytes
+_PACK = _TENSOR.pack_into
 _SLOTS = 10
+
+
+def _current_stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The same without the Stream object, where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 class OpsError(RuntimeError):
@@ -68,28 +77,39 @@ class Ops:
 
     # ── arguments ──
     def _put(self, slot: int, t, name: str):
-        """Describes one tensor to the library; the address of its view."""
+        """Describes one tensor to the library; the address of its view. (The
+        common ranks are written out: this is most of a small call's time.)"""
         if t is None:
             return None
+        try:
+            code, n = _DTYPES[t.dtype], t.dim()
+            if t.get_device() == self.device:  # -1 is the host's
+                if n == 2:
+                    a, b = t.shape
+                    s, u = t.stride()
+                    _PACK(self._buf, slot << 6, t.data_ptr(), a, b, 0, s, u, 0, code, 2)
+                    return self._at[slot]
+                if n == 3:
+                    a, b, c = t.shape
+                    s, u, v = t.stride()
+                    _PACK(self._buf, slot << 6, t.data_ptr(), a, b, c, s, u, v, code, 3)
+                    return self._at[slot]
+                if n == 1:
+                    _PACK(self._buf, slot << 6, t.data_ptr(), t.shape[0], 0, 0, t.stride(0), 0, 0, code, 1)
+                    return self._at[slot]
+        except (AttributeError, KeyError):
+            pass
         if not isinstance(t, torch.Tensor):
             raise OpsError(f"{name} has to be a torch tensor, not {type(t).__name__}")
-        if self.device < 0:
-            if t.device.type != "cpu":
-                raise OpsError(f"{name} is on {t.device}: a host-only handle checks CPU tensors")
-        elif t.get_device() != self.device:
-            raise OpsError(f"{name} is on {t.device}, the handle's GPU is cuda:{self.device}")
-        code = _DTYPES.get(t.dtype)
-        if code is None:
+        if t.get_device() != self.device:
+            where = "a host-only handle checks CPU tensors" if self.device < 0 else f"the handle's GPU is cuda:{self.device}"
+            raise OpsError(f"{name} is on {t.device}: {where}")
+        if t.dtype not in _DTYPES:
             raise OpsError(f"{name} is {t.dtype}, expected float32, bfloat16 or a mask of uint8 or bool")
-        n = t.dim()
-        if not 1 <= n <= 3:
-            raise OpsError(f"{name} has {n} dimensions, expected 1 to 3")
-        pad = (0,) * (3 - n)
-        _TENSOR.pack_into(self._buf, slot * _TENSOR.size, t.data_ptr(), *t.shape, *pad, *t.stride(), *pad, code, n)
-        return self._at[slot]
+        raise OpsError(f"{name} has {t.dim()} dimensions, expected 1 to 3")
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream if self.device >= 0 else None
+        return _raw_stream(self.device) if self.device >= 0 else None
 
     def _check(self, rc: int):
         if rc != 0:

@@ -191,6 +191,26 @@ def test_infinite_and_nan_inputs(ops, dtype, rows):
     assert torch.equal(y[1, same].float(), sign)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_infinite_inputs_of_large_products(ops, dtype):
+    """The same through the large products, forward and backward, split sums too."""
+    m, k, n = 2000, 520, 1032
+    d = data(m, k, n, dtype)
+    clean = ops.linear(d["x"], d["w"])
+    dxc, dwc, _ = ops.linear_backward(d["dy"], d["x"], d["w"])
+    x, dy = d["x"].clone(), d["dy"].clone()
+    x[7, 3], dy[1500, 9] = float("inf"), float("-inf")
+    y = ops.linear(x, d["w"])
+    assert torch.equal(y[7].float(), torch.sign(d["w"][:, 3].float()) * float("inf"))
+    y[7] = clean[7]
+    assert torch.equal(y, clean)
+    dx, dw, _ = ops.linear_backward(dy, d["x"], d["w"])
+    assert torch.equal(dx[1500].float(), torch.sign(d["w"][9].float()) * float("-inf"))
+    assert torch.equal(dw[9].float(), torch.sign(d["x"][1500].float()) * float("-inf"))
+    dx[1500], dw[9] = dxc[1500], dwc[9]
+    assert torch.equal(dx, dxc) and torch.equal(dw, dwc)
+
+
 def test_wide_range_in_f32(ops):
     """f32 operands keep their range and all 24 bits: magnitudes from 2^-60 to
     2^60 in one product."""
