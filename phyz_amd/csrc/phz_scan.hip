@@ -13,7 +13,7 @@
 //
 //   lane    VEC neighbouring channels of one world; the state in f32 registers
 //   wave    64 lanes, U steps loaded ahead of the ones being computed
-//   group   NW waves take NW consecutive runs of U steps of the same channels
+//   group   NW waves (4 or 16) take NW consecutive runs of U steps of the same channels
 //           (a slab): each wave composes its run from registers, the runs'
 //           (A, H) meet in LDS, and each wave then runs its steps from the
 //           state that the earlier ones leave. The data is read once.
@@ -105,7 +105,9 @@ __device__ __forceinline__ void store(void* base, int64_t at, const float* v) {
 template <class E, int VEC, int U, bool BACK, bool NEED_X>
 struct Run {
   Pack<E, VEC> z[U], x[NEED_X ? U : 1], a[BACK ? U : 1], hp[BACK ? U : 1];
-  uint32_t reset;  // bit u: an episode begins at this step
+  // Whether episodes begin, as loaded: step u in reset[u], or, where a wave's
+  // lanes are of one world, step u in lane u's reset[0].
+  uint32_t reset[U];
 };
 
 template <class E, int FORM, bool BACK, int VEC, int NW, int U, bool AGG>
@@ -146,17 +148,27 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
       for (int v = 0; v < VEC; v++) s[v] = p.start[b * p.start_b + d + v];
     }
     // The state that the earlier chunks leave.
-    for (int j = 0; j < chunk; j++) {
-      const float* a = p.agg + ((int64_t)j * 2 * p.lanes + idc) * VEC;
-      const Pack<float, VEC> A = load<float, VEC>(a, 0), H = load<float, VEC>(a, p.lanes * VEC);
+    constexpr int kAhead = 32 / VEC;  // chunks whose (A, H) are loaded together
+    for (int j0 = 0; j0 < chunk; j0 += kAhead) {
+      Pack<float, VEC> A[kAhead], H[kAhead];
 #pragma unroll
-      for (int v = 0; v < VEC; v++) s[v] = compose(A.v[v], s[v], H.v[v]);
+      for (int j = 0; j < kAhead; j++) {
+        const float* a = p.agg + ((int64_t)min(j0 + j, chunk - 1) * 2 * p.lanes + idc) * VEC;
+        A[j] = load<float, VEC>(a, 0), H[j] = load<float, VEC>(a, p.lanes * VEC);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        if (j0 + j < chunk) {
+#pragma unroll
+          for (int v = 0; v < VEC; v++) s[v] = compose(A[j].v[v], s[v], H[j].v[v]);
+        }
     }
   }
 
   auto step_of = [&](int i) { return (int64_t)(BACK ? p.steps - 1 - i : i); };
+  const bool one_world = __all(b == (int64_t)__builtin_amdgcn_readfirstlane((int)b));
   auto fetch = [&](R& r, int base) {
-    r.reset = 0;
+    if (rs && one_world) r.reset[0] = lane < U && base + lane < last ? rs[step_of(base + lane) * p.r_t] : 0;
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int i = base + u;
@@ -166,7 +178,7 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
         if (kNeedX) r.x[u] = load<E, VEC>(x, t * p.x_t);
         if (BACK) r.a[u] = load<E, VEC>(dh, t * p.dh_t);
         if (kNeedH && t > 0) r.hp[u] = load<E, VEC>(h, (t - 1) * p.h_t);
-        if (rs) r.reset |= (rs[t * p.r_t] ? 1u : 0u) << u;
+        if (rs && !one_world) r.reset[u] = rs[t * p.r_t];
       }
     }
   };
@@ -178,6 +190,13 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
   int buf = 0;
   for (int slab = first; slab < last; slab += stride, base += stride) {
     if (slab + stride < last) fetch(nxt, base + stride);
+    uint32_t reset = 0;  // bit u: an episode begins at step u of the run
+    if (rs && one_world) {
+      reset = (uint32_t)__ballot(cur.reset[0] != 0);
+    } else if (rs) {
+#pragma unroll
+      for (int u = 0; u < U; u++) reset |= (base + u < last && cur.reset[u] ? 1u : 0u) << u;
+    }
     float q[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -199,7 +218,7 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
 #pragma unroll
       for (int u = 0; u < U; u++)
         if (base + u < last) {
-          const bool rst = (cur.reset >> u) & 1u;
+          const bool rst = (reset >> u) & 1u;
 #pragma unroll
           for (int v = 0; v < VEC; v++) {
             H[v] = advance(H[v], u, v, rst);
@@ -243,7 +262,7 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
           for (int u = 0; u < U; u++)
             if (base + u < last) {
               const int64_t t = step_of(base + u);
-              const bool rst = (cur.reset >> u) & 1u;
+              const bool rst = (reset >> u) & 1u;
               if (BACK) {
                 float dz[VEC], dx[VEC];
 #pragma unroll
@@ -280,7 +299,7 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
       for (int u = 0; u < U; u++)
         if (base + u < last) {
           const int64_t t = step_of(base + u);
-          const bool rst = (cur.reset >> u) & 1u;
+          const bool rst = (reset >> u) & 1u;
           if (BACK) {
             float dz[VEC], dx[VEC];
 #pragma unroll
@@ -321,29 +340,43 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
   }
 }
 
-template <class E, int FORM, bool BACK, int VEC>
-void launch(const ScanArgs& p, int nw, hipStream_t stream) {
-  constexpr int U = BACK ? 4 : 8;
-  const dim3 grid((unsigned)ceil_div(p.lanes, kWaveLanes), (unsigned)p.chunks);
-  if (p.chunks > 1) {
-    const dim3 front(grid.x, p.chunks - 1);  // nobody starts from the last chunk
-    if (nw == 1)
-      hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 1, U, true>), front, dim3(64), 0, stream, p);
-    else
-      hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 8, U, true>), front, dim3(512), 0, stream, p);
+// How waves share a sequence's steps, and the steps that each loads ahead of
+// the ones it computes: more hide more of memory's latency, and leave registers
+// for fewer waves.
+enum Spread {
+  ALONE = 1,   // a wave takes all of them
+  CHUNKS = 4,  // a group of four shares a slab, and takes one of several chunks
+  SLABS = 16   // a group of sixteen shares a slab, and takes all of them
+};
+template <class E>
+constexpr int run_steps(bool back, int spread) {
+  return spread == ALONE ? (back ? 2 : 4) : back && sizeof(E) == 4 ? 4 : 8;
+}
+
+template <class E, int FORM, bool BACK, int VEC, int NW>
+void launch_as(const ScanArgs& p, hipStream_t stream) {
+  constexpr int U = run_steps<E>(BACK, NW);
+  const unsigned groups = (unsigned)ceil_div(p.lanes, kWaveLanes);
+  if constexpr (NW == CHUNKS) {
+    if (p.chunks > 1)  // nobody starts from the last chunk
+      hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, NW, U, true>), dim3(groups, p.chunks - 1), dim3(NW * 64), 0,
+                         stream, p);
   }
-  if (nw == 1)
-    hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 1, U, false>), grid, dim3(64), 0, stream, p);
-  else
-    hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, 8, U, false>), grid, dim3(512), 0, stream, p);
+  hipLaunchKernelGGL((gated_scan_kernel<E, FORM, BACK, VEC, NW, U, false>), dim3(groups, p.chunks), dim3(NW * 64), 0, stream,
+                     p);
+}
+
+template <class E, int FORM, bool BACK>
+void launch(const ScanArgs& p, int vec, int spread, hipStream_t stream) {
+  if (spread == SLABS) vec == 2 ? launch_as<E, FORM, BACK, 2, SLABS>(p, stream) : launch_as<E, FORM, BACK, 1, SLABS>(p, stream);
+  else if (spread == CHUNKS)
+    vec == 4 ? launch_as<E, FORM, BACK, 4, CHUNKS>(p, stream) : launch_as<E, FORM, BACK, 1, CHUNKS>(p, stream);
+  else vec == 4 ? launch_as<E, FORM, BACK, 4, ALONE>(p, stream) : launch_as<E, FORM, BACK, 1, ALONE>(p, stream);
 }
 
 template <class E>
-void launch_any(const ScanArgs& p, int form, bool back, int vec, int nw, hipStream_t stream) {
-  auto go = [&](auto f, auto bk) {
-    if (vec == 4) launch<E, decltype(f)::value, decltype(bk)::value, 4>(p, nw, stream);
-    else launch<E, decltype(f)::value, decltype(bk)::value, 1>(p, nw, stream);
-  };
+void launch_any(const ScanArgs& p, int form, bool back, int vec, int spread, hipStream_t stream) {
+  auto go = [&](auto f, auto bk) { launch<E, decltype(f)::value, decltype(bk)::value>(p, vec, spread, stream); };
   using Sg = std::integral_constant<int, PHZ_GATE_SIGMOID>;
   using Dc = std::integral_constant<int, PHZ_GATE_DECAY>;
   if (form == PHZ_GATE_SIGMOID) back ? go(Sg{}, std::true_type{}) : go(Sg{}, std::false_type{});
@@ -386,26 +419,47 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const void* z, int64_t 
   }
 }
 
-// How the steps and channels are spread. Lanes of four channels, two waves a
-// SIMD wanted (8 a compute unit).
+// Which spread. Waves alone where the channels, four a lane, give four waves a
+// compute unit; groups of sixteen, two channels a lane, where those are one for
+// every second compute unit, so that the data is read once; below, chunks of at
+// least two slabs up to 16 waves a compute unit in all, at most 64 chunks (each
+// start folds its predecessors), of lanes of four channels, or of one where
+// even so the waves would be few.
+// One MI355X, us:                    alone  sixteen  chunks  bytes at a copy's rate
+//   64 x 4096 x 256 f32, forward     158    158      161     173
+//   512 x 64 x 512 f32, forward      .      42       61      43
+//   512 x 64 x 512 f32, backward     90     78       89      86
+//   1023 x 61 x 515 bf16, backward   .      92       115     69
+//   4000 x 100 x 128 f32, backward   .      394      325     264
+//   32768 x 1 x 2048 bf16, forward   .      .        157     86
+//   4096 x 1 x 512 f32, forward      .      .        14.5    5.4
+// What chunks cost above their bytes is the second reading.
 struct Plan {
-  int vec, nw, chunk, chunks;
+  int vec, spread, chunk, chunks;
   int64_t groups, lanes;
 };
 
-Plan plan(const phz_ops* o, int64_t steps, int64_t worlds, int64_t width, bool back) {
-  Plan p;
-  p.vec = width >= 4 ? 4 : 1;
-  p.groups = ceil_div(width, p.vec);
-  p.lanes = worlds * p.groups;
-  const int64_t waves = ceil_div(p.lanes, kWaveLanes), want = 8ll * o->cus;
-  const int u = back ? 4 : 8;
-  p.nw = waves >= want / 2 || steps <= 2 * u ? 1 : 8;
-  const int64_t slab = (int64_t)p.nw * u;
-  int64_t chunks = std::min<int64_t>(ceil_div(want, waves * p.nw), steps / (4 * slab));
-  chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, 64));
-  p.chunk = (int)(ceil_div(ceil_div(steps, chunks), slab) * slab);
-  p.chunks = (int)std::max<int64_t>(1, ceil_div(steps, p.chunk));
+Plan plan(const phz_ops* o, int dtype, int64_t steps, int64_t worlds, int64_t width, bool back) {
+  Plan p{};
+  auto lay = [&](int vec, Spread spread) {
+    p.spread = spread;
+    p.vec = width >= vec ? vec : 1;
+    p.groups = ceil_div(width, p.vec);
+    p.lanes = worlds * p.groups;
+    p.chunk = (int)steps;
+    p.chunks = 1;
+    return ceil_div(p.lanes, kWaveLanes);
+  };
+  if (lay(4, ALONE) >= 4 * o->cus || steps <= 16) return p;
+  if (lay(2, SLABS) >= o->cus / 2) return p;
+  for (int vec : {4, 1}) {
+    const int64_t want = 16ll * o->cus, waves = lay(vec, CHUNKS) * CHUNKS;
+    const int64_t slab = CHUNKS * (dtype == PHZ_F32 ? run_steps<float>(back, CHUNKS) : run_steps<bf16>(back, CHUNKS));
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({ceil_div(want, waves), steps / (2 * slab), 64}));
+    p.chunk = (int)(ceil_div(ceil_div(steps, chunks), slab) * slab);
+    p.chunks = (int)ceil_div(steps, p.chunk);
+    if (waves * p.chunks >= want / 2) break;
+  }
   return p;
 }
 
@@ -442,7 +496,7 @@ int scan(phz_ops* o, hipStream_t stream, int form, bool back, ScanArgs a, int dt
     }
     return launched(o, "gated scan") ? 0 : 1;
   }
-  const Plan p = plan(o, steps, worlds, width, back);
+  const Plan p = plan(o, dtype, steps, worlds, width, back);
   a.steps = (int32_t)steps;
   a.width = (int32_t)width;
   a.groups = (int32_t)p.groups;
@@ -453,8 +507,8 @@ int scan(phz_ops* o, hipStream_t stream, int form, bool back, ScanArgs a, int dt
     a.agg = (float*)o->workspace(stream, (uint64_t)p.chunks * 2 * p.lanes * p.vec * sizeof(float));
     if (!a.agg) return 1;
   }
-  if (dtype == PHZ_F32) launch_any<float>(a, form, back, p.vec, p.nw, stream);
-  else launch_any<bf16>(a, form, back, p.vec, p.nw, stream);
+  if (dtype == PHZ_F32) launch_any<float>(a, form, back, p.vec, p.spread, stream);
+  else launch_any<bf16>(a, form, back, p.vec, p.spread, stream);
   return launched(o, "gated scan") ? 0 : 1;
 }
 
