@@ -67,8 +67,40 @@ struct Source {
   }
 };
 
-// m <- mu m + g, and partial sums of the matrix's squares in f64: gradients
-// whose squares leave f32's range have a norm too.
+// m <- mu m + g where there is a momentum, for eight elements; the sum of the
+// squares of what is orthogonalised, in f64: gradients whose squares leave
+// f32's range have a norm too.
+template <class E>
+__device__ __forceinline__ double update8(const Source<E>& s, int q, int64_t i, int j, int cols) {
+  float v[8];
+  if (s.m.data) {
+    float d[8];
+    load8<float>(s.m, q, i, j, cols, v);
+    load8<E>(s.g, q, i, j, cols, d);
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
+    float* mp = (float*)s.m.data + q * s.m.batch + i * s.m.row + j;
+    if (j + 8 <= cols) {
+      Pack<float, 8> w;
+#pragma unroll
+      for (int c = 0; c < 8; c++) w.v[c] = v[c];
+      *(Pack<float, 8>*)mp = w;
+    } else {
+      for (int c = 0; j + c < cols; c++) mp[c] = v[c];
+    }
+    if (s.nesterov) {
+#pragma unroll
+      for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
+    }
+  } else {
+    load8<E>(s.g, q, i, j, cols, v);
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int c = 0; c < 8; c++) sum = fma((double)v[c], (double)v[c], sum);
+  return sum;
+}
+
 template <class E>
 __global__ __launch_bounds__(256) void norm_kernel(Source<E> s, double* part, int32_t rows, int32_t cols) {
   const int q = blockIdx.y;
@@ -76,32 +108,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Source<E> s, double* part, in
   double sum = 0.0;
   for (uint32_t t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
     const uint32_t i = t / per;
-    const int j = (t - i * per) * 8;
-    float v[8];
-    if (s.m.data) {
-      float d[8];
-      load8<float>(s.m, q, i, j, cols, v);
-      load8<E>(s.g, q, i, j, cols, d);
-#pragma unroll
-      for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
-      float* mp = (float*)s.m.data + q * s.m.batch + i * s.m.row + j;
-      if (j + 8 <= cols) {
-        Pack<float, 8> w;
-#pragma unroll
-        for (int c = 0; c < 8; c++) w.v[c] = v[c];
-        *(Pack<float, 8>*)mp = w;
-      } else {
-        for (int c = 0; j + c < cols; c++) mp[c] = v[c];
-      }
-      if (s.nesterov) {
-#pragma unroll
-        for (int c = 0; c < 8; c++) v[c] = fmaf(s.mu, v[c], d[c]);
-      }
-    } else {
-      load8<E>(s.g, q, i, j, cols, v);
-    }
-#pragma unroll
-    for (int c = 0; c < 8; c++) sum = fma((double)v[c], (double)v[c], sum);
+    sum += update8(s, q, i, (t - i * per) * 8, cols);
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) part[(int64_t)q * gridDim.x + blockIdx.x] = sum;
@@ -298,6 +305,9 @@ Bounds bounds(const phz_muon_cfg& g) {
   return m;
 }
 
+// The power of two that puts values up to `bound` within half of f16's range.
+double f16_scale(double bound) { return exp2(floor(log2(32768.0 / bound))); }
+
 // Any coefficients: products of f32 operands at any size (phz_gemm.h).
 template <class G, class O>
 int newton_schulz_any(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t batch, int32_t rows,
@@ -383,8 +393,7 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
   half_t* h = (half_t*)(ws + part_bytes + split_bytes);
   Planes x{h, xn, c8, 2 * xn}, y{h + 2 * batch * xn, xn, c8, 2 * xn};
   const Planes a{h + 4 * batch * xn, an, s8, P * an}, p{h + (4 * xn + P * an) * batch, an, s8, P * an};
-  auto scale = [](double bound) { return exp2(floor(log2(32768.0 / bound))); };
-  const double sx = scale(top.x), sa = scale(top.a), sp = scale(top.p > 0 ? top.p : 1.0);
+  const double sx = f16_scale(top.x), sa = f16_scale(top.a), sp = f16_scale(top.p > 0 ? top.p : 1.0);
   hipLaunchKernelGGL(norm_kernel<G>, dim3(parts, (unsigned)batch), dim3(256), 0, stream, src, part, rows, cols);
   const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 2048), 2048);
   hipLaunchKernelGGL(scale_kernel<G>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, src, part, parts, cfg.eps,
@@ -412,6 +421,226 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
   return launched(o, "orthogonalize") ? 0 : 1;
 }
 
+// ── a matrix that fits a compute unit ───────────────────────────────────────
+//
+// Up to about 128 x 160 or 64 x 500, one workgroup does all of it: the
+// seventeen launches of the path above would each take a few microseconds for
+// next to no work. X lies in LDS as hi + lo, shorter side along rows (tall
+// matrices transposed on the way in and out), A and then b A + c A^2 beside it.
+// Each product's 32 x 32 blocks are shared among sixteen waves, which hold their
+// sums until everybody has read what they replace. Sums come out with four
+// neighbouring rows in a lane: A and the polynomial are symmetric and X' is
+// taken as X^T P, so those are four neighbours along a row of LDS, too.
+// Rows of LDS are eight elements longer than whole 32, which puts 16 rows'
+// reads on all banks.
+constexpr int kOneWaves = 16, kOneBlocks = 3, kOneLds = 156 * 1024, kOneLittle = 40 * 1024;
+
+struct OneShape {
+  int32_t s, l;    // shorter and longer side, in whole 32
+  int32_t xr, ar;  // elements between rows of X and of A
+  int64_t bytes;
+};
+OneShape one_shape(int64_t rows, int64_t cols, int planes) {
+  OneShape o{};
+  o.s = (int32_t)((std::min(rows, cols) + 31) / 32 * 32), o.l = (int32_t)((std::max(rows, cols) + 31) / 32 * 32);
+  o.xr = o.l + 8, o.ar = o.s + 8;
+  o.bytes = (int64_t)o.s * o.xr * 4 + (int64_t)o.s * o.ar * 2 * planes;
+  return o;
+}
+
+struct Four {
+  half_t v[4];
+};
+
+template <class G, class O, int P, int LDS>
+__global__ __launch_bounds__(kOneWaves * 64) void one_kernel(Source<G> src, phz_muon_cfg cfg, OneShape sh, float sx, float sa,
+                                                             float sp, Result<O> out, int32_t rows, int32_t cols) {
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
+  __shared__ double norm;
+  half_t* xh = (half_t*)lds;
+  half_t* xl = xh + sh.s * sh.xr;
+  half_t* ah = xl + sh.s * sh.xr;
+  half_t* al = ah + sh.s * sh.ar;  // P = 2
+  const int q = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool wide = rows <= cols;
+  constexpr int T = kOneWaves * 64;
+
+  // The matrix's norm (and the momentum's update), then X over it; a thread
+  // meets the same elements in both passes.
+  for (int t = threadIdx.x; t < sh.s * sh.xr / 4; t += T) ((uint64_t*)lds)[t] = 0, ((uint64_t*)xl)[t] = 0;
+  const uint32_t per = (cols + 7) / 8, n = (uint32_t)rows * per;  // eights
+  double sum = 0.0;
+  for (uint32_t t = threadIdx.x; t < n; t += T) {
+    const uint32_t i = t / per;
+    sum += update8(src, q, i, (t - i * per) * 8, cols);
+  }
+  __shared__ double part[kOneWaves];
+#pragma unroll
+  for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < kOneWaves; w++) all += part[w];
+    norm = sx / (sqrt(all) + cfg.eps);
+  }
+  __syncthreads();
+  const double inv = norm;
+  for (uint32_t t = threadIdx.x; t < n; t += T) {
+    const uint32_t i = t / per;
+    const int j = (t - i * per) * 8;
+    float v[8];
+    src.at(q, i, j, cols, v);
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+      if (j + c >= cols) break;
+      const float x = (float)(v[c] * inv);
+      const int at = wide ? i * sh.xr + j + c : (j + c) * sh.xr + i;
+      xh[at] = from_f32<half_t>(x);
+      xl[at] = from_f32<half_t>(x - to_f32(xh[at]));
+    }
+  }
+  __syncthreads();
+
+  const int fr = lane & 31, fk = (lane >> 5) * 8;  // fragments: row lane % 32, eight k from here
+  auto along = [&](const half_t* p, int pitch, int row, int k) { return *(const s16x8*)(p + (row + fr) * pitch + k + fk); };
+  // Eight k (rows of X) of column col + lane % 32.
+  auto across = [&](const half_t* p, int col, int k) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const half_t* at = p + (k + fk + ((lane & 15) >> 2)) * sh.xr + col + (lane & 16) + (lane & 3) * 4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 4 * sh.xr));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto times = [&](s16x8 ahi, s16x8 alo, s16x8 bhi, s16x8 blo, f32x16 c) {
+    if (P == 2) {
+      c = Mfma<half_t>::run(alo, bhi, c);
+      c = Mfma<half_t>::run(ahi, blo, c);
+    }
+    return Mfma<half_t>::run(ahi, bhi, c);
+  };
+  auto put4 = [&](half_t* hi, half_t* lo, int at, const float* v) {
+    Four h, l;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      h.v[c] = from_f32<half_t>(v[c]);
+      if (lo) l.v[c] = from_f32<half_t>(v[c] - to_f32(h.v[c]));
+    }
+    *(Four*)(hi + at) = h;
+    if (lo) *(Four*)(lo + at) = l;
+  };
+  // Where a block's group of four sums lies: column `col` + lane % 32 of the
+  // product, its row `row` + 8 g + 4 (lane / 32).
+  auto place = [&](int pitch, int row, int col, int g) { return (col + fr) * pitch + row + g * 8 + (lane >> 5) * 4; };
+  const int sb = sh.s / 32, lb = sh.l / 32, ablocks = sb * sb, xblocks = sb * lb;  // at most 16, 48
+  const int ai = wave / sb * 32, aj = wave % sb * 32;
+  const float to_a = sa / (sx * sx), to_c = (float)cfg.c * (sp / (sa * sa)), to_b = (float)cfg.b * (sp / sa);
+  for (int step = 0; step < cfg.steps; step++) {
+    // A = X X^T: nothing is replaced that others read.
+    f32x16 c;
+    if (wave < ablocks) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) c[r] = 0.0f;
+#pragma unroll 2
+      for (int k = 0; k < sh.l; k += 16)
+        c = times(along(xh, sh.xr, ai, k), P == 2 ? along(xl, sh.xr, ai, k) : s16x8{}, along(xh, sh.xr, aj, k),
+                  P == 2 ? along(xl, sh.xr, aj, k) : s16x8{}, c);
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = c[g * 4 + r] * to_a;
+        put4(ah, P == 2 ? al : nullptr, place(sh.ar, ai, aj, g), v);
+      }
+    }
+    __syncthreads();
+    // b A + c A^2, in A's place once everybody has read A.
+    if (wave < ablocks) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) c[r] = 0.0f;
+#pragma unroll 2
+      for (int k = 0; k < sh.s; k += 16)
+        c = times(along(ah, sh.ar, ai, k), P == 2 ? along(al, sh.ar, ai, k) : s16x8{}, along(ah, sh.ar, aj, k),
+                  P == 2 ? along(al, sh.ar, aj, k) : s16x8{}, c);
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const Four h = *(const Four*)(ah + place(sh.ar, ai, aj, g));
+        Four l{};
+        if (P == 2) l = *(const Four*)(al + place(sh.ar, ai, aj, g));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          c[g * 4 + r] = fmaf(to_c, c[g * 4 + r], to_b * (P == 2 ? to_f32(h.v[r]) + to_f32(l.v[r]) : to_f32(h.v[r])));
+      }
+    }
+    __syncthreads();
+    if (wave < ablocks) {
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = c[g * 4 + r];
+        put4(ah, P == 2 ? al : nullptr, place(sh.ar, ai, aj, g), v);
+      }
+    }
+    __syncthreads();
+    // X' = a X + (X^T P)^T, block columns of X by block rows of P.
+    f32x16 d[kOneBlocks];
+#pragma unroll
+    for (int u = 0; u < kOneBlocks; u++) {
+      const int t = wave + u * kOneWaves;
+      if (t < xblocks) {
+        const int col = t / sb * 32, row = t % sb * 32;
+#pragma unroll
+        for (int r = 0; r < 16; r++) d[u][r] = 0.0f;
+#pragma unroll 2
+        for (int k = 0; k < sh.s; k += 16)
+          d[u] = times(across(xh, col, k), P == 2 ? across(xl, col, k) : s16x8{}, along(ah, sh.ar, row, k),
+                       P == 2 ? along(al, sh.ar, row, k) : s16x8{}, d[u]);
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int at = place(sh.xr, col, row, g);
+          const Four h = *(const Four*)(xh + at), l = *(const Four*)(xl + at);
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            d[u][g * 4 + r] = fmaf((float)cfg.a, to_f32(h.v[r]) + to_f32(l.v[r]), d[u][g * 4 + r] * (1.0f / sp));
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOneBlocks; u++) {
+      const int t = wave + u * kOneWaves;
+      if (t < xblocks) {
+        const int col = t / sb * 32, row = t % sb * 32;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) v[r] = d[u][g * 4 + r];
+          put4(xh, xl, place(sh.xr, col, row, g), v);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (uint32_t t = threadIdx.x; t < n; t += T) {
+    const uint32_t i = t / per;
+    const int j = (t - i * per) * 8;
+    const bool whole = j + 8 <= cols;
+    Pack<O, 8> before{};
+    if (out.update && whole) before = *(const Pack<O, 8>*)(out.o + q * out.batch + i * out.row + j);
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+      const int at = min(j + c, cols - 1) * (wide ? 1 : sh.xr) + i * (wide ? sh.xr : 1);
+      v[c] = (to_f32(xh[at]) + to_f32(xl[at])) * (1.0f / sx);
+    }
+    if (whole) out.put8(q, i, j, v, before);
+    else
+      for (int c = 0; j + c < cols; c++) out.put(q, i, j + c, v[c]);
+  }
+}
+
 template <class G, class O>
 int orthogonal(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t batch, int64_t rows, int64_t cols,
                View g, View m, const Result<O>& out) {
@@ -421,6 +650,17 @@ int orthogonal(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, int64_t 
   if (cfg.steps == 0 || !(top.x <= 64) || !(top.a <= 4096) || !(top.p <= 4096))
     return newton_schulz_any<G, O>(o, stream, cfg, batch, (int32_t)rows, (int32_t)cols, src, out);
   constexpr int P = sizeof(O) == 2 ? 1 : 2;
+  const OneShape shape = one_shape(rows, cols, P);
+  if (shape.s <= 128 && shape.bytes <= kOneLds && shape.s / 32 * (shape.l / 32) <= kOneBlocks * kOneWaves) {
+    const float sx = (float)f16_scale(top.x), sa = (float)f16_scale(top.a), sp = (float)f16_scale(top.p > 0 ? top.p : 1.0);
+    if (shape.bytes <= kOneLittle)
+      hipLaunchKernelGGL((one_kernel<G, O, P, kOneLittle>), dim3((unsigned)batch), dim3(kOneWaves * 64), 0, stream, src, cfg,
+                         shape, sx, sa, sp, out, (int32_t)rows, (int32_t)cols);
+    else
+      hipLaunchKernelGGL((one_kernel<G, O, P, kOneLds>), dim3((unsigned)batch), dim3(kOneWaves * 64), 0, stream, src, cfg,
+                         shape, sx, sa, sp, out, (int32_t)rows, (int32_t)cols);
+    return launched(o, "orthogonalize") ? 0 : 1;
+  }
   return newton_schulz<G, O, P>(o, stream, cfg, top, batch, (int32_t)rows, (int32_t)cols, src, out);
 }
 

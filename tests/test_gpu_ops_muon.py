@@ -57,6 +57,18 @@ def test_orthogonalize(ops, shape, dtype):
     assert torch.equal(ops.orthogonalize(g), o)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(128, 160), (160, 128), (129, 160), (128, 161), (96, 281), (64, 530), (530, 64),
+                                   (32, 1150), (1150, 17), (20, 3000), (100, 100)], ids=str)
+def test_sizes_about_one_workgroup(ops, shape, dtype):
+    """What one workgroup holds, and what it just does not; a batch of each."""
+    g = matrices(5, *shape, dtype, seed=6)
+    o = ops.orthogonalize(g)
+    for k in range(5):
+        assert off(o[k], R.orthogonalize(g[k])) <= TOL[dtype]
+    assert torch.equal(ops.orthogonalize(g[3]), o[3])
+
+
 @pytest.mark.parametrize("steps", [0, 1, 2, 7])
 def test_steps_and_coefficients(ops, steps):
     g = matrices(2, 40, 72, F32)
