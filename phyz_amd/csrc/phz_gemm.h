@@ -144,14 +144,22 @@ __device__ __forceinline__ f32x16 multiply(const float* a, const float* b, f32x1
 
 // Any size and layout: a workgroup of four waves per BM x BN tile, registers
 // holding the next k tile while the matrix cores work on the one in LDS.
-// `epi.put1(q, split, i, j, sum)` takes each element.
+//
+// An epilogue has
+//   Columns, columns(j, c)                what it reads for eight columns, once
+//   Held, fetch(q, i, j, held)            what it reads for eight elements, ahead
+//   put8(q, split, i, j, sums, held, c)   eight neighbouring sums of row i
+//   put1(q, split, i, j, sum)             one, at a ragged end
 template <class E, bool AK, bool BKD, int BM, int BN, class Epi>
 __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape s, Epi epi) {
   constexpr int BK = Any<E>::tile_k, LD = Any<E>::ld, PER = 16 / sizeof(E);
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
   using SA = Stage<E, AK, BM>;
   using SB = Stage<E, BKD, BN>;
-  __shared__ __attribute__((aligned(16))) E la[BM * LD], lb[BN * LD];
+  constexpr int kOutRow = WN + 4;  // floats of one staged output row
+  static_assert(4 * 32 * kOutRow * 4 <= (BM + BN) * LD * (int)sizeof(E), "output rows fit the tiles");
+  __shared__ __attribute__((aligned(16))) E la[(BM + BN) * LD];
+  E* lb = la + BM * LD;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
   const int q = blockIdx.z / s.splits, split = blockIdx.z - q * s.splits;
@@ -190,22 +198,54 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
           acc[i][j] = multiply(la + (wm + i * 32 + fr) * LD + kk + fk, lb + (wn + j * 32 + fr) * LD + kk + fk, acc[i][j]);
   }
 
-  // Accumulator layout: register r of a lane is row (r / 4) 8 + (lane / 32) 4 +
-  // r % 4, column lane % 32 of its 32 x 32 block.
+  // Out through LDS, 32 rows of a wave's part at a time, so that each lane
+  // holds eight neighbouring columns. Accumulator layout: register r of a lane
+  // is row (r / 4) 8 + (lane / 32) 4 + r % 4, column lane % 32 of its block.
+  __syncthreads();
+  float* out = (float*)la + wave * 32 * kOutRow;
+  constexpr int kLanes = WN / 8, kRows = 64 / kLanes, kPuts = 32 / kRows;
+  const int col = n0 + wn + (lane % kLanes) * 8;
+  typename Epi::Columns columns;
+  if (col + 8 <= s.n) epi.columns(col, columns);
 #pragma unroll
-  for (int i = 0; i < TM; i++)
+  for (int i = 0; i < TM; i++) {
+    typename Epi::Held held[kPuts];
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-      const int col = n0 + wn + j * 32 + fr;
-      if (col < s.n) {
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int row = m0 + wm + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-          if (row < s.m) epi.put1(q, split, row, col, acc[i][j][r]);
-        }
-      }
+    for (int r = 0; r < kPuts; r++) {
+      const int row = m0 + wm + i * 32 + r * kRows + lane / kLanes;
+      if (row < s.m && col + 8 <= s.n) epi.fetch(q, row, col, held[r]);
     }
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        out[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * kOutRow + j * 32 + fr] = acc[i][j][r];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < kPuts; r++) {
+      const int row = m0 + wm + i * 32 + r * kRows + lane / kLanes;
+      float v[8];
+      const float* p = out + (r * kRows + lane / kLanes) * kOutRow + (lane % kLanes) * 8;
+      *(f32x4*)v = *(const f32x4*)p;
+      *(f32x4*)(v + 4) = *(const f32x4*)(p + 4);
+      if (row >= s.m) continue;
+      if (col + 8 <= s.n) epi.put8(q, split, row, col, v, held[r], columns);
+      else
+        for (int c = 0; c < 8 && col + c < s.n; c++) epi.put1(q, split, row, col + c, v[c]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
 }
+
+// For epilogues that read nothing for columns, or nothing ahead.
+struct NoColumns {
+  struct Columns {};
+  __device__ __forceinline__ void columns(int, Columns&) const {}
+};
+struct NothingAhead : NoColumns {
+  struct Held {};
+  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
+};
 
 // Launches gemm_any with the tile that fills the chip: 128 x 128 where those
 // are two for every compute unit and not mostly beyond the edge, 64 x 64 below.

@@ -156,11 +156,6 @@ struct FastTile {
   }
 };
 
-// An epilogue has
-//   Held, fetch(q, i, j, held)         what it reads for eight elements, ahead
-//   put8(q, split, i, j, sums, held)   eight neighbouring sums of row i
-//   put1(q, split, i, j, sum)          one, at a ragged end
-//
 // A tile BM x BN, BK slots of contraction a stage (SK = BK / planes of k), NS stages of LDS, MW x NW waves, and
 // NG such groups of waves: each takes every NG-th stage of the contraction, and
 // their sums are added in order at the end. One group where the tiles fill the
@@ -291,7 +286,9 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
     for (int r = 0; r < kPuts; r++)
       if (mine && row_of(i, r) < p.m && col + 8 <= p.n) epi.fetch(q, row_of(i, r), col, held[i & 1][r]);
   };
+  typename Epi::Columns columns;
   arrive(steps - 1);
+  if (col + 8 <= p.n) epi.columns(col, columns);
   fetch(0);
   if (NG == 1 || (steps - 1) * NG + group < total) compute();  // a group may have no last stage
 
@@ -323,7 +320,7 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
       for (int g = 1; g < NG; g++)
 #pragma unroll
         for (int c = 0; c < 8; c++) v[c] += s[g * kGroup + c];
-      if (col + 8 <= p.n) epi.put8(q, split, row, col, v, held[i & 1][r]);
+      if (col + 8 <= p.n) epi.put8(q, split, row, col, v, held[i & 1][r], columns);
       else
         for (int c = 0; c < 8 && col + c < p.n; c++) epi.put1(q, split, row, col + c, v[c]);
     }
@@ -410,12 +407,11 @@ inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int
 }
 
 // Sums of one split, joined by join_kernel.
-struct PartOut {
+struct PartOut : NothingAhead {
   float* part;
   int64_t row, batch, split;
-  struct Held {};
-  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held&) const {
+  PartOut(float* p, int64_t r, int64_t b, int64_t s) : part(p), row(r), batch(b), split(s) {}
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held&, const Columns&) const {
     float* at = part + s * split + q * batch + i * row + j;
     *(f32x4*)at = *(const f32x4*)sums;
     *(f32x4*)(at + 4) = *(const f32x4*)(sums + 4);
@@ -434,7 +430,8 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
     const int i = (int)(t / per), j = (int)(t - (int64_t)i * per) * 8;
     const float* at = p.part + q * p.batch + i * p.row + j;
     typename Epi::Held held;
-    if (j + 8 <= n) epi.fetch(q, i, j, held);
+    typename Epi::Columns columns;
+    if (j + 8 <= n) epi.fetch(q, i, j, held), epi.columns(j, columns);
     float v[8];
     *(f32x4*)v = *(const f32x4*)at;
     *(f32x4*)(v + 4) = *(const f32x4*)(at + 4);
@@ -443,7 +440,7 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
 #pragma unroll
       for (int c = 0; c < 4; c++) v[c] += lo[c], v[4 + c] += hi[c];
     }
-    if (j + 8 <= n) epi.put8(q, 0, i, j, v, held);
+    if (j + 8 <= n) epi.put8(q, 0, i, j, v, held, columns);
     else
       for (int c = 0; c < 8 && j + c < n; c++) epi.put1(q, 0, i, j + c, v[c]);
   }

@@ -78,28 +78,29 @@ struct LinearOut {
   E *pre, *y;
   int64_t residual_row, pre_row, y_row, bias_step;
   int act;
+  struct Columns {
+    Pack<E, 8> bias;
+  };
   struct Held {
     Pack<E, 8> residual;
   };
+  __device__ __forceinline__ void columns(int j, Columns& c) const {
+    if (!bias) return;
+    if (bias_step == 1) {
+      c.bias = *(const Pack<E, 8>*)(bias + j);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) c.bias.v[k] = bias[(j + k) * bias_step];
+    }
+  }
   __device__ __forceinline__ void fetch(int, int i, int j, Held& h) const {
     if (residual) h.residual = *(const Pack<E, 8>*)(residual + i * residual_row + j);
   }
-  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held& h) const {
+  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held& h, const Columns& col) const {
     float p[8];
     Pack<E, 8> out;
 #pragma unroll
-    for (int c = 0; c < 8; c++) p[c] = sums[c];
-    if (bias) {
-      Pack<E, 8> b;
-      if (bias_step == 1) {
-        b = *(const Pack<E, 8>*)(bias + j);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 8; c++) b.v[c] = bias[(j + c) * bias_step];
-      }
-#pragma unroll
-      for (int c = 0; c < 8; c++) p[c] += to_f32(b.v[c]);
-    }
+    for (int c = 0; c < 8; c++) p[c] = bias ? sums[c] + to_f32(col.bias.v[c]) : sums[c];
     if (pre) {
 #pragma unroll
       for (int c = 0; c < 8; c++) out.v[c] = from_f32<E>(p[c]);
@@ -120,12 +121,11 @@ struct LinearOut {
 };
 
 template <class E>
-struct PlainOut {
+struct PlainOut : NothingAhead {
   E* y;
   int64_t row;
-  struct Held {};
-  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
-  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held&) const {
+  PlainOut(E* p, int64_t r) : y(p), row(r) {}
+  __device__ __forceinline__ void put8(int, int, int i, int j, const float* sums, const Held&, const Columns&) const {
     Pack<E, 8> out;
 #pragma unroll
     for (int c = 0; c < 8; c++) out.v[c] = from_f32<E>(sums[c]);
@@ -144,6 +144,8 @@ struct Repair {
   int64_t a_i, a_k, a_plane, b_j, b_k, b_plane;  // elements
   int32_t k;
   typedef typename Epi::Held Held;
+  typedef typename Epi::Columns Columns;
+  __device__ __forceinline__ void columns(int j, Columns& c) const { to.columns(j, c); }
   __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const { to.fetch(q, i, j, h); }
   __device__ __noinline__ float again(int i, int j) const {
     float sum = 0.0f;
@@ -154,14 +156,14 @@ struct Repair {
     }
     return sum;
   }
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held& h) const {
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held& h, const Columns& col) const {
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) {
       v[c] = sums[c];
       if (!(fabsf(v[c]) < __builtin_inff())) v[c] = again(i, j + c);
     }
-    to.put8(q, s, i, j, v, h);
+    to.put8(q, s, i, j, v, h, col);
   }
   __device__ __forceinline__ void put1(int q, int s, int i, int j, float v) const {
     if (!(fabsf(v) < __builtin_inff())) v = again(i, j);
@@ -170,9 +172,16 @@ struct Repair {
 };
 
 // Sums of one split of the contraction, joined by join_splits.
-struct SplitOut {
+struct SplitOut : NothingAhead {
   float* part;
   int64_t row, split;
+  SplitOut(float* p, int64_t r, int64_t s) : part(p), row(r), split(s) {}
+  __device__ __forceinline__ void put8(int, int s, int i, int j, const float* sums, const Held&, const Columns&) const {
+    Pack<float, 8> out;
+#pragma unroll
+    for (int c = 0; c < 8; c++) out.v[c] = sums[c];
+    *(Pack<float, 8>*)(part + s * split + i * row + j) = out;
+  }
   __device__ __forceinline__ void put1(int, int s, int i, int j, float p) const { part[s * split + i * row + j] = p; }
 };
 

@@ -174,15 +174,16 @@ __global__ __launch_bounds__(256) void scale_kernel(Source<E> s, const double* p
 
 // y = alpha sum + beta d, as PY planes; d has PD.
 template <int PY, int PD>
-struct PlanesOut {
+struct PlanesOut : NoColumns {
   Planes y, d;
   float alpha, beta;
   int32_t cols;  // columns that exist: zeros beyond
+  PlanesOut(Planes y_, Planes d_, float al, float be, int32_t c) : y(y_), d(d_), alpha(al), beta(be), cols(c) {}
   typedef PlaneEight<PD> Held;
   __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const {
     if (d.data) h.get(d, q * d.batch + i * d.row + j);
   }
-  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h) const {
+  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h, const Columns&) const {
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++)
@@ -213,11 +214,12 @@ struct Result {
 
 // alpha sum + beta X into the result.
 template <class O>
-struct LastOut {
+struct LastOut : NoColumns {
   Planes x;
   float alpha, beta;
   int32_t cols;
   Result<O> out;
+  LastOut(Planes x_, float al, float be, int32_t c, const Result<O>& o) : x(x_), alpha(al), beta(be), cols(c), out(o) {}
   struct Held {
     PlaneEight<2> x;
     Pack<O, 8> before;
@@ -226,7 +228,7 @@ struct LastOut {
     h.x.get(x, q * x.batch + i * x.row + j);
     if (out.update && j + 8 <= cols) h.before = *(const Pack<O, 8>*)(out.o + q * out.batch + i * out.row + j);
   }
-  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h) const {
+  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h, const Columns&) const {
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) v[c] = fmaf(alpha, sums[c], beta * h.x.value(c));
@@ -238,11 +240,16 @@ struct LastOut {
 };
 
 // C = alpha product + beta D in f32 (any coefficients; see newton_schulz_any).
-struct Axpby {
+struct Axpby : NothingAhead {
   float *y;
   const float* d;
   float alpha, beta;
   int64_t row, batch;
+  Axpby(float* y_, const float* d_, float al, float be, int64_t r, int64_t b)
+      : y(y_), d(d_), alpha(al), beta(be), row(r), batch(b) {}
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* p, const Held&, const Columns&) const {
+    for (int c = 0; c < 8; c++) put1(q, s, i, j + c, p[c]);
+  }
   __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
     const int64_t at = q * batch + i * row + j;
     y[at] = fmaf(alpha, p, d ? beta * d[at] : 0.0f);
@@ -250,11 +257,15 @@ struct Axpby {
 };
 
 template <class O>
-struct LastAny {
+struct LastAny : NothingAhead {
   const float* x;
   float a;
   int64_t row, batch;
   Result<O> out;
+  LastAny(const float* x_, float a_, int64_t r, int64_t b, const Result<O>& o) : x(x_), a(a_), row(r), batch(b), out(o) {}
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* p, const Held&, const Columns&) const {
+    for (int c = 0; c < 8; c++) put1(q, s, i, j + c, p[c]);
+  }
   __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
     out.put(q, i, j, fmaf(a, x[q * batch + i * row + j], p));
   }
