@@ -9,6 +9,8 @@
    kernels (csrc/phz_io.hip), the PPO update pass (csrc/phz_train.hip) and the
    operators of sequence policies (csrc/phz_ops.hip, phz_scan.hip,
    phz_linear.hip, phz_muon.hip) for gfx950 and link them with hiprtc.
+3. Compile the module that describes torch tensors to the library
+   (csrc/phz_describe.cpp, g++, Python's headers): _describe.so.
 
 Packed FP32 instructions are disabled in every device compile.
 """
@@ -18,11 +20,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libphyz_amd.so")
+DESCRIBE = os.path.join(HERE, "_describe.so")
 ARCH = "gfx950"
 KERNELS = ["phz_io", "phz_train", "phz_ops", "phz_scan", "phz_linear", "phz_muon"]  # csrc/*.hip, ahead of time
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -70,6 +74,9 @@ def build(verbose: bool = False) -> str:
              os.path.join(CSRC, name + ".hip"), "-o", obj(name)] for name in KERNELS]
     jobs.append([cc, "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-c",
                  os.path.join(CSRC, "phz_host.cpp"), "-o", obj("phz_host")])
+    describe_tmp = DESCRIBE + ".tmp"
+    jobs.append(["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-I" + sysconfig.get_paths()["include"],
+                 os.path.join(CSRC, "phz_describe.cpp"), "-o", describe_tmp])
     with ThreadPoolExecutor(4) as pool:
         for done in [pool.submit(_run, j, verbose) for j in jobs]:
             done.result()
@@ -77,6 +84,7 @@ def build(verbose: bool = False) -> str:
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(obj, KERNELS), obj("phz_host"), "-o", tmp,
           "-L/opt/rocm/lib", "-lhiprtc", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib"], verbose)
     os.replace(tmp, LIB)
+    os.replace(describe_tmp, DESCRIBE)
     return LIB
 
 

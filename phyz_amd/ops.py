@@ -24,7 +24,7 @@ and then raises.
 from __future__ import annotations
 
 import ctypes as C
-import struct
+import os
 
 import torch
 
@@ -36,10 +36,25 @@ ACTS = {"none": 0, "tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
 # 0.7 to 1.2.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
-_DTYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.uint8: 3, torch.bool: 3}
-_TENSOR = struct.Struct("=q3q3qii")  # phz_tensor, 64 bytes
-_PACK = _TENSOR.pack_into
-_SLOTS = 10
+_DTYPES = (torch.float32, torch.float64, torch.bfloat16, torch.uint8, torch.bool)
+# The entry points, in the order of phz_describe.cpp's table.
+_ENTRIES = ("phz_gated_scan", "phz_gated_scan_backward", "phz_gated_step", "phz_linear", "phz_linear_backward",
+            "phz_orthogonalize", "phz_muon_step")
+_SCAN, _SCAN_BACKWARD, _STEP, _LINEAR, _LINEAR_BACKWARD, _ORTHOGONALIZE, _MUON = range(7)
+_describe = None
+
+
+def _bound():
+    """The module that hands tensors to the library, bound to its entry points."""
+    global _describe
+    if _describe is None:
+        if not os.path.exists(os.path.join(_lib.HERE, "_describe.so")):
+            raise ImportError("phyz_amd/_describe.so is not built; run `python -m phyz_amd.build`")
+        from . import _describe as module
+        L = _lib.load()
+        module.bind(tuple(C.cast(getattr(L, name), C.c_void_p).value for name in _ENTRIES), _DTYPES)
+        _describe = module
+    return _describe
 
 
 def _current_stream(device: int) -> int:
@@ -59,15 +74,12 @@ class Ops:
 
     def __init__(self, device: int = 0):
         self._L = _lib.load()
+        self._call = _bound().call
         self.device = int(device)
         h = C.c_void_p()
         if self._L.phz_ops_create(self.device, C.byref(h)) != 0:
             raise OpsError(self._L.phz_ops_last_error(None).decode())
-        self._h = h
-        self._buf = bytearray(_SLOTS * _TENSOR.size)
-        self._keep = (C.c_char * len(self._buf)).from_buffer(self._buf)
-        base = C.addressof(self._keep)
-        self._at = [base + i * _TENSOR.size for i in range(_SLOTS)]
+        self._h = h.value
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -75,30 +87,16 @@ class Ops:
             self._L.phz_ops_destroy(h)
             self._h = None
 
-    # ── arguments ──
-    def _put(self, slot: int, t, name: str):
-        """Describes one tensor to the library; the address of its view. (The
-        common ranks are written out: this is most of a small call's time.)"""
-        if t is None:
-            return None
-        try:
-            code, n = _DTYPES[t.dtype], t.dim()
-            if t.get_device() == self.device:  # -1 is the host's
-                if n == 2:
-                    a, b = t.shape
-                    s, u = t.stride()
-                    _PACK(self._buf, slot << 6, t.data_ptr(), a, b, 0, s, u, 0, code, 2)
-                    return self._at[slot]
-                if n == 3:
-                    a, b, c = t.shape
-                    s, u, v = t.stride()
-                    _PACK(self._buf, slot << 6, t.data_ptr(), a, b, c, s, u, v, code, 3)
-                    return self._at[slot]
-                if n == 1:
-                    _PACK(self._buf, slot << 6, t.data_ptr(), t.shape[0], 0, 0, t.stride(0), 0, 0, code, 1)
-                    return self._at[slot]
-        except (AttributeError, KeyError):
-            pass
+    # ── calls ──
+    def _run(self, op: int, head: int, names: str, *tensors):
+        """One entry point on the current stream; `names` are the tensors'."""
+        rc = self._call(op, self._h, _raw_stream(self.device) if self.device >= 0 else 0, self.device, head, tensors)
+        if rc > 0:
+            raise OpsError(self._L.phz_ops_last_error(self._h).decode())
+        if rc < 0:
+            self._complain(names.split()[-1 - rc], tensors[-1 - rc])
+
+    def _complain(self, name: str, t):
         if not isinstance(t, torch.Tensor):
             raise OpsError(f"{name} has to be a torch tensor, not {type(t).__name__}")
         if t.get_device() != self.device:
@@ -114,6 +112,12 @@ class Ops:
     def _check(self, rc: int):
         if rc != 0:
             raise OpsError(self._L.phz_ops_last_error(self._h).decode())
+
+    @staticmethod
+    def _tensor(t, name: str):
+        if not isinstance(t, torch.Tensor):
+            raise OpsError(f"{name} has to be a torch tensor, not {type(t).__name__}")
+        return t
 
     @staticmethod
     def _choice(table, key, what):
@@ -139,39 +143,31 @@ class Ops:
         [worlds, width] float32, zeros if None; where reset [steps, worlds] is
         set an episode begins and h_{t-1} counts as 0."""
         f = self._choice(FORMS, form, "gate form")
-        az, ax = self._put(0, z, "z"), self._put(1, x, "x")
         if out is not None:
             h, last = out
         else:
-            h = torch.empty_like(x)
+            h = torch.empty_like(self._tensor(x, "x"))
             last = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device)
-        self._check(self._L.phz_gated_scan(self._h, self._stream(), f, az, ax, self._put(2, h0, "h0"),
-                                           self._put(3, reset, "reset"), self._put(4, h, "h"),
-                                           self._put(5, last, "h_last")))
+        self._run(_SCAN, f, "z x h0 reset h h_last", z, x, h0, reset, h, last)
         return h, last
 
     def gated_scan_backward(self, dh, z, x, h, h0=None, reset=None, dh_last=None, form: str = "sigmoid", out=None):
         """The gradients (dz, dx, dh0) of gated_scan, from those of h and of the
         last state (None: zero) and the stored h. dh0 is float32."""
         f = self._choice(FORMS, form, "gate form")
-        az, ax = self._put(0, z, "z"), self._put(1, x, "x")
         if out is not None:
             dz, dx, dh0 = out
         else:
-            dz, dx = torch.empty_like(z), torch.empty_like(x)
+            dz, dx = torch.empty_like(self._tensor(z, "z")), torch.empty_like(self._tensor(x, "x"))
             dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device)
-        self._check(self._L.phz_gated_scan_backward(
-            self._h, self._stream(), f, self._put(2, dh, "dh"), self._put(3, dh_last, "dh_last"), az, ax,
-            self._put(4, h, "h"), self._put(5, h0, "h0"), self._put(6, reset, "reset"), self._put(7, dz, "dz"),
-            self._put(8, dx, "dx"), self._put(9, dh0, "dh0")))
+        self._run(_SCAN_BACKWARD, f, "dh dh_last z x h h0 reset dz dx dh0", dh, dh_last, z, x, h, h0, reset, dz, dx, dh0)
         return dz, dx, dh0
 
     def gated_step(self, z, x, h, reset=None, form: str = "sigmoid"):
         """One step for z, x [worlds, width]: h [worlds, width] float32 is
         replaced, and returned."""
         f = self._choice(FORMS, form, "gate form")
-        self._check(self._L.phz_gated_step(self._h, self._stream(), f, self._put(0, z, "z"), self._put(1, x, "x"),
-                                           self._put(2, reset, "reset"), self._put(3, h, "h")))
+        self._run(_STEP, f, "z x reset h", z, x, reset, h)
         return h
 
     # ── the linear layer ──
@@ -184,14 +180,12 @@ class Ops:
         with save_pre, (y, x w^T + bias). All of one type, float32 or bfloat16.
         `out` (2-D) may be the residual."""
         a = self._choice(ACTS, act, "activation")
-        x2, r2 = self._rows(x), self._rows(residual)
-        ax, aw = self._put(0, x2, "x"), self._put(1, w, "w")
-        if w.dim() != 2:
+        x2, r2 = self._rows(self._tensor(x, "x")), self._rows(residual)
+        if self._tensor(w, "w").dim() != 2:
             raise OpsError(f"w has {w.dim()} dimensions, expected 2")
         y = out if out is not None else torch.empty((x2.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
         pre = torch.empty((x2.shape[0], w.shape[0]), dtype=x.dtype, device=x.device) if save_pre else None
-        self._check(self._L.phz_linear(self._h, self._stream(), a, ax, aw, self._put(2, bias, "bias"),
-                                       self._put(3, r2, "residual"), self._put(4, pre, "pre"), self._put(5, y, "y")))
+        self._run(_LINEAR, a, "x w bias residual pre y", x2, w, bias, r2, pre, y)
         shape = (*x.shape[:-1], w.shape[0])
         if out is None and x.dim() != 2:
             y = y.view(shape)
@@ -202,14 +196,12 @@ class Ops:
         """The gradients (dx, dw, db) of linear for dz = dy act'(pre); those not
         needed are None. The residual's gradient is dy itself."""
         a = self._choice(ACTS, act, "activation")
-        x2, dy2, p2 = self._rows(x), self._rows(dy), self._rows(pre)
-        ax, aw = self._put(0, x2, "x"), self._put(1, w, "w")
+        x2, dy2, p2 = self._rows(self._tensor(x, "x")), self._rows(dy), self._rows(pre)
+        self._tensor(w, "w")
         dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
         db = torch.empty(w.shape[:1], dtype=w.dtype, device=w.device) if need_db else None
-        self._check(self._L.phz_linear_backward(
-            self._h, self._stream(), a, self._put(2, dy2, "dy"), ax, aw, self._put(3, p2, "pre"),
-            self._put(4, dx, "dx"), self._put(5, dw, "dw"), self._put(6, db, "db")))
+        self._run(_LINEAR_BACKWARD, a, "dy x w pre dx dw db", dy2, x2, w, p2, dx, dw, db)
         return (dx.view(x.shape) if need_dx else None), dw, db
 
     # ── the orthogonalised update ──
@@ -222,9 +214,8 @@ class Ops:
         """Each [rows, cols] matrix of g after `steps` Newton-Schulz steps from
         g / (|g|_F + eps): nearly the orthogonal factor of g."""
         cfg = self._muon(steps, coef, eps)
-        ag = self._put(0, g, "g")
-        o = out if out is not None else torch.empty_like(g)
-        self._check(self._L.phz_orthogonalize(self._h, self._stream(), C.byref(cfg), ag, self._put(1, o, "o")))
+        o = out if out is not None else torch.empty_like(self._tensor(g, "g"))
+        self._run(_ORTHOGONALIZE, C.addressof(cfg), "g o", g, o)
         return o
 
     def muon_step(self, w, g, m, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
@@ -232,5 +223,4 @@ class Ops:
         """Muon's update of w (and the momentum m, both float32, in place) for
         the gradient g: matrices [rows, cols], or a batch of them."""
         cfg = self._muon(steps, coef, eps, lr, momentum, nesterov, weight_decay)
-        self._check(self._L.phz_muon_step(self._h, self._stream(), C.byref(cfg), self._put(0, w, "w"),
-                                          self._put(1, g, "g"), self._put(2, m, "m")))
+        self._run(_MUON, C.addressof(cfg), "w g m", w, g, m)
