@@ -336,6 +336,7 @@ template <class T, int PL> struct Tiles {
   typedef Tile<128, 128, 64, 2, 2, 2, 2> Mid;
   typedef Tile<64, 64, 64, 4, 2, 2, 2> Deep;   // one a compute unit
   typedef Tile<64, 64, 64, 2, 2, 2, 2> Small;  // two
+  typedef Tile<128, 128, 64, 2, 2, 2> Two;     // two
 };
 template <> struct Tiles<bf16, 3> {
   typedef Tile<256, 128, 96, 2, 4, 2> Big;
@@ -351,7 +352,7 @@ template <> struct Tiles<float, 1> {
 enum { PLANES_F32 = 0 };  // plan_fast's name for f32 operands as they are
 
 struct FastPlan {
-  int tile;  // 0 big, 1 mid, 2 deep, 3 small
+  int tile;  // 0 big, 1 mid, 2 deep, 3 small, 4 two
   int32_t splits, k_split;
   uint64_t part_bytes;  // workspace for the splits' sums
 };
@@ -360,15 +361,17 @@ struct FastPlan {
 // stages of a workgroup's contraction at the tile's measured time, and for a
 // split contraction the sums' way through memory. One MI355X, bf16, us:
 //
-//                         256x256  128x128  64x64 deep  64x64 small  library
-//   8192 x 8192 x 8192    903      1023     .           .            860
-//   4096 x 4096 x 1024    36.7     38.3     .           .            29.8
-//   2048 x 2048 x 2048    51.6     23.9     42.9        30.3         21.9
-//   1024 x 4096 x 1024    28.1     14.2     25.4        18.4         14.0
-//   1500 x 1000 x 3000    78.1     36.8     31.3        26.6         26.6
-//   1024 x 1024 x 4096    91.2     36.5     21.1        26.3         19.3
-//   512 x 512 x 2048      47.4     19.2     10.9        10.8         7.4
-//   4096 x 256 x 256      11.0     6.1      4.4         4.3          6.1
+//                         256x256  128x128  128x128g2  64x64g2  64x64g2  library
+//                         one a CU two      one        one      two
+//   8192 x 8192 x 8192    903      1023     .          .        .        860
+//   4096 x 4096 x 1024    36.7     38.3     .          .        .        29.8
+//   8192 x 1000 x 1000    .        24.2     28.1       51.4     40.7     .
+//   2048 x 2048 x 2048    51.6     24.6     21.9       36.6     28.6     21.9
+//   1024 x 4096 x 1024    28.1     13.4     12.9       21.7     16.6     14.0
+//   1024 x 1024 x 4096    91.2     40.8     33.8       17.8     23.0     19.3
+//   1024 x 1024 x 1024    27.1     11.6     11.1       6.4      6.4      8.3
+//   512 x 512 x 2048      47.4     .        19.2       10.9     10.8     7.4
+//   4096 x 256 x 256      11.0     .        6.1        4.4      4.3      6.1
 //
 // Large tiles read LDS and L2 least for each product and win where there are
 // enough of them; below, what counts is that every compute unit has one. f32
@@ -376,22 +379,28 @@ struct FastPlan {
 // (4096 x 2048 x 2048: 64x64 four a CU 265, 128x128 273; 1024 x 1024 x 1024:
 // 64x64g2 21, 128x128 66).
 inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int64_t batch, int planes, bool may_split) {
-  struct Kind { int bm, bn, per_cu; double stage; };
-  // Time of a stage of 64 (of 32 for two and three planes) with the chip full.
-  const Kind one[4] = {{256, 256, 1, 1.7}, {128, 128, 1, 0.65}, {64, 64, 1, 0.29}, {64, 64, 2, 0.43}};
-  const Kind three[4] = {{256, 128, 1, 2.8}, {128, 128, 1, 1.5}, {64, 64, 1, 0.45}, {64, 64, 2, 0.8}};
-  const Kind f32[4] = {{}, {}, {64, 64, 1, 0.57}, {64, 64, 4, 2.0}};
+  // Time of a stage of 64 (of 32 for two and three planes, and for f32) with
+  // one workgroup a compute unit, and with all that fit.
+  struct Kind { int bm, bn, per_cu; double alone, full; };
+  const Kind one[5] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 1, 0.6, 0.6}, {64, 64, 1, 0.24, 0.24}, {64, 64, 2, 0.32, 0.42},
+                       {128, 128, 2, 0.68, 1.3}};
+  const Kind three[4] = {{256, 128, 1, 2.8, 2.8}, {128, 128, 1, 1.5, 1.5}, {64, 64, 1, 0.45, 0.45}, {64, 64, 2, 0.6, 0.8}};
+  const Kind f32[4] = {{}, {}, {64, 64, 1, 0.57, 0.57}, {64, 64, 4, 0.6, 2.0}};
   const Kind* kinds = planes == 3 ? three : planes == PLANES_F32 ? f32 : one;
   const int64_t sk = planes == 1 ? 64 : 32, stages = std::max<int64_t>(1, ceil_div(k, sk));
   FastPlan best{};
   double least = 1e30;
-  for (int t = planes == PLANES_F32 ? 2 : 0; t < 4; t++) {
-    const int64_t tiles = ceil_div(m, kinds[t].bm) * ceil_div(n, kinds[t].bn) * batch;
+  for (int t = planes == PLANES_F32 ? 2 : 0; t < (kinds == one ? 5 : 4); t++) {
+    const Kind& kind = kinds[t];
+    const int64_t tiles = ceil_div(m, kind.bm) * ceil_div(n, kind.bn) * batch;
     for (int64_t splits = 1; splits <= (may_split ? 64 : 1); splits *= 2) {
       if (splits > 1 && stages < 8 * splits) break;
-      const int64_t rounds = ceil_div(tiles * splits, (int64_t)o->cus * kinds[t].per_cu);
-      double us = rounds * (3.0 + ceil_div(stages, splits) * kinds[t].stage);
-      if (splits > 1) us += 4.0 + (2.0 * splits + 1) * m * n * batch * 4 / 4e6;
+      const int64_t rounds = ceil_div(tiles * splits, (int64_t)o->cus * kind.per_cu);
+      const int64_t beside = std::min<int64_t>(kind.per_cu, ceil_div(tiles * splits, o->cus));
+      const double stage =
+          kind.per_cu == 1 ? kind.full : kind.alone + (kind.full - kind.alone) * (beside - 1) / (kind.per_cu - 1);
+      double us = rounds * (3.0 + ceil_div(stages, splits) * stage);
+      if (splits > 1) us += 3.0 + 0.1 * splits + (2.0 * splits + 1) * m * n * batch * 4 / 8e6;  // sums stay in the caches
       if (us < least) {
         least = us;
         best.tile = t;
@@ -421,28 +430,45 @@ struct PartOut : NothingAhead {
   }
 };
 
-// The splits' sums, added in order, to the epilogue.
+// The splits' sums to the epilogue, added in a fixed order: four threads for
+// eight elements, each every fourth split.
 template <class Epi>
 __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_t m, int32_t n, Epi epi) {
+  __shared__ float s[3][64][9];
   const uint32_t per = (n + 7) / 8;
-  const int q = blockIdx.y;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)m * per; t += (int64_t)gridDim.x * 256) {
-    const int i = (int)(t / per), j = (int)(t - (int64_t)i * per) * 8;
+  const int q = blockIdx.y, unit = threadIdx.x & 63, lane = threadIdx.x >> 6;
+  for (int64_t t0 = (int64_t)blockIdx.x * 64; t0 < (int64_t)m * per; t0 += (int64_t)gridDim.x * 64) {
+    const int64_t t = t0 + unit;
+    const bool live = t < (int64_t)m * per;
+    const int i = live ? (int)(t / per) : 0, j = live ? (int)(t - (int64_t)i * per) * 8 : 0;
     const float* at = p.part + q * p.batch + i * p.row + j;
     typename Epi::Held held;
     typename Epi::Columns columns;
-    if (j + 8 <= n) epi.fetch(q, i, j, held), epi.columns(j, columns);
+    if (live && lane == 0 && j + 8 <= n) epi.fetch(q, i, j, held), epi.columns(j, columns);
     float v[8];
-    *(f32x4*)v = *(const f32x4*)at;
-    *(f32x4*)(v + 4) = *(const f32x4*)(at + 4);
-    for (int s = 1; s < splits; s++) {
-      const f32x4 lo = *(const f32x4*)(at + s * p.split), hi = *(const f32x4*)(at + s * p.split + 4);
+#pragma unroll
+    for (int c = 0; c < 8; c++) v[c] = 0.0f;
+#pragma unroll 4
+    for (int k = lane; k < splits; k += 4) {
+      const f32x4 lo = *(const f32x4*)(at + k * p.split), hi = *(const f32x4*)(at + k * p.split + 4);
 #pragma unroll
       for (int c = 0; c < 4; c++) v[c] += lo[c], v[4 + c] += hi[c];
     }
-    if (j + 8 <= n) epi.put8(q, 0, i, j, v, held, columns);
-    else
-      for (int c = 0; c < 8 && j + c < n; c++) epi.put1(q, 0, i, j + c, v[c]);
+    if (lane) {
+#pragma unroll
+      for (int c = 0; c < 8; c++) s[lane - 1][unit][c] = v[c];
+    }
+    __syncthreads();
+    if (lane == 0 && live) {
+#pragma unroll
+      for (int l = 0; l < 3; l++)
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[c] += s[l][unit][c];
+      if (j + 8 <= n) epi.put8(q, 0, i, j, v, held, columns);
+      else
+        for (int c = 0; c < 8 && j + c < n; c++) epi.put1(q, 0, i, j + c, v[c]);
+    }
+    __syncthreads();
   }
 }
 
@@ -469,10 +495,13 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
     if (plan.tile == 0) go(typename Tiles<T, PL>::Big{});
     if (plan.tile == 1) go(typename Tiles<T, PL>::Mid{});
   }
+  if constexpr (sizeof(T) == 2 && PL < 3) {
+    if (plan.tile == 4) go(typename Tiles<T, PL>::Two{});
+  }
   if (plan.tile == 2) go(typename Tiles<T, PL>::Deep{});
   if (plan.tile == 3) go(typename Tiles<T, PL>::Small{});
   if (p.splits > 1) {
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 256), 4096);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 64), 8192);
     hipLaunchKernelGGL(join_kernel<Epi>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, sums, p.splits, p.m, p.n,
                        epi);
   }

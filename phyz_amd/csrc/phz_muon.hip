@@ -406,7 +406,7 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
   const Planes a{h + 4 * batch * xn, an, s8, P * an}, p{h + (4 * xn + P * an) * batch, an, s8, P * an};
   const double sx = f16_scale(top.x), sa = f16_scale(top.a), sp = f16_scale(top.p > 0 ? top.p : 1.0);
   hipLaunchKernelGGL(norm_kernel<G>, dim3(parts, (unsigned)batch), dim3(256), 0, stream, src, part, rows, cols);
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 2048), 2048);
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 4096), 1024);
   hipLaunchKernelGGL(scale_kernel<G>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, src, part, parts, cfg.eps,
                      (float)sx, x, nullptr, rows, cols);
   for (int k = 0; k < cfg.steps; k++) {
