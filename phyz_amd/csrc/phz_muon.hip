@@ -310,8 +310,11 @@ Bounds bounds(const phz_muon_cfg& g) {
     m.p = std::max(m.p, fabs(t * (g.b + g.c * t)));
     if (g.c != 0.0 && -g.b / (2 * g.c) > 0 && -g.b / (2 * g.c) < t) m.p = std::max(m.p, g.b * g.b / fabs(4 * g.c));
     top = quintic_top(g.a, g.b, g.c, top) * 1.001;
+    if (!(top < 1e30)) {  // or NaN
+      m.x = INFINITY;
+      break;
+    }
     m.x = std::max(m.x, top);
-    if (!(m.x < 1e30)) break;
   }
   return m;
 }

@@ -211,6 +211,28 @@ def test_infinite_inputs_of_large_products(ops, dtype):
     assert torch.equal(dx, dxc) and torch.equal(dw, dwc)
 
 
+def test_f32_in_pieces(ops):
+    """Large enough to be cut into bf16 pieces: within the bounds of f32, and an
+    infinite input reaches its own row alone, with its sign."""
+    m, k, n = 4100, 2056, 1032
+    d = data(m, k, n, F32, seed=8)
+    y = ops.linear(d["x"], d["w"], bias=d["bias"], act="silu")
+    wy, _, by, _ = R.linear(d["x"], d["w"], d["bias"], None, "silu", F32)
+    R.within(y, wy, by, "y")
+    got = ops.linear_backward(d["dy"], d["x"], d["w"], pre=d["pre"], act="gelu")
+    want, bounds = R.linear_backward(d["dy"], d["x"], d["w"], d["pre"], "gelu", F32)
+    for name, a, b, c in zip(("dx", "dw", "db"), got, want, bounds):
+        R.within(a, b, c, name)
+    plain = ops.linear(d["x"], d["w"])
+    x = d["x"].clone()
+    x[17, 2000] = float("-inf")
+    x[4099, 1] = float("nan")
+    y = ops.linear(x, d["w"])
+    assert torch.equal(y[17], torch.sign(d["w"][:, 2000]) * float("-inf")) and torch.isnan(y[4099]).all()
+    y[17], y[4099] = plain[17], plain[4099]
+    assert torch.equal(y, plain)
+
+
 def test_wide_range_in_f32(ops):
     """f32 operands keep their range and all 24 bits: magnitudes from 2^-60 to
     2^60 in one product."""

@@ -77,6 +77,16 @@ def test_steps_and_coefficients(ops, steps):
         assert off(o, R.orthogonalize(g, steps, coef, 1e-3)) <= TOL[F32]
 
 
+def test_coefficients_beyond_f16(ops):
+    """Steps that raise every singular value a hundredfold: the iterates leave
+    f16's range and the f32 products take over. a X alone is exact to a few U;
+    its error here is that of one rounding a step."""
+    for shape in ((40, 72), (72, 40), (200, 150)):
+        g = matrices(2, *shape, F32)
+        o = ops.orthogonalize(g, steps=4, coef=(100.0, 0.0, 0.0))
+        assert off(o, R.orthogonalize(g, 4, (100.0, 0.0, 0.0))) <= TOL[F32]
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-18, 1e12, 1e30])
 def test_any_magnitude(ops, scale):
     """The norm's squares leave f32's range; the result does not depend on it."""
