@@ -430,14 +430,22 @@ struct PartOut : NothingAhead {
   }
 };
 
+// What a join's first blocks may do beside it, to save a launch.
+struct NothingBeside {
+  static constexpr unsigned blocks = 0;
+  __device__ __forceinline__ void run(unsigned) const {}
+};
+
 // The splits' sums to the epilogue, added in a fixed order: four threads for
 // eight elements, each every fourth split.
-template <class Epi>
-__global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_t m, int32_t n, Epi epi) {
+template <class Epi, class Beside>
+__global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_t m, int32_t n, Epi epi, Beside beside) {
+  if (blockIdx.x < beside.blocks) return beside.run(blockIdx.x);
   __shared__ float s[3][64][9];
   const uint32_t per = (n + 7) / 8;
   const int q = blockIdx.y, unit = threadIdx.x & 63, lane = threadIdx.x >> 6;
-  for (int64_t t0 = (int64_t)blockIdx.x * 64; t0 < (int64_t)m * per; t0 += (int64_t)gridDim.x * 64) {
+  const int64_t stride = (int64_t)(gridDim.x - beside.blocks) * 64;
+  for (int64_t t0 = (int64_t)(blockIdx.x - beside.blocks) * 64; t0 < (int64_t)m * per; t0 += stride) {
     const int64_t t = t0 + unit;
     const bool live = t < (int64_t)m * per;
     const int i = live ? (int)(t / per) : 0, j = live ? (int)(t - (int64_t)i * per) * 8 : 0;
@@ -472,10 +480,11 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
   }
 }
 
-// `part`: plan.part_bytes of workspace.
-template <class T, int PL, bool AK, bool BKD, class Epi>
+// `part`: plan.part_bytes of workspace. `beside` goes with the join: to plans
+// with splits, and one matrix, only.
+template <class T, int PL, bool AK, bool BKD, class Epi, class Beside = NothingBeside>
 void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batch, const FastPlan& plan, float* part,
-                      const Epi& epi) {
+                      const Epi& epi, const Beside& beside = {}) {
   p.zeros = (const char*)o->zeros;
   p.splits = plan.splits;
   p.k_split = plan.k_split;
@@ -502,8 +511,8 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
   if (plan.tile == 3) go(typename Tiles<T, PL>::Small{});
   if (p.splits > 1) {
     const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 64), 8192);
-    hipLaunchKernelGGL(join_kernel<Epi>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, sums, p.splits, p.m, p.n,
-                       epi);
+    hipLaunchKernelGGL((join_kernel<Epi, Beside>), dim3(beside.blocks + blocks, (unsigned)batch), dim3(256), 0, stream, sums,
+                       p.splits, p.m, p.n, epi, beside);
   }
 }
 

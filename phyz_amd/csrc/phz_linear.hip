@@ -12,8 +12,8 @@ namespace {
 // ── activations ─────────────────────────────────────────────────────────────
 
 // tanh(p) = 1 - 2 / (1 + exp(2 p)), and where that cancels (|p| < 0.3) its
-// series to p^9, whose next term is below 1e-8 of it. ocml's tanhf is as exact
-// and took 60 us more over 134 million elements.
+// series to p^9, whose next term is 1382/155925 p^10 < 6e-8 of it. The device
+// library's took 60 us more over 134 million elements.
 __device__ __forceinline__ float tanh_of(float p) {
   const float s = p * p;
   const float small = p * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
@@ -313,32 +313,6 @@ void launch_few_rows(const phz_ops* o, hipStream_t stream, const phz_tensor* x, 
   else wide ? go(few_rows<E, 2, 2, Epi>, 32) : go(few_rows<E, 2, 1, Epi>, 16);
 }
 
-// y[i][j] = the splits' sums, added in a fixed order: eight threads an element,
-// each every eighth split.
-template <class E>
-__global__ __launch_bounds__(256) void join_splits(const float* part, int splits, int64_t split, E* y, int64_t row,
-                                                   int32_t n, int64_t total) {
-  __shared__ float s[8][32];
-  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  for (int64_t t0 = (int64_t)blockIdx.x * 32; t0 < total; t0 += (int64_t)gridDim.x * 32) {
-    const int64_t t = t0 + c;
-    float v = 0.0f;
-    if (t < total) {
-#pragma unroll 8
-      for (int k = lane; k < splits; k += 8) v += part[k * split + t];
-    }
-    s[lane][c] = v;
-    __syncthreads();
-    if (lane == 0 && t < total) {
-#pragma unroll
-      for (int l = 1; l < 8; l++) v += s[l][c];
-      const int64_t i = t / n;
-      y[i * row + (t - i * n)] = from_f32<E>(v);
-    }
-    __syncthreads();
-  }
-}
-
 // Eight f32 as three planes of bf16.
 __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v) {
   Pack<bf16, 8> h, m, l;
@@ -351,7 +325,7 @@ __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v)
 
 // dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
 // rows of `dz_row` with zeros past n, or cut into three planes of such rows, and the sums of dz over each block's rows,
-// which column_sums adds up in order. A thread takes eight columns; `across`
+// which ColumnSums adds up in order. A thread takes eight columns; `across`
 // (a power of two, at most 32) of them lie along a row, the others take rows in
 // turn.
 template <class E>
@@ -414,22 +388,60 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
   }
 }
 
-// Eight threads a column, each every eighth block's sum.
+// db from the blocks' sums of dz: eight columns a workgroup, 32 threads a
+// column, each every 32nd block's sum.
 template <class E>
-__global__ __launch_bounds__(256) void column_sums(const float* sums, int32_t blocks, int32_t n, E* db, int64_t step) {
-  __shared__ float s[8][32];
-  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5, j = blockIdx.x * 32 + c;
-  float v = 0.0f;
-  if (j < n) {
+struct ColumnSums {
+  const float* sums;
+  E* db;
+  int64_t step;
+  int32_t parts, n;
+  unsigned blocks;  // workgroups, 0 where there is no db
+  __device__ __forceinline__ void run(unsigned block) const {
+    __shared__ float s[4][8];
+    const int c = threadIdx.x & 7, j = block * 8 + c;
+    float v = 0.0f;
+    if (j < n) {
 #pragma unroll 8
-    for (int i = lane; i < blocks; i += 8) v += sums[(int64_t)i * n + j];
-  }
-  s[lane][c] = v;
-  __syncthreads();
-  if (lane == 0 && j < n) {
+      for (int i = threadIdx.x >> 3; i < parts; i += 32) v += sums[(int64_t)i * n + j];
+    }
 #pragma unroll
-    for (int l = 1; l < 8; l++) v += s[l][c];
-    db[j * step] = from_f32<E>(v);
+    for (int k = 8; k < 64; k *= 2) v += __shfl_xor(v, k);
+    if ((threadIdx.x & 63) < 8) s[threadIdx.x >> 6][c] = v;
+    __syncthreads();
+    if (threadIdx.x < 8 && j < n) db[j * step] = from_f32<E>((s[0][c] + s[1][c]) + (s[2][c] + s[3][c]));
+  }
+};
+template <class E>
+__global__ __launch_bounds__(256) void column_sums(ColumnSums<E> c) {
+  c.run(blockIdx.x);
+}
+
+// y[i][j] = the splits' sums, added in a fixed order: eight threads an element,
+// each every eighth split.
+template <class E>
+__global__ __launch_bounds__(256) void join_splits(const float* part, int splits, int64_t split, E* y, int64_t row,
+                                                   int32_t n, int64_t total, ColumnSums<E> beside) {
+  if (blockIdx.x < beside.blocks) return beside.run(blockIdx.x);
+  __shared__ float s[8][32];
+  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const int64_t stride = (int64_t)(gridDim.x - beside.blocks) * 32;
+  for (int64_t t0 = (int64_t)(blockIdx.x - beside.blocks) * 32; t0 < total; t0 += stride) {
+    const int64_t t = t0 + c;
+    float v = 0.0f;
+    if (t < total) {
+#pragma unroll 8
+      for (int k = lane; k < splits; k += 8) v += part[k * split + t];
+    }
+    s[lane][c] = v;
+    __syncthreads();
+    if (lane == 0 && t < total) {
+#pragma unroll
+      for (int l = 1; l < 8; l++) v += s[l][c];
+      const int64_t i = t / n;
+      y[i * row + (t - i * n)] = from_f32<E>(v);
+    }
+    __syncthreads();
   }
 }
 
@@ -547,9 +559,9 @@ FastPlan plan(const phz_ops* o, Way way, int64_t m, int64_t n, int64_t k) {
 
 // The product of two operands, C of m x n, contraction k; AK, BK: dense along
 // it. Epilogues of cut products are repaired where sums are not finite.
-template <class E, bool AK, bool BK, class Epi>
+template <class E, bool AK, bool BK, class Epi, class Beside = NothingBeside>
 void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<E>& b, int64_t m, int64_t n, int64_t k,
-             const FastPlan& plan, float* part, const Epi& epi) {
+             const FastPlan& plan, float* part, const Epi& epi, const Beside& beside = {}) {
   const int64_t e = a.way == CUT ? 2 : sizeof(E);
   FastArgs f{};
   f.a = (const char*)a.data(), f.b = (const char*)b.data(), f.a_row = a.row() * e, f.b_row = b.row() * e;
@@ -560,10 +572,10 @@ void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<
     if (a.way == CUT) {
       const Repair<Epi> safe{epi, (const bf16*)a.data(), (const bf16*)b.data(), AK ? a.row() : 1, AK ? 1 : a.row(),
                              a.plane(), BK ? b.row() : 1, BK ? 1 : b.row(), b.plane(), (int32_t)k};
-      return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, safe);
+      return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, safe, beside);
     }
   }
-  launch_gemm_fast<E, 1, AK, BK>(o, stream, f, 1, plan, part, epi);
+  launch_gemm_fast<E, 1, AK, BK>(o, stream, f, 1, plan, part, epi, beside);
 }
 
 template <class E>
@@ -628,8 +640,12 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
     splits = (int32_t)ceil_div(m, k_split);
   }
   const bool lay_d = (need_dx || need_dw) && (fast ? !d.well : act != PHZ_ACT_NONE);
-  // Blocks of rows whose sums of dz are added up in the end, at most 256.
-  const int64_t rows = std::max<int64_t>(32, ceil_div(ceil_div(m, 256), 8) * 8), blocks = ceil_div(m, rows);
+  // Blocks of rows whose sums of dz are added up in the end: four workgroups a
+  // compute unit in all, 64 to 512 blocks of at least 16 rows.
+  int across = 32;
+  while (across > 1 && across * 4 >= n) across /= 2;
+  const int64_t wanted = std::min<int64_t>(512, std::max<int64_t>(64, 4 * o->cus / ceil_div(n, across * 8)));
+  const int64_t rows = std::max<int64_t>(16, ceil_div(ceil_div(m, wanted), 8) * 8), blocks = ceil_div(m, rows);
 
   Carve c;
   float *sums = nullptr, *part = nullptr;
@@ -643,15 +659,15 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
     if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
   }
   if (m > 0 && (lay_d || db)) {
-    int across = 32;
-    while (across > 1 && across * 4 >= n) across /= 2;
     hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, across * 8), (unsigned)blocks), dim3(256), 0, stream, act,
                        (const E*)dy->data, dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0,
                        (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(), pad8(n), sums, (int32_t)m, (int32_t)n, (int32_t)rows, across);
   }
-  if (db)
-    hipLaunchKernelGGL(column_sums<E>, dim3((unsigned)ceil_div(n, 32)), dim3(256), 0, stream, sums, (int32_t)blocks,
-                       (int32_t)n, (E*)db->data, db->stride[0]);
+  // db goes with the join of dw's splits where there is one.
+  const ColumnSums<E> bias{sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)blocks, (int32_t)n,
+                           db ? (unsigned)ceil_div(n, 8) : 0u};
+  const bool joined = need_dw && (fast ? dw_plan.splits : splits) > 1;
+  if (db && !joined) hipLaunchKernelGGL(column_sums<E>, dim3(bias.blocks), dim3(256), 0, stream, bias);
   if (fast) {
     if (need_dx) {
       wo.lay(stream);
@@ -659,7 +675,7 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
     }
     if (need_dw) {
       xo.lay(stream);
-      product<E, false, false>(o, stream, d, xo, n, k, m, dw_plan, part, PlainOut<E>{(E*)dw->data, dw->stride[0]});
+      product<E, false, false>(o, stream, d, xo, n, k, m, dw_plan, part, PlainOut<E>{(E*)dw->data, dw->stride[0]}, bias);
     }
   } else {
     const int32_t mi = (int32_t)m, ni = (int32_t)n, ki = (int32_t)k;
@@ -674,8 +690,8 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
         launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, PlainOut<E>{(E*)dw->data, dw->stride[0]});
       } else {
         launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, SplitOut{part, k, n * k});
-        hipLaunchKernelGGL(join_splits<E>, dim3((unsigned)std::min<int64_t>(ceil_div(n * k, 32), 8192)), dim3(256), 0,
-                           stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k);
+        hipLaunchKernelGGL(join_splits<E>, dim3(bias.blocks + (unsigned)std::min<int64_t>(ceil_div(n * k, 32), 8192)),
+                           dim3(256), 0, stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k, bias);
       }
     }
   }

@@ -24,14 +24,12 @@ struct View {
 int norm_blocks(int64_t elements) { return (int)std::max<int64_t>(1, std::min<int64_t>(512, elements / 4096)); }
 
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double s[256];
-  s[threadIdx.x] = v;
+  __shared__ double s[4];
+#pragma unroll
+  for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  for (int k = 128; k; k >>= 1) {
-    if (threadIdx.x < k) s[threadIdx.x] += s[threadIdx.x + k];
-    __syncthreads();
-  }
-  return s[0];
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // Eight neighbouring elements of a row (fewer at its end: zeros).
@@ -153,13 +151,13 @@ template <class E>
 __global__ __launch_bounds__(256) void scale_kernel(Source<E> s, const double* part, int parts, double eps, float scale,
                                                     Planes x, float* xf, int32_t rows, int32_t cols) {
   const int q = blockIdx.y;
-  const double inv = inverse_norm(part, parts, q, eps) * scale;
   const uint32_t per = (cols + 7) / 8, n = (uint32_t)rows * per;
-  for (uint32_t t = blockIdx.x * 256 + threadIdx.x; t < n; t += gridDim.x * 256) {
-    const uint32_t i = t / per;
-    const int j = (t - i * per) * 8;
-    float v[8];
-    s.at(q, i, j, cols, v);
+  uint32_t t = blockIdx.x * 256 + threadIdx.x, i = t / per;
+  int j = (t - i * per) * 8;
+  float v[8];
+  if (t < n) s.at(q, i, j, cols, v);  // on its way during the norm's sum
+  const double inv = inverse_norm(part, parts, q, eps) * scale;
+  while (t < n) {
 #pragma unroll
     for (int c = 0; c < 8; c++) v[c] = (float)(v[c] * inv);
     if (xf) {
@@ -169,6 +167,9 @@ __global__ __launch_bounds__(256) void scale_kernel(Source<E> s, const double* p
     } else {
       put_planes<2>(x, q * x.batch + i * x.row + j, v);
     }
+    t += gridDim.x * 256;
+    i = t / per, j = (t - i * per) * 8;
+    if (t < n) s.at(q, i, j, cols, v);
   }
 }
 
@@ -409,7 +410,7 @@ int newton_schulz(phz_ops* o, hipStream_t stream, const phz_muon_cfg& cfg, const
   const Planes a{h + 4 * batch * xn, an, s8, P * an}, p{h + (4 * xn + P * an) * batch, an, s8, P * an};
   const double sx = f16_scale(top.x), sa = f16_scale(top.a), sp = f16_scale(top.p > 0 ? top.p : 1.0);
   hipLaunchKernelGGL(norm_kernel<G>, dim3(parts, (unsigned)batch), dim3(256), 0, stream, src, part, rows, cols);
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 4096), 1024);
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)rows * c8, 2048), 1024);
   hipLaunchKernelGGL(scale_kernel<G>, dim3(blocks, (unsigned)batch), dim3(256), 0, stream, src, part, parts, cfg.eps,
                      (float)sx, x, nullptr, rows, cols);
   for (int k = 0; k < cfg.steps; k++) {
