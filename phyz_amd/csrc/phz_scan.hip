@@ -51,10 +51,13 @@ struct ScanArgs {
 // A span in which an episode begins keeps nothing of the state before it, be
 // that infinite or NaN: its A is this NaN, and stands for "forget", which a
 // product that underflows to 0 does not. (A gate that is NaN makes H NaN, so
-// no other NaN in A matters.)
+// no other NaN in A matters.) A state of 0 passes a span as 0 although gates
+// above 1 may take A past f32's range.
 constexpr uint32_t kForget = 0x7fc5a5a5u;
 __device__ __forceinline__ bool forgets(float a) { return __builtin_bit_cast(uint32_t, a) == kForget; }
-__device__ __forceinline__ float compose(float a, float s, float h) { return forgets(a) ? h : fmaf(a, s, h); }
+__device__ __forceinline__ float compose(float a, float s, float h) {
+  return forgets(a) || s == 0.0f ? h : fmaf(a, s, h);
+}
 
 // One step's affine map and outputs. `s` is h (forward) or k (backward).
 template <int FORM>
@@ -112,6 +115,7 @@ struct Run {
 
 template <class E, int FORM, bool BACK, int VEC, int NW, int U, bool AGG>
 __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p) {
+  static_assert(NW > 1 || !AGG, "chunks are of several waves");
   using S = Step<FORM>;
   // What a chunk's map needs: forward z, x; backward z and dh only.
   constexpr bool kNeedX = BACK ? (FORM == PHZ_GATE_SIGMOID && !AGG) : true;
@@ -209,12 +213,12 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
       return S::next(rst ? 0.0f : st, q[u][v], to_f32(cur.x[kNeedX ? u : 0].v[v]));
     };
 
-    if (AGG || NW > 1) {
-      // Compose this wave's run (onto the chunk's so far, where a wave works alone).
+    if constexpr (NW > 1) {
+      // Compose this wave's run.
       float A[VEC], H[VEC];
       bool forget = false;
 #pragma unroll
-      for (int v = 0; v < VEC; v++) A[v] = NW > 1 ? 1.0f : prod[v], H[v] = NW > 1 ? 0.0f : s[v];
+      for (int v = 0; v < VEC; v++) A[v] = 1.0f, H[v] = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; u++)
         if (base + u < last) {
@@ -226,74 +230,68 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
           }
           forget = forget || rst;
         }
-      if (NW > 1) {
-        float* mine = lds + buf * (NW * 2 * VEC * kWaveLanes);
+      float* mine = lds + buf * (NW * 2 * VEC * kWaveLanes);
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        mine[(wave * 2 * kWaveLanes + lane) * VEC + v] = forget ? __builtin_bit_cast(float, kForget) : A[v];
+        mine[((wave * 2 + 1) * kWaveLanes + lane) * VEC + v] = H[v];
+      }
+      __syncthreads();
+      // Fold every run of the slab in order; keep the state before this
+      // wave's own.
+      float before[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; v++) before[v] = s[v];
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        if (w == wave) {
+#pragma unroll
+          for (int v = 0; v < VEC; v++) before[v] = s[v];
+        }
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
-          mine[(wave * 2 * kWaveLanes + lane) * VEC + v] = forget ? __builtin_bit_cast(float, kForget) : A[v];
-          mine[((wave * 2 + 1) * kWaveLanes + lane) * VEC + v] = H[v];
-        }
-        __syncthreads();
-        // Fold every run of the slab in order; keep the state before this
-        // wave's own.
-        float before[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; v++) before[v] = s[v];
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-          if (w == wave) {
-#pragma unroll
-            for (int v = 0; v < VEC; v++) before[v] = s[v];
-          }
-#pragma unroll
-          for (int v = 0; v < VEC; v++) {
-            const float a = mine[(w * 2 * kWaveLanes + lane) * VEC + v];
-            const float g = mine[((w * 2 + 1) * kWaveLanes + lane) * VEC + v];
-            s[v] = compose(a, s[v], g);
-            if (AGG) {
-              forgot = forgot || forgets(a);
-              prod[v] *= a;
-            }
+          const float a = mine[(w * 2 * kWaveLanes + lane) * VEC + v];
+          const float g = mine[((w * 2 + 1) * kWaveLanes + lane) * VEC + v];
+          s[v] = compose(a, s[v], g);
+          if (AGG) {
+            forgot = forgot || forgets(a);
+            prod[v] *= a;
           }
         }
-        if (!AGG) {
-          // The outputs, from the state before the run; s stays the slab's end.
-#pragma unroll
-          for (int u = 0; u < U; u++)
-            if (base + u < last) {
-              const int64_t t = step_of(base + u);
-              const bool rst = (reset >> u) & 1u;
-              if (BACK) {
-                float dz[VEC], dx[VEC];
-#pragma unroll
-                for (int v = 0; v < VEC; v++) {
-                  const float e = to_f32(cur.a[u].v[v]) + before[v];
-                  float hp = 0.0f;
-                  if (!rst) {
-                    if (t > 0) hp = to_f32(cur.hp[kNeedH ? u : 0].v[v]);
-                    else if (p.h0) hp = p.h0[b * p.h0_b + d + v];
-                  }
-                  dz[v] = S::dz(e, hp, kNeedX ? to_f32(cur.x[kNeedX ? u : 0].v[v]) : 0.0f, q[u][v]);
-                  dx[v] = S::write(q[u][v]) * e;
-                  before[v] = rst ? 0.0f : S::keep(q[u][v]) * e;
-                }
-                if (live) {
-                  store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, dz);
-                  store<E, VEC>(p.o2, b * p.o2_b + d + t * p.o2_t, dx);
-                }
-              } else {
-#pragma unroll
-                for (int v = 0; v < VEC; v++) before[v] = advance(before[v], u, v, rst);
-                if (live) store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, before);
-              }
-            }
-        }
-        buf ^= 1;
-      } else {
-#pragma unroll
-        for (int v = 0; v < VEC; v++) prod[v] = A[v], s[v] = H[v];
-        forgot = forgot || forget;
       }
+      if (!AGG) {
+        // The outputs, from the state before the run; s stays the slab's end.
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (base + u < last) {
+            const int64_t t = step_of(base + u);
+            const bool rst = (reset >> u) & 1u;
+            if (BACK) {
+              float dz[VEC], dx[VEC];
+#pragma unroll
+              for (int v = 0; v < VEC; v++) {
+                const float e = to_f32(cur.a[u].v[v]) + before[v];
+                float hp = 0.0f;
+                if (!rst) {
+                  if (t > 0) hp = to_f32(cur.hp[kNeedH ? u : 0].v[v]);
+                  else if (p.h0) hp = p.h0[b * p.h0_b + d + v];
+                }
+                dz[v] = S::dz(e, hp, kNeedX ? to_f32(cur.x[kNeedX ? u : 0].v[v]) : 0.0f, q[u][v]);
+                dx[v] = S::write(q[u][v]) * e;
+                before[v] = rst ? 0.0f : S::keep(q[u][v]) * e;
+              }
+              if (live) {
+                store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, dz);
+                store<E, VEC>(p.o2, b * p.o2_b + d + t * p.o2_t, dx);
+              }
+            } else {
+#pragma unroll
+              for (int v = 0; v < VEC; v++) before[v] = advance(before[v], u, v, rst);
+              if (live) store<E, VEC>(p.o1, b * p.o1_b + d + t * p.o1_t, before);
+            }
+          }
+      }
+      buf ^= 1;
     } else {
 #pragma unroll
       for (int u = 0; u < U; u++)
@@ -479,7 +477,8 @@ bool check_type(phz_ops* o, const char* name, const phz_tensor* t) {
 bool check_limits(phz_ops* o, int64_t steps, int64_t worlds, int64_t width) {
   if (steps > 0x7fff0000ll || width > 0x7fff0000ll || worlds > 0x7fff0000ll)
     return o->err = "steps, worlds and width have to be below 2^31", false;
-  if (worlds * ((width + 3) / 4) > 64ll * 0x7fff0000ll) return o->err = "too many channels", false;
+  // Lanes (of four channels) are counted in the launch's 32 bits.
+  if (worlds * (width < 4 ? width : ceil_div(width, 4)) > 0xffff0000ll) return o->err = "too many channels", false;
   return true;
 }
 

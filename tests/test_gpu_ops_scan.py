@@ -122,6 +122,20 @@ def test_saturated_gates(ops, T):
         assert torch.equal(h, torch.full_like(x, 0.3))
 
 
+@pytest.mark.parametrize("shape", [(600, 1, 64), (600, 300, 64), (4000, 2, 33)], ids=str)
+def test_zero_states_pass_growing_gates(ops, shape):
+    """Gates of 2 over hundreds of steps, of which the product is past f32: a
+    state of 0 stays 0, and what enters late grows exactly."""
+    z, x = torch.full(shape, 2.0, device="cuda"), torch.zeros(shape, device="cuda")
+    want, tail = torch.zeros(shape, device="cuda"), torch.tensor([1.0, 3.0, 7.0], device="cuda")[:, None, None]
+    x[-3:], want[-3:] = 1.0, tail
+    h, last = ops.gated_scan(z, x, form="decay")
+    assert torch.equal(h, want) and torch.equal(last, want[-1])
+    dh = x.flip(0)
+    dz, dx, dh0 = ops.gated_scan_backward(dh, z, x, h, form="decay")
+    assert torch.equal(dx, want.flip(0)) and not dz.any() and torch.equal(dh0, 2 * want[-1])
+
+
 def test_empty(ops):
     z = torch.zeros(0, 3, 5, device="cuda")
     h0 = torch.randn(3, 5, device="cuda")
