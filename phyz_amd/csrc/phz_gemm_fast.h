@@ -480,6 +480,14 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
   }
 }
 
+template <class Epi, class Beside>
+void launch_join(hipStream_t stream, const PartOut& sums, int batch, int splits, int32_t m, int32_t n, const Epi& epi,
+                 const Beside& beside) {
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)m * ((n + 7) / 8), 64), 8192);
+  hipLaunchKernelGGL((join_kernel<Epi, Beside>), dim3(beside.blocks + blocks, (unsigned)batch), dim3(256), 0, stream, sums,
+                     splits, m, n, epi, beside);
+}
+
 // `part`: plan.part_bytes of workspace. `beside` goes with the join: to plans
 // with splits, and one matrix, only.
 template <class T, int PL, bool AK, bool BKD, class Epi, class Beside = NothingBeside>
@@ -509,11 +517,35 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
   }
   if (plan.tile == 2) go(typename Tiles<T, PL>::Deep{});
   if (plan.tile == 3) go(typename Tiles<T, PL>::Small{});
-  if (p.splits > 1) {
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)p.m * ((p.n + 7) / 8), 64), 8192);
-    hipLaunchKernelGGL((join_kernel<Epi, Beside>), dim3(beside.blocks + blocks, (unsigned)batch), dim3(256), 0, stream, sums,
-                       p.splits, p.m, p.n, epi, beside);
-  }
+  if (p.splits > 1) launch_join(stream, sums, batch, p.splits, p.m, p.n, epi, beside);
+}
+
+// gemm_any's contraction in splits where its tiles are few: a stage of tile_k
+// takes about 1.1 us alone, a join 4, so splits keep at least four stages, and
+// there are at most two workgroups a compute unit.
+struct AnyPlan {
+  int32_t splits, k_split;
+  uint64_t part_bytes;
+};
+template <class E>
+AnyPlan plan_any(const phz_ops* o, int64_t m, int64_t n, int64_t k) {
+  const int64_t bk = Any<E>::tile_k, stages = ceil_div(k, bk), tiles = ceil_div(m, 64) * ceil_div(n, 64);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(2 * o->cus, tiles), stages / 4));
+  AnyPlan p{};
+  p.k_split = (int32_t)(std::max<int64_t>(1, ceil_div(stages, want)) * bk);
+  p.splits = (int32_t)std::max<int64_t>(1, ceil_div(k, p.k_split));
+  p.part_bytes = p.splits > 1 ? (uint64_t)p.splits * m * ((n + 7) / 8 * 8) * 4 : 0;
+  return p;
+}
+template <class E, bool AK, bool BKD, class Epi, class Beside = NothingBeside>
+void launch_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b, int64_t m, int64_t n, int64_t k,
+                const AnyPlan& plan, float* part, const Epi& epi, const Beside& beside = {}) {
+  const GemmShape s{(int32_t)m, (int32_t)n, (int32_t)k, plan.k_split, plan.splits};
+  if (plan.splits == 1) return launch_gemm_any<E, AK, BKD>(o, stream, a, b, s, 1, epi);
+  const int64_t row = (n + 7) / 8 * 8;
+  const PartOut sums{part, row, m * row, m * row};
+  launch_gemm_any<E, AK, BKD>(o, stream, a, b, s, 1, sums);
+  launch_join(stream, sums, 1, plan.splits, s.m, s.n, epi, beside);
 }
 
 }  // namespace phzop

@@ -179,20 +179,6 @@ struct Repair {
   }
 };
 
-// Sums of one split of the contraction, joined by join_splits.
-struct SplitOut : NothingAhead {
-  float* part;
-  int64_t row, split;
-  SplitOut(float* p, int64_t r, int64_t s) : part(p), row(r), split(s) {}
-  __device__ __forceinline__ void put8(int, int s, int i, int j, const float* sums, const Held&, const Columns&) const {
-    Pack<float, 8> out;
-#pragma unroll
-    for (int c = 0; c < 8; c++) out.v[c] = sums[c];
-    *(Pack<float, 8>*)(part + s * split + i * row + j) = out;
-  }
-  __device__ __forceinline__ void put1(int, int s, int i, int j, float p) const { part[s * split + i * row + j] = p; }
-};
-
 // ── few rows ────────────────────────────────────────────────────────────────
 //
 // Up to 32 rows (a policy acting, a serving batch): the weights are read once
@@ -417,34 +403,6 @@ __global__ __launch_bounds__(256) void column_sums(ColumnSums<E> c) {
   c.run(blockIdx.x);
 }
 
-// y[i][j] = the splits' sums, added in a fixed order: eight threads an element,
-// each every eighth split.
-template <class E>
-__global__ __launch_bounds__(256) void join_splits(const float* part, int splits, int64_t split, E* y, int64_t row,
-                                                   int32_t n, int64_t total, ColumnSums<E> beside) {
-  if (blockIdx.x < beside.blocks) return beside.run(blockIdx.x);
-  __shared__ float s[8][32];
-  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  const int64_t stride = (int64_t)(gridDim.x - beside.blocks) * 32;
-  for (int64_t t0 = (int64_t)(blockIdx.x - beside.blocks) * 32; t0 < total; t0 += stride) {
-    const int64_t t = t0 + c;
-    float v = 0.0f;
-    if (t < total) {
-#pragma unroll 8
-      for (int k = lane; k < splits; k += 8) v += part[k * split + t];
-    }
-    s[lane][c] = v;
-    __syncthreads();
-    if (lane == 0 && t < total) {
-#pragma unroll
-      for (int l = 1; l < 8; l++) v += s[l][c];
-      const int64_t i = t / n;
-      y[i * row + (t - i * n)] = from_f32<E>(v);
-    }
-    __syncthreads();
-  }
-}
-
 // Rows of n elements into rows of `to_row`, zeros between: as they are, or f32
 // cut into three planes.
 template <class E>
@@ -609,9 +567,11 @@ int linear(phz_ops* o, hipStream_t stream, int act, const phz_tensor* x, const p
     b.lay(stream);
     product<E, true, true>(o, stream, a, b, m, n, k, how, part, out);
   } else {
-    launch_gemm_any<E, true, true>(o, stream, Operand{x->data, x->stride[0], 0}, Operand{w->data, w->stride[0], 0},
-                                   GemmShape{(int32_t)m, (int32_t)n, (int32_t)k, (int32_t)std::max<int64_t>(k, 1), 1}, 1,
-                                   out);
+    const AnyPlan how = plan_any<E>(o, m, n, k);
+    float* part = how.part_bytes ? (float*)o->workspace(stream, how.part_bytes) : nullptr;
+    if (how.part_bytes && !part) return 1;
+    launch_any<E, true, true>(o, stream, Operand{x->data, x->stride[0], 0}, Operand{w->data, w->stride[0], 0}, m, n, k, how,
+                              part, out);
   }
   return launched(o, "linear") ? 0 : 1;
 }
@@ -630,15 +590,9 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   FastPlan dx_plan{}, dw_plan{};
   if (fast && need_dx) dx_plan = plan<E>(o, way, m, k, pad8(n));
   if (fast && need_dw) dw_plan = plan<E>(o, way, n, k, m);
-  int32_t splits = 1, k_split = (int32_t)std::max<int64_t>(m, 1);
-  if (!fast && need_dw) {
-    // The contraction of dw runs over rows: split where its few tiles would
-    // not fill the chip.
-    const int64_t bk = Any<E>::tile_k;
-    const int64_t want = std::min<int64_t>(ceil_div(2 * o->cus, ceil_div(n, 64) * ceil_div(k, 64)), ceil_div(m, 4 * bk));
-    k_split = (int32_t)(ceil_div(ceil_div(m, std::max<int64_t>(1, std::min<int64_t>(want, 256))), bk) * bk);
-    splits = (int32_t)ceil_div(m, k_split);
-  }
+  AnyPlan dx_any{1, 1, 0}, dw_any{1, 1, 0};
+  if (!fast && need_dx) dx_any = plan_any<E>(o, m, k, n);
+  if (!fast && need_dw) dw_any = plan_any<E>(o, n, k, m);
   const bool lay_d = (need_dx || need_dw) && (fast ? !d.well : act != PHZ_ACT_NONE);
   // Blocks of rows whose sums of dz are added up in the end: four workgroups a
   // compute unit in all, 64 to 512 blocks of at least 16 rows.
@@ -655,7 +609,7 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
     if (db) sums = c.take<float>(blocks * n * 4);
     if (fast && need_dw && !xo.well) xo.copy = c.take<char>(xo.bytes());
     if (fast && need_dx && !wo.well) wo.copy = c.take<char>(wo.bytes());
-    part = c.take<float>(std::max({dx_plan.part_bytes, dw_plan.part_bytes, splits > 1 ? (uint64_t)splits * n * k * 4 : 0}));
+    part = c.take<float>(std::max({dx_plan.part_bytes, dw_plan.part_bytes, dx_any.part_bytes, dw_any.part_bytes}));
     if (pass == 0 && c.used && !(c.base = o->workspace(stream, c.used))) return 1;
   }
   if (m > 0 && (lay_d || db)) {
@@ -666,7 +620,7 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   // db goes with the join of dw's splits where there is one.
   const ColumnSums<E> bias{sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)blocks, (int32_t)n,
                            db ? (unsigned)ceil_div(n, 8) : 0u};
-  const bool joined = need_dw && (fast ? dw_plan.splits : splits) > 1;
+  const bool joined = need_dw && (fast ? dw_plan.splits : dw_any.splits) > 1;
   if (db && !joined) hipLaunchKernelGGL(column_sums<E>, dim3(bias.blocks), dim3(256), 0, stream, bias);
   if (fast) {
     if (need_dx) {
@@ -678,22 +632,12 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
       product<E, false, false>(o, stream, d, xo, n, k, m, dw_plan, part, PlainOut<E>{(E*)dw->data, dw->stride[0]}, bias);
     }
   } else {
-    const int32_t mi = (int32_t)m, ni = (int32_t)n, ki = (int32_t)k;
     const Operand dop{d.copy ? d.copy : dy->data, d.copy ? pad8(n) : dy->stride[0], 0}, xa{x->data, x->stride[0], 0},
         wa{w->data, w->stride[0], 0};
     if (need_dx)
-      launch_gemm_any<E, true, false>(o, stream, dop, wa, GemmShape{mi, ki, ni, ni, 1}, 1,
-                                      PlainOut<E>{(E*)dx->data, dx->stride[0]});
-    if (need_dw) {
-      const GemmShape shape{ni, ki, mi, k_split, splits};
-      if (splits == 1) {
-        launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, PlainOut<E>{(E*)dw->data, dw->stride[0]});
-      } else {
-        launch_gemm_any<E, false, false>(o, stream, dop, xa, shape, 1, SplitOut{part, k, n * k});
-        hipLaunchKernelGGL(join_splits<E>, dim3(bias.blocks + (unsigned)std::min<int64_t>(ceil_div(n * k, 32), 8192)),
-                           dim3(256), 0, stream, part, splits, n * k, (E*)dw->data, dw->stride[0], ki, n * k, bias);
-      }
-    }
+      launch_any<E, true, false>(o, stream, dop, wa, m, k, n, dx_any, part, PlainOut<E>{(E*)dx->data, dx->stride[0]});
+    if (need_dw)
+      launch_any<E, false, false>(o, stream, dop, xa, n, k, m, dw_any, part, PlainOut<E>{(E*)dw->data, dw->stride[0]}, bias);
   }
   if (dw && k > 0 && m == 0)
     hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], (int32_t)k, n * k);
