@@ -179,9 +179,11 @@ struct Repair {
   }
 };
 
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
 // ── few rows ────────────────────────────────────────────────────────────────
 //
-// Up to 32 rows (a policy acting, a serving batch): the weights are read once
+// Up to 64 rows (a policy acting, a serving batch): the weights are read once
 // and everything else is small, so the floor is their way from memory. A
 // workgroup takes 16 TN outputs, its eight waves every eighth run of 128 bytes
 // of each weight row, straight into the matrix cores' fragments: lane l holds
@@ -189,7 +191,10 @@ struct Repair {
 // 16; which k an instruction pairs is the same on both sides and does not
 // matter to the sum. The waves' sums meet in LDS in order. f32 takes the f32
 // matrix instructions: exact products, and still below the weights' time.
-// 16 x 2048 -> 8192 bf16: 8.2 us of 7.2 for 33.6 MB at a large copy's rate.
+// 16 x 2048 -> 8192 bf16: 8.8 us, 3.8 TB/s (a large copy: 7.2 us). From 33 rows
+// on the inputs' way from L2 counts too: 64 x 2048 -> 4096 bf16 13.2 us against
+// 10.7 by tiles, but 64 x 1852 -> 3995 13.3 against 21.8, f32 512 -> 2048 7.3
+// against 11.0, and equal elsewhere.
 
 template <class E> struct Small;
 template <> struct Small<bf16> {
@@ -207,11 +212,11 @@ template <> struct Small<float> {
   }
 };
 
-constexpr int kSmallRows = 32, kSmallWaves = 8;
+constexpr int kSmallRows = 64, kSmallWaves = 8;
 
 template <class E, int TM, int TN, class Epi>
 __global__ __launch_bounds__(kSmallWaves * 64) void few_rows(const E* x, int64_t x_row, const E* w, int64_t w_row,
-                                                             int32_t m, int32_t n, int32_t k, Epi epi) {
+                                                             int32_t m, int32_t n, int32_t k, int32_t k_split, Epi epi) {
   constexpr int PER = Small<E>::kPer, U = 2;  // U loads of 64 bytes a row make a line
   typedef Pack<E, PER> Frag;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -229,7 +234,9 @@ __global__ __launch_bounds__(kSmallWaves * 64) void few_rows(const E* x, int64_t
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kRun = 4 * PER * U;
-  int k0 = wave * kRun;
+  const int split = blockIdx.y;
+  int k0 = split * k_split + wave * kRun;
+  k = min(k, (split + 1) * k_split);
 #pragma unroll 2
   for (; k0 + kRun <= k; k0 += kSmallWaves * kRun) {
     Frag fw[U][TN], fx[U][TM];
@@ -282,21 +289,42 @@ __global__ __launch_bounds__(kSmallWaves * 64) void few_rows(const E* x, int64_t
     float v = sums[0][i][j];
 #pragma unroll
     for (int g = 1; g < kSmallWaves; g++) v += sums[g][i][j];
-    if (i < m && n0 + j < n) epi.put1(0, 0, i, n0 + j, v);
+    if (i < m && n0 + j < n) epi.put1(0, split, i, n0 + j, v);
   }
 }
 
+// 32 outputs a workgroup where that still is one for every compute unit, and
+// the contraction in splits where 16 leave units idle and their time (of runs
+// of k, by rows and type, measured) pays for the join: 32 x 4096 -> 1024 15.2 us
+// in one, 10.5 in four.
+struct FewPlan {
+  bool wide;
+  int32_t splits, k_split;
+  uint64_t part_bytes;
+};
+template <class E>
+FewPlan plan_few(const phz_ops* o, int64_t m, int64_t n, int64_t k) {
+  constexpr int64_t kAll = kSmallWaves * 8 * Small<E>::kPer;  // a run of every wave
+  const double us = k * (sizeof(E) == 2 ? 1.5 + 0.045 * m : 2.0 + 0.105 * m) / 1000;
+  FewPlan p{ceil_div(n, 32) >= o->cus, 1, 0, 0};
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(o->cus / ceil_div(n, 16), k / (2 * kAll)));
+  if (us * (1 - 1.0 / splits) < 5) splits = 1;
+  p.k_split = (int32_t)(std::max<int64_t>(1, ceil_div(ceil_div(k, splits), kAll)) * kAll);
+  p.splits = (int32_t)std::max<int64_t>(1, ceil_div(k, p.k_split));
+  p.part_bytes = p.splits > 1 ? (uint64_t)p.splits * m * pad8(n) * 4 : 0;
+  return p;
+}
+
 template <class E, class Epi>
-void launch_few_rows(const phz_ops* o, hipStream_t stream, const phz_tensor* x, const phz_tensor* w, Epi epi) {
+void launch_few_rows(hipStream_t stream, const phz_tensor* x, const phz_tensor* w, const FewPlan& p, Epi epi) {
   const int32_t m = (int32_t)x->size[0], k = (int32_t)x->size[1], n = (int32_t)w->size[0];
   auto go = [&](auto kernel, int per) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, per)), dim3(kSmallWaves * 64), 0, stream, (const E*)x->data,
-                       x->stride[0], (const E*)w->data, w->stride[0], m, n, k, epi);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, per), (unsigned)p.splits), dim3(kSmallWaves * 64), 0, stream,
+                       (const E*)x->data, x->stride[0], (const E*)w->data, w->stride[0], m, n, k, p.k_split, epi);
   };
-  // 32 outputs a workgroup where that still is one for every compute unit.
-  const bool wide = ceil_div(n, 32) >= o->cus;
-  if (m <= 16) wide ? go(few_rows<E, 1, 2, Epi>, 32) : go(few_rows<E, 1, 1, Epi>, 16);
-  else wide ? go(few_rows<E, 2, 2, Epi>, 32) : go(few_rows<E, 2, 1, Epi>, 16);
+  if (m <= 16) p.wide ? go(few_rows<E, 1, 2, Epi>, 32) : go(few_rows<E, 1, 1, Epi>, 16);
+  else if (m <= 32) p.wide ? go(few_rows<E, 2, 2, Epi>, 32) : go(few_rows<E, 2, 1, Epi>, 16);
+  else p.wide ? go(few_rows<E, 4, 2, Epi>, 32) : go(few_rows<E, 4, 1, Epi>, 16);
 }
 
 // Eight f32 as three planes of bf16.
@@ -316,8 +344,8 @@ __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v)
 // turn.
 template <class E>
 __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_row, const E* pre, int64_t pre_row,
-                                               E* dz, bf16* cut, int64_t plane, int64_t dz_row, float* sums, int32_t m,
-                                               int32_t n, int32_t rows, int32_t across) {
+                                               E* dz, bf16* cut, int64_t plane, int64_t dz_row, float* sums, E* db,
+                                               int64_t db_step, int32_t m, int32_t n, int32_t rows, int32_t across) {
   const int lanes = 256 / across, at = threadIdx.x & (across - 1), lane = threadIdx.x / across;
   const int j = (blockIdx.x * across + at) * 8;
   const int64_t i0 = (int64_t)blockIdx.y * rows, i1 = min((int64_t)m, i0 + rows);
@@ -359,18 +387,24 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
       if (cut) put_cut(cut + i * dz_row + j, plane, all);
     }
   }
-  if (!sums) return;
+  if (!sums && !db) return;
   __shared__ float s[256][9];  // [lane][eight of columns][column], one apart
+  __shared__ float part[256];
 #pragma unroll
   for (int c = 0; c < 8; c++) s[threadIdx.x][c] = total[c];
   __syncthreads();
-  for (int t = threadIdx.x; t < across * 8; t += 256) {
-    const int col = blockIdx.x * across * 8 + t;
-    if (col < n) {
-      float v = 0.0f;
-      for (int l = 0; l < lanes; l++) v += s[l * across + t / 8][t % 8];
-      sums[(int64_t)blockIdx.y * n + col] = v;
-    }
+  // A thread adds eight lanes of a column, and the first ones those sums.
+  const int wide = across * 8, at_col = threadIdx.x & (wide - 1), first = threadIdx.x / wide * 8;
+  float v = 0.0f;
+#pragma unroll
+  for (int l = 0; l < 8; l++) v += s[(first + l) * across + at_col / 8][at_col % 8];
+  part[threadIdx.x] = v;
+  __syncthreads();
+  const int col = blockIdx.x * wide + at_col;
+  if (first == 0 && col < n) {
+    for (int l = wide; l < 256; l += wide) v += part[l + at_col];
+    if (sums) sums[(int64_t)blockIdx.y * n + col] = v;
+    else db[col * db_step] = from_f32<E>(v);
   }
 }
 
@@ -462,8 +496,6 @@ struct Carve {
   }
 };
 
-int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
-
 // How a product's operands go to gemm_fast: as they are, copied into whole
 // eights where they do not lie well (rows of whole 16 bytes, and a tile's rows
 // within 32-bit offsets); or, f32, cut in three planes.
@@ -547,7 +579,16 @@ int linear(phz_ops* o, hipStream_t stream, int act, const phz_tensor* x, const p
   out.y = (E*)y->data, out.y_row = y->stride[0];
   out.act = act;
   if (m <= kSmallRows) {
-    launch_few_rows<E>(o, stream, x, w, out);
+    const FewPlan how = plan_few<E>(o, m, n, k);
+    if (how.splits == 1) {
+      launch_few_rows<E>(stream, x, w, how, out);
+    } else {
+      float* part = (float*)o->workspace(stream, how.part_bytes);
+      if (!part) return 1;
+      const PartOut sums{part, pad8(n), m * pad8(n), m * pad8(n)};
+      launch_few_rows<E>(stream, x, w, how, sums);
+      launch_join(stream, sums, 1, how.splits, (int32_t)m, (int32_t)n, out, NothingBeside{});
+    }
     return launched(o, "linear") ? 0 : 1;
   }
   const Way way = k == 0 ? ANY : way_of<E>(m, n, k, k % (16 / sizeof(E)) == 0);
@@ -595,18 +636,20 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   if (!fast && need_dw) dw_any = plan_any<E>(o, n, k, m);
   const bool lay_d = (need_dx || need_dw) && (fast ? !d.well : act != PHZ_ACT_NONE);
   // Blocks of rows whose sums of dz are added up in the end: four workgroups a
-  // compute unit in all, 64 to 512 blocks of at least 16 rows.
-  int across = 32;
+  // compute unit in all, 64 to 512 blocks of at least 16 rows. Up to 512 rows
+  // are one block, of 64 rows at a time, which leaves db itself.
+  const bool one = m <= 512;
+  int across = one ? 4 : 32;
   while (across > 1 && across * 4 >= n) across /= 2;
   const int64_t wanted = std::min<int64_t>(512, std::max<int64_t>(64, 4 * o->cus / ceil_div(n, across * 8)));
-  const int64_t rows = std::max<int64_t>(16, ceil_div(ceil_div(m, wanted), 8) * 8), blocks = ceil_div(m, rows);
+  const int64_t rows = one ? 512 : std::max<int64_t>(16, ceil_div(ceil_div(m, wanted), 8) * 8), blocks = ceil_div(m, rows);
 
   Carve c;
   float *sums = nullptr, *part = nullptr;
   for (int pass = 0; pass < 2; pass++) {
     c.used = 0;
     if (lay_d) d.copy = c.take<char>(d.bytes());
-    if (db) sums = c.take<float>(blocks * n * 4);
+    if (db && !one) sums = c.take<float>(blocks * n * 4);
     if (fast && need_dw && !xo.well) xo.copy = c.take<char>(xo.bytes());
     if (fast && need_dx && !wo.well) wo.copy = c.take<char>(wo.bytes());
     part = c.take<float>(std::max({dx_plan.part_bytes, dw_plan.part_bytes, dx_any.part_bytes, dw_any.part_bytes}));
@@ -615,13 +658,14 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   if (m > 0 && (lay_d || db)) {
     hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, across * 8), (unsigned)blocks), dim3(256), 0, stream, act,
                        (const E*)dy->data, dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0,
-                       (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(), pad8(n), sums, (int32_t)m, (int32_t)n, (int32_t)rows, across);
+                       (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(), pad8(n), sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)m, (int32_t)n,
+                       (int32_t)rows, across);
   }
   // db goes with the join of dw's splits where there is one.
   const ColumnSums<E> bias{sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)blocks, (int32_t)n,
-                           db ? (unsigned)ceil_div(n, 8) : 0u};
+                           db && (!one || m == 0) ? (unsigned)ceil_div(n, 8) : 0u};
   const bool joined = need_dw && (fast ? dw_plan.splits : dw_any.splits) > 1;
-  if (db && !joined) hipLaunchKernelGGL(column_sums<E>, dim3(bias.blocks), dim3(256), 0, stream, bias);
+  if (bias.blocks && !joined) hipLaunchKernelGGL(column_sums<E>, dim3(bias.blocks), dim3(256), 0, stream, bias);
   if (fast) {
     if (need_dx) {
       wo.lay(stream);

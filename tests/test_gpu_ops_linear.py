@@ -50,6 +50,18 @@ def test_forward_and_backward(ops, shape, dtype):
         R.within(a, b, c, name)
 
 
+#: Few tiles and a long contraction, in one product or another, at sizes off the
+#: vector; and rows about where another kernel or another split of rows begins.
+LONG = [(2, 57, 914), (125, 1618, 2), (357, 1647, 67), (2149, 45, 1003), (40, 3001, 9), (33, 520, 300), (48, 2048, 515),
+        (64, 1000, 72), (65, 1000, 72), (512, 40, 33), (513, 40, 33), (511, 24, 700)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_contractions(ops, shape, dtype):
+    test_forward_and_backward(ops, shape, dtype)
+
+
 #: Large enough for every tile, for split contractions and for operands that
 #: are copied first, on and off the tiles' sizes.
 LARGE = [(4096, 4096, 64, "silu"), (3001, 1024, 2056, "none"), (257, 4104, 520, "tanh"), (9000, 131, 1003, "gelu"),
