@@ -146,11 +146,36 @@ __device__ __forceinline__ f32x16 multiply(const float* a, const float* b, f32x1
 // holding the next k tile while the matrix cores work on the one in LDS.
 //
 // An epilogue has
-//   Columns, columns(j, c)                what it reads for eight columns, once
-//   Held, fetch(q, i, j, held)            what it reads for eight elements, ahead
-//   put8(q, split, i, j, sums, held, c)   eight neighbouring sums of row i
-//   put1(q, split, i, j, sum)             one, at a ragged end
-template <class E, bool AK, bool BKD, int BM, int BN, class Epi>
+//   Columns, columns(j, left, c)                what it reads for eight columns, once
+//   Held, fetch(q, i, j, left, held)            what it reads for eight elements, ahead
+//   put8(q, split, i, j, left, sums, held, c)   eight neighbouring sums of row i
+//   kRagged                                     whether rows may end inside eight
+// of which, at a ragged end, only the first `left` exist; else that is the
+// constant 8. RAGGED is a kernel of its own: its single accesses, all on their
+// way together, take registers that whole rows would miss (32768 x 1024 -> 4096
+// bf16 388 us, 412 with both in one), and one at a time, after each other, cost
+// a load's latency each (54038 x 252 -> 135: 73 us, so 49).
+template <class E>
+__device__ __forceinline__ void load_some(Pack<E, 8>& to, const E* p, int left) {
+  if (left >= 8) {
+    to = *(const Pack<E, 8>*)p;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; c++) to.v[c] = c < left ? p[c] : E{};
+  }
+}
+template <class E>
+__device__ __forceinline__ void store_some(E* p, const Pack<E, 8>& from, int left) {
+  if (left >= 8) {
+    *(Pack<E, 8>*)p = from;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      if (c < left) p[c] = from.v[c];
+  }
+}
+
+template <class E, bool AK, bool BKD, int BM, int BN, bool RAGGED, class Epi>
 __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape s, Epi epi) {
   constexpr int BK = Any<E>::tile_k, LD = Any<E>::ld, PER = 16 / sizeof(E);
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
@@ -206,14 +231,15 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
   constexpr int kLanes = WN / 8, kRows = 64 / kLanes, kPuts = 32 / kRows;
   const int col = n0 + wn + (lane % kLanes) * 8;
   typename Epi::Columns columns;
-  if (col + 8 <= s.n) epi.columns(col, columns);
+  const int left = RAGGED ? min(8, s.n - col) : 8;
+  if (col < s.n) epi.columns(col, left, columns);
 #pragma unroll
   for (int i = 0; i < TM; i++) {
     typename Epi::Held held[kPuts];
 #pragma unroll
     for (int r = 0; r < kPuts; r++) {
       const int row = m0 + wm + i * 32 + r * kRows + lane / kLanes;
-      if (row < s.m && col + 8 <= s.n) epi.fetch(q, row, col, held[r]);
+      if (row < s.m && col < s.n) epi.fetch(q, row, col, left, held[r]);
     }
 #pragma unroll
     for (int j = 0; j < TN; j++)
@@ -228,10 +254,9 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
       const float* p = out + (r * kRows + lane / kLanes) * kOutRow + (lane % kLanes) * 8;
       *(f32x4*)v = *(const f32x4*)p;
       *(f32x4*)(v + 4) = *(const f32x4*)(p + 4);
-      if (row >= s.m) continue;
-      if (col + 8 <= s.n) epi.put8(q, split, row, col, v, held[r], columns);
-      else
-        for (int c = 0; c < 8 && col + c < s.n; c++) epi.put1(q, split, row, col + c, v[c]);
+      if (row >= s.m || col >= s.n) continue;
+      if (!RAGGED || left == 8) epi.put8(q, split, row, col, 8, v, held[r], columns);
+      else epi.put8(q, split, row, col, left, v, held[r], columns);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -240,11 +265,11 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
 // For epilogues that read nothing for columns, or nothing ahead.
 struct NoColumns {
   struct Columns {};
-  __device__ __forceinline__ void columns(int, Columns&) const {}
+  __device__ __forceinline__ void columns(int, int, Columns&) const {}
 };
 struct NothingAhead : NoColumns {
   struct Held {};
-  __device__ __forceinline__ void fetch(int, int, int, Held&) const {}
+  __device__ __forceinline__ void fetch(int, int, int, int, Held&) const {}
 };
 
 // Launches gemm_any with the tile that fills the chip: 128 x 128 where those
@@ -252,12 +277,18 @@ struct NothingAhead : NoColumns {
 template <class E, bool AK, bool BKD, class Epi>
 void launch_gemm_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b, GemmShape s, int batch, Epi epi) {
   const int64_t z = (int64_t)batch * s.splits;
-  if (s.m > 64 && s.n > 64 && ceil_div(s.m, 128) * ceil_div(s.n, 128) * z >= 2ll * o->cus)
-    hipLaunchKernelGGL((gemm_any<E, AK, BKD, 128, 128, Epi>), dim3(ceil_div(s.n, 128), ceil_div(s.m, 128), z),
-                       dim3(256), 0, stream, a, b, s, epi);
-  else
-    hipLaunchKernelGGL((gemm_any<E, AK, BKD, 64, 64, Epi>), dim3(ceil_div(s.n, 64), ceil_div(s.m, 64), z), dim3(256), 0,
-                       stream, a, b, s, epi);
+  const bool large = s.m > 64 && s.n > 64 && ceil_div(s.m, 128) * ceil_div(s.n, 128) * z >= 2ll * o->cus;
+  const int tile = large ? 128 : 64;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(s.n, tile), ceil_div(s.m, tile), z), dim3(256), 0, stream, a, b, s, epi);
+  };
+  if constexpr (Epi::kRagged) {
+    if (s.n % 8) {
+      large ? go(gemm_any<E, AK, BKD, 128, 128, true, Epi>) : go(gemm_any<E, AK, BKD, 64, 64, true, Epi>);
+      return;
+    }
+  }
+  large ? go(gemm_any<E, AK, BKD, 128, 128, false, Epi>) : go(gemm_any<E, AK, BKD, 64, 64, false, Epi>);
 }
 
 }  // namespace phzop

@@ -167,7 +167,7 @@ struct Tile {
   static constexpr int kThreads = MW_ * NW_ * NG_ * 64;
 };
 
-template <class T, int PL, bool AK, bool BKD, class Shape, class Epi>
+template <class T, int PL, bool AK, bool BKD, class Shape, bool RAGGED, class Epi>
 __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi epi) {
   constexpr int BM = Shape::BM, BN = Shape::BN, BK = Shape::BK, NS = Shape::NS, NG = Shape::NG;
   constexpr int NWAVE = Shape::MW * Shape::NW;
@@ -278,17 +278,18 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
   constexpr int kShare = 32 / NG;  // rows that a group puts out; where they are fewer than kRows, lanes idle
   constexpr int kPuts = kShare < kRows ? 1 : kShare / kRows;
   const int col = n0 + wn + (lane % kLanes) * 8;
+  const int left = RAGGED ? min(8, p.n - col) : 8;
   const bool mine = kShare >= kRows || lane / kLanes < kShare;
   auto row_of = [&](int i, int r) { return m0 + wm + i * 32 + group * kShare + r * kRows + lane / kLanes; };
   typename Epi::Held held[2][kPuts];
   auto fetch = [&](int i) {
 #pragma unroll
     for (int r = 0; r < kPuts; r++)
-      if (mine && row_of(i, r) < p.m && col + 8 <= p.n) epi.fetch(q, row_of(i, r), col, held[i & 1][r]);
+      if (mine && row_of(i, r) < p.m && col < p.n) epi.fetch(q, row_of(i, r), col, left, held[i & 1][r]);
   };
   typename Epi::Columns columns;
   arrive(steps - 1);
-  if (col + 8 <= p.n) epi.columns(col, columns);
+  if (col < p.n) epi.columns(col, left, columns);
   fetch(0);
   if (NG == 1 || (steps - 1) * NG + group < total) compute();  // a group may have no last stage
 
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
 #pragma unroll
     for (int r = 0; r < kPuts; r++) {
       const int row = row_of(i, r);
-      if (!mine || row >= p.m) continue;
+      if (!mine || row >= p.m || col >= p.n) continue;
       float v[8];
       const float* s = out + (group * kShare + r * kRows + lane / kLanes) * kOutRow + (lane % kLanes) * 8;
       *(f32x4*)v = *(const f32x4*)s;
@@ -320,9 +321,8 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
       for (int g = 1; g < NG; g++)
 #pragma unroll
         for (int c = 0; c < 8; c++) v[c] += s[g * kGroup + c];
-      if (col + 8 <= p.n) epi.put8(q, split, row, col, v, held[i & 1][r], columns);
-      else
-        for (int c = 0; c < 8 && col + c < p.n; c++) epi.put1(q, split, row, col + c, v[c]);
+      if (!RAGGED || left == 8) epi.put8(q, split, row, col, 8, v, held[i & 1][r], columns);
+      else epi.put8(q, split, row, col, left, v, held[i & 1][r], columns);
     }
     if (NG > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
@@ -415,12 +415,13 @@ inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int
   return best;
 }
 
-// Sums of one split, joined by join_kernel.
+// Sums of one split, joined by join_kernel, in rows of whole eights.
 struct PartOut : NothingAhead {
+  static constexpr bool kRagged = false;
   float* part;
   int64_t row, batch, split;
   PartOut(float* p, int64_t r, int64_t b, int64_t s) : part(p), row(r), batch(b), split(s) {}
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* sums, const Held&, const Columns&) const {
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, int, const float* sums, const Held&, const Columns&) const {
     float* at = part + s * split + q * batch + i * row + j;
     *(f32x4*)at = *(const f32x4*)sums;
     *(f32x4*)(at + 4) = *(const f32x4*)(sums + 4);
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
     const float* at = p.part + q * p.batch + i * p.row + j;
     typename Epi::Held held;
     typename Epi::Columns columns;
-    if (live && lane == 0 && j + 8 <= n) epi.fetch(q, i, j, held), epi.columns(j, columns);
+    if (live && lane == 0) epi.fetch(q, i, j, min(8, n - j), held), epi.columns(j, min(8, n - j), columns);
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) v[c] = 0.0f;
@@ -472,9 +473,8 @@ __global__ __launch_bounds__(256) void join_kernel(PartOut p, int splits, int32_
       for (int l = 0; l < 3; l++)
 #pragma unroll
         for (int c = 0; c < 8; c++) v[c] += s[l][unit][c];
-      if (j + 8 <= n) epi.put8(q, 0, i, j, v, held, columns);
-      else
-        for (int c = 0; c < 8 && j + c < n; c++) epi.put1(q, 0, i, j + c, v[c]);
+      if (j + 8 <= n) epi.put8(q, 0, i, j, 8, v, held, columns);
+      else epi.put8(q, 0, i, j, n - j, v, held, columns);
     }
     __syncthreads();
   }
@@ -503,10 +503,18 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
     p.tiles_m = (int32_t)ceil_div(p.m, S::BM);
     p.tiles_n = (int32_t)ceil_div(p.n, S::BN);
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch, (unsigned)p.splits);
-    if (p.splits == 1)
-      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, Epi>), grid, dim3(S::kThreads), 0, stream, p, epi);
-    else
-      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, PartOut>), grid, dim3(S::kThreads), 0, stream, p, sums);
+    const dim3 block(S::kThreads);
+    if (p.splits > 1) {
+      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, false, PartOut>), grid, block, 0, stream, p, sums);
+      return;
+    }
+    if constexpr (Epi::kRagged) {
+      if (p.n % 8) {
+        hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, true, Epi>), grid, block, 0, stream, p, epi);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, false, Epi>), grid, block, 0, stream, p, epi);
   };
   if constexpr (sizeof(T) == 2) {
     if (plan.tile == 0) go(typename Tiles<T, PL>::Big{});

@@ -176,22 +176,22 @@ __global__ __launch_bounds__(256) void scale_kernel(Source<E> s, const double* p
 // y = alpha sum + beta d, as PY planes; d has PD.
 template <int PY, int PD>
 struct PlanesOut : NoColumns {
+  static constexpr bool kRagged = false;  // rows of planes are whole eights
   Planes y, d;
   float alpha, beta;
   int32_t cols;  // columns that exist: zeros beyond
   PlanesOut(Planes y_, Planes d_, float al, float be, int32_t c) : y(y_), d(d_), alpha(al), beta(be), cols(c) {}
   typedef PlaneEight<PD> Held;
-  __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const {
+  __device__ __forceinline__ void fetch(int q, int i, int j, int, Held& h) const {
     if (d.data) h.get(d, q * d.batch + i * d.row + j);
   }
-  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h, const Columns&) const {
+  __device__ __forceinline__ void put8(int q, int, int i, int j, int, const float* sums, const Held& h, const Columns&) const {
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++)
       v[c] = j + c < cols ? (d.data ? fmaf(alpha, sums[c], beta * h.value(c)) : alpha * sums[c]) : 0.0f;
     put_planes<PY>(y, q * y.batch + i * y.row + j, v);
   }
-  __device__ __forceinline__ void put1(int, int, int, int, float) const {}  // rows are whole eights
 };
 
 // The last X' as o, or into the weights: w <- keep w - step X'.
@@ -216,6 +216,7 @@ struct Result {
 // alpha sum + beta X into the result.
 template <class O>
 struct LastOut : NoColumns {
+  static constexpr bool kRagged = false;  // rows of planes are whole eights
   Planes x;
   float alpha, beta;
   int32_t cols;
@@ -225,11 +226,11 @@ struct LastOut : NoColumns {
     PlaneEight<2> x;
     Pack<O, 8> before;
   };
-  __device__ __forceinline__ void fetch(int q, int i, int j, Held& h) const {
+  __device__ __forceinline__ void fetch(int q, int i, int j, int, Held& h) const {
     h.x.get(x, q * x.batch + i * x.row + j);
     if (out.update && j + 8 <= cols) h.before = *(const Pack<O, 8>*)(out.o + q * out.batch + i * out.row + j);
   }
-  __device__ __forceinline__ void put8(int q, int, int i, int j, const float* sums, const Held& h, const Columns&) const {
+  __device__ __forceinline__ void put8(int q, int, int i, int j, int, const float* sums, const Held& h, const Columns&) const {
     float v[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) v[c] = fmaf(alpha, sums[c], beta * h.x.value(c));
@@ -237,19 +238,19 @@ struct LastOut : NoColumns {
     else
       for (int c = 0; c < 8 && j + c < cols; c++) out.put(q, i, j + c, v[c]);
   }
-  __device__ __forceinline__ void put1(int, int, int, int, float) const {}  // rows are whole eights
 };
 
 // C = alpha product + beta D in f32 (any coefficients; see newton_schulz_any).
 struct Axpby : NothingAhead {
+  static constexpr bool kRagged = true;
   float *y;
   const float* d;
   float alpha, beta;
   int64_t row, batch;
   Axpby(float* y_, const float* d_, float al, float be, int64_t r, int64_t b)
       : y(y_), d(d_), alpha(al), beta(be), row(r), batch(b) {}
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* p, const Held&, const Columns&) const {
-    for (int c = 0; c < 8; c++) put1(q, s, i, j + c, p[c]);
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, int left, const float* p, const Held&, const Columns&) const {
+    for (int c = 0; c < 8 && c < left; c++) put1(q, s, i, j + c, p[c]);
   }
   __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
     const int64_t at = q * batch + i * row + j;
@@ -259,13 +260,14 @@ struct Axpby : NothingAhead {
 
 template <class O>
 struct LastAny : NothingAhead {
+  static constexpr bool kRagged = true;
   const float* x;
   float a;
   int64_t row, batch;
   Result<O> out;
   LastAny(const float* x_, float a_, int64_t r, int64_t b, const Result<O>& o) : x(x_), a(a_), row(r), batch(b), out(o) {}
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, const float* p, const Held&, const Columns&) const {
-    for (int c = 0; c < 8; c++) put1(q, s, i, j + c, p[c]);
+  __device__ __forceinline__ void put8(int q, int s, int i, int j, int left, const float* p, const Held&, const Columns&) const {
+    for (int c = 0; c < 8 && c < left; c++) put1(q, s, i, j + c, p[c]);
   }
   __device__ __forceinline__ void put1(int q, int, int i, int j, float p) const {
     out.put(q, i, j, fmaf(a, x[q * batch + i * row + j], p));

@@ -53,7 +53,7 @@ def test_forward_and_backward(ops, shape, dtype):
 #: Few tiles and a long contraction, in one product or another, at sizes off the
 #: vector; and rows about where another kernel or another split of rows begins.
 LONG = [(2, 57, 914), (125, 1618, 2), (357, 1647, 67), (2149, 45, 1003), (40, 3001, 9), (33, 520, 300), (48, 2048, 515),
-        (64, 1000, 72), (65, 1000, 72), (512, 40, 33), (513, 40, 33), (511, 24, 700)]
+        (64, 1000, 72), (65, 1000, 72), (512, 40, 33), (513, 40, 33), (511, 24, 700), (128, 40, 33), (129, 40, 33)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
