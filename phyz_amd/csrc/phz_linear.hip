@@ -338,10 +338,12 @@ __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v)
 }
 
 // dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
-// rows of `dz_row` with zeros past n, or cut into three planes of such rows, and the sums of dz over each block's rows,
-// which ColumnSums adds up in order. A thread takes eight columns; `across`
-// (a power of two, at most 32) of them lie along a row, the others take rows in
-// turn.
+// rows of `dz_row` with zeros past n, or cut into three planes of such rows, and
+// the sums of dz over each block's rows, which ColumnSums adds up in order. A
+// thread takes eight columns; `across` (a power of two, at most 32) of them lie
+// along a row, the others take rows in turn. Bound by memory: 40793 x 1760 bf16
+// 77 us for 431 MB (5.6 TB/s), 16384 x 256 f32 10.7 us for 50 MB, of which some
+// 4 us are the launch's ramp and the sums.
 template <class E>
 __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_row, const E* pre, int64_t pre_row,
                                                E* dz, bf16* cut, int64_t plane, int64_t dz_row, float* sums, E* db,
@@ -409,7 +411,8 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
 }
 
 // db from the blocks' sums of dz: eight columns a workgroup, 32 threads a
-// column, each every 32nd block's sum.
+// column, each every 32nd block's sum. Latency only (3 to 4 us by itself), so it
+// goes beside the join of dw's splits where there is one.
 template <class E>
 struct ColumnSums {
   const float* sums;
@@ -438,7 +441,7 @@ __global__ __launch_bounds__(256) void column_sums(ColumnSums<E> c) {
 }
 
 // Rows of n elements into rows of `to_row`, zeros between: as they are, or f32
-// cut into three planes.
+// cut into three planes. Bound by memory: 54038 x 252 bf16 12 us, 4.5 TB/s.
 template <class E>
 __global__ __launch_bounds__(256) void pack_rows(const E* from, int64_t from_row, E* to, bf16* cut, int64_t to_row,
                                                  int64_t plane, int32_t m, int32_t n) {

@@ -390,8 +390,9 @@ __global__ void copy_rows(const float* src, int64_t src_b, float* dst, int64_t d
   }
 }
 
-// One step for every channel, the state replaced in place. Bound by launch
-// latency below about a million channels, by memory above.
+// One step for every channel, the state replaced in place: 16 bytes a channel
+// in f32. Bound by a launch's latency below about a million channels (1024 x
+// 256: 2.7 us, 0.9 of them at a copy's rate), by memory above.
 template <class E, int FORM, int VEC>
 __global__ __launch_bounds__(256) void gated_step_kernel(const void* z, int64_t z_b, const void* x, int64_t x_b,
                                                          const uint8_t* reset, int64_t r_b, float* h, int64_t h_b,
