@@ -402,7 +402,9 @@ enum { PHZ_GATE_SIGMOID = 0, PHZ_GATE_DECAY = 1 };
  * h0 [worlds][width] f32: the state before the first step (NULL: zeros).
  * reset [steps][worlds] u8: where nonzero, an episode begins at that step and
  * h_{t-1} counts as 0, whatever it holds. h_last [worlds][width] f32 (or NULL)
- * receives the state after the last step. The state is held in f32. */
+ * receives the state after the last step. The state is held in f32. DECAY's
+ * gates may be any numbers: products of many of them that leave f32's range do
+ * not reach states that stay in it. */
 int phz_gated_scan(phz_ops* ops, void* stream, int form, const phz_tensor* z, const phz_tensor* x, const phz_tensor* h0,
                    const phz_tensor* reset, const phz_tensor* h, const phz_tensor* h_last);
 /* Its gradients: dh, dh_last (f32, or NULL) are the loss's gradients for h and

@@ -34,6 +34,13 @@ namespace {
 
 constexpr int kWaveLanes = 64;
 
+// How waves share a sequence's steps.
+enum Spread {
+  ALONE = 1,   // a wave takes all of them
+  CHUNKS = 4,  // a group of four shares a slab, and takes one of several chunks
+  SLABS = 16   // a group of sixteen shares a slab, and takes all of them
+};
+
 struct ScanArgs {
   const void *z, *x, *h, *dh;   // h and dh: backward only
   void *o1, *o2;                // h | dz, dx
@@ -45,19 +52,47 @@ struct ScanArgs {
   int64_t lanes;                // worlds * groups
   int32_t steps, width, groups; // groups: lanes that cover one world's width
   int32_t chunk, chunks;        // steps per chunk
-  float* agg;                   // [chunks][2][lanes][VEC]: each chunk's A, then H
+  float* agg;                   // [chunks][chunk_words][lanes][VEC]: each chunk's A, H (decay: m, H, e of A = m 2^e)
 };
+constexpr int chunk_words(int form) { return form == PHZ_GATE_DECAY ? 3 : 2; }
 
 // A span in which an episode begins keeps nothing of the state before it, be
 // that infinite or NaN: its A is this NaN, and stands for "forget", which a
 // product that underflows to 0 does not. (A gate that is NaN makes H NaN, so
-// no other NaN in A matters.) A state of 0 passes a span as 0 although gates
-// above 1 may take A past f32's range.
+// no other NaN in A matters.) A state of 0 passes a span as 0.
 constexpr uint32_t kForget = 0x7fc5a5a5u;
 __device__ __forceinline__ bool forgets(float a) { return __builtin_bit_cast(uint32_t, a) == kForget; }
 __device__ __forceinline__ float compose(float a, float s, float h) {
   return forgets(a) || s == 0.0f ? h : fmaf(a, s, h);
 }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
+
+// A where f32 does not hold it: m 2^e, with 1 <= |m| < 2, or 0. In the decay form
+// a product of gates may leave f32's range, and come back, where product times
+// state does not (130 gates of 2 on a state of 0.001, then 130 of 1/2). Sigmoid
+// gates are at most 1: a product below f32's range never grows again, and what it
+// loses is below 2^-126 of the state.
+struct Wide {
+  float m = 1.0f;
+  int32_t e = 0;
+  // A run of these between settles: each at most halves m.
+  __device__ __forceinline__ void times(float c) {
+    m *= __builtin_amdgcn_frexp_mantf(c);
+    e += __builtin_amdgcn_frexp_expf(c);
+  }
+  __device__ __forceinline__ void settle() {
+    e = min(max(e + __builtin_amdgcn_frexp_expf(m) - 1, -(1 << 30)), 1 << 30);
+    m = 2.0f * __builtin_amdgcn_frexp_mantf(m);
+  }
+  __device__ __forceinline__ float compose(float s, float h) const {
+    return forgets(m) ? h : fmaf(m, __builtin_amdgcn_ldexpf(s, e), h);
+  }
+};
+// A run's A is plain f32 where all its gates are within 2^-15 and 2^15, so that
+// the products of its up to eight are in range; else it is this mark, and the
+// Wide product stands beside it.
+constexpr uint32_t kApart = 0x7fc5a5a6u;
+constexpr uint32_t kNarrowLeast = 0x38000000u, kNarrowMost = 0x47000000u;  // 2^-15 and 2^15
 
 // One step's affine map and outputs. `s` is h (forward) or k (backward).
 template <int FORM>
@@ -117,12 +152,15 @@ template <class E, int FORM, bool BACK, int VEC, int NW, int U, bool AGG>
 __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p) {
   static_assert(NW > 1 || !AGG, "chunks are of several waves");
   using S = Step<FORM>;
+  constexpr bool kWide = FORM == PHZ_GATE_DECAY;
+  constexpr int kWords = kWide ? 4 : 2;  // of a run in LDS: A, H, and m and e of an A apart
+  constexpr int kChunkWords = chunk_words(FORM);
   // What a chunk's map needs: forward z, x; backward z and dh only.
   constexpr bool kNeedX = BACK ? (FORM == PHZ_GATE_SIGMOID && !AGG) : true;
   constexpr bool kNeedH = BACK && !AGG;
   using R = Run<E, VEC, U, BACK, kNeedX>;
   // Double-buffered, so one barrier a slab is enough.
-  __shared__ float lds[NW > 1 ? 2 * NW * 2 * VEC * kWaveLanes : 1];
+  __shared__ float lds[NW > 1 ? 2 * NW * kWords * VEC * kWaveLanes : 1];
 
   const int lane = threadIdx.x & 63;
   const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -142,10 +180,38 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
   const E* h = kNeedH ? (const E*)p.h + b * p.h_b + d : nullptr;
   const uint8_t* rs = p.reset ? p.reset + b * p.r_b : nullptr;
 
-  float s[VEC], prod[VEC];
+  auto step_of = [&](int i) { return (int64_t)(BACK ? p.steps - 1 - i : i); };
+  float s[VEC];
+  float prod[VEC];
+  Wide wide[VEC];       // the same, where gates may be above 1
   bool forgot = false;  // the chunk so far (AGG)
 #pragma unroll
   for (int v = 0; v < VEC; v++) s[v] = 0.0f, prod[v] = 1.0f;
+
+  // The steps [from, to) themselves, one after the other. A span's H grows from
+  // 0 and may leave f32's range, or a gate be infinite, where the state that
+  // goes through the span stays finite: where A and H make a state that is not
+  // finite of one that is, the steps decide. Once a state is not finite it stays
+  // so until the next episode, so this is taken about once an episode at most.
+  auto walk = [&](float st, int v, int from, int to) {
+#pragma unroll 1
+    for (int i = from; i < to; i++) {
+      const int64_t t = step_of(i);
+      const float q = S::gate(to_f32(z[t * p.z_t + v])), a = to_f32(BACK ? dh[t * p.dh_t + v] : x[t * p.x_t + v]);
+      const bool rst = rs && rs[t * p.r_t];
+      if (BACK) st = rst ? 0.0f : S::keep(q) * (a + st);
+      else st = S::next(rst ? 0.0f : st, q, a);
+    }
+    return st;
+  };
+  // Channel v's state after the steps [from, to), whose map is (a, h). (An
+  // infinite state stays so whatever finite inputs add, be the sum of those
+  // alone the other infinity.)
+  auto pass = [&](const Wide& a, float h, int v, int from, int to) {
+    const float r = a.compose(s[v], fabsf(s[v]) == __builtin_inff() && fabsf(h) == __builtin_inff() && !forgets(a.m) ? 0.0f : h);
+    s[v] = !forgets(a.m) && finite(s[v]) && !finite(r) ? walk(s[v], v, from, to) : r;
+  };
+
   if (!AGG) {
     if (p.start) {
 #pragma unroll
@@ -153,23 +219,46 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
     }
     // The state that the earlier chunks leave.
     constexpr int kAhead = 32 / VEC;  // chunks whose (A, H) are loaded together
+    constexpr bool kWideChunks = kWide && NW == CHUNKS;
+    const int64_t word = p.lanes * VEC;
+    bool odd = false;
     for (int j0 = 0; j0 < chunk; j0 += kAhead) {
-      Pack<float, VEC> A[kAhead], H[kAhead];
+      Pack<float, VEC> A[kAhead], X[kWideChunks ? kAhead : 1], H[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; j++) {
-        const float* a = p.agg + ((int64_t)min(j0 + j, chunk - 1) * 2 * p.lanes + idc) * VEC;
-        A[j] = load<float, VEC>(a, 0), H[j] = load<float, VEC>(a, p.lanes * VEC);
+        const float* a = p.agg + ((int64_t)min(j0 + j, chunk - 1) * kChunkWords * p.lanes + idc) * VEC;
+        A[j] = load<float, VEC>(a, 0), H[j] = load<float, VEC>(a, word);
+        if constexpr (kWideChunks) X[j] = load<float, VEC>(a, 2 * word);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; j++)
         if (j0 + j < chunk) {
 #pragma unroll
-          for (int v = 0; v < VEC; v++) s[v] = compose(A[j].v[v], s[v], H[j].v[v]);
+          for (int v = 0; v < VEC; v++) {
+            if constexpr (kWideChunks) {
+              s[v] = Wide{A[j].v[v], __builtin_bit_cast(int32_t, X[j].v[v])}.compose(s[v], H[j].v[v]);
+              odd = odd || !finite(s[v]);
+            } else {
+              s[v] = compose(A[j].v[v], s[v], H[j].v[v]);
+            }
+          }
         }
+    }
+    if constexpr (kWideChunks) {
+      if (odd) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          s[v] = p.start ? p.start[b * p.start_b + d + v] : 0.0f;
+#pragma unroll 1
+          for (int j = 0; j < chunk; j++) {
+            const float* a = p.agg + ((int64_t)j * kChunkWords * p.lanes + idc) * VEC + v;
+            pass(Wide{a[0], __builtin_bit_cast(int32_t, a[2 * word])}, a[word], v, j * p.chunk, (j + 1) * p.chunk);
+          }
+        }
+      }
     }
   }
 
-  auto step_of = [&](int i) { return (int64_t)(BACK ? p.steps - 1 - i : i); };
   const bool one_world = __all(b == (int64_t)__builtin_amdgcn_readfirstlane((int)b));
   auto fetch = [&](R& r, int base) {
     if (rs && one_world) r.reset[0] = lane < U && base + lane < last ? rs[step_of(base + lane) * p.r_t] : 0;
@@ -217,6 +306,7 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
       // Compose this wave's run.
       float A[VEC], H[VEC];
       bool forget = false;
+      uint32_t reach = 0;  // of the gates' magnitudes above the least that is narrow
 #pragma unroll
       for (int v = 0; v < VEC; v++) A[v] = 1.0f, H[v] = 0.0f;
 #pragma unroll
@@ -227,21 +317,37 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
           for (int v = 0; v < VEC; v++) {
             H[v] = advance(H[v], u, v, rst);
             A[v] *= S::keep(q[u][v]);
+            if (kWide) reach = max(reach, 2 * __builtin_bit_cast(uint32_t, q[u][v]) - 2 * kNarrowLeast);
           }
           forget = forget || rst;
         }
-      float* mine = lds + buf * (NW * 2 * VEC * kWaveLanes);
+      constexpr int kWord = kWaveLanes * VEC;
+      float* mine = lds + buf * (NW * kWords * kWord);
+      auto word_of = [&](int w, int i, int v) -> float& { return mine[(w * kWords + i) * kWord + lane * VEC + v]; };
+      if (kWide && !forget && reach > 2 * (kNarrowMost - kNarrowLeast)) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          Wide a;
+#pragma unroll
+          for (int u = 0; u < U; u++)
+            if (base + u < last) a.times(q[u][v]);
+          a.settle();
+          word_of(wave, 2, v) = a.m, word_of(wave, 3, v) = __builtin_bit_cast(float, a.e);
+          A[v] = __builtin_bit_cast(float, kApart);
+        }
+      }
 #pragma unroll
       for (int v = 0; v < VEC; v++) {
-        mine[(wave * 2 * kWaveLanes + lane) * VEC + v] = forget ? __builtin_bit_cast(float, kForget) : A[v];
-        mine[((wave * 2 + 1) * kWaveLanes + lane) * VEC + v] = H[v];
+        word_of(wave, 0, v) = forget ? __builtin_bit_cast(float, kForget) : A[v];
+        word_of(wave, 1, v) = H[v];
       }
       __syncthreads();
       // Fold every run of the slab in order; keep the state before this
       // wave's own.
-      float before[VEC];
+      float before[VEC], slab_s[VEC];
+      float odd = 0.0f;  // NaN where some state is not finite
 #pragma unroll
-      for (int v = 0; v < VEC; v++) before[v] = s[v];
+      for (int v = 0; v < VEC; v++) before[v] = slab_s[v] = s[v];
 #pragma unroll
       for (int w = 0; w < NW; w++) {
         if (w == wave) {
@@ -250,13 +356,46 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
         }
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
-          const float a = mine[(w * 2 * kWaveLanes + lane) * VEC + v];
-          const float g = mine[((w * 2 + 1) * kWaveLanes + lane) * VEC + v];
-          s[v] = compose(a, s[v], g);
+          const float a = word_of(w, 0, v);
+          s[v] = compose(a, s[v], word_of(w, 1, v));
+          if (kWide) odd = fmaf(0.0f, s[v], odd);
           if (AGG) {
             forgot = forgot || forgets(a);
             prod[v] *= a;
           }
+        }
+      }
+      if constexpr (kWide) {
+        auto run_of = [&](int w, int v) {
+          const float a = word_of(w, 0, v);
+          Wide r{a, 0};
+          if (__builtin_bit_cast(uint32_t, a) == kApart)
+            r.m = word_of(w, 2, v), r.e = __builtin_bit_cast(int32_t, word_of(w, 3, v));
+          return r;
+        };
+        // An A apart, or a state that is not finite: each run with care.
+        if (odd != odd) {
+#pragma unroll
+          for (int v = 0; v < VEC; v++) {
+            s[v] = slab_s[v];
+#pragma unroll 1
+            for (int w = 0; w < NW; w++) {
+              if (w == wave) before[v] = s[v];
+              pass(run_of(w, v), word_of(w, 1, v), v, min(slab + w * U, last), min(slab + (w + 1) * U, last));
+            }
+          }
+        }
+        if (AGG && wave == 0) {  // who stores it
+#pragma unroll
+          for (int w = 0; w < NW; w++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+              const Wide r = run_of(w, v);
+              wide[v].times(r.m);
+              wide[v].e += r.e;
+            }
+#pragma unroll
+          for (int v = 0; v < VEC; v++) wide[v].settle();
         }
       }
       if (!AGG) {
@@ -328,9 +467,13 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
 
   if (AGG) {
     if (live && wave == 0) {
-      float* a = p.agg + ((int64_t)chunk * 2 * p.lanes + id) * VEC;
+      const int64_t word = p.lanes * VEC;
+      float* a = p.agg + ((int64_t)chunk * kChunkWords * p.lanes + id) * VEC;
 #pragma unroll
-      for (int v = 0; v < VEC; v++) a[v] = forgot ? __builtin_bit_cast(float, kForget) : prod[v], a[p.lanes * VEC + v] = s[v];
+      for (int v = 0; v < VEC; v++) {
+        a[v] = forgot ? __builtin_bit_cast(float, kForget) : kWide ? wide[v].m : prod[v], a[word + v] = s[v];
+        if (kWide) a[2 * word + v] = __builtin_bit_cast(float, wide[v].e);
+      }
     }
   } else if (p.end && chunk == p.chunks - 1 && live && wave == 0) {
 #pragma unroll
@@ -338,14 +481,8 @@ __global__ __launch_bounds__(NW * kWaveLanes) void gated_scan_kernel(ScanArgs p)
   }
 }
 
-// How waves share a sequence's steps, and the steps that each loads ahead of
-// the ones it computes: more hide more of memory's latency, and leave registers
-// for fewer waves.
-enum Spread {
-  ALONE = 1,   // a wave takes all of them
-  CHUNKS = 4,  // a group of four shares a slab, and takes one of several chunks
-  SLABS = 16   // a group of sixteen shares a slab, and takes all of them
-};
+// The steps that each wave loads ahead of the ones it computes: more hide more
+// of memory's latency, and leave registers for fewer waves.
 template <class E>
 constexpr int run_steps(bool back, int spread) {
   return spread == ALONE ? (back ? 2 : 4) : back && sizeof(E) == 4 ? 4 : 8;
@@ -504,7 +641,7 @@ int scan(phz_ops* o, hipStream_t stream, int form, bool back, ScanArgs a, int dt
   a.chunk = p.chunk;
   a.chunks = p.chunks;
   if (p.chunks > 1) {
-    a.agg = (float*)o->workspace(stream, (uint64_t)p.chunks * 2 * p.lanes * p.vec * sizeof(float));
+    a.agg = (float*)o->workspace(stream, (uint64_t)p.chunks * chunk_words(form) * p.lanes * p.vec * sizeof(float));
     if (!a.agg) return 1;
   }
   if (dtype == PHZ_F32) launch_any<float>(a, form, back, p.vec, p.spread, stream);
