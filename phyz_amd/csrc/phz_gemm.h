@@ -44,7 +44,11 @@ template <> struct Any<float> { static constexpr int tile_k = 32, ld = 36; };
 // the six largest are taken (hh, hm, mh, mm, hl, lh); what is left out is below
 // 2^-22 of |a||b|. Six products of the bf16 rate are 2.7 times the rate of the
 // f32 matrix instructions.
-// The three pieces of x. Where x is not finite, all of it is in the first.
+//
+// The three pieces of x. One that is not finite is (+-1, 0, x): the last piece
+// meets only the other operand's first one, which is 0 where the operand is, so
+// every product is what f32 makes of it: infinity times a number that infinity,
+// times 0 NaN, times infinity (h l and l h) theirs.
 __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t& l) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
   const bool finite = (b & 0x7f800000u) != 0x7f800000u;
@@ -52,10 +56,10 @@ __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t
   const float r = finite ? x - hf : 0.0f;
   const uint32_t rb = __builtin_bit_cast(uint32_t, r);
   const float mf = __builtin_bit_cast(float, rb & 0xffff0000u);
-  const bool nan = !finite && (b & 0x007fffffu);
-  h = nan ? (uint16_t)0x7fc0u : (uint16_t)(b >> 16);
+  const bool nan = b & 0x007fffffu;
+  h = (uint16_t)(finite ? b >> 16 : (b >> 16 & 0x8000u) | 0x3f80u);
   m = (uint16_t)(rb >> 16);
-  l = (uint16_t)(__builtin_bit_cast(uint32_t, r - mf) >> 16);
+  l = (uint16_t)(finite ? __builtin_bit_cast(uint32_t, r - mf) >> 16 : nan ? 0x7fc0u : b >> 16);
 }
 
 // Moves one operand's tile of ROWS rows by tile_k through registers into LDS,

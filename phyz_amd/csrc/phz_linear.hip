@@ -144,41 +144,6 @@ struct PlainOut : NothingAhead {
   }
 };
 
-// For f32 operands cut in three planes: a sum that is not finite is taken again
-// from the operands themselves, one element at a time. An infinite element
-// times the zero pieces of a finite one would have made it NaN.
-template <class Epi>
-struct Repair {
-  static constexpr bool kRagged = Epi::kRagged;
-  Epi to;
-  const bf16 *a, *b;
-  int64_t a_i, a_k, a_plane, b_j, b_k, b_plane;  // elements
-  int32_t k;
-  typedef typename Epi::Held Held;
-  typedef typename Epi::Columns Columns;
-  __device__ __forceinline__ void columns(int j, int left, Columns& c) const { to.columns(j, left, c); }
-  __device__ __forceinline__ void fetch(int q, int i, int j, int left, Held& h) const { to.fetch(q, i, j, left, h); }
-  __device__ __noinline__ float again(int i, int j) const {
-    float sum = 0.0f;
-    for (int t = 0; t < k; t++) {
-      const bf16 *x = a + i * a_i + t * a_k, *y = b + j * b_j + t * b_k;
-      sum = fmaf(to_f32(x[0]) + (to_f32(x[a_plane]) + to_f32(x[2 * a_plane])),
-                 to_f32(y[0]) + (to_f32(y[b_plane]) + to_f32(y[2 * b_plane])), sum);
-    }
-    return sum;
-  }
-  __device__ __forceinline__ void put8(int q, int s, int i, int j, int left, const float* sums, const Held& h,
-                                       const Columns& col) const {
-    float v[8];
-#pragma unroll
-    for (int c = 0; c < 8; c++) {
-      v[c] = sums[c];
-      if (c < left && !(fabsf(v[c]) < __builtin_inff())) v[c] = again(i, j + c);
-    }
-    to.put8(q, s, i, j, left, v, h, col);
-  }
-};
-
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // ── few rows ────────────────────────────────────────────────────────────────
@@ -551,7 +516,7 @@ FastPlan plan(const phz_ops* o, Way way, int64_t m, int64_t n, int64_t k) {
 }
 
 // The product of two operands, C of m x n, contraction k; AK, BK: dense along
-// it. Epilogues of cut products are repaired where sums are not finite.
+// it.
 template <class E, bool AK, bool BK, class Epi, class Beside = NothingBeside>
 void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<E>& b, int64_t m, int64_t n, int64_t k,
              const FastPlan& plan, float* part, const Epi& epi, const Beside& beside = {}) {
@@ -561,13 +526,8 @@ void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<
   f.a_plane = (uint32_t)(a.plane() * 2), f.b_plane = (uint32_t)(b.plane() * 2);
   f.m = (int32_t)m, f.n = (int32_t)n, f.k = (int32_t)k;
   f.a_rows = (int32_t)(AK ? a.rows : a.whole_cols()), f.b_rows = (int32_t)(BK ? b.rows : b.whole_cols());
-  if constexpr (sizeof(E) == 4) {
-    if (a.way == CUT) {
-      const Repair<Epi> safe{epi, (const bf16*)a.data(), (const bf16*)b.data(), AK ? a.row() : 1, AK ? 1 : a.row(),
-                             a.plane(), BK ? b.row() : 1, BK ? 1 : b.row(), b.plane(), (int32_t)k};
-      return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, safe, beside);
-    }
-  }
+  if constexpr (sizeof(E) == 4)
+    if (a.way == CUT) return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, epi, beside);
   launch_gemm_fast<E, 1, AK, BK>(o, stream, f, 1, plan, part, epi, beside);
 }
 
