@@ -39,11 +39,15 @@ template <class E> struct Any;
 template <> struct Any<bf16> { static constexpr int tile_k = 64, ld = 72; };
 template <> struct Any<float> { static constexpr int tile_k = 32, ld = 36; };
 
-// x = h + m + l in bf16 pieces by truncation: 8 bits of the significand each,
-// 24 in all, so the cut is exact. Of the nine products of two numbers' pieces
-// the six largest are taken (hh, hm, mh, mm, hl, lh); what is left out is below
-// 2^-22 of |a||b|. Six products of the bf16 rate are 2.7 times the rate of the
-// f32 matrix instructions.
+// x = h + m + l in bf16 pieces, each the nearest to what the ones before leave
+// (h cut off where the nearest is infinite). For |x| in [2^e, 2^(e+1)) what h
+// leaves is at most 2^(e-8) and a multiple of 2^(e-23), what m leaves at most
+// 2^(e-17): seven bits, so the cut is exact (from 2^-110 on; a smaller x loses
+// what is below bf16's least, 2^-133). Of the nine products of two numbers'
+// pieces the six largest are taken (hh, hm, mh, mm, hl, lh); what is left out,
+// ml + lm + ll, is at most 2^-24 (1 + 2^-9) of |a||b|, of either sign: no more
+// than one rounding to f32. Six products of the bf16 rate are 2.7 times the rate
+// of the f32 matrix instructions.
 //
 // The three pieces of x. One that is not finite is (+-1, 0, x): the last piece
 // meets only the other operand's first one, which is 0 where the operand is, so
@@ -51,15 +55,16 @@ template <> struct Any<float> { static constexpr int tile_k = 32, ld = 36; };
 // times 0 NaN, times infinity (h l and l h) theirs.
 __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t& l) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
-  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-  const float hf = __builtin_bit_cast(float, b & 0xffff0000u);
-  const float r = finite ? x - hf : 0.0f;
-  const uint32_t rb = __builtin_bit_cast(uint32_t, r);
-  const float mf = __builtin_bit_cast(float, rb & 0xffff0000u);
-  const bool nan = b & 0x007fffffu;
-  h = (uint16_t)(finite ? b >> 16 : (b >> 16 & 0x8000u) | 0x3f80u);
-  m = (uint16_t)(rb >> 16);
-  l = (uint16_t)(finite ? __builtin_bit_cast(uint32_t, r - mf) >> 16 : nan ? 0x7fc0u : b >> 16);
+  if ((b & 0x7f800000u) == 0x7f800000u) {
+    h = (uint16_t)((b >> 16 & 0x8000u) | 0x3f80u), m = 0;
+    l = (uint16_t)(b & 0x007fffffu ? 0x7fc0u : b >> 16);
+    return;
+  }
+  bf16 p = from_f32<bf16>(x);
+  if ((p.bits & 0x7f80u) == 0x7f80u) p.bits = (uint16_t)(b >> 16);
+  const float r = x - to_f32(p);
+  const bf16 q = from_f32<bf16>(r);
+  h = p.bits, m = q.bits, l = from_f32<bf16>(r - to_f32(q)).bits;
 }
 
 // Moves one operand's tile of ROWS rows by tile_k through registers into LDS,

@@ -4,8 +4,9 @@
 //
 // Operands are one plane of 16-bit elements, f32 (through the f32 matrix
 // instructions: exact products at a sixteenth of the rate), or a sum of planes:
-//   two    A = hi + lo, f32 data cut in f16: lo hi + hi lo + hi hi (lo lo is
-//          below what f32 sums hold), for data of a known range;
+//   two    A = hi + lo, f32 data cut in f16: lo hi + hi lo + hi hi (lo lo, at
+//          most 2^-22 of a product, is left out as the cut's own 2^-23 are), for
+//          data of a known range;
 //   three  A = h + m + l, f32 data cut in bf16 without loss (cut3): six of the
 //          nine products, as in phz_gemm.h, for any data.
 // Rows are 16-byte aligned and, along k (or along rows, for
