@@ -24,6 +24,7 @@ and then raises.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 
 import torch
@@ -173,7 +174,9 @@ class Ops:
     # ── the linear layer ──
     @staticmethod
     def _rows(t):
-        return t.reshape(-1, t.shape[-1]) if isinstance(t, torch.Tensor) and t.dim() > 2 else t
+        if not isinstance(t, torch.Tensor) or t.dim() <= 2:
+            return t
+        return t.reshape(math.prod(t.shape[:-1]), t.shape[-1])  # -1 says nothing where no element is
 
     def linear(self, x, w, bias=None, act: str = "none", residual=None, save_pre: bool = False, out=None):
         """y = act(x w^T + bias) + residual for x [..., n_in], w [n_out, n_in];
