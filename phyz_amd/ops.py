@@ -105,7 +105,9 @@ class Ops:
             raise OpsError(f"{name} is on {t.device}: {where}")
         if t.dtype not in _DTYPES:
             raise OpsError(f"{name} is {t.dtype}, expected float32, bfloat16 or a mask of uint8 or bool")
-        raise OpsError(f"{name} has {t.dim()} dimensions, expected 1 to 3")
+        if not 1 <= t.dim() <= 3:
+            raise OpsError(f"{name} has {t.dim()} dimensions, expected 1 to 3")
+        raise OpsError(f"{name} has no strided memory to read here (a sparse tensor, or one inside vmap or a trace)")
 
     def _stream(self):
         return _raw_stream(self.device) if self.device >= 0 else None
@@ -184,6 +186,8 @@ class Ops:
         `out` (2-D) may be the residual."""
         a = self._choice(ACTS, act, "activation")
         x2, r2 = self._rows(self._tensor(x, "x")), self._rows(residual)
+        if x.dim() < 2:
+            raise OpsError(f"x has {x.dim()} dimensions, expected 2 or more")
         if self._tensor(w, "w").dim() != 2:
             raise OpsError(f"w has {w.dim()} dimensions, expected 2")
         y = out if out is not None else torch.empty((x2.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
@@ -200,7 +204,8 @@ class Ops:
         needed are None. The residual's gradient is dy itself."""
         a = self._choice(ACTS, act, "activation")
         x2, dy2, p2 = self._rows(self._tensor(x, "x")), self._rows(dy), self._rows(pre)
-        self._tensor(w, "w")
+        if self._tensor(w, "w").dim() != 2:
+            raise OpsError(f"w has {w.dim()} dimensions, expected 2")
         dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
         db = torch.empty(w.shape[:1], dtype=w.dtype, device=w.device) if need_db else None

@@ -28,3 +28,19 @@ def test_batches_without_elements(ops, call):
     """As their two-dimensional forms: right, and only then without a device."""
     with pytest.raises(OpsError, match="host-only"):
         call(ops)
+
+
+@pytest.mark.parametrize("call, message", [
+    (lambda o: torch.vmap(lambda z: o.gated_scan(z, z))(t(3, 6, 2, 5)), "z has no strided memory"),
+    (lambda o: torch.vmap(lambda z: o.gated_step(z, z, t(2, 5)))(t(3, 2, 5)), "z has no strided memory"),
+    (lambda o: torch.vmap(lambda x: o.linear(x, t(7, 3)))(t(3, 4, 3)), "x has no strided memory"),
+    (lambda o: o.gated_scan(t(6, 2, 5).to_sparse(), t(6, 2, 5)), "z has no strided memory"),
+    (lambda o: o.gated_scan(t(()), t(())), "z has 0 dimensions, expected 1 to 3"),
+    (lambda o: o.linear(t(()), t(7, 3)), "x has 0 dimensions, expected 2 or more"),
+    (lambda o: o.linear(t(3), t(7, 3)), "x has 1 dimensions, expected 2 or more"),
+    (lambda o: o.linear_backward(t(4, 7), t(4, 3), t(3)), "w has 1 dimensions, expected 2"),
+    (lambda o: o.linear_backward(t(4, 7), t(4, 3), t(())), "w has 0 dimensions, expected 2"),
+])
+def test_refusals_name_the_reason(ops, call, message):
+    with pytest.raises(OpsError, match=message):
+        call(ops)
