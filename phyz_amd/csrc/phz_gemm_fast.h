@@ -68,10 +68,10 @@ struct FastArgs {
 // output register; the wait state is the one that a write of m0 needs.
 __device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void dma16(uint32_t lds, const char* at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory", "m0");
 }
 
 // One operand's tile of ROWS rows by BK: how it lies in LDS, how NW waves
