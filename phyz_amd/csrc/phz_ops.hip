@@ -124,25 +124,24 @@ bool apart(phz_ops* o, const char* an, const phz_tensor* a, const char* bn, cons
   span(a, &al, &ah);
   span(b, &bl, &bh);
   if (ah <= bl || bh <= al) return true;
-  // Interleaved views: rows of the same steps, whose dense parts lie beside
-  // each other within the smallest step.
-  if (a->ndim == b->ndim && a->ndim > 1 && a->dtype == b->dtype) {
-    const int last = a->ndim - 1;
-    const int64_t e = elem_bytes(a->dtype);
-    int64_t step = 0;
-    bool same = (a->size[last] <= 1 || a->stride[last] == 1) && (b->size[last] <= 1 || b->stride[last] == 1);
-    for (int i = 0; i < last && same; i++) {
-      if (a->size[i] <= 1 && b->size[i] <= 1) continue;
-      same = a->stride[i] == b->stride[i] && a->stride[i] > 0;
-      if (same) step = step ? std::min(step, a->stride[i]) : a->stride[i];
-    }
-    for (int i = 0; i < last && same && step; i++)
-      if ((a->size[i] > 1 || b->size[i] > 1) && a->stride[i] % step) same = false;
-    if (same && step) {
-      const int64_t delta = (int64_t)(bl - al), pitch = step * e;
-      const int64_t off = ((delta % pitch) + pitch) % pitch;
-      if (off >= a->size[last] * e && pitch - off >= b->size[last] * e) return true;
-    }
+  // Interleaved views (halves of a buffer's rows, a record's first step beside its
+  // others): modulo a stride of either, axes whose strides are its multiples
+  // vanish, and the rest of each view is within one stretch of residues. Where
+  // those do not meet, no element does.
+  const int64_t ea = elem_bytes(a->dtype), eb = elem_bytes(b->dtype);
+  auto stretch = [](const phz_tensor* t, int64_t e, int64_t mod) {
+    int64_t n = e;
+    for (int i = 0; i < t->ndim; i++)
+      if (t->size[i] > 1 && t->stride[i] * e % mod) n += (t->size[i] - 1) * t->stride[i] * e;
+    return n;
+  };
+  for (int k = 0; k < a->ndim + b->ndim; k++) {
+    const phz_tensor* t = k < a->ndim ? a : b;
+    const int i = k < a->ndim ? k : k - a->ndim;
+    const int64_t mod = t->size[i] > 1 ? t->stride[i] * (t == a ? ea : eb) : 0;
+    if (mod <= 0) continue;
+    const int64_t off = (((int64_t)(bl - al) % mod) + mod) % mod;
+    if (off >= stretch(a, ea, mod) && mod - off >= stretch(b, eb, mod)) return true;
   }
   o->err = fmt("%s overlaps %s", an, bn);
   return false;

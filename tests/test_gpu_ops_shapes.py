@@ -43,3 +43,19 @@ def test_rows_far_apart_give_the_same_bits(ops):
     dx = ops.linear_backward(x, dy, torch.randn(k, n, device="cuda").to(BF16), need_dx=False, need_db=False)[1]
     assert torch.equal(dx, ops.linear_backward(x.contiguous(), dy, torch.zeros(k, n, device="cuda").to(BF16), need_dx=False,
                                                need_db=False)[1])
+
+
+@pytest.mark.parametrize("T, B, D", [(40, 3, 13), (600, 300, 64), (4000, 2, 33)])
+def test_a_record_of_states(ops, T, B, D):
+    """h0 and the states, or the states and the last one, side by side in one record
+    [worlds, steps + 1, width]."""
+    z, x = torch.randn(T, B, D, device="cuda"), torch.randn(T, B, D, device="cuda")
+    h0 = torch.randn(B, D, device="cuda")
+    h, last = ops.gated_scan(z, x, h0=h0)
+    record = torch.full((B, T + 1, D), 7.0, device="cuda")
+    record[:, 0] = h0
+    end = torch.empty(B, D, device="cuda")
+    ops.gated_scan(z, x, h0=record[:, 0], out=(record[:, 1:].transpose(0, 1), end))
+    assert torch.equal(record[:, 0], h0) and torch.equal(record[:, 1:].transpose(0, 1), h) and torch.equal(end, last)
+    ops.gated_scan(z, x, h0=h0, out=(record[:, :T].transpose(0, 1), record[:, T]))
+    assert torch.equal(record[:, :T].transpose(0, 1), h) and torch.equal(record[:, T], last)
