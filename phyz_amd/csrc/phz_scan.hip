@@ -102,18 +102,19 @@ template <>
 struct Step<PHZ_GATE_SIGMOID> {
   // The gate as its smaller side c with z's sign (signed_gate):
   // h' = h + c (x - h) where the gate keeps, x + c (h - x) where it writes, so
-  // a gate at rest leaves the state exactly as it is.
+  // a gate at rest leaves the state exactly as it is. Differences are taken of
+  // halves, which stay in f32's range where x - h does not; the bits are the same.
   static __device__ __forceinline__ float gate(float z) { return signed_gate(z); }
   static __device__ __forceinline__ float keep(float q) { return __float_as_int(q) < 0 ? fabsf(q) : 1.0f - fabsf(q); }
   static __device__ __forceinline__ float write(float q) { return __float_as_int(q) < 0 ? 1.0f - fabsf(q) : fabsf(q); }
   static __device__ __forceinline__ float next(float h, float q, float x) {
     const bool w = __float_as_int(q) < 0;
     const float base = w ? x : h, other = w ? h : x;
-    return fmaf(fabsf(q), other - base, base);
+    return fmaf(2.0f * fabsf(q), fmaf(-0.5f, base, 0.5f * other), base);
   }
   static __device__ __forceinline__ float dz(float e, float hp, float x, float q) {
     const float c = fabsf(q);
-    return e * (hp - x) * (c * (1.0f - c));
+    return e * fmaf(-0.5f, x, 0.5f * hp) * (2.0f * c * (1.0f - c));
   }
 };
 
