@@ -20,6 +20,9 @@ torch's current stream and return without waiting. Errors raise OpsError with
 the library's message. There is no host fallback: the kernels run on a HIP
 device or not at all. Ops(device=-1) checks arguments only (of CPU tensors)
 and then raises.
+
+Autograd records none of this: gradients come from the _backward calls. What a
+call writes in place or into `out` counts as changed for graphs that saved it.
 """
 from __future__ import annotations
 
@@ -64,6 +67,11 @@ def _current_stream(device: int) -> int:
 
 # The same without the Stream object, where this torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
+
+
+# Tells autograd that tensors were written to, so that a graph which saved their
+# values refuses to use them.
+_written = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
 class OpsError(RuntimeError):
@@ -152,6 +160,8 @@ class Ops:
             h = torch.empty_like(self._tensor(x, "x"))
             last = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device)
         self._run(_SCAN, f, "z x h0 reset h h_last", z, x, h0, reset, h, last)
+        if out is not None:
+            _written([t for t in out if t is not None])
         return h, last
 
     def gated_scan_backward(self, dh, z, x, h, h0=None, reset=None, dh_last=None, form: str = "sigmoid", out=None):
@@ -164,6 +174,8 @@ class Ops:
             dz, dx = torch.empty_like(self._tensor(z, "z")), torch.empty_like(self._tensor(x, "x"))
             dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device)
         self._run(_SCAN_BACKWARD, f, "dh dh_last z x h h0 reset dz dx dh0", dh, dh_last, z, x, h, h0, reset, dz, dx, dh0)
+        if out is not None:
+            _written([t for t in out if t is not None])
         return dz, dx, dh0
 
     def gated_step(self, z, x, h, reset=None, form: str = "sigmoid"):
@@ -171,6 +183,7 @@ class Ops:
         replaced, and returned."""
         f = self._choice(FORMS, form, "gate form")
         self._run(_STEP, f, "z x reset h", z, x, reset, h)
+        _written((h,))
         return h
 
     # ── the linear layer ──
@@ -193,6 +206,8 @@ class Ops:
         y = out if out is not None else torch.empty((x2.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
         pre = torch.empty((x2.shape[0], w.shape[0]), dtype=x.dtype, device=x.device) if save_pre else None
         self._run(_LINEAR, a, "x w bias residual pre y", x2, w, bias, r2, pre, y)
+        if out is not None:
+            _written((y,))
         shape = (*x.shape[:-1], w.shape[0])
         if out is None and x.dim() != 2:
             y = y.view(shape)
@@ -224,6 +239,8 @@ class Ops:
         cfg = self._muon(steps, coef, eps)
         o = out if out is not None else torch.empty_like(self._tensor(g, "g"))
         self._run(_ORTHOGONALIZE, C.addressof(cfg), "g o", g, o)
+        if out is not None:
+            _written((o,))
         return o
 
     def muon_step(self, w, g, m, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
@@ -232,3 +249,4 @@ class Ops:
         the gradient g: matrices [rows, cols], or a batch of them."""
         cfg = self._muon(steps, coef, eps, lr, momentum, nesterov, weight_decay)
         self._run(_MUON, C.addressof(cfg), "w g m", w, g, m)
+        _written((w, m))
