@@ -28,8 +28,11 @@ union {
   void* at[7];
 } g_entries;
 const int kTensors[7] = {6, 10, 4, 6, 7, 2, 3};
+// Whose results a user may expect autograd to know: not the gradients' own
+// operators and the update's.
+const bool kForward[7] = {true, false, true, true, false, true, false};
 
-PyObject *g_dtypes[5], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device;
+PyObject *g_dtypes[5], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device, *g_requires_grad;
 const int kCodes[5] = {PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_U8};
 
 // False, with no Python error left, where `o` is no tensor that can be
@@ -74,11 +77,12 @@ bool describe(PyObject* o, long device, phz_tensor* t) {
   return ok;
 }
 
-// call(op, handle, stream, device, head, tensors): the entry point's result, or
-// -1 - i where tensor i cannot be described.
+// call(op, handle, stream, device, head, tensors, unrecorded): the entry point's
+// result, -1 - i where tensor i cannot be described, or, unless `unrecorded`,
+// -101 - i where a forward operator's tensor i requires gradients.
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 6 || !PyTuple_Check(args[5])) {
-    PyErr_SetString(PyExc_TypeError, "call(op, handle, stream, device, head, tensors)");
+  if (n != 7 || !PyTuple_Check(args[5])) {
+    PyErr_SetString(PyExc_TypeError, "call(op, handle, stream, device, head, tensors, unrecorded)");
     return nullptr;
   }
   const long op = PyLong_AsLong(args[0]), device = PyLong_AsLong(args[3]);
@@ -96,6 +100,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyObject* o = PyTuple_GET_ITEM(args[5], i);
     if (o == Py_None) continue;
     if (!describe(o, device, &d[i])) return PyLong_FromLong(-1 - i);
+    if (kForward[op] && args[6] == Py_False) {
+      PyObject* v = PyObject_GetAttr(o, g_requires_grad);
+      if (!v) return nullptr;
+      Py_DECREF(v);
+      if (v == Py_True) return PyLong_FromLong(-101 - i);
+    }
     t[i] = &d[i];
   }
   const Entries& f = g_entries.fn;
@@ -141,7 +151,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_describe", nullptr, -1, g_metho
 PyMODINIT_FUNC PyInit__describe() {
   static_assert(sizeof(phz_tensor) == 64, "phz_tensor");
   const struct { PyObject** at; const char* name; } names[] = {
-      {&g_data_ptr, "data_ptr"}, {&g_shape, "shape"}, {&g_stride, "stride"}, {&g_dtype, "dtype"}, {&g_get_device, "get_device"}};
+      {&g_data_ptr, "data_ptr"}, {&g_shape, "shape"}, {&g_stride, "stride"}, {&g_dtype, "dtype"}, {&g_get_device, "get_device"},
+      {&g_requires_grad, "requires_grad"}};
   for (auto& s : names)
     if (!(*s.at = PyUnicode_InternFromString(s.name))) return nullptr;
   return PyModule_Create(&g_module);

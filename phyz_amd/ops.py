@@ -21,8 +21,11 @@ the library's message. There is no host fallback: the kernels run on a HIP
 device or not at all. Ops(device=-1) checks arguments only (of CPU tensors)
 and then raises.
 
-Autograd records none of this: gradients come from the _backward calls. What a
-call writes in place or into `out` counts as changed for graphs that saved it.
+Autograd records none of this: gradients come from the _backward calls. The
+forward operators refuse tensors that require gradients while it is recording
+(call them under torch.no_grad(), or on detached tensors); the _backward calls
+and muon_step take them as they are. What a call writes in place or into `out`
+counts as changed for graphs that saved it.
 """
 from __future__ import annotations
 
@@ -99,7 +102,13 @@ class Ops:
     # ── calls ──
     def _run(self, op: int, head: int, names: str, *tensors):
         """One entry point on the current stream; `names` are the tensors'."""
-        rc = self._call(op, self._h, _raw_stream(self.device) if self.device >= 0 else 0, self.device, head, tensors)
+        stream = _raw_stream(self.device) if self.device >= 0 else 0
+        rc = self._call(op, self._h, stream, self.device, head, tensors, False)
+        if rc < -100:
+            if torch.is_grad_enabled():
+                raise OpsError(f"{names.split()[-101 - rc]} requires gradients, which these operators do not record: call under "
+                               "torch.no_grad() or with detach(), and take the gradients from the _backward calls")
+            rc = self._call(op, self._h, stream, self.device, head, tensors, True)
         if rc > 0:
             raise OpsError(self._L.phz_ops_last_error(self._h).decode())
         if rc < 0:
