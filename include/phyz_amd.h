@@ -365,7 +365,10 @@ int phz_train_time_update(phz_train* t, const uint32_t* const* order, const uint
  *   - Workspace belongs to the handle, one block per stream, grown on demand.
  *     A call that would have to grow it while its stream is being captured is
  *     refused: run the call once before the capture, or phz_ops_reserve. A
- *     captured graph uses the block of the stream it was captured on.
+ *     captured graph has a block of its own, the size of its stream's, so it may
+ *     be replayed on any stream, beside other graphs and other calls (not beside
+ *     itself). The handle keeps that block until it is destroyed, which is only
+ *     allowed once no such graph will run again.
  *   - A handle is not thread-safe. Results do not depend on timing: the same
  *     call on the same inputs gives the same bits. ── */
 typedef struct phz_ops phz_ops;
@@ -391,6 +394,8 @@ const char* phz_ops_last_error(const phz_ops* ops);
 int phz_ops_reserve(phz_ops* ops, void* stream, uint64_t bytes);
 /* Workspace bytes that the handle holds, over all streams. */
 uint64_t phz_ops_workspace_bytes(const phz_ops* ops);
+/* Those of them that captured graphs work in. */
+uint64_t phz_ops_graph_bytes(const phz_ops* ops);
 
 /* How a recurrence reads its gate z:
  * SIGMOID  c = sigmoid(z), h_t = c h_{t-1} + (1 - c) x_t

@@ -135,6 +135,7 @@ SIGNATURES = {
     "phz_ops_last_error": (C.c_char_p, [OPS]),
     "phz_ops_reserve": (C.c_int, [OPS, STREAM, C.c_uint64]),
     "phz_ops_workspace_bytes": (C.c_uint64, [OPS]),
+    "phz_ops_graph_bytes": (C.c_uint64, [OPS]),
     "phz_gated_scan": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 6),
     "phz_gated_scan_backward": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 10),
     "phz_gated_step": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 4),

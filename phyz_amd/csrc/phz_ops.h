@@ -17,11 +17,10 @@ struct phz_ops {
   int cus = 256;
   std::string err;
   // Zeros that out-of-range lanes of direct-to-LDS loads read.
-  void* zeros = nullptr;
-  struct Block { void* stream; void* data; uint64_t bytes; };
-  std::vector<Block> blocks;  // one per stream
-  std::vector<Block> retired; // outgrown blocks that a captured graph may use
-  bool captured = false;
+  const void* zeros = nullptr;
+  // One for a stream's own calls, and for each capture on it that needed one.
+  struct Block { void* stream; void* data; uint64_t bytes; bool graph; unsigned long long capture; };
+  std::vector<Block> blocks;
 
   int fail(const std::string& m) {
     err = m;

@@ -6,6 +6,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
 
 using namespace phzop;
 
@@ -13,49 +15,93 @@ namespace {
 
 thread_local std::string g_ops_create_error;
 
+// 256 zero bytes on a device, which captured graphs read too: one for all handles,
+// never freed.
+const void* zeros_of(phz_ops* o) {
+  static std::mutex lock;
+  static std::map<int, void*> made;
+  std::lock_guard<std::mutex> hold(lock);
+  void*& z = made[o->device];
+  if (!z) {
+    void* p = nullptr;
+    if (!o->hip_ok(hipMalloc(&p, 256), "zeros")) return nullptr;
+    if (!o->hip_ok(hipMemset(p, 0, 256), "zeros") || !o->hip_ok(hipDeviceSynchronize(), "create")) {
+      (void)hipFree(p);
+      return nullptr;
+    }
+    z = p;
+  }
+  return z;
+}
+
 }  // namespace
 
+// A stream's own calls and each capture on it work in blocks of their own, since
+// a graph may be replayed on any stream, beside another one's replay and beside
+// the stream's own calls. A capture takes the block that the stream's calls have
+// grown (they get another when they next need one), or, where an earlier capture
+// has taken that, allocates its like.
 char* phz_ops::workspace(hipStream_t stream, uint64_t bytes) {
   bytes = std::max<uint64_t>((bytes + 255) & ~255ull, 256);
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long capture = 0;
   if (!hip_ok(hipStreamIsCapturing(stream, &status), "hipStreamIsCapturing")) return nullptr;
   const bool capturing = status != hipStreamCaptureStatusNone;
-  Block* b = nullptr;
+  if (capturing && !hip_ok(hipStreamGetCaptureInfo(stream, &status, &capture), "hipStreamGetCaptureInfo")) return nullptr;
+  Block *own = nullptr, *eager = nullptr;
+  uint64_t known = 0;  // the most that the stream's calls or captures have had
   for (auto& x : blocks)
-    if (x.stream == (void*)stream) b = &x;
-  if (!b || b->bytes < bytes) {
-    if (capturing) {
+    if (x.stream == (void*)stream) {
+      known = std::max(known, x.bytes);
+      if (!x.graph) eager = &x;
+      if (x.graph == capturing && x.capture == capture && (!own || own->bytes < x.bytes)) own = &x;
+    }
+  if (own && own->bytes >= bytes) return (char*)own->data;
+  if (capturing) {
+    if (eager && eager->bytes >= bytes) {
+      eager->graph = true;
+      eager->capture = capture;
+      return (char*)eager->data;
+    }
+    if (known < bytes) {
       err = fmt("the stream is being captured and its workspace would have to grow to %llu bytes: run the call once "
                 "before, or phz_ops_reserve",
                 (unsigned long long)bytes);
       return nullptr;
     }
-    // Half as much again as asked, so that growing sizes do not allocate on
-    // every call.
-    uint64_t want = bytes + bytes / 2;
+    // An allocation is no part of the capture; this mode lets it pass.
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (!hip_ok(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode")) return nullptr;
     void* p = nullptr;
-    if (hipMalloc(&p, want) != hipSuccess) {
+    const bool ok = hip_ok(hipMalloc(&p, known), "workspace");
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) {
       (void)hipGetLastError();
-      want = bytes;
-      if (!hip_ok(hipMalloc(&p, want), "workspace")) {
-        (void)hipGetLastError();
-        return nullptr;
-      }
+      return nullptr;
     }
-    if (b) {
-      // hipFree waits for the device, so work in flight has ended; a captured
-      // graph may run again, and keeps its block.
-      if (captured) retired.push_back(*b);
-      else (void)hipFree(b->data);
-      b->data = p;
-      b->bytes = want;
-    } else {
-      blocks.push_back(Block{(void*)stream, p, want});
-      b = &blocks.back();
+    blocks.push_back(Block{(void*)stream, p, known, true, capture});
+    return (char*)p;
+  }
+  // Half as much again as asked, so that growing sizes do not allocate on
+  // every call.
+  uint64_t want = std::max(bytes + bytes / 2, known);
+  void* p = nullptr;
+  if (hipMalloc(&p, want) != hipSuccess) {
+    (void)hipGetLastError();
+    want = bytes;
+    if (!hip_ok(hipMalloc(&p, want), "workspace")) {
+      (void)hipGetLastError();
+      return nullptr;
     }
   }
-  captured = captured || capturing;
-  return (char*)b->data;
+  if (own) {
+    (void)hipFree(own->data);  // waits for the device, so work in flight has ended
+    own->data = p;
+    own->bytes = want;
+  } else {
+    blocks.push_back(Block{(void*)stream, p, want, false, 0});
+  }
+  return (char*)p;
 }
 
 namespace phzop {
@@ -170,11 +216,9 @@ int phz_ops_create(int device_ordinal, phz_ops** out) {
     int cus = 0;
     bool ok = g.ok && o->hip_ok(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device_ordinal),
                                 "compute units");
-    ok = ok && o->hip_ok(hipMalloc(&o->zeros, 256), "zeros") && o->hip_ok(hipMemset(o->zeros, 0, 256), "zeros") &&
-         o->hip_ok(hipDeviceSynchronize(), "create");
+    ok = ok && (o->zeros = zeros_of(o));
     if (!ok) {
       g_ops_create_error = o->err;
-      if (o->zeros) (void)hipFree(o->zeros);
       delete o;
       return 1;
     }
@@ -192,8 +236,6 @@ void phz_ops_destroy(phz_ops* o) {
   if (o->device >= 0) {
     DeviceGuard g(o);
     for (auto& b : o->blocks) (void)hipFree(b.data);
-    for (auto& b : o->retired) (void)hipFree(b.data);
-    if (o->zeros) (void)hipFree(o->zeros);
   }
   delete o;
 }
@@ -212,8 +254,14 @@ uint64_t phz_ops_workspace_bytes(const phz_ops* o) {
   uint64_t n = 0;
   if (o) {
     for (auto& b : o->blocks) n += b.bytes;
-    for (auto& b : o->retired) n += b.bytes;
   }
+  return n;
+}
+
+uint64_t phz_ops_graph_bytes(const phz_ops* o) {
+  uint64_t n = 0;
+  if (o)
+    for (auto& b : o->blocks) n += b.graph ? b.bytes : 0;
   return n;
 }
 

@@ -82,7 +82,9 @@ class OpsError(RuntimeError):
 
 
 class Ops:
-    """A handle: one GPU's operators and their workspaces (one per stream)."""
+    """A handle: one GPU's operators and their workspaces, one per stream and one
+    per captured graph. A handle whose workspace a captured graph holds is kept to
+    the end of the process, so that the graph outlives the last reference to it."""
 
     def __init__(self, device: int = 0):
         self._L = _lib.load()
@@ -96,7 +98,8 @@ class Ops:
     def __del__(self):
         h = getattr(self, "_h", None)
         if h:
-            self._L.phz_ops_destroy(h)
+            if not self._L.phz_ops_graph_bytes(h):
+                self._L.phz_ops_destroy(h)
             self._h = None
 
     # ── calls ──
