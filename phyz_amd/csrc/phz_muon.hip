@@ -714,9 +714,9 @@ bool sizes(phz_ops* o, const char* name, const phz_tensor* t, Sizes* s) {
     return o->err = fmt("%s has %d dimensions, expected a matrix or a batch of them", name, t->ndim), false;
   const int k = t->ndim - 2;
   *s = Sizes{k ? t->size[0] : 1, t->size[k], t->size[k + 1]};
-  if (s->rows > 32768 || s->cols > 1 << 20 || s->cols * s->rows > 1ll << 30 || std::min(s->rows, s->cols) > 32768)
-    return o->err = fmt("%s is %lld x %lld: at most 32768 rows and 2^30 elements a matrix", name, (long long)s->rows,
-                        (long long)s->cols),
+  if (s->rows > 32768 || s->cols > 1 << 20 || s->cols * s->rows > 1ll << 30)
+    return o->err = fmt("%s is %lld x %lld: at most 32768 rows, 2^20 columns and 2^30 elements a matrix", name,
+                        (long long)s->rows, (long long)s->cols),
            false;
   if (s->batch > 65535) return o->err = "at most 65535 matrices a call", false;
   return true;

@@ -44,3 +44,10 @@ def test_batches_without_elements(ops, call):
 def test_refusals_name_the_reason(ops, call, message):
     with pytest.raises(OpsError, match=message):
         call(ops)
+
+
+@pytest.mark.parametrize("rows, cols", [(32769, 1), (1, (1 << 20) + 1), (32768, 32769)])
+def test_limits_of_a_matrix_are_named(ops, rows, cols):
+    g = t(1, 1).expand(rows, cols)
+    with pytest.raises(OpsError, match=f"g is {rows} x {cols}: at most 32768 rows, 2\\^20 columns and 2\\^30 elements"):
+        ops.orthogonalize(g, out=g)
