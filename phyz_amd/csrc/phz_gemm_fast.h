@@ -171,8 +171,9 @@ struct Tile {
 // Bound by the matrix cores and the reads of LDS that feed them, which take
 // about as long on 64 x 64 of a wave and two thirds on 128 x 64: 8192 x 8192 x
 // 8192 bf16 903 us, 1217 TFLOP/s; 32768 x 1024 -> 4096 with GELU and residual
-// 386 us, 712 TFLOP/s, where every 16 stages a tile's way out has the compute
-// unit to itself.
+// 381 to 404 us (720 to 680 TFLOP/s) by card in a steady train of launches, 420
+// after an idle moment and up to 480 in the first ten, where every 16 stages a
+// tile's way out has the compute unit to itself.
 template <class T, int PL, bool AK, bool BKD, class Shape, bool RAGGED, class Epi>
 __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi epi) {
   constexpr int BM = Shape::BM, BN = Shape::BN, BK = Shape::BK, NS = Shape::NS, NG = Shape::NG;

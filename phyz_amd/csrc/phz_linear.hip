@@ -305,8 +305,12 @@ __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v)
 
 // dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
 // rows of `dz_row` with zeros past n, or cut into three planes of such rows, and
-// the sums of dz over each block's rows, which ColumnSums adds up in order. A
-// thread takes eight columns; `across` (a power of two, at most 32) of them lie
+// the sums of dz over each block's rows, which ColumnSums adds up in order. For
+// bf16 operands dz goes to the products in bf16, as the matrix cores take it
+// (db's sums have it in f32): gradients are then 0.0023 off 64 bits, relative,
+// where rounding the results alone gives 0.0017 (8191 x 1000 -> 1001), and both
+// products take half the instructions and dz half the bytes that a second plane
+// of it would cost. A thread takes eight columns; `across` (a power of two, at most 32) of them lie
 // along a row, the others take rows in turn. Bound by memory: 40793 x 1760 bf16
 // 77 us for 431 MB (5.6 TB/s), 16384 x 256 f32 10.7 us for 50 MB, of which some
 // 4 us are the launch's ramp and the sums.
@@ -474,8 +478,9 @@ enum Way { AS_IS, CUT, ANY };  // ANY: gemm_any
 // the sizes along dense axes are whole 16 bytes, so that usually nothing needs
 // a copy; from `copy_from` multiply-adds on the copies pay all the same. f32
 // goes to bf16 pieces from 2^33 multiply-adds on, where their rate pays for the
-// cuts (us, f32 instructions / pieces: 2048 x 1024 -> 1024 43 / 50, 4096 x 1024
-// -> 1024 80 / 71, 8192 x 1024 -> 1024 140 / 110).
+// cuts (us, f32 instructions / pieces: 2048 x 1024 -> 1024 45 / 53, 4096 x 1024
+// -> 1024 77 / 70, 8192 x 1024 -> 1024 139 / 107, 16384 x 1024 -> 1024 265 / 198;
+// not at every size: 4100 x 2056 -> 1032 174 / 200).
 template <class E>
 Way way_of(int64_t m, int64_t n, int64_t k, bool whole) {
   constexpr int64_t copy_from = 1ll << 30;

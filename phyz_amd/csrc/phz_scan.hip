@@ -562,14 +562,16 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const void* z, int64_t 
 // least two slabs up to 16 waves a compute unit in all, at most 64 chunks (each
 // start folds its predecessors), of lanes of four channels, or of one where
 // even so the waves would be few.
-// One MI355X, us:                    alone  sixteen  chunks  bytes at a copy's rate
-//   64 x 4096 x 256 f32, forward     158    158      161     173
-//   512 x 64 x 512 f32, forward      .      42       61      43
-//   512 x 64 x 512 f32, backward     90     78       89      86
-//   1023 x 61 x 515 bf16, backward   .      92       115     69
-//   4000 x 100 x 128 f32, backward   .      394      325     264
-//   32768 x 1 x 2048 bf16, forward   .      .        157     86
-//   4096 x 1 x 512 f32, forward      .      .        14.5    5.4
+// One MI355X, us:                            alone  sixteen  chunks  bytes at a copy's rate
+//   64 x 4096 x 256 f32, forward             159    214      164     173
+//   512 x 64 x 512 f32, forward              155    39       63      43
+//   512 x 64 x 512 f32, backward             393    87       100     86
+//   1023 x 61 x 515 bf16 decay, backward     662    96       119     69
+//   4000 x 100 x 128 f32, backward           .      448      372     264
+//   32768 x 1 x 2048 bf16, forward           .      1261     167     86
+//   4096 x 1 x 512 f32, forward              .      162      15.8    5.4
+// (sigmoid where not said otherwise; decay takes less, though the exponents of its
+// products are 1 to 7% of its sixteen and 2 to 15% of its chunks.)
 // What chunks cost above their bytes is the second reading.
 struct Plan {
   int vec, spread, chunk, chunks;
