@@ -435,8 +435,9 @@ int phz_linear(phz_ops* ops, void* stream, int act, const phz_tensor* x, const p
                const phz_tensor* residual, const phz_tensor* pre, const phz_tensor* y);
 /* Its gradients for dz = dy act'(pre): dx = dz W, dw = dz^T x, db = the sum of
  * dz over rows; each of dx, dw, db may be NULL. The residual's gradient is dy.
- * pre may be NULL for PHZ_ACT_NONE. In bf16, dz is rounded to bf16 before the
- * products, as the matrix cores take it. */
+ * pre may be NULL for PHZ_ACT_NONE. In bf16, the products take dz in two pieces
+ * (to 2^-16 of itself), so that gradients are rounded once, where they are
+ * stored. */
 int phz_linear_backward(phz_ops* ops, void* stream, int act, const phz_tensor* dy, const phz_tensor* x,
                         const phz_tensor* w, const phz_tensor* pre, const phz_tensor* dx, const phz_tensor* dw,
                         const phz_tensor* db);

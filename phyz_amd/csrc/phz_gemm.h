@@ -24,6 +24,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct Operand {
   const void* data;
   int64_t row, batch;
+  int64_t plane;  // of A, where it is the sum of two planes
 };
 
 struct GemmShape {
@@ -65,6 +66,17 @@ __device__ __forceinline__ void cut3(float x, uint16_t& h, uint16_t& m, uint16_t
   const float r = x - to_f32(p);
   const bf16 q = from_f32<bf16>(r);
   h = p.bits, m = q.bits, l = from_f32<bf16>(r - to_f32(q)).bits;
+}
+
+// v = hi + lo to 2^-16 of itself, of one sign: hi v's first eight bits, lo the
+// nearest to the rest. lo is never 0 beside a number hi (2^-30 of it instead, or
+// 1 beside infinity), so that infinity times v is infinity in both products.
+__device__ __forceinline__ void cut2(float v, bf16& hi, bf16& lo) {
+  hi.bits = (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16);
+  const float h = to_f32(hi);
+  if (v != v) hi.bits = 0x7fc0u;
+  const float rest = fabsf(h) < __builtin_inff() ? v - h : copysignf(1.0f, h);
+  lo = from_f32<bf16>(rest != 0.0f ? rest : h * 0x1p-30f);
 }
 
 // Moves one operand's tile of ROWS rows by tile_k through registers into LDS,
@@ -187,7 +199,9 @@ __device__ __forceinline__ void store_some(E* p, const Pack<E, 8>& from, int lef
 // way together, take registers that whole rows would miss (32768 x 1024 -> 4096
 // bf16 388 us, 412 with both in one), and one at a time, after each other, cost
 // a load's latency each (54038 x 252 -> 135: 73 us, so 49).
-template <class E, bool AK, bool BKD, int BM, int BN, bool RAGGED, class Epi>
+//
+// PA: planes of A, both in a stage.
+template <class E, bool AK, bool BKD, int PA, int BM, int BN, bool RAGGED, class Epi>
 __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape s, Epi epi) {
   constexpr int BK = Any<E>::tile_k, LD = Any<E>::ld, PER = 16 / sizeof(E);
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
@@ -195,8 +209,8 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
   using SB = Stage<E, BKD, BN>;
   constexpr int kOutRow = WN + 4;  // floats of one staged output row
   static_assert(4 * 32 * kOutRow * 4 <= (BM + BN) * LD * (int)sizeof(E), "output rows fit the tiles");
-  __shared__ __attribute__((aligned(16))) E la[(BM + BN) * LD];
-  E* lb = la + BM * LD;
+  __shared__ __attribute__((aligned(16))) E la[(PA * BM + BN) * LD];
+  E* lb = la + PA * BM * LD;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
   const int q = blockIdx.z / s.splits, split = blockIdx.z - q * s.splits;
@@ -213,26 +227,30 @@ __global__ __launch_bounds__(256) void gemm_any(Operand a, Operand b, GemmShape 
     for (int j = 0; j < TN; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
-  SA sa;
+  SA sa[PA];
   SB sb;
-  sa.load(pa, a.row, m0, s.m, k0, k_end);
-  sb.load(pb, b.row, n0, s.n, k0, k_end);
+  auto load = [&](int k) {
+#pragma unroll
+    for (int h = 0; h < PA; h++) sa[h].load(h ? pa + a.plane : pa, a.row, m0, s.m, k, k_end);
+    sb.load(pb, b.row, n0, s.n, k, k_end);
+  };
+  load(k0);
   for (int k = k0; k < k_end; k += BK) {
     __syncthreads();
-    sa.store(la);
+#pragma unroll
+    for (int h = 0; h < PA; h++) sa[h].store(la + h * BM * LD);
     sb.store(lb);
     __syncthreads();
-    if (k + BK < k_end) {
-      sa.load(pa, a.row, m0, s.m, k + BK, k_end);
-      sb.load(pb, b.row, n0, s.n, k + BK, k_end);
-    }
+    if (k + BK < k_end) load(k + BK);
 #pragma unroll
     for (int kk = 0; kk < BK; kk += 2 * PER)
 #pragma unroll
       for (int i = 0; i < TM; i++)
 #pragma unroll
         for (int j = 0; j < TN; j++)
-          acc[i][j] = multiply(la + (wm + i * 32 + fr) * LD + kk + fk, lb + (wn + j * 32 + fr) * LD + kk + fk, acc[i][j]);
+#pragma unroll
+          for (int h = PA - 1; h >= 0; h--)
+            acc[i][j] = multiply(la + (h * BM + wm + i * 32 + fr) * LD + kk + fk, lb + (wn + j * 32 + fr) * LD + kk + fk, acc[i][j]);
   }
 
   // Out through LDS, 32 rows of a wave's part at a time, so that each lane
@@ -286,7 +304,7 @@ struct NothingAhead : NoColumns {
 
 // Launches gemm_any with the tile that fills the chip: 128 x 128 where those
 // are two for every compute unit and not mostly beyond the edge, 64 x 64 below.
-template <class E, bool AK, bool BKD, class Epi>
+template <class E, bool AK, bool BKD, int PA = 1, class Epi>
 void launch_gemm_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b, GemmShape s, int batch, Epi epi) {
   const int64_t z = (int64_t)batch * s.splits;
   const bool large = s.m > 64 && s.n > 64 && ceil_div(s.m, 128) * ceil_div(s.n, 128) * z >= 2ll * o->cus;
@@ -296,11 +314,11 @@ void launch_gemm_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b,
   };
   if constexpr (Epi::kRagged) {
     if (s.n % 8) {
-      large ? go(gemm_any<E, AK, BKD, 128, 128, true, Epi>) : go(gemm_any<E, AK, BKD, 64, 64, true, Epi>);
+      large ? go(gemm_any<E, AK, BKD, PA, 128, 128, true, Epi>) : go(gemm_any<E, AK, BKD, PA, 64, 64, true, Epi>);
       return;
     }
   }
-  large ? go(gemm_any<E, AK, BKD, 128, 128, false, Epi>) : go(gemm_any<E, AK, BKD, 64, 64, false, Epi>);
+  large ? go(gemm_any<E, AK, BKD, PA, 128, 128, false, Epi>) : go(gemm_any<E, AK, BKD, PA, 64, 64, false, Epi>);
 }
 
 }  // namespace phzop

@@ -9,6 +9,7 @@
 //          data of a known range;
 //   three  A = h + m + l, f32 data cut in bf16 without loss (cut3): six of the
 //          nine products, as in phz_gemm.h, for any data.
+// A may have two planes where B has one: lo b + hi b, f32 data (cut2) with bf16.
 // Rows are 16-byte aligned and, along k (or along rows, for
 // operands dense along rows), whole 16 bytes long or padded with zeros to them.
 #pragma once
@@ -174,13 +175,14 @@ struct Tile {
 // 381 to 404 us (720 to 680 TFLOP/s) by card in a steady train of launches, 420
 // after an idle moment and up to 480 in the first ten, where every 16 stages a
 // tile's way out has the compute unit to itself.
-template <class T, int PL, bool AK, bool BKD, class Shape, bool RAGGED, class Epi>
+// PL, PB: planes of A and of B.
+template <class T, int PL, int PB, bool AK, bool BKD, class Shape, bool RAGGED, class Epi>
 __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi epi) {
   constexpr int BM = Shape::BM, BN = Shape::BN, BK = Shape::BK, NS = Shape::NS, NG = Shape::NG;
   constexpr int NWAVE = Shape::MW * Shape::NW;
   constexpr int WM = BM / Shape::MW, WN = BN / Shape::NW, TM = WM / 32, TN = WN / 32, SK = BK / PL;
   using TA = FastTile<T, AK, BM, BK, NWAVE, PL>;
-  using TB = FastTile<T, BKD, BN, BK, NWAVE, PL>;
+  using TB = FastTile<T, BKD, BN, SK * PB, NWAVE, PB>;
   constexpr int kOne = TA::kBytes + TB::kBytes, kStage = NG * kOne, kLoads = TA::kPerWave + TB::kPerWave;
   constexpr int kOutRow = WN + 4;  // floats of one staged output row
   constexpr int kOut = NG * NWAVE * 32 * kOutRow * 4;
@@ -248,13 +250,15 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
     now = now == (NS - 1) * kStage ? 0 : now + kStage;
 #pragma unroll
     for (int kk = 0; kk < SK; kk += Mfma<T>::kStep) {
-      s16x8 fa[PL][TM], fb[PL][TN];
+      s16x8 fa[PL][TM], fb[PB][TN];
 #pragma unroll
       for (int h = 0; h < PL; h++) {
 #pragma unroll
         for (int i = 0; i < TM; i++) fa[h][i] = TA::read(l, lane, wm + i * 32, h, kk);
+        if (h < PB) {
 #pragma unroll
-        for (int j = 0; j < TN; j++) fb[h][j] = TB::read(l + TA::kBytes, lane, wn + j * 32, h, kk);
+          for (int j = 0; j < TN; j++) fb[h][j] = TB::read(l + TA::kBytes, lane, wn + j * 32, h, kk);
+        }
       }
 #pragma unroll
       for (int i = 0; i < TM; i++)
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void gemm_fast(FastArgs p, Epi 
           }
           if constexpr (PL >= 2) {
             acc[i][j] = Mfma<T>::run(fa[1][i], fb[0][j], acc[i][j]);
-            acc[i][j] = Mfma<T>::run(fa[0][i], fb[1][j], acc[i][j]);
+            if constexpr (PB >= 2) acc[i][j] = Mfma<T>::run(fa[0][i], fb[1][j], acc[i][j]);
           }
           acc[i][j] = Mfma<T>::run(fa[0][i], fb[0][j], acc[i][j]);
         }
@@ -356,7 +360,8 @@ template <> struct Tiles<float, 1> {
   typedef Tile<64, 64, 32, 2, 2, 2> Small;  // four
 };
 
-enum { PLANES_F32 = 0 };  // plan_fast's name for f32 operands as they are
+// plan_fast's names for f32 operands as they are, and for two planes by one.
+enum { PLANES_F32 = 0, PLANES_2BY1 = 21 };
 
 struct FastPlan {
   int tile;  // 0 big, 1 mid, 2 deep, 3 small, 4 two
@@ -391,13 +396,15 @@ inline FastPlan plan_fast(const phz_ops* o, int64_t m, int64_t n, int64_t k, int
   struct Kind { int bm, bn, per_cu; double alone, full; };
   const Kind one[5] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 1, 0.6, 0.6}, {64, 64, 1, 0.24, 0.24}, {64, 64, 2, 0.32, 0.42},
                        {128, 128, 2, 0.68, 1.3}};
+  const Kind two_by_one[5] = {{256, 256, 1, 1.6, 1.6}, {128, 128, 1, 0.62, 0.62}, {64, 64, 1, 0.24, 0.24}, {64, 64, 2, 0.32, 0.44},
+                              {128, 128, 2, 0.8, 1.05}};
   const Kind three[4] = {{256, 128, 1, 2.8, 2.8}, {128, 128, 1, 1.5, 1.5}, {64, 64, 1, 0.45, 0.45}, {64, 64, 2, 0.6, 0.8}};
   const Kind f32[4] = {{}, {}, {64, 64, 1, 0.57, 0.57}, {64, 64, 4, 0.6, 2.0}};
-  const Kind* kinds = planes == 3 ? three : planes == PLANES_F32 ? f32 : one;
+  const Kind* kinds = planes == 3 ? three : planes == PLANES_F32 ? f32 : planes == PLANES_2BY1 ? two_by_one : one;
   const int64_t sk = planes == 1 ? 64 : 32, stages = std::max<int64_t>(1, ceil_div(k, sk));
   FastPlan best{};
   double least = 1e30;
-  for (int t = planes == PLANES_F32 ? 2 : 0; t < (kinds == one ? 5 : 4); t++) {
+  for (int t = planes == PLANES_F32 ? 2 : 0; t < (kinds == three || kinds == f32 ? 4 : 5); t++) {
     const Kind& kind = kinds[t];
     const int64_t tiles = ceil_div(m, kind.bm) * ceil_div(n, kind.bn) * batch;
     for (int64_t splits = 1; splits <= (may_split ? 64 : 1); splits *= 2) {
@@ -497,7 +504,7 @@ void launch_join(hipStream_t stream, const PartOut& sums, int batch, int splits,
 
 // `part`: plan.part_bytes of workspace. `beside` goes with the join: to plans
 // with splits, and one matrix, only.
-template <class T, int PL, bool AK, bool BKD, class Epi, class Beside = NothingBeside>
+template <class T, int PL, bool AK, bool BKD, int PB = PL, class Epi, class Beside = NothingBeside>
 void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batch, const FastPlan& plan, float* part,
                       const Epi& epi, const Beside& beside = {}) {
   p.zeros = (const char*)o->zeros;
@@ -512,16 +519,16 @@ void launch_gemm_fast(const phz_ops* o, hipStream_t stream, FastArgs p, int batc
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)batch, (unsigned)p.splits);
     const dim3 block(S::kThreads);
     if (p.splits > 1) {
-      hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, false, PartOut>), grid, block, 0, stream, p, sums);
+      hipLaunchKernelGGL((gemm_fast<T, PL, PB, AK, BKD, S, false, PartOut>), grid, block, 0, stream, p, sums);
       return;
     }
     if constexpr (Epi::kRagged) {
       if (p.n % 8) {
-        hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, true, Epi>), grid, block, 0, stream, p, epi);
+        hipLaunchKernelGGL((gemm_fast<T, PL, PB, AK, BKD, S, true, Epi>), grid, block, 0, stream, p, epi);
         return;
       }
     }
-    hipLaunchKernelGGL((gemm_fast<T, PL, AK, BKD, S, false, Epi>), grid, block, 0, stream, p, epi);
+    hipLaunchKernelGGL((gemm_fast<T, PL, PB, AK, BKD, S, false, Epi>), grid, block, 0, stream, p, epi);
   };
   if constexpr (sizeof(T) == 2) {
     if (plan.tile == 0) go(typename Tiles<T, PL>::Big{});
@@ -552,14 +559,14 @@ AnyPlan plan_any(const phz_ops* o, int64_t m, int64_t n, int64_t k) {
   p.part_bytes = p.splits > 1 ? (uint64_t)p.splits * m * ((n + 7) / 8 * 8) * 4 : 0;
   return p;
 }
-template <class E, bool AK, bool BKD, class Epi, class Beside = NothingBeside>
+template <class E, bool AK, bool BKD, int PA = 1, class Epi, class Beside = NothingBeside>
 void launch_any(const phz_ops* o, hipStream_t stream, Operand a, Operand b, int64_t m, int64_t n, int64_t k,
                 const AnyPlan& plan, float* part, const Epi& epi, const Beside& beside = {}) {
   const GemmShape s{(int32_t)m, (int32_t)n, (int32_t)k, plan.k_split, plan.splits};
-  if (plan.splits == 1) return launch_gemm_any<E, AK, BKD>(o, stream, a, b, s, 1, epi);
+  if (plan.splits == 1) return launch_gemm_any<E, AK, BKD, PA>(o, stream, a, b, s, 1, epi);
   const int64_t row = (n + 7) / 8 * 8;
   const PartOut sums{part, row, m * row, m * row};
-  launch_gemm_any<E, AK, BKD>(o, stream, a, b, s, 1, sums);
+  launch_gemm_any<E, AK, BKD, PA>(o, stream, a, b, s, 1, sums);
   launch_join(stream, sums, 1, plan.splits, s.m, s.n, epi, beside);
 }
 

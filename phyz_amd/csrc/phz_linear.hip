@@ -4,6 +4,7 @@
 #include "phz_gemm_fast.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace phzop;
 
@@ -293,6 +294,15 @@ void launch_few_rows(hipStream_t stream, const phz_tensor* x, const phz_tensor* 
   else p.wide ? go(few_rows<E, 4, 2, Epi>, 32) : go(few_rows<E, 4, 1, Epi>, 16);
 }
 
+// Eight f32 as two planes of bf16, the second `plane` elements on.
+__device__ __forceinline__ void put_two(bf16* to, int64_t plane, const float* v) {
+  Pack<bf16, 8> hi, lo;
+#pragma unroll
+  for (int c = 0; c < 8; c++) cut2(v[c], hi.v[c], lo.v[c]);
+  *(Pack<bf16, 8>*)to = hi;
+  *(Pack<bf16, 8>*)(to + plane) = lo;
+}
+
 // Eight f32 as three planes of bf16.
 __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v) {
   Pack<bf16, 8> h, m, l;
@@ -306,11 +316,10 @@ __device__ __forceinline__ void put_cut(bf16* to, int64_t plane, const float* v)
 // dz = dy act'(pre) (where there is an activation, or the copy is wanted) in
 // rows of `dz_row` with zeros past n, or cut into three planes of such rows, and
 // the sums of dz over each block's rows, which ColumnSums adds up in order. For
-// bf16 operands dz goes to the products in bf16, as the matrix cores take it
-// (db's sums have it in f32): gradients are then 0.0023 off 64 bits, relative,
-// where rounding the results alone gives 0.0017 (8191 x 1000 -> 1001), and both
-// products take half the instructions and dz half the bytes that a second plane
-// of it would cost. A thread takes eight columns; `across` (a power of two, at most 32) of them lie
+// bf16 operands with an activation dz is two planes of bf16 (cut2), the second
+// `plane` on in the same row: rounded to one, it would be a second rounding of
+// the gradients, as large as their own (1 x 33 -> 13: 0.0033 off 64 bits,
+// relative, for 0.0020). A thread takes eight columns; `across` (a power of two, at most 32) of them lie
 // along a row, the others take rows in turn. Bound by memory: 40793 x 1760 bf16
 // 77 us for 431 MB (5.6 TB/s), 16384 x 256 f32 10.7 us for 50 MB, of which some
 // 4 us are the launch's ramp and the sums.
@@ -339,8 +348,13 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
         out.v[c] = from_f32<E>(v);
         all[c] = v;
       }
-      if (dz) *(Pack<E, 8>*)(dz + i * dz_row + j) = out;
-      if (cut) put_cut(cut + i * dz_row + j, plane, all);
+      if constexpr (sizeof(E) == 2) {
+        if (dz && plane) put_two(dz + i * dz_row + j, plane, all);
+        else if (dz) *(Pack<E, 8>*)(dz + i * dz_row + j) = out;
+      } else {
+        if (dz) *(Pack<E, 8>*)(dz + i * dz_row + j) = out;
+        if (cut) put_cut(cut + i * dz_row + j, plane, all);
+      }
     }
   } else if (j < n) {
     for (int64_t i = i0 + lane; i < i1; i += lanes) {
@@ -354,9 +368,13 @@ __global__ __launch_bounds__(256) void dz_rows(int act, const E* dy, int64_t dy_
           total[c] += v;
         }
         all[c] = v;
-        if (dz) dz[i * dz_row + j + c] = from_f32<E>(v);  // dz_row is whole eights
+        if (dz && !(sizeof(E) == 2 && plane)) dz[i * dz_row + j + c] = from_f32<E>(v);  // rows are whole eights
       }
-      if (cut) put_cut(cut + i * dz_row + j, plane, all);
+      if constexpr (sizeof(E) == 2) {
+        if (dz && plane) put_two(dz + i * dz_row + j, plane, all);
+      } else {
+        if (cut) put_cut(cut + i * dz_row + j, plane, all);
+      }
     }
   }
   if (!sums && !db) return;
@@ -495,7 +513,7 @@ struct Lain {
   const E* from;
   int64_t from_row, rows, cols;
   Way way;
-  bool well;
+  bool well, two = false;  // two: a copy of two planes, a row of one beside the other's
   char* copy = nullptr;
   Lain(const phz_tensor* t, Way w)
       : from((const E*)t->data), from_row(t->stride[0]), rows(t->size[0]), cols(t->size[1]), way(w) {
@@ -503,10 +521,12 @@ struct Lain {
     well = way == ANY || (way == AS_IS && (uintptr_t)from % 16 == 0 && from_row % el == 0 && cols % el == 0 &&
                           from_row <= 1 << 22);
   }
-  int64_t plane() const { return way == CUT ? (rows * pad8(cols) + 127) / 128 * 128 : 0; }  // elements
-  uint64_t bytes() const { return way == CUT ? 3 * plane() * 2 : rows * pad8(cols) * sizeof(E); }
+  int64_t plane() const {  // elements
+    return way == CUT ? (rows * pad8(cols) + 127) / 128 * 128 : two ? pad8(cols) : 0;
+  }
+  uint64_t bytes() const { return way == CUT ? 3 * plane() * 2 : rows * row() * sizeof(E); }
   const void* data() const { return well ? (const void*)from : copy; }
-  int64_t row() const { return well ? from_row : pad8(cols); }
+  int64_t row() const { return well ? from_row : pad8(cols) * (two ? 2 : 1); }
   int64_t whole_cols() const { return well ? cols : pad8(cols); }
   void lay(hipStream_t stream) const {
     const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows * (pad8(cols) / 8), 256), 8192);
@@ -517,8 +537,8 @@ struct Lain {
 };
 
 template <class E>
-FastPlan plan(const phz_ops* o, Way way, int64_t m, int64_t n, int64_t k) {
-  return plan_fast(o, m, n, k, 1, way == CUT ? 3 : sizeof(E) == 4 ? (int)PLANES_F32 : 1, true);
+FastPlan plan(const phz_ops* o, Way way, int64_t m, int64_t n, int64_t k, bool two = false) {
+  return plan_fast(o, m, n, k, 1, way == CUT ? 3 : sizeof(E) == 4 ? (int)PLANES_F32 : two ? (int)PLANES_2BY1 : 1, true);
 }
 
 // The product of two operands, C of m x n, contraction k; AK, BK: dense along
@@ -532,8 +552,11 @@ void product(const phz_ops* o, hipStream_t stream, const Lain<E>& a, const Lain<
   f.a_plane = (uint32_t)(a.plane() * 2), f.b_plane = (uint32_t)(b.plane() * 2);
   f.m = (int32_t)m, f.n = (int32_t)n, f.k = (int32_t)k;
   f.a_rows = (int32_t)(AK ? a.rows : a.whole_cols()), f.b_rows = (int32_t)(BK ? b.rows : b.whole_cols());
-  if constexpr (sizeof(E) == 4)
+  if constexpr (sizeof(E) == 4) {
     if (a.way == CUT) return launch_gemm_fast<bf16, 3, AK, BK>(o, stream, f, 1, plan, part, epi, beside);
+  } else if constexpr (!BK) {  // A is dz
+    if (a.two) return launch_gemm_fast<bf16, 2, AK, BK, 1>(o, stream, f, 1, plan, part, epi, beside);
+  }
   launch_gemm_fast<E, 1, AK, BK>(o, stream, f, 1, plan, part, epi, beside);
 }
 
@@ -597,9 +620,10 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   const bool fast = way != ANY;
   Lain<E> d(dy, way), xo(x, way), wo(w, way);
   if (act != PHZ_ACT_NONE) d.well = false;  // dz is made here
+  d.two = sizeof(E) == 2 && act != PHZ_ACT_NONE;
   FastPlan dx_plan{}, dw_plan{};
-  if (fast && need_dx) dx_plan = plan<E>(o, way, m, k, pad8(n));
-  if (fast && need_dw) dw_plan = plan<E>(o, way, n, k, m);
+  if (fast && need_dx) dx_plan = plan<E>(o, way, m, k, pad8(n), d.two);
+  if (fast && need_dw) dw_plan = plan<E>(o, way, n, k, m, d.two);
   AnyPlan dx_any{1, 1, 0}, dw_any{1, 1, 0};
   if (!fast && need_dx) dx_any = plan_any<E>(o, m, k, n);
   if (!fast && need_dw) dw_any = plan_any<E>(o, n, k, m);
@@ -628,8 +652,8 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
   if (m > 0 && (lay_d || db)) {
     hipLaunchKernelGGL(dz_rows<E>, dim3((unsigned)ceil_div(n, across * 8), (unsigned)blocks), dim3(256), 0, stream, act,
                        (const E*)dy->data, dy->stride[0], pre ? (const E*)pre->data : nullptr, pre ? pre->stride[0] : 0,
-                       (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(), pad8(n), sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)m, (int32_t)n,
-                       (int32_t)rows, across);
+                       (E*)(way == CUT ? nullptr : d.copy), (bf16*)(way == CUT ? d.copy : nullptr), d.plane(),
+                       pad8(n) * (d.two ? 2 : 1), sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)m, (int32_t)n, (int32_t)rows, across);
   }
   // db goes with the join of dw's splits where there is one.
   const ColumnSums<E> bias{sums, db ? (E*)db->data : nullptr, db ? db->stride[0] : 0, (int32_t)blocks, (int32_t)n,
@@ -646,12 +670,21 @@ int linear_backward(phz_ops* o, hipStream_t stream, int act, const phz_tensor* d
       product<E, false, false>(o, stream, d, xo, n, k, m, dw_plan, part, PlainOut<E>{(E*)dw->data, dw->stride[0]}, bias);
     }
   } else {
-    const Operand dop{d.copy ? d.copy : dy->data, d.copy ? pad8(n) : dy->stride[0], 0}, xa{x->data, x->stride[0], 0},
-        wa{w->data, w->stride[0], 0};
-    if (need_dx)
-      launch_any<E, true, false>(o, stream, dop, wa, m, k, n, dx_any, part, PlainOut<E>{(E*)dx->data, dx->stride[0]});
-    if (need_dw)
-      launch_any<E, false, false>(o, stream, dop, xa, n, k, m, dw_any, part, PlainOut<E>{(E*)dw->data, dw->stride[0]}, bias);
+    const Operand dop{d.copy ? d.copy : dy->data, d.copy ? pad8(n) * (d.two ? 2 : 1) : dy->stride[0], 0, d.plane()},
+        xa{x->data, x->stride[0], 0}, wa{w->data, w->stride[0], 0};
+    auto both = [&](auto planes) {
+      constexpr int PA = decltype(planes)::value;
+      if (need_dx)
+        launch_any<E, true, false, PA>(o, stream, dop, wa, m, k, n, dx_any, part, PlainOut<E>{(E*)dx->data, dx->stride[0]});
+      if (need_dw)
+        launch_any<E, false, false, PA>(o, stream, dop, xa, n, k, m, dw_any, part, PlainOut<E>{(E*)dw->data, dw->stride[0]},
+                                        bias);
+    };
+    if constexpr (sizeof(E) == 2) {
+      d.two ? both(std::integral_constant<int, 2>{}) : both(std::integral_constant<int, 1>{});
+    } else {
+      both(std::integral_constant<int, 1>{});
+    }
   }
   if (dw && k > 0 && m == 0)
     hipLaunchKernelGGL(fill_zero<E>, dim3(256), dim3(256), 0, stream, (E*)dw->data, dw->stride[0], (int32_t)k, n * k);
