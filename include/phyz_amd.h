@@ -452,7 +452,9 @@ typedef struct {
 } phz_muon_cfg;
 
 /* o = `steps` Newton-Schulz steps on each [rows][cols] matrix of g (2 or 3
- * dimensions; f32 or bf16, rows dense), in o's type, which is g's. */
+ * dimensions; f32 or bf16, rows dense), in o's type, which is g's. X is held to
+ * 2^-38, with singular values of about 1: of a matrix whose norm is far below eps,
+ * and whose result is as far below 1, what is smaller than that is lost. */
 int phz_orthogonalize(phz_ops* ops, void* stream, const phz_muon_cfg* cfg, const phz_tensor* g, const phz_tensor* o);
 /* m <- momentum m + g; u = g + momentum m (nesterov) or m;
  * w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u).
