@@ -373,14 +373,15 @@ int phz_train_time_update(phz_train* t, const uint32_t* const* order, const uint
  *     call on the same inputs gives the same bits. ── */
 typedef struct phz_ops phz_ops;
 
-enum { PHZ_BF16 = 2, PHZ_U8 = 3 }; /* further phz_tensor dtypes, beside PHZ_F32 */
+/* further phz_tensor dtypes, beside PHZ_F32 and PHZ_F64 */
+enum { PHZ_BF16 = 2, PHZ_U8 = 3, PHZ_I32 = 4, PHZ_I64 = 5 };
 
 /* A view of up to three dimensions; sizes and strides in elements. */
 typedef struct {
   void* data;
   int64_t size[3];
   int64_t stride[3];
-  int32_t dtype; /* PHZ_F32, PHZ_BF16 or PHZ_U8 */
+  int32_t dtype; /* PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_I32 or PHZ_I64 */
   int32_t ndim;  /* 1..3; the entries beyond it are ignored */
 } phz_tensor;
 
@@ -461,6 +462,90 @@ int phz_orthogonalize(phz_ops* ops, void* stream, const phz_muon_cfg* cfg, const
  * w and m are f32, g f32 or bf16. */
 int phz_muon_step(phz_ops* ops, void* stream, const phz_muon_cfg* cfg, const phz_tensor* w, const phz_tensor* g,
                   const phz_tensor* m);
+
+/* Sizes of linear attention's heads, 1 to 128 each, and the outputs' scale. */
+typedef struct {
+  double scale;
+  int32_t size_k, size_v;
+} phz_attention_cfg;
+
+/* Linear attention with a decay for each head, the recurrence of a state
+ * S [size_k][size_v] a head:
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
+ * for q [steps][worlds][q heads * size_k], k [..][k heads * size_k], v [..][v
+ * heads * size_v] (f32 or bf16, any strides of the first two axes, the last one
+ * dense) and g [steps][worlds][heads] f32, any strides. Heads of q, k and v that
+ * are fewer than g's serve heads / their own in a row each. s0
+ * [worlds][heads][size_k * size_v] f32: the state before the first step (NULL:
+ * zeros). Where reset [steps][worlds] u8 is nonzero, or g below -104 (exp(g) is 0
+ * in f32), S_{t-1} counts as 0, whatever it holds. o [steps][worlds][heads *
+ * size_v] in q's type; s_last like s0 (or NULL) receives the state after the last
+ * step. States are held in f32, sums in f32. g is at most 0 where gates decay;
+ * above, states grow as the recurrence does, up to exp(g) of 2^32 in 16 steps. */
+int phz_linear_attention(phz_ops* ops, void* stream, const phz_attention_cfg* cfg, const phz_tensor* q,
+                         const phz_tensor* k, const phz_tensor* v, const phz_tensor* g, const phz_tensor* s0,
+                         const phz_tensor* reset, const phz_tensor* o, const phz_tensor* s_last);
+/* Its gradients: d_o and ds (like s_last, or NULL) are the loss's gradients for o
+ * and s_last. dq, dk and dv like q, k and v (summed over the heads that share
+ * them), dg [steps][worlds][heads] f32 or NULL, ds0 like s0 or NULL. */
+int phz_linear_attention_backward(phz_ops* ops, void* stream, const phz_attention_cfg* cfg, const phz_tensor* d_o,
+                                  const phz_tensor* ds, const phz_tensor* q, const phz_tensor* k, const phz_tensor* v,
+                                  const phz_tensor* g, const phz_tensor* s0, const phz_tensor* reset,
+                                  const phz_tensor* dq, const phz_tensor* dk, const phz_tensor* dv, const phz_tensor* dg,
+                                  const phz_tensor* ds0);
+/* One step: q, k, v, g and reset without the axis of steps; s is read and
+ * replaced, o [worlds][heads * size_v]. */
+int phz_linear_attention_step(phz_ops* ops, void* stream, const phz_attention_cfg* cfg, const phz_tensor* q,
+                              const phz_tensor* k, const phz_tensor* v, const phz_tensor* g, const phz_tensor* reset,
+                              const phz_tensor* s, const phz_tensor* o);
+
+/* Which elements of a head make a pair: i and i + pairs, or 2i and 2i + 1. */
+enum { PHZ_PAIRS_HALF = 0, PHZ_PAIRS_INTERLEAVED = 1 };
+typedef struct {
+  double scale;
+  int32_t heads, pairs; /* how many heads x has; PHZ_PAIRS_HALF or PHZ_PAIRS_INTERLEAVED */
+  int32_t inverse;      /* turns the other way: the gradient's direction */
+} phz_rotary_cfg;
+
+/* Rotary positions: in each head of x [steps][worlds][heads * size] (f32 or bf16,
+ * the last axis dense), pair i < pairs turns by the angle positions * freq[i]
+ * and is multiplied by scale,
+ *   y0 = scale (x0 cos - x1 sin),   y1 = scale (x0 sin + x1 cos),
+ * and the elements behind the 2 * pairs first are copied. positions
+ * [steps][worlds], i32 or i64, of either sign; freq [pairs] f64, radians a
+ * position. Angles are held in f64 until whole turns are taken off. y like x; it
+ * may be the same view as x. */
+int phz_rotary(phz_ops* ops, void* stream, const phz_rotary_cfg* cfg, const phz_tensor* x, const phz_tensor* positions,
+               const phz_tensor* freq, const phz_tensor* y);
+
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  uint32_t seed;
+} phz_adamw_cfg;
+
+/* One AdamW step over n tensors, each a dense vector: with t = ++*step,
+ *   m <- beta1 m + (1 - beta1) g,   v <- beta2 v + (1 - beta2) g^2,
+ *   w <- (1 - lr weight_decay) w - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps).
+ * w and g are f32 or bf16, each tensor its own; step is one i64 on the device, so
+ * that a replayed graph counts on. Two forms of the moments, one for all tensors:
+ *   f32   exponents is NULL;
+ *   u8    8 bits an element, and for each 256 elements of a tensor an exponent:
+ *         exponents[i] is u8 [2][ceil(size / 256)], m's row and v's, zeros to begin
+ *         with. A code is three binary digits behind a leading one, and an exponent
+ *         below the block's: m's code c (a sign and 7 bits) is
+ *         (8 + c % 8) 2^(E - 144 + c / 8), or c % 8 times 2^(E - 143) where c / 8 is
+ *         0, v's (8 bits) the same with 160 and 159; E is the biased exponent of the
+ *         block's largest element, at least 40. What is not finite is 0x80 or 0xff.
+ *         Values are rounded up with the probability that makes them right on
+ *         average (to nearest, v would stand still where g^2 changes it by less than
+ *         a sixteenth a step), by bits that depend on seed, t, the tensor's place in
+ *         the list and the element's in the tensor; a positive v never rounds to 0. */
+int phz_adamw_step(phz_ops* ops, void* stream, const phz_adamw_cfg* cfg, int64_t n, const phz_tensor* w,
+                   const phz_tensor* g, const phz_tensor* m, const phz_tensor* v, const phz_tensor* exponents,
+                   const phz_tensor* step);
+/* The values that moments of 8 bits stand for, in bf16, which holds them exactly. */
+int phz_adamw_values(phz_ops* ops, void* stream, int64_t n, const phz_tensor* m, const phz_tensor* v,
+                     const phz_tensor* exponents, const phz_tensor* m_values, const phz_tensor* v_values);
 
 #ifdef __cplusplus
 }

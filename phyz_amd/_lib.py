@@ -49,6 +49,19 @@ class MuonCfg(C.Structure):
                 ("momentum", C.c_double), ("weight_decay", C.c_double), ("steps", C.c_int32), ("nesterov", C.c_int32)]
 
 
+class AttentionCfg(C.Structure):
+    _fields_ = [("scale", C.c_double), ("size_k", C.c_int32), ("size_v", C.c_int32)]
+
+
+class RotaryCfg(C.Structure):
+    _fields_ = [("scale", C.c_double), ("heads", C.c_int32), ("pairs", C.c_int32), ("inverse", C.c_int32)]
+
+
+class AdamWCfg(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("seed", C.c_uint32)]
+
+
 fp = C.POINTER(C.c_float)
 
 # name -> (restype, argtypes); every symbol declared in include/phyz_amd.h.
@@ -143,6 +156,12 @@ SIGNATURES = {
     "phz_linear_backward": (C.c_int, [OPS, STREAM, C.c_int] + [TENSOR] * 7),
     "phz_orthogonalize": (C.c_int, [OPS, STREAM, C.POINTER(MuonCfg), TENSOR, TENSOR]),
     "phz_muon_step": (C.c_int, [OPS, STREAM, C.POINTER(MuonCfg), TENSOR, TENSOR, TENSOR]),
+    "phz_linear_attention": (C.c_int, [OPS, STREAM, C.POINTER(AttentionCfg)] + [TENSOR] * 8),
+    "phz_linear_attention_backward": (C.c_int, [OPS, STREAM, C.POINTER(AttentionCfg)] + [TENSOR] * 13),
+    "phz_linear_attention_step": (C.c_int, [OPS, STREAM, C.POINTER(AttentionCfg)] + [TENSOR] * 7),
+    "phz_rotary": (C.c_int, [OPS, STREAM, C.POINTER(RotaryCfg)] + [TENSOR] * 4),
+    "phz_adamw_step": (C.c_int, [OPS, STREAM, C.POINTER(AdamWCfg), C.c_int64] + [TENSOR] * 6),
+    "phz_adamw_values": (C.c_int, [OPS, STREAM, C.c_int64] + [TENSOR] * 5),
 }
 
 

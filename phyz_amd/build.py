@@ -8,7 +8,8 @@
 2. Compile the host library (csrc/phz_host.cpp), the ahead-of-time layout
    kernels (csrc/phz_io.hip), the PPO update pass (csrc/phz_train.hip) and the
    operators of sequence policies (csrc/phz_ops.hip, phz_scan.hip,
-   phz_linear.hip, phz_muon.hip) for gfx950 and link them with hiprtc.
+   phz_linear.hip, phz_muon.hip, phz_attend.hip, phz_rotary.hip, phz_adamw.hip)
+   for gfx950 and link them with hiprtc.
 3. Compile the module that describes torch tensors to the library
    (csrc/phz_describe.cpp, g++, Python's headers): _describe.so.
 
@@ -28,7 +29,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libphyz_amd.so")
 DESCRIBE = os.path.join(HERE, "_describe.so")
 ARCH = "gfx950"
-KERNELS = ["phz_io", "phz_train", "phz_ops", "phz_scan", "phz_linear", "phz_muon"]  # csrc/*.hip, ahead of time
+KERNELS = ["phz_io", "phz_train", "phz_ops", "phz_scan", "phz_linear", "phz_muon", "phz_attend", "phz_rotary", "phz_adamw"]  # csrc/*.hip, ahead of time
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

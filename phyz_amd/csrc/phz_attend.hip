@@ -1,0 +1,544 @@
+// phz_attend.hip — linear attention with a decay for each head, over rollouts
+// and one step at a time, with its gradients.
+//
+//   S_t = a_t S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,  a_t = exp(g_t), or 0
+//                                                           where an episode begins
+//   E_t = scale q_t do_t^T + a_{t+1} E_{t+1}
+//   dq_t = scale S_t do_t,  dk_t = E_t v_t,  dv_t = E_t^T k_t,
+//   dg_t = a_t <E_t, S_{t-1}>,  ds0 = a_0 E_0
+#include "phz_ops.h"
+
+#include <algorithm>
+
+using namespace phzop;
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxSize = 128;       // of a head's keys and values
+constexpr float kForgets = -104.0f; // exp of less is 0 in f32: an episode begins
+
+// One of q, k, v, o and their gradients: [steps][worlds][heads of its own * size].
+struct Rows {
+  void* p;
+  int64_t t, b;  // strides
+  int32_t per;   // heads of g that one of its heads serves
+};
+// States [worlds][heads][size_k * size_v], or null.
+struct States {
+  float* p;
+  int64_t b, h;
+};
+
+struct AttendArgs {
+  Rows q, k, v, o, dq, dk, dv;  // o: the output, or its gradient
+  const float* g;
+  float* dg;
+  const uint8_t* reset;
+  States s0, s1, ds, ds0;  // first and last state, their gradients
+  int64_t g_t, g_b, g_h, dg_t, dg_b, dg_h, r_t, r_b;
+  int32_t steps, worlds, heads, nk, nv;
+  float scale;
+  const uint32_t* flags;  // heads to take, or null: all
+};
+
+template <class E>
+__device__ __forceinline__ const E* row_of(const Rows& r, int b, int h, int size) {
+  return (const E*)r.p + b * r.b + (int64_t)(h / r.per) * size;
+}
+
+// ── one step after another ──────────────────────────────────────────────────
+//
+// A wave holds 16 columns of one head's state: lane (c, g) = (lane % 16, lane /
+// 16) has its column's rows 16 i + 4 g + r. A sweep is
+//   s <- a s + key val^T,  out = s^T read
+// over the steps in either direction; the four gradients' and the forward pass's
+// are all of this form.
+struct Sweep {
+  const void *read, *key, *val;
+  int64_t read_t, key_t, val_t;
+  int32_t rows, cols;   // key's (and read's) size, and val's
+  float key_scale, out_scale;
+  const float* first;   // the state that it starts from, or null
+  int64_t f_row, f_col; // strides of its elements
+  bool back;
+};
+
+template <class E, class Out>
+__device__ __forceinline__ void sweep(const AttendArgs& a, const Sweep& w, int b, int h, int col0, float (&s)[8][4], Out&& out) {
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int col = col0 + c;
+  const bool live = col < w.cols;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int d = 16 * i + 4 * g + r;
+      s[i][r] = w.first && live && d < w.rows ? w.first[d * w.f_row + col * w.f_col] : 0.0f;
+    }
+  const float* gate = a.g + b * a.g_b + h * a.g_h;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  for (int n = 0; n < a.steps; n++) {
+    const int64_t t = w.back ? a.steps - 1 - n : n;
+    // Backwards the state of step t + 1 comes in by that step's gate.
+    const int64_t tg = w.back ? t + 1 : t;
+    float x = 0.0f;
+    bool forget = false;
+    if (tg < a.steps) {
+      x = gate[tg * a.g_t];
+      forget = x < kForgets || (reset && reset[tg * a.r_t]);
+    }
+    const float keep = expf(x);
+    const E* key = (const E*)w.key + t * w.key_t;
+    const E* read = (const E*)w.read + t * w.read_t;
+    const float val = live ? to_f32(((const E*)w.val)[t * w.val_t + col]) * w.key_scale : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = 16 * i + 4 * g + r;
+        if (d >= w.rows) continue;
+        const float kept = forget ? 0.0f : keep * s[i][r];
+        s[i][r] = fmaf(to_f32(key[d]), val, kept);
+        sum = fmaf(to_f32(read[d]), s[i][r], sum);
+      }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    out(t, col, live, sum * w.out_scale);
+  }
+}
+
+template <class E>
+__device__ __forceinline__ void put(const Rows& r, int64_t t, int b, int h, int size, int col, float v, bool wide) {
+  // Heads that share one of theirs leave f32 sums of their own, joined later.
+  if (wide) ((float*)r.p)[t * r.t + b * r.b + (int64_t)h * size + col] = v;
+  else ((E*)r.p)[t * r.t + b * r.b + (int64_t)h * size + col] = from_f32<E>(v);
+}
+
+// The elements of the state that a lane holds, rows and columns within the head.
+template <class F>
+__device__ __forceinline__ void each_element(int rows, int col, bool live, float (&s)[8][4], F&& f) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int d = 16 * i + 4 * g + r;
+      if (live && d < rows) f(d, s[i][r]);
+    }
+}
+
+// A head whose steps are taken one after the other: what the chunks' products
+// cannot do is right here, infinities and NaN that a reset cuts off from the
+// steps behind it. Workgroups look through the heads' flags. 2 waves a SIMD.
+template <class E>
+__global__ __launch_bounds__(512) void attend_sequential(AttendArgs a, int32_t marks) {
+  const int wave = threadIdx.x >> 6, c = threadIdx.x & 15, col0 = 16 * wave;
+  const int64_t all = (int64_t)a.worlds * a.heads;
+  for (int64_t bh = blockIdx.x; bh < all; bh += gridDim.x) {
+    if (a.flags) {
+      uint32_t any = 0;
+      for (int m = 0; m < marks; m++) any |= a.flags[m * all + bh];
+      if (!any) continue;
+    }
+    const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+    if (col0 >= a.nv) continue;
+    Sweep w{row_of<E>(a.q, b, h, a.nk), row_of<E>(a.k, b, h, a.nk), row_of<E>(a.v, b, h, a.nv), a.q.t, a.k.t, a.v.t, a.nk, a.nv,
+            1.0f, a.scale, a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, false};
+    float s[8][4];
+    sweep<E>(a, w, b, h, col0, s, [&](int64_t t, int col, bool live, float v) {
+      if (live && (threadIdx.x & 63) < 16) put<E>(a.o, t, b, h, a.nv, col, v, false);
+    });
+    if (a.s1.p) {
+      float* last = a.s1.p + b * a.s1.b + h * a.s1.h;
+      const int col = col0 + c;
+      each_element(a.nk, col, col < a.nv, s, [&](int d, float v) { last[(int64_t)d * a.nv + col] = v; });
+    }
+  }
+}
+
+// Its gradients. dg by <E_t, S_t> = q_t dq_t + dg_{t+1} = dg_t + k_t dk_t, in f64.
+// `wide`: which of dq, dk, dv are sums of each head's own (1, 2, 4).
+template <class E>
+__global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, int32_t marks, int32_t wide) {
+  __shared__ float part[8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, col0 = 16 * wave;
+  const int64_t all = (int64_t)a.worlds * a.heads;
+  // The sum of one value of each column over the workgroup, in thread 0.
+  auto total = [&](float v) {
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) v += __shfl_xor(v, m);
+    if (lane == 0) part[wave] = v;
+    __syncthreads();
+    float sum = 0.0f;
+    for (int i = 0; i < 8; i++) sum += part[i];
+    __syncthreads();
+    return sum;
+  };
+  for (int64_t bh = blockIdx.x; bh < all; bh += gridDim.x) {
+    if (a.flags) {
+      uint32_t any = 0;
+      for (int m = 0; m < marks; m++) any |= a.flags[m * all + bh];
+      if (!any) continue;
+    }
+    const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+    const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv),
+            *d_o = row_of<E>(a.o, b, h, a.nv);
+    const float* s0 = a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr;
+    const float* ds = a.ds.p ? a.ds.p + b * a.ds.b + h * a.ds.h : nullptr;
+    float* dg = a.dg ? a.dg + b * a.dg_b + h * a.dg_h : nullptr;
+    const float* gate = a.g + b * a.g_b + h * a.g_h;
+    const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+    float s[8][4];
+    // dq: the state's transpose, over its columns d.
+    sweep<E>(a, Sweep{d_o, v, k, a.o.t, a.v.t, a.k.t, a.nv, a.nk, 1.0f, a.scale, s0, 1, a.nv, false}, b, h, col0, s,
+             [&](int64_t t, int col, bool live, float x) {
+               if (live && lane < 16) put<E>(a.dq, t, b, h, a.nk, col, x, wide & 1);
+               if (dg) {
+                 const float sum = total(live ? to_f32(q[t * a.q.t + col]) * x : 0.0f);
+                 if (threadIdx.x == 0) dg[t * a.dg_t] = sum;
+               }
+             });
+    double later = 0.0;
+    if (dg) {
+      float mine = 0.0f;
+      const int col = col0 + c;
+      if (ds)
+        each_element(a.nv, col, col < a.nk, s, [&](int j, float x) { mine = fmaf(ds[(int64_t)col * a.nv + j], x, mine); });
+      mine += __shfl_xor(mine, 16);
+      mine += __shfl_xor(mine, 32);
+      later = total(mine);
+    }
+    sweep<E>(a, Sweep{v, d_o, q, a.v.t, a.o.t, a.q.t, a.nv, a.nk, a.scale, 1.0f, ds, 1, a.nv, true}, b, h, col0, s,
+             [&](int64_t t, int col, bool live, float x) {
+               if (live && lane < 16) put<E>(a.dk, t, b, h, a.nk, col, x, wide & 2);
+               if (dg) {
+                 const float sum = total(live ? to_f32(k[t * a.k.t + col]) * x : 0.0f);
+                 if (threadIdx.x == 0) {
+                   later += (double)dg[t * a.dg_t] - (double)sum;
+                   const float y = gate[t * a.g_t];
+                   if (y < kForgets || (reset && reset[t * a.r_t])) later = 0.0;
+                   dg[t * a.dg_t] = (float)later;
+                 }
+               }
+             });
+    sweep<E>(a, Sweep{k, q, d_o, a.k.t, a.q.t, a.o.t, a.nk, a.nv, a.scale, 1.0f, ds, a.nv, 1, true}, b, h, col0, s,
+             [&](int64_t t, int col, bool live, float x) {
+               if (live && lane < 16) put<E>(a.dv, t, b, h, a.nv, col, x, wide & 4);
+             });
+    if (a.ds0.p) {
+      float* out = a.ds0.p + b * a.ds0.b + h * a.ds0.h;
+      const float y = gate[0], keep = expf(y);
+      const bool forget = y < kForgets || (reset && reset[0]);
+      const int col = col0 + c;
+      each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = forget ? 0.0f : keep * x; });
+    }
+  }
+}
+
+// ── a single step ───────────────────────────────────────────────────────────
+//
+// A workgroup takes `width` columns of one head's state: a thread four
+// neighbouring columns of every RP-th row, read, replaced and read by q; the
+// rows' sums meet in LDS.
+constexpr int kStepThreads = 256;
+
+template <class E>
+__global__ __launch_bounds__(kStepThreads) void attend_step(AttendArgs a, int32_t parts, int32_t width) {
+  __shared__ float sum[kStepThreads * 4];
+  const int64_t at = blockIdx.x;
+  const int part = (int)(at % parts);
+  const int64_t bh = at / parts;
+  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  const int j0 = part * width, cols = min(width, a.nv - j0);
+  const int groups = (cols + 3) / 4, rows = kStepThreads / groups;
+  const int jj = threadIdx.x % groups, rr = threadIdx.x / groups;
+  const float x = a.g[b * a.g_b + h * a.g_h];
+  const bool forget = x < kForgets || (a.reset && a.reset[b * a.r_b]);
+  const float keep = expf(x);
+  float* s = a.s1.p + b * a.s1.b + h * a.s1.h + j0;
+  const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv) + j0;
+  float acc[4] = {};
+  const int j = 4 * jj, n = min(4, cols - j);
+  if (rr < rows) {
+    float val[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) val[i] = i < n ? to_f32(v[j + i]) : 0.0f;
+    if (n == 4) {
+#pragma unroll 8
+      for (int d = rr; d < a.nk; d += rows) {
+        auto* at = (Pack<float, 4>*)(s + (int64_t)d * a.nv + j);
+        Pack<float, 4> w = *at;
+        const float kd = to_f32(k[d]), qd = to_f32(q[d]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          w.v[i] = fmaf(kd, val[i], forget ? 0.0f : keep * w.v[i]);
+          acc[i] = fmaf(qd, w.v[i], acc[i]);
+        }
+        *at = w;
+      }
+    } else {
+      for (int d = rr; d < a.nk; d += rows) {
+        const float kd = to_f32(k[d]), qd = to_f32(q[d]);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (i < n) {
+            float& w = s[(int64_t)d * a.nv + j + i];
+            w = fmaf(kd, val[i], forget ? 0.0f : keep * w);
+            acc[i] = fmaf(qd, w, acc[i]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) sum[threadIdx.x * 4 + i] = acc[i];
+  __syncthreads();
+  const int used = min(rows, a.nk);
+  for (int i = threadIdx.x; i < cols; i += kStepThreads) {
+    float o = 0.0f;
+    for (int r = 0; r < used; r++) o += sum[r * groups * 4 + i];
+    ((E*)a.o.p)[b * a.o.b + (int64_t)h * a.nv + j0 + i] = from_f32<E>(o * a.scale);
+  }
+}
+
+// ── the rest ────────────────────────────────────────────────────────────────
+
+// States copied, or zeros, where there are no steps.
+__global__ void copy_states(States from, States to, int32_t heads, int32_t n) {
+  const int b = blockIdx.x / heads, h = blockIdx.x % heads;
+  for (int i = threadIdx.x; i < n; i += blockDim.x)
+    to.p[b * to.b + h * to.h + i] = from.p ? from.p[b * from.b + h * from.h + i] : 0.0f;
+}
+
+// The sums of heads that share one: from [steps][worlds][heads * size] f32, dense.
+template <class E>
+__global__ void join_heads(const float* from, Rows to, int64_t rows, int32_t worlds, int32_t heads, int32_t size) {
+  const int32_t own = heads / to.per, width = own * size;
+  const int64_t n = rows * width;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / width;
+    const int32_t x = (int32_t)(i % width), h = x / size, d = x % size;
+    const float* f = from + (row * heads + (int64_t)h * to.per) * size + d;
+    float s = 0.0f;
+    for (int p = 0; p < to.per; p++) s += f[(int64_t)p * size];
+    ((E*)to.p)[row / worlds * to.t + row % worlds * to.b + x] = from_f32<E>(s);
+  }
+}
+
+// ── arguments ───────────────────────────────────────────────────────────────
+
+struct Named {
+  const char* name;
+  const phz_tensor* t;
+};
+
+// Sizes from cfg, q, k, v and g; false, with the error set, where they do not fit.
+// ndim 3: with the axis of steps.
+bool take(phz_ops* o, const phz_attention_cfg* cfg, const phz_tensor* q, const phz_tensor* k, const phz_tensor* v,
+          const phz_tensor* g, const phz_tensor* reset, int ndim, AttendArgs* a) {
+  if (!cfg) return o->err = "configuration is missing", false;
+  if (cfg->size_k < 1 || cfg->size_k > kMaxSize || cfg->size_v < 1 || cfg->size_v > kMaxSize)
+    return o->err = fmt("size_k and size_v have to be 1 to %d, not %d and %d", kMaxSize, cfg->size_k, cfg->size_v), false;
+  if (!(cfg->scale >= -3e38 && cfg->scale <= 3e38)) return o->err = "scale has to be finite", false;
+  if (!q) return o->err = "q is missing", false;
+  if (q->dtype != PHZ_F32 && q->dtype != PHZ_BF16)
+    return o->err = fmt("q is %s, expected f32 or bf16", dtype_name(q->dtype)), false;
+  const int last = ndim - 1;
+  Want any{ndim, {-1, -1, -1}, q->dtype, true, false};
+  if (!check(o, "q", q, any)) return false;
+  const int64_t T = ndim == 3 ? q->size[0] : 1, B = q->size[last - 1];
+  Want rows = any;
+  rows.size[0] = ndim == 3 ? T : B;
+  if (ndim == 3) rows.size[1] = B;
+  if (!check(o, "k", k, rows) || !check(o, "v", v, rows)) return false;
+  rows.dtype = PHZ_F32;
+  rows.dense = false;
+  if (!check(o, "g", g, rows)) return false;
+  const int64_t H = g->size[last];
+  if (T > 0x3fff0000ll || B > 0x3fff0000ll || H > 0xffffll || H < 1)
+    return o->err = "steps and worlds have to be below 2^30, heads 1 to 65535", false;
+  if (B * H > 0x3fff0000ll) return o->err = "too many heads of all worlds", false;
+  const struct { const char* name; const phz_tensor* t; int size; Rows* to; } each[] = {
+      {"q", q, cfg->size_k, &a->q}, {"k", k, cfg->size_k, &a->k}, {"v", v, cfg->size_v, &a->v}};
+  for (auto& x : each) {
+    const int64_t n = x.t->size[last];
+    if (n < 1 || n % x.size || H % (n / x.size))
+      return o->err = fmt("%s has %lld elements along axis %d: heads of %d, as many as g's %lld or a divisor of them", x.name,
+                          (long long)n, last, x.size, (long long)H),
+             false;
+    *x.to = Rows{x.t->data, ndim == 3 ? x.t->stride[0] : 0, x.t->stride[last - 1], (int32_t)(H / (n / x.size))};
+  }
+  Want mask{ndim - 1, {ndim == 3 ? T : B, B, 0}, PHZ_U8, false, false};
+  if (reset && !check(o, "reset", reset, mask)) return false;
+  a->g = (const float*)g->data;
+  a->g_t = ndim == 3 ? g->stride[0] : 0, a->g_b = g->stride[last - 1], a->g_h = g->stride[last];
+  if (reset) {
+    a->reset = (const uint8_t*)reset->data;
+    a->r_t = ndim == 3 ? reset->stride[0] : 0, a->r_b = reset->stride[ndim - 2];
+  }
+  a->steps = (int32_t)T, a->worlds = (int32_t)B, a->heads = (int32_t)H;
+  a->nk = cfg->size_k, a->nv = cfg->size_v;
+  a->scale = (float)cfg->scale;
+  return true;
+}
+
+// One of the tensors of whole states.
+bool take_states(phz_ops* o, const char* name, const phz_tensor* t, bool output, const AttendArgs& a, States* to) {
+  if (!t) return true;
+  const Want want{3, {a.worlds, a.heads, (int64_t)a.nk * a.nv}, PHZ_F32, true, output};
+  if (!check(o, name, t, want)) return false;
+  *to = States{(float*)t->data, t->stride[0], t->stride[1]};
+  return true;
+}
+
+// Outputs that share elements with inputs or with each other.
+bool all_apart(phz_ops* o, std::initializer_list<Named> outs, std::initializer_list<Named> ins) {
+  for (auto u = outs.begin(); u != outs.end(); u++) {
+    for (auto& v : ins)
+      if (!apart(o, u->name, u->t, v.name, v.t)) return false;
+    for (auto v = u + 1; v != outs.end(); v++)
+      if (!apart(o, u->name, u->t, v->name, v->t)) return false;
+  }
+  return true;
+}
+
+unsigned sequential_blocks(const phz_ops* o, const AttendArgs& a) {
+  return (unsigned)std::min<int64_t>((int64_t)a.worlds * a.heads, 2 * o->cus);
+}
+
+}  // namespace
+
+extern "C" {
+
+int phz_linear_attention(phz_ops* o, void* stream_, const phz_attention_cfg* cfg, const phz_tensor* q, const phz_tensor* k,
+                         const phz_tensor* v, const phz_tensor* g, const phz_tensor* s0, const phz_tensor* reset,
+                         const phz_tensor* out, const phz_tensor* s_last) {
+  return guarded(o, [&] {
+    AttendArgs a{};
+    if (!take(o, cfg, q, k, v, g, reset, 3, &a)) return 1;
+    const Want like{3, {a.steps, a.worlds, (int64_t)a.heads * a.nv}, q->dtype, true, true};
+    if (!check(o, "o", out, like) || !take_states(o, "s0", s0, false, a, &a.s0) ||
+        !take_states(o, "s_last", s_last, true, a, &a.s1) ||
+        !all_apart(o, {{"o", out}, {"s_last", s_last}},
+                   {{"q", q}, {"k", k}, {"v", v}, {"g", g}, {"s0", s0}, {"reset", reset}}))
+      return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    if (a.worlds == 0) return 0;
+    a.o = Rows{out->data, out->stride[0], out->stride[1], 1};
+    auto stream = (hipStream_t)stream_;
+    DeviceGuard guard(o);
+    if (!guard.ok) return 1;
+    if (a.steps == 0) {
+      if (a.s1.p)
+        hipLaunchKernelGGL(copy_states, dim3(a.worlds * a.heads), dim3(256), 0, stream, a.s0, a.s1, a.heads, a.nk * a.nv);
+      return launched(o, "linear attention") ? 0 : 1;
+    }
+    const unsigned blocks = sequential_blocks(o, a);
+    if (q->dtype == PHZ_F32) hipLaunchKernelGGL(attend_sequential<float>, dim3(blocks), dim3(512), 0, stream, a, 0);
+    else hipLaunchKernelGGL(attend_sequential<bf16>, dim3(blocks), dim3(512), 0, stream, a, 0);
+    return launched(o, "linear attention") ? 0 : 1;
+  });
+}
+
+int phz_linear_attention_backward(phz_ops* o, void* stream_, const phz_attention_cfg* cfg, const phz_tensor* d_o,
+                                  const phz_tensor* ds, const phz_tensor* q, const phz_tensor* k, const phz_tensor* v,
+                                  const phz_tensor* g, const phz_tensor* s0, const phz_tensor* reset, const phz_tensor* dq,
+                                  const phz_tensor* dk, const phz_tensor* dv, const phz_tensor* dg, const phz_tensor* ds0) {
+  return guarded(o, [&] {
+    AttendArgs a{};
+    if (!take(o, cfg, q, k, v, g, reset, 3, &a)) return 1;
+    const int64_t T = a.steps, B = a.worlds, H = a.heads;
+    const Want grad{3, {T, B, H * a.nv}, q->dtype, true, false};
+    const Want gates{3, {T, B, H}, PHZ_F32, false, true};
+    if (!check(o, "do", d_o, grad)) return 1;
+    for (const auto& x : {std::pair<Named, const phz_tensor*>{{"dq", dq}, q}, {{"dk", dk}, k}, {{"dv", dv}, v}})
+      if (!check(o, x.first.name, x.first.t, Want{3, {T, B, x.second->size[2]}, q->dtype, true, true})) return 1;
+    if ((dg && !check(o, "dg", dg, gates)) || !take_states(o, "s0", s0, false, a, &a.s0) ||
+        !take_states(o, "ds", ds, false, a, &a.ds) || !take_states(o, "ds0", ds0, true, a, &a.ds0) ||
+        !all_apart(o, {{"dq", dq}, {"dk", dk}, {"dv", dv}, {"dg", dg}, {"ds0", ds0}},
+                   {{"do", d_o}, {"ds", ds}, {"q", q}, {"k", k}, {"v", v}, {"g", g}, {"s0", s0}, {"reset", reset}}))
+      return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    if (B == 0) return 0;
+    auto stream = (hipStream_t)stream_;
+    DeviceGuard guard(o);
+    if (!guard.ok) return 1;
+    if (T == 0) {
+      if (a.ds0.p)
+        hipLaunchKernelGGL(copy_states, dim3((unsigned)(B * H)), dim3(256), 0, stream, a.ds, a.ds0, a.heads, a.nk * a.nv);
+      return launched(o, "linear attention backward") ? 0 : 1;
+    }
+    a.o = Rows{d_o->data, d_o->stride[0], d_o->stride[1], 1};
+    if (dg) a.dg = (float*)dg->data, a.dg_t = dg->stride[0], a.dg_b = dg->stride[1], a.dg_h = dg->stride[2];
+    // Gradients of shared heads: each head's own in f32, then their sums.
+    struct { const phz_tensor* t; Rows* row; Rows to; int size; int64_t at; } outs[] = {
+        {dq, &a.dq, {dq->data, dq->stride[0], dq->stride[1], a.q.per}, a.nk, -1},
+        {dk, &a.dk, {dk->data, dk->stride[0], dk->stride[1], a.k.per}, a.nk, -1},
+        {dv, &a.dv, {dv->data, dv->stride[0], dv->stride[1], a.v.per}, a.nv, -1}};
+    int64_t need = 0;
+    for (auto& x : outs)
+      if (x.to.per > 1) x.at = need, need += T * B * H * x.size * 4;
+    char* work = nullptr;
+    if (need && !(work = o->workspace(stream, need))) return 1;
+    int wide = 0;
+    for (int i = 0; i < 3; i++) {
+      *outs[i].row = outs[i].to;
+      if (outs[i].at >= 0) {
+        wide |= 1 << i;
+        *outs[i].row = Rows{work + outs[i].at, B * H * outs[i].size, H * outs[i].size, 1};
+      }
+    }
+    const unsigned blocks = sequential_blocks(o, a);
+    if (q->dtype == PHZ_F32)
+      hipLaunchKernelGGL(attend_sequential_backward<float>, dim3(blocks), dim3(512), 0, stream, a, 0, wide);
+    else
+      hipLaunchKernelGGL(attend_sequential_backward<bf16>, dim3(blocks), dim3(512), 0, stream, a, 0, wide);
+    for (auto& x : outs) {
+      if (x.at < 0) continue;
+      const unsigned n = (unsigned)std::min<int64_t>(ceil_div(T * B * (H / x.to.per) * x.size, 256), 16 * o->cus);
+      if (q->dtype == PHZ_F32)
+        hipLaunchKernelGGL(join_heads<float>, dim3(n), dim3(256), 0, stream, (const float*)x.row->p, x.to, T * B, a.worlds,
+                           a.heads, x.size);
+      else
+        hipLaunchKernelGGL(join_heads<bf16>, dim3(n), dim3(256), 0, stream, (const float*)x.row->p, x.to, T * B, a.worlds,
+                           a.heads, x.size);
+    }
+    return launched(o, "linear attention backward") ? 0 : 1;
+  });
+}
+
+int phz_linear_attention_step(phz_ops* o, void* stream_, const phz_attention_cfg* cfg, const phz_tensor* q,
+                              const phz_tensor* k, const phz_tensor* v, const phz_tensor* g, const phz_tensor* reset,
+                              const phz_tensor* s, const phz_tensor* out) {
+  return guarded(o, [&] {
+    AttendArgs a{};
+    if (!take(o, cfg, q, k, v, g, reset, 2, &a)) return 1;
+    const Want like{2, {a.worlds, (int64_t)a.heads * a.nv, 0}, q->dtype, true, true};
+    if (!s) return o->fail("s is missing");
+    if (!check(o, "o", out, like) || !take_states(o, "s", s, true, a, &a.s1) ||
+        !all_apart(o, {{"s", s}, {"o", out}}, {{"q", q}, {"k", k}, {"v", v}, {"g", g}, {"reset", reset}}))
+      return 1;
+    if (o->device < 0) return o->fail("host-only handle (device -1)");
+    if (a.worlds == 0) return 0;
+    a.o = Rows{out->data, 0, out->stride[0], 1};
+    DeviceGuard guard(o);
+    if (!guard.ok) return 1;
+    const int64_t all = (int64_t)a.worlds * a.heads;
+    // Few heads: several workgroups to one, of 16 columns at least.
+    int width = (a.nv + 3) / 4 * 4;
+    while (all * ceil_div(a.nv, width) < 2 * o->cus && width % 32 == 0) width /= 2;
+    const int parts = (int)ceil_div(a.nv, width);
+    if (all * parts > 0x7fffffffll) return o->fail("too many heads of all worlds");
+    if (q->dtype == PHZ_F32)
+      hipLaunchKernelGGL(attend_step<float>, dim3((unsigned)(all * parts)), dim3(kStepThreads), 0, (hipStream_t)stream_, a, parts,
+                         width);
+    else
+      hipLaunchKernelGGL(attend_step<bf16>, dim3((unsigned)(all * parts)), dim3(kStepThreads), 0, (hipStream_t)stream_, a, parts,
+                         width);
+    return launched(o, "linear attention step") ? 0 : 1;
+  });
+}
+
+}  // extern "C"

@@ -8,6 +8,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <new>
+#include <vector>
+
 #include "../../include/phyz_amd.h"
 
 namespace {
@@ -22,29 +25,37 @@ struct Entries {
   int (*linear_backward)(phz_ops*, void*, int, T, T, T, T, T, T, T);
   int (*orthogonalize)(phz_ops*, void*, const phz_muon_cfg*, T, T);
   int (*muon)(phz_ops*, void*, const phz_muon_cfg*, T, T, T);
+  int (*attention)(phz_ops*, void*, const phz_attention_cfg*, T, T, T, T, T, T, T, T);
+  int (*attention_backward)(phz_ops*, void*, const phz_attention_cfg*, T, T, T, T, T, T, T, T, T, T, T, T, T);
+  int (*attention_step)(phz_ops*, void*, const phz_attention_cfg*, T, T, T, T, T, T, T);
+  int (*rotary)(phz_ops*, void*, const phz_rotary_cfg*, T, T, T, T);
+  int (*adamw)(phz_ops*, void*, const phz_adamw_cfg*, int64_t, T, T, T, T, T, T);
+  int (*adamw_values)(phz_ops*, void*, int64_t, T, T, T, T, T);
 };
+constexpr int kEntries = 13, kPlain = 11, kMost = 13, kDtypes = 7;  // the last two take lists (call_lists)
 union {
   Entries fn;
-  void* at[7];
+  void* at[kEntries];
 } g_entries;
-const int kTensors[7] = {6, 10, 4, 6, 7, 2, 3};
+const int kTensors[kPlain] = {6, 10, 4, 6, 7, 2, 3, 8, 13, 7, 4};
 // Whose results a user may expect autograd to know: not the gradients' own
 // operators and the update's.
-const bool kForward[7] = {true, false, true, true, false, true, false};
+const bool kForward[kPlain] = {true, false, true, true, false, true, false, true, false, true, true};
 
-PyObject *g_dtypes[5], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device, *g_requires_grad;
-const int kCodes[5] = {PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_U8};
+PyObject *g_dtypes[kDtypes], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device, *g_requires_grad;
+const int kCodes[kDtypes] = {PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_U8, PHZ_I32, PHZ_I64};
 
 // False, with no Python error left, where `o` is no tensor that can be
-// described (the caller finds out why and says so).
-bool describe(PyObject* o, long device, phz_tensor* t) {
+// described (the caller finds out why and says so). `flat`: as a vector, which a
+// contiguous tensor of any number of axes is.
+bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false) {
   PyObject* v = PyObject_CallMethodNoArgs(o, g_get_device);
   bool ok = v && PyLong_AsLong(v) == device;
   Py_XDECREF(v);
   if (ok) {
     v = PyObject_GetAttr(o, g_dtype);
     int code = -1;
-    for (int i = 0; i < 5; i++)
+    for (int i = 0; i < kDtypes; i++)
       if (v == g_dtypes[i]) code = kCodes[i];
     Py_XDECREF(v);
     t->dtype = code;
@@ -61,12 +72,24 @@ bool describe(PyObject* o, long device, phz_tensor* t) {
   ok = ok && shape && stride && PyTuple_Check(shape) && PyTuple_Check(stride);
   if (ok) {
     const Py_ssize_t n = PyTuple_GET_SIZE(shape);
-    ok = n >= 1 && n <= 3 && PyTuple_GET_SIZE(stride) == n;
-    for (Py_ssize_t i = 0; ok && i < n; i++) {
-      t->size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
-      t->stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i));
+    ok = PyTuple_GET_SIZE(stride) == n && (flat || (n >= 1 && n <= 3));
+    if (flat) {
+      int64_t all = 1;
+      for (Py_ssize_t i = n; ok && i-- > 0;) {
+        const int64_t size = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+        ok = size <= 1 || PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i)) == all || all == 0;
+        all *= size;
+      }
+      t->size[0] = all;
+      t->stride[0] = 1;
+      t->ndim = 1;
+    } else {
+      for (Py_ssize_t i = 0; ok && i < n; i++) {
+        t->size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+        t->stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i));
+      }
+      t->ndim = (int32_t)n;
     }
-    t->ndim = (int32_t)n;
   }
   Py_XDECREF(shape);
   Py_XDECREF(stride);
@@ -90,12 +113,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(args[2]);
   const long long head = PyLong_AsLongLong(args[4]);
   if (PyErr_Occurred()) return nullptr;
-  if (op < 0 || op > 6 || PyTuple_GET_SIZE(args[5]) != kTensors[op] || !g_entries.at[op]) {
+  if (op < 0 || op >= kPlain || PyTuple_GET_SIZE(args[5]) != kTensors[op] || !g_entries.at[op]) {
     PyErr_SetString(PyExc_ValueError, "unknown operator, or not its tensors");
     return nullptr;
   }
-  phz_tensor d[10];
-  T t[10] = {};
+  phz_tensor d[kMost];
+  T t[kMost] = {};
   for (int i = 0; i < kTensors[op]; i++) {
     PyObject* o = PyTuple_GET_ITEM(args[5], i);
     if (o == Py_None) continue;
@@ -111,6 +134,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Entries& f = g_entries.fn;
   const int h = (int)head;
   const auto* cfg = (const phz_muon_cfg*)(intptr_t)head;
+  const auto* att = (const phz_attention_cfg*)(intptr_t)head;
+  const auto* rot = (const phz_rotary_cfg*)(intptr_t)head;
   int rc = 1;
   switch (op) {
     case 0: rc = f.scan(ops, stream, h, t[0], t[1], t[2], t[3], t[4], t[5]); break;
@@ -120,20 +145,75 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     case 4: rc = f.linear_backward(ops, stream, h, t[0], t[1], t[2], t[3], t[4], t[5], t[6]); break;
     case 5: rc = f.orthogonalize(ops, stream, cfg, t[0], t[1]); break;
     case 6: rc = f.muon(ops, stream, cfg, t[0], t[1], t[2]); break;
+    case 7: rc = f.attention(ops, stream, att, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]); break;
+    case 8:
+      rc = f.attention_backward(ops, stream, att, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], t[10], t[11],
+                                t[12]);
+      break;
+    case 9: rc = f.attention_step(ops, stream, att, t[0], t[1], t[2], t[3], t[4], t[5], t[6]); break;
+    case 10: rc = f.rotary(ops, stream, rot, t[0], t[1], t[2], t[3]); break;
   }
   return PyLong_FromLong(rc);
 }
 
-// bind(entry points' addresses, (float32, float64, bfloat16, uint8, bool))
-PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 2 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != 7 || !PyTuple_Check(args[1]) ||
-      PyTuple_GET_SIZE(args[1]) != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind(seven addresses, five dtypes)");
+// call_lists(op, handle, stream, device, head, lists, single): an entry point of
+// lists of tensors, each a vector. Lists are tuples of one length, or None;
+// `single` is a tensor or None. The result as in call(), -1 - (5 i + l) for tensor
+// i of list l (l = 0 .. 4) and -1 - 5 n for the single one.
+PyObject* call_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7 || !PyTuple_Check(args[5]) || PyTuple_GET_SIZE(args[5]) != 5) {
+    PyErr_SetString(PyExc_TypeError, "call_lists(op, handle, stream, device, head, five lists, single)");
     return nullptr;
   }
-  for (int i = 0; i < 7; i++) g_entries.at[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args[0], i));
+  const long op = PyLong_AsLong(args[0]), device = PyLong_AsLong(args[3]);
+  auto* ops = (phz_ops*)PyLong_AsVoidPtr(args[1]);
+  void* stream = PyLong_AsVoidPtr(args[2]);
+  const auto* cfg = (const phz_adamw_cfg*)(intptr_t)PyLong_AsLongLong(args[4]);
   if (PyErr_Occurred()) return nullptr;
-  for (int i = 0; i < 5; i++) {
+  PyObject* const* lists = &PyTuple_GET_ITEM(args[5], 0);
+  Py_ssize_t n = -1;
+  bool fits = op >= kPlain && op < kEntries && g_entries.at[op];
+  for (int l = 0; l < 5; l++) {
+    if (lists[l] == Py_None) continue;
+    fits = fits && PyTuple_Check(lists[l]) && (n < 0 || PyTuple_GET_SIZE(lists[l]) == n);
+    if (fits) n = PyTuple_GET_SIZE(lists[l]);
+  }
+  if (!fits || n < 0) {
+    PyErr_SetString(PyExc_ValueError, "unknown operator, or not its lists");
+    return nullptr;
+  }
+  std::vector<phz_tensor> d;
+  try {
+    d.resize((size_t)n * 5 + 1);
+  } catch (const std::bad_alloc&) {
+    return PyErr_NoMemory();
+  }
+  T t[6] = {};
+  for (int l = 0; l < 5; l++) {
+    if (lists[l] == Py_None) continue;
+    t[l] = d.data() + n * l;
+    for (Py_ssize_t i = 0; i < n; i++)
+      if (!describe(PyTuple_GET_ITEM(lists[l], i), device, &d[n * l + i], true)) return PyLong_FromSsize_t(-1 - (5 * i + l));
+  }
+  if (args[6] != Py_None) {
+    if (!describe(args[6], device, &d[n * 5], true)) return PyLong_FromSsize_t(-1 - 5 * n);
+    t[5] = &d[n * 5];
+  }
+  const Entries& f = g_entries.fn;
+  return PyLong_FromLong(op == kPlain ? f.adamw(ops, stream, cfg, n, t[0], t[1], t[2], t[3], t[4], t[5])
+                                      : f.adamw_values(ops, stream, n, t[0], t[1], t[2], t[3], t[4]));
+}
+
+// bind(entry points' addresses, (float32, float64, bfloat16, uint8, bool, int32, int64))
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != kEntries || !PyTuple_Check(args[1]) ||
+      PyTuple_GET_SIZE(args[1]) != kDtypes) {
+    PyErr_SetString(PyExc_TypeError, "bind(the entry points' addresses, the dtypes)");
+    return nullptr;
+  }
+  for (int i = 0; i < kEntries; i++) g_entries.at[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args[0], i));
+  if (PyErr_Occurred()) return nullptr;
+  for (int i = 0; i < kDtypes; i++) {
     PyObject* o = PyTuple_GET_ITEM(args[1], i);
     Py_INCREF(o);
     Py_XSETREF(g_dtypes[i], o);
@@ -142,6 +222,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef g_methods[] = {{"call", (PyCFunction)(void*)call, METH_FASTCALL, nullptr},
+                           {"call_lists", (PyCFunction)(void*)call_lists, METH_FASTCALL, nullptr},
                            {"bind", (PyCFunction)(void*)bind, METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_describe", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

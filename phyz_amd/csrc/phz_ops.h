@@ -83,9 +83,17 @@ int guarded(phz_ops* o, F&& body) {
 }
 
 inline const char* dtype_name(int d) {
-  return d == PHZ_F32 ? "f32" : d == PHZ_BF16 ? "bf16" : d == PHZ_U8 ? "u8" : d == PHZ_F64 ? "f64" : "unknown";
+  return d == PHZ_F32    ? "f32"
+         : d == PHZ_BF16 ? "bf16"
+         : d == PHZ_U8   ? "u8"
+         : d == PHZ_F64  ? "f64"
+         : d == PHZ_I32  ? "i32"
+         : d == PHZ_I64  ? "i64"
+                         : "unknown";
 }
-inline int64_t elem_bytes(int d) { return d == PHZ_F32 ? 4 : d == PHZ_BF16 ? 2 : 1; }
+inline int64_t elem_bytes(int d) {
+  return d == PHZ_F64 || d == PHZ_I64 ? 8 : d == PHZ_F32 || d == PHZ_I32 ? 4 : d == PHZ_BF16 ? 2 : 1;
+}
 
 // Shape, type and layout of one argument. `size`: what each axis has to be,
 // -1 for any. The last axis has to be dense where `dense` is set; strides may
@@ -106,7 +114,7 @@ inline bool empty(const phz_tensor* t) {
   return false;
 }
 inline bool launched(phz_ops* o, const char* what) { return o->hip_ok(hipGetLastError(), what); }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ── device side ─────────────────────────────────────────────────────────────
 

@@ -1,5 +1,6 @@
 """Operators of sequence policies on the device, over the C ABI of
-phyz_amd/csrc/phz_scan.hip, phz_linear.hip and phz_muon.hip.
+phyz_amd/csrc/phz_scan.hip, phz_linear.hip, phz_muon.hip, phz_attend.hip,
+phz_rotary.hip and phz_adamw.hip.
 
 A policy with memory is a stack of blocks: a linear layer into gates and
 values, a gated linear recurrence over the rollout's steps, and a linear layer
@@ -14,6 +15,16 @@ weight matrices:
     dh, dw_out, _ = ops.linear_backward(dy, h, w_out)
     dz, dx, dh0 = ops.gated_scan_backward(dh, z, x, h, h0=h0, reset=reset)
     ops.muon_step(w_out, dw_out, momentum_out, lr=0.02)
+
+The recurrence's state may be a matrix for each head instead of a vector, read
+by queries and written by keys and values (linear attention with a decay), with
+positions as rotations of queries and keys; and parameters of any shapes take
+one AdamW step together:
+
+    qk = ops.rotary(qkv[..., :2 * n], positions, freq, heads=2 * heads)
+    o, s = ops.linear_attention(qk[..., :n], qk[..., n:], qkv[..., 2 * n:], g, reset=reset)
+    o = ops.linear_attention_step(q, k, v, g, s)              # acting: s advances
+    ops.adamw_step(params, grads, m, v, step)
 
 Arguments are torch tensors on the handle's GPU; calls enqueue their work on
 torch's current stream and return without waiting. Errors raise OpsError with
@@ -43,11 +54,15 @@ ACTS = {"none": 0, "tanh": 1, "relu": 2, "silu": 3, "gelu": 4}
 # 0.7 to 1.2.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
-_DTYPES = (torch.float32, torch.float64, torch.bfloat16, torch.uint8, torch.bool)
+PAIRS = {"half": 0, "interleaved": 1}
+
+_DTYPES = (torch.float32, torch.float64, torch.bfloat16, torch.uint8, torch.bool, torch.int32, torch.int64)
 # The entry points, in the order of phz_describe.cpp's table.
 _ENTRIES = ("phz_gated_scan", "phz_gated_scan_backward", "phz_gated_step", "phz_linear", "phz_linear_backward",
-            "phz_orthogonalize", "phz_muon_step")
-_SCAN, _SCAN_BACKWARD, _STEP, _LINEAR, _LINEAR_BACKWARD, _ORTHOGONALIZE, _MUON = range(7)
+            "phz_orthogonalize", "phz_muon_step", "phz_linear_attention", "phz_linear_attention_backward",
+            "phz_linear_attention_step", "phz_rotary", "phz_adamw_step", "phz_adamw_values")
+(_SCAN, _SCAN_BACKWARD, _STEP, _LINEAR, _LINEAR_BACKWARD, _ORTHOGONALIZE, _MUON, _ATTENTION, _ATTENTION_BACKWARD,
+ _ATTENTION_STEP, _ROTARY, _ADAMW, _ADAMW_VALUES) = range(13)
 _describe = None
 
 
@@ -81,6 +96,26 @@ class OpsError(RuntimeError):
     pass
 
 
+def rotary_frequencies(size: int, base: float = 10000.0, stretch: float = 1.0, turns=None, context: int = 0) -> torch.Tensor:
+    """Radians a position for the size / 2 pairs of Ops.rotary, float64 on the CPU:
+    base^(-2 i / size). For contexts `stretch` times as long as those trained on,
+    all are divided by it, or, given turns=(few, many) and the trained context,
+    only pairs that turn at most `few` times in it; pairs that turn `many` times or
+    more are kept, those between blended."""
+    if size < 0 or size % 2:
+        raise OpsError(f"the rotated part of a head has to be even, not {size}")
+    if not (base > 0 and stretch > 0 and math.isfinite(base) and math.isfinite(stretch)):
+        raise OpsError("base and stretch have to be positive and finite")
+    f = base ** (-torch.arange(size // 2, dtype=torch.float64) * 2 / max(size, 1))
+    if turns is None:
+        return f / stretch
+    few, many = turns
+    if not (0 <= few < many and math.isfinite(many) and context > 0):
+        raise OpsError("turns have to be (few, many), few below many, with the trained context")
+    keep = ((f * context / (2 * math.pi) - few) / (many - few)).clamp(0, 1)
+    return f * (keep + (1 - keep) / stretch)
+
+
 class Ops:
     """A handle: one GPU's operators and their workspaces, one per stream and one
     per captured graph. A handle whose workspace a captured graph holds is kept to
@@ -88,7 +123,7 @@ class Ops:
 
     def __init__(self, device: int = 0):
         self._L = _lib.load()
-        self._call = _bound().call
+        self._call, self._call_lists = _bound().call, _bound().call_lists
         self.device = int(device)
         h = C.c_void_p()
         if self._L.phz_ops_create(self.device, C.byref(h)) != 0:
@@ -128,6 +163,28 @@ class Ops:
         if not 1 <= t.dim() <= 3:
             raise OpsError(f"{name} has {t.dim()} dimensions, expected 1 to 3")
         raise OpsError(f"{name} has no strided memory to read here (a sparse tensor, or one inside vmap or a trace)")
+
+    def _run_lists(self, op: int, head: int, names: str, lists, single=None):
+        """One entry point of lists of tensors on the current stream."""
+        names = names.split()
+        for name, x in zip(names, lists):
+            if x is not None and not isinstance(x, (list, tuple)):
+                raise OpsError(f"{name} has to be a list of tensors, not {type(x).__name__}")
+        lists = [None if x is None else tuple(x) for x in lists]
+        n = len(lists[0])
+        for name, x in zip(names, lists):
+            if x is not None and len(x) != n:
+                raise OpsError(f"{name} has {len(x)} tensors, {names[0]} has {n}")
+        rc = self._call_lists(op, self._h, _raw_stream(self.device) if self.device >= 0 else 0, self.device, head,
+                              tuple(lists), single)
+        if rc > 0:
+            raise OpsError(self._L.phz_ops_last_error(self._h).decode())
+        if rc < 0:
+            i, l = divmod(-1 - rc, 5)
+            name, t = (names[5], single) if i == n else (f"{names[l]}[{i}]", lists[l][i])
+            if isinstance(t, torch.Tensor) and t.get_device() == self.device and t.dtype in _DTYPES and not t.is_contiguous():
+                raise OpsError(f"{name} is not contiguous")
+            self._complain(name, t)
 
     def _stream(self):
         return _raw_stream(self.device) if self.device >= 0 else None
@@ -262,3 +319,165 @@ class Ops:
         cfg = self._muon(steps, coef, eps, lr, momentum, nesterov, weight_decay)
         self._run(_MUON, C.addressof(cfg), "w g m", w, g, m)
         _written((w, m))
+
+    # ── linear attention with a decay for each head ──
+    @staticmethod
+    def _heads(q, v, g, size_k, size_v, scale):
+        """(heads, the head sizes and scale as the library takes them)."""
+        heads = g.shape[-1]
+        if heads < 1:
+            raise OpsError("g has no heads")
+        size_k = q.shape[-1] // heads if size_k is None else int(size_k)
+        size_v = v.shape[-1] // heads if size_v is None else int(size_v)
+        if not (1 <= size_k <= 128 and 1 <= size_v <= 128):
+            raise OpsError(f"size_k and size_v have to be 1 to 128, not {size_k} and {size_v}")
+        return heads, _lib.AttentionCfg(size_k ** -0.5 if scale is None else float(scale), size_k, size_v)
+
+    @staticmethod
+    def _matrices(s, name: str, cfg):
+        """States [worlds, heads, size_k, size_v] with one axis for each's elements."""
+        if s is None:
+            return None
+        if not isinstance(s, torch.Tensor) or s.dim() != 4:
+            raise OpsError(f"{name} has to be a tensor [worlds, heads, size_k, size_v]")
+        for axis, n in ((2, cfg.size_k), (3, cfg.size_v)):
+            if s.shape[axis] != n:
+                raise OpsError(f"{name} has {s.shape[axis]} elements along axis {axis}, expected {n}")
+        try:
+            return s.view(s.shape[0], s.shape[1], s.shape[2] * s.shape[3])
+        except RuntimeError:
+            raise OpsError(f"{name}: each head's state has to be dense") from None
+
+    def _rates(self, g, like):
+        """g of all steps and worlds, from one of the heads alone."""
+        if self._tensor(g, "g").dim() == 1 and like.dim() > 1:
+            return g.expand(*like.shape[:-1], g.shape[0])
+        return g
+
+    def linear_attention(self, q, k, v, g, s0=None, reset=None, size_k=None, size_v=None, scale=None, out=None):
+        """S_t = exp(g_t) S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t for q, k
+        [steps, worlds, heads * size_k] and v [steps, worlds, heads * size_v] (views
+        with a dense last axis) and g [steps, worlds, heads] float32, or [heads]: (o
+        like v's heads, the last state [worlds, heads, size_k, size_v] float32).
+        Given size_k and size_v, q, k and v may each have fewer heads than g: each
+        then serves heads / its heads of g's in a row. s0 are the states before the
+        first step (None: zeros); where reset [steps, worlds] is set, or g is below
+        -104, an episode begins and S_{t-1} counts as 0. scale: size_k^-0.5 if None."""
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g")):
+            self._tensor(t, name)
+        if q.dim() != 3:
+            raise OpsError(f"q has {q.dim()} dimensions, expected 3")
+        g = self._rates(g, q)
+        heads, cfg = self._heads(q, v, g, size_k, size_v, scale)
+        if out is not None:
+            o, last = out
+        else:
+            o = torch.empty((*q.shape[:-1], heads * cfg.size_v), dtype=q.dtype, device=q.device)
+            last = torch.empty((q.shape[1], heads, cfg.size_k, cfg.size_v), dtype=torch.float32, device=q.device)
+        self._run(_ATTENTION, C.addressof(cfg), "q k v g s0 reset o s_last", q, k, v, g, self._matrices(s0, "s0", cfg), reset, o,
+                  self._matrices(last, "s_last", cfg))
+        if out is not None:
+            _written([t for t in out if t is not None])
+        return o, last
+
+    def linear_attention_backward(self, do, q, k, v, g, s0=None, reset=None, ds=None, size_k=None, size_v=None, scale=None,
+                                  need_dg: bool = True, out=None):
+        """The gradients (dq, dk, dv, dg, ds0) of linear_attention, from those of o
+        and of the last state (None: zero). dq, dk and dv are like q, k and v, summed
+        over the heads that share them; dg [steps, worlds, heads] is every step's and
+        world's own also where g is one of the heads alone, None if not needed; dg and
+        ds0 are float32."""
+        for t, name in ((do, "do"), (q, "q"), (k, "k"), (v, "v"), (g, "g")):
+            self._tensor(t, name)
+        if q.dim() != 3:
+            raise OpsError(f"q has {q.dim()} dimensions, expected 3")
+        g = self._rates(g, q)
+        heads, cfg = self._heads(q, v, g, size_k, size_v, scale)
+        if out is not None:
+            dq, dk, dv, dg, ds0 = out
+        else:
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            dg = torch.empty((*q.shape[:-1], heads), dtype=torch.float32, device=q.device) if need_dg else None
+            ds0 = torch.empty((q.shape[1], heads, cfg.size_k, cfg.size_v), dtype=torch.float32, device=q.device)
+        self._run(_ATTENTION_BACKWARD, C.addressof(cfg), "do ds q k v g s0 reset dq dk dv dg ds0", do, self._matrices(ds, "ds", cfg),
+                  q, k, v, g, self._matrices(s0, "s0", cfg), reset, dq, dk, dv, dg, self._matrices(ds0, "ds0", cfg))
+        if out is not None:
+            _written([t for t in out if t is not None])
+        return dq, dk, dv, dg, ds0
+
+    def linear_attention_step(self, q, k, v, g, s, reset=None, size_k=None, size_v=None, scale=None, out=None):
+        """One step for q, k, v and g without the axis of steps: o [worlds, heads *
+        size_v]; the states s [worlds, heads, size_k, size_v] float32 are replaced."""
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g")):
+            self._tensor(t, name)
+        if q.dim() != 2:
+            raise OpsError(f"q has {q.dim()} dimensions, expected 2")
+        g = self._rates(g, q)
+        heads, cfg = self._heads(q, v, g, size_k, size_v, scale)
+        o = out if out is not None else torch.empty((q.shape[0], heads * cfg.size_v), dtype=q.dtype, device=q.device)
+        self._run(_ATTENTION_STEP, C.addressof(cfg), "q k v g reset s o", q, k, v, g, reset,
+                  self._matrices(self._tensor(s, "s"), "s", cfg), o)
+        _written((s,) if out is None else (s, o))
+        return o
+
+    # ── rotary positions ──
+    def rotary(self, x, positions, freq, heads: int = 1, layout: str = "half", scale: float = 1.0, inverse: bool = False,
+               out=None):
+        """x [..., heads * size] with the first 2 len(freq) elements of each head
+        turned by positions * freq, in pairs (i, i + len(freq)) ("half") or (2 i, 2 i
+        + 1) ("interleaved"), and multiplied by scale; the others are copied. positions
+        (int32 or int64) have x's axes but the last, of which there are one or two;
+        freq is float64 (rotary_frequencies). inverse turns back: the gradient for x is
+        rotary(dy, ..., inverse=True). `out` may be x."""
+        p = self._choice(PAIRS, layout, "layout")
+        cfg = _lib.RotaryCfg(float(scale), int(heads), p, int(bool(inverse)))
+        y = out if out is not None else torch.empty_like(self._tensor(x, "x"))
+        x3, p2, y3 = x, positions, y
+        if isinstance(x, torch.Tensor) and x.dim() == 2:
+            x3, p2, y3 = (t[None] if isinstance(t, torch.Tensor) else t for t in (x, positions, y))
+        self._run(_ROTARY, C.addressof(cfg), "x positions freq y", x3, p2, freq, y3)
+        if out is not None:
+            _written((y,))
+        return y
+
+    # ── AdamW ──
+    @staticmethod
+    def adamw_state(params, bits: int = 32):
+        """(m, v, exponents, step) of adamw_step for tensors like params, before the
+        first step: moments in 32 bits (exponents None), or in 8 with an exponent for
+        each 256 elements."""
+        params = list(params)
+        if bits not in (32, 8):
+            raise OpsError(f"moments have 32 or 8 bits, not {bits}")
+        dt = torch.float32 if bits == 32 else torch.uint8
+        m, v = ([torch.zeros(p.shape, dtype=dt, device=p.device) for p in params] for _ in range(2))
+        e = None if bits == 32 else [torch.zeros(2, -(-p.numel() // 256), dtype=torch.uint8, device=p.device) for p in params]
+        where = params[0].device if params else torch.device("cpu")
+        return m, v, e, torch.zeros(1, dtype=torch.int64, device=where)
+
+    def adamw_step(self, w, g, m, v, step, exponents=None, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                   weight_decay: float = 0.01, seed: int = 0):
+        """One AdamW step of the tensors w (float32 or bfloat16, in place) for the
+        gradients g (either), with the moments m and v (in place; float32, or uint8
+        with their exponents): lists of one length, of contiguous tensors of any
+        shapes, best made by adamw_state. step, an int64 tensor of one element, counts
+        the steps, also in replays of a captured graph. Moments of 8 bits are rounded
+        by random bits that follow from seed and step."""
+        cfg = _lib.AdamWCfg(lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xffffffff)
+        self._run_lists(_ADAMW, C.addressof(cfg), "w g m v exponents step", (w, g, m, v, exponents), self._tensor(step, "step"))
+        _written([*w, *m, *v, *(exponents or ()), step])
+
+    def adamw_values(self, m, v, exponents, out=None):
+        """The values of 8-bit moments, lists of bfloat16 tensors, which hold them
+        exactly: (m's, v's)."""
+        if out is None:
+            for name, x in (("m", m), ("v", v)):
+                if not isinstance(x, (list, tuple)):
+                    raise OpsError(f"{name} has to be a list of tensors, not {type(x).__name__}")
+            out = tuple([torch.empty(self._tensor(t, "m").shape, dtype=torch.bfloat16, device=t.device) for t in x]
+                        for x in (m, v))
+            self._run_lists(_ADAMW_VALUES, 0, "m v exponents m_values v_values", (m, v, exponents, *out))
+        else:
+            self._run_lists(_ADAMW_VALUES, 0, "m v exponents m_values v_values", (m, v, exponents, *out))
+            _written([t for x in out for t in x])
+        return out
