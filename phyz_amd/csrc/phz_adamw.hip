@@ -88,6 +88,18 @@ __device__ __forceinline__ uint32_t encode(float x, int e, uint32_t dither) {
   return bits ? max(code, 1u) : 0;
 }
 
+// x a + y b and x^2 with every product and sum rounded: codes follow from them, and
+// are the same in any implementation that does so.
+__device__ __forceinline__ float blend(float x, float a, float y, float b) {
+#pragma clang fp contract(off)
+  const float p = x * a, q = y * b;
+  return p + q;
+}
+__device__ __forceinline__ float square(float x) {
+#pragma clang fp contract(off)
+  return x * x;
+}
+
 // The largest biased exponent of a wave's finite values, at least 40.
 __device__ __forceinline__ int block_exponent(uint32_t most) {
 #pragma unroll
@@ -125,8 +137,7 @@ __device__ __forceinline__ void stash(E* p, int n, const float* x) {
 }
 
 // A wave takes 256 elements at a time, a lane four of them. In 8 bits that is a
-// block, whose exponent the wave's lanes find together. Products and sums are
-// rounded one by one where codes follow from them.
+// block, whose exponent the wave's lanes find together.
 template <class W, class G, bool EIGHT>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWArgs a) {
   int at = 0;
@@ -159,8 +170,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      m[i] = __fadd_rn(__fmul_rn(m[i], a.b1), __fmul_rn(g[i], a.c1));
-      v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g[i], g[i]), a.c2));
+      m[i] = blend(m[i], a.b1, g[i], a.c1);
+      v[i] = blend(v[i], a.b2, square(g[i]), a.c2);
       w[i] = w[i] * a.keep - (m[i] / fix1) * a.lr / (sqrtf(v[i] / fix2) + a.eps);
     }
     stash((W*)t.w + i0, n, w);

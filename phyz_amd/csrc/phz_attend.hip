@@ -6,15 +6,29 @@
 //   E_t = scale q_t do_t^T + a_{t+1} E_{t+1}
 //   dq_t = scale S_t do_t,  dk_t = E_t v_t,  dv_t = E_t^T k_t,
 //   dg_t = a_t <E_t, S_{t-1}>,  ds0 = a_0 E_0
+//
+// Steps are taken in chunks of C (64 in bf16, 32 in f32), in which the recurrence
+// is four matrix products. With L[t][s] = a_{s+1} .. a_t for s <= t (0 where an
+// episode begins between), e_t = L from the chunk's start, r_s = L to its end and
+// f over all of it,
+//   A = scale (Q K^T) o L,   O = A V + scale e o (Q S),   S <- f S + K^T (r o V)
+// A workgroup takes one head of one world through its chunks (or a segment of
+// them, where heads are few), the state in its waves' registers: the data is read
+// once. L comes from running sums of g in f64, as differences of long ones are
+// taken.
 #include "phz_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace phzop;
 
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxSize = 128;       // of a head's keys and values
 constexpr float kForgets = -104.0f; // exp of less is 0 in f32: an episode begins
@@ -238,6 +252,514 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
   }
 }
 
+// ── chunks: products of tiles of 16 ─────────────────────────────────────────
+//
+// A fragment is, of a lane (c, g) = (lane % 16, lane / 16), four neighbouring
+// elements 4 g .. 4 g + 3 of a block of 16 along the contraction, of row (or
+// column) c. The matrix instructions' result has that form too, its rows along the
+// contraction: a state that one product leaves in registers is the next one's
+// operand as it is.
+template <class E> struct Kind;
+template <> struct Kind<float> {
+  typedef f32x4 Frag;
+  static constexpr int C = 32, kScores = 1, kState = 1, kExact = 1;
+};
+// bf16: operands that are f32 go in pieces, each the rounding of what the ones
+// before leave: scores and the state as it is read in two (2^-17 of them: the
+// results are rounded to 2^-9), what is added to the state in three, as f32 holds it.
+template <> struct Kind<bf16> {
+  typedef s16x4 Frag;
+  static constexpr int C = 64, kScores = 2, kState = 2, kExact = 3;
+};
+
+// c + A B over N blocks of 16.
+template <int N>
+__device__ __forceinline__ f32x4 mma(const f32x4* a, const f32x4* b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][r], b[i][r], c, 0, 0, 0);
+  return c;
+}
+template <int N>
+__device__ __forceinline__ f32x4 mma(const s16x4* a, const s16x4* b, f32x4 c) {
+  static_assert(N % 2 == 0, "an instruction takes two blocks");
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const s16x8 x = __builtin_shufflevector(a[i], a[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    const s16x8 y = __builtin_shufflevector(b[i], b[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  }
+  return c;
+}
+
+// v in NP pieces, each `stride` fragments from the last.
+template <int NP>
+__device__ __forceinline__ void cut(f32x4 v, f32x4* out, int) {
+  static_assert(NP == 1, "f32 is whole");
+  out[0] = v;
+}
+template <int NP>
+__device__ __forceinline__ void cut(f32x4 v, s16x4* out, int stride) {
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    s16x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const bf16 h = from_f32<bf16>(v[i]);
+      x[i] = (short)h.bits;
+      if (p + 1 < NP) v[i] -= to_f32(h);
+    }
+    out[p * stride] = x;
+  }
+}
+__device__ __forceinline__ f32x4 widen(f32x4 v) { return v; }
+__device__ __forceinline__ f32x4 widen(s16x4 v) {
+  f32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = to_f32(bf16{(uint16_t)v[i]});
+  return x;
+}
+// a where it is kept, 0 (whatever x is) where nothing is left of it.
+__device__ __forceinline__ f32x4 scaled(f32x4 x, float by) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = by != 0.0f ? x[i] * by : 0.0f;
+  return x;
+}
+
+// A tile of ROWS x D in LDS, rows 16 bytes apart from whole banks: fragments along
+// a row and down a column fall into all banks.
+template <class E, int D>
+struct Tile {
+  typedef typename Kind<E>::Frag Frag;
+  static constexpr int kRow = D * sizeof(E) + 16;
+  static __device__ __forceinline__ Frag along(const char* l, int row, int block) {
+    const int lane = threadIdx.x & 63;
+    return *(const Frag*)(l + (row + (lane & 15)) * kRow + (16 * block + (lane >> 4) * 4) * (int)sizeof(E));
+  }
+  // Rows 16 block + 4 g .. + 3 of column col + c.
+  static __device__ __forceinline__ Frag down(const char* l, int block, int col) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    if constexpr (sizeof(E) == 4) {
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; r++) v[r] = *(const float*)(l + (16 * block + 4 * g + r) * kRow + (col + c) * 4);
+      return v;
+    } else {
+      // The transposing read hands each lane of 16 a column of a 4 x 16 block.
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(l + (16 * block + 4 * g + (c >> 2)) * kRow + col * 2 + (c & 3) * 8));
+    }
+  }
+};
+
+// A chunk's rows of one tensor on their way from memory to LDS through registers,
+// NT threads; rows and columns that do not exist are 0.
+template <class E, int D, int NT>
+struct Load {
+  static constexpr int C = Kind<E>::C, EL = 16 / sizeof(E), kPer = D / EL, kStep = NT / kPer;
+  static constexpr int N = (C + kStep - 1) / kStep;
+  Pack<E, EL> x[N];
+  __device__ __forceinline__ void fetch(const E* base, int64_t stride, int left, int d) {
+    const int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int row = row0 + i * kStep;
+      const E* p = base + row * stride + col;
+      if (row < left && col + EL <= d) {
+        x[i] = *(const Pack<E, EL>*)p;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EL; e++) x[i].v[e] = row < left && col + e < d ? p[e] : E{};
+      }
+    }
+  }
+  __device__ __forceinline__ void stash(char* l) const {
+    const int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int row = row0 + i * kStep;
+      if (C % kStep == 0 || row < C) *(f32x4*)(l + row * Tile<E, D>::kRow + col * (int)sizeof(E)) = __builtin_bit_cast(f32x4, x[i]);
+    }
+  }
+};
+
+// What the gates of a chunk come to.
+template <int C>
+struct Decays {
+  double sum[C];            // of log2 of the gates up to t
+  float e[C], r[C];         // from the start to t, from t to the end; 0 behind or before a reset
+  float u[C], w[C];         // from the end of the tile of 16 before to t, from t to the end of its tile
+  int32_t since[C];         // the last step up to t at which an episode begins, or 0
+  float f;                  // over all of it, or 0
+  double all;               // log2 of it without resets
+  uint64_t resets;
+};
+struct Gate {
+  float x;
+  bool reset;
+};
+// A lane a step; by one wave.
+__device__ __forceinline__ Gate fetch_gate(const float* g, int64_t g_t, const uint8_t* reset, int64_t r_t, int left) {
+  const int lane = threadIdx.x & 63;
+  Gate v{0.0f, false};
+  if (lane < left) {
+    v.x = g[lane * g_t];
+    v.reset = reset && reset[lane * r_t];
+  }
+  return v;
+}
+template <int C>
+__device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
+  const int lane = threadIdx.x & 63;
+  const bool reset = v.reset || v.x < kForgets;
+  // A reset's own gate does not count: what is left of before is nothing.
+  double x = reset ? 0.0 : (double)v.x * 1.4426950408889634074;
+#pragma unroll
+  for (int m = 1; m < C; m *= 2) {
+    const double y = __shfl_up(x, m);
+    if (lane >= m) x += y;
+  }
+  const uint64_t resets = __ballot(reset);
+  const double all = __shfl(x, C - 1);
+  const double before = __shfl(x, max((lane & ~15) - 1, 0)), last = __shfl(x, lane | 15);
+  if (lane >= C) return;
+  const uint64_t upto = resets & (2ull << lane) - 1ull;
+  const int at = resets ? 63 - __builtin_clzll(resets) : 0;
+  d->sum[lane] = x;
+  d->e[lane] = upto ? 0.0f : __builtin_amdgcn_exp2f((float)x);
+  d->r[lane] = lane >= at ? __builtin_amdgcn_exp2f((float)(all - x)) : 0.0f;
+  d->u[lane] = __builtin_amdgcn_exp2f((float)(lane < 16 ? x : x - before));
+  d->w[lane] = __builtin_amdgcn_exp2f((float)(last - x));
+  d->since[lane] = upto ? 63 - __builtin_clzll(upto) : 0;
+  if (lane == 0) {
+    d->f = resets ? 0.0f : __builtin_amdgcn_exp2f((float)all);
+    d->all = all;
+    d->resets = resets;
+  }
+}
+// L[t][s] for the lane's t = 16 b + c and s = 16 a + 4 g .. + 3: between tiles the
+// product of the way from s to its tile's end, from there to t's tile, and on to t.
+template <int C>
+__device__ __forceinline__ f32x4 decay_between(const Decays<C>& d, int a, int b) {
+  const int lane = threadIdx.x & 63, t = 16 * b + (lane & 15), s = 16 * a + (lane >> 4) * 4, since = d.since[t];
+  f32x4 x;
+  if (a == b) {
+    const double at = d.sum[t];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      x[r] = s + r <= t && s + r >= since ? __builtin_amdgcn_exp2f((float)(at - d.sum[s + r])) : 0.0f;
+  } else {
+    float way = d.u[t];
+    if (b > a + 1) way *= __builtin_amdgcn_exp2f((float)(d.sum[16 * b - 1] - d.sum[16 * a + 15]));
+    const f32x4 w = *(const f32x4*)&d.w[s];
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = s + r >= since ? way * w[r] : 0.0f;
+  }
+  return x;
+}
+// Tile n of the C / 16 (C / 16 + 1) / 2 with a <= b.
+__device__ __forceinline__ void tile_of(int n, int* a, int* b) {
+  *b = n >= 6 ? 3 : n >= 3 ? 2 : n >= 1 ? 1 : 0;
+  *a = n - *b * (*b + 1) / 2;
+}
+
+// Segments: `chunks` chunks each, one a workgroup. States before them stand in
+// `states` [segments][heads of all worlds][kR * kC] as the waves hold them: of
+// rows x columns (kR x kC after padding), lane's four rows of a column together.
+struct Segments {
+  int32_t chunks, count;
+  float* states;
+  float* decay;     // [segments][heads]: over a segment, negative where a reset is in it
+  uint32_t* flags;  // [segments][heads]: results that are not finite
+};
+
+// A workgroup's head and segment. Neighbouring heads share lines of memory: they
+// go to one XCD.
+__device__ __forceinline__ void place_of(int64_t heads, int64_t* bh, int* segment) {
+  const uint32_t n = gridDim.x, per = n / 8, i = blockIdx.x;
+  const uint32_t id = i < per * 8 ? i % 8 * per + i / 8 : i;
+  *bh = id % heads;
+  *segment = (int)(id / heads);
+}
+
+__device__ __forceinline__ bool not_finite(float sum_of_zeros) { return sum_of_zeros != 0.0f || sum_of_zeros != sum_of_zeros; }
+__device__ __forceinline__ float zeros_of(f32x4 x, float z) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) z = fmaf(x[i], 0.0f, z);
+  return z;
+}
+
+// The wave's 16 columns of a state in the caller's layout (element (row, col) at
+// row * row_stride + col * col_stride).
+template <int NB>
+__device__ __forceinline__ void read_state(const float* p, int64_t row_stride, int64_t col_stride, int rows, int cols, int col0,
+                                           f32x4 (&s)[NB]) {
+  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < NB; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int row = 16 * i + 4 * g + r;
+      s[i][r] = p && row < rows && col < cols ? p[row * row_stride + col * col_stride] : 0.0f;
+    }
+}
+template <int NB>
+__device__ __forceinline__ void write_state(float* p, int64_t row_stride, int64_t col_stride, int rows, int cols, int col0,
+                                            const f32x4 (&s)[NB]) {
+  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < NB; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int row = 16 * i + 4 * g + r;
+      if (row < rows && col < cols) p[row * row_stride + col * col_stride] = s[i][r];
+    }
+}
+
+// s <- f s + rows^T (weight o cols) of one chunk: the wave's 16 columns.
+template <class E, int DR, int DC>
+__device__ __forceinline__ void advance_state(const char* rows, const char* cols, const float* weight, float scale, float f, int col0,
+                                              f32x4 (&s)[DR / 16]) {
+  typedef Kind<E> K;
+  typedef typename K::Frag Frag;
+  constexpr int NB = K::C / 16;
+  const int g = (threadIdx.x & 63) >> 4;
+  Frag v[K::kExact][NB];
+#pragma unroll
+  for (int i = 0; i < NB; i++) {
+    f32x4 x = widen(Tile<E, DC>::down(cols, i, col0));
+    const f32x4 w = *(const f32x4*)(weight + 16 * i + 4 * g);
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[r] *= w[r] * scale;
+    cut<K::kExact>(x, &v[0][i], NB);
+  }
+#pragma unroll
+  for (int i = 0; i < DR / 16; i++) {
+    Frag k[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) k[j] = Tile<E, DR>::down(rows, j, 16 * i);
+    f32x4 x = scaled(s[i], f);
+#pragma unroll
+    for (int p = K::kExact - 1; p >= 0; p--) x = mma<NB>(k, v[p], x);
+    s[i] = x;
+  }
+}
+
+// The forward pass. Wave w has columns 16 w .. 16 w + 15 of the state and of o.
+// Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS.
+template <class E, int DK, int DV>
+__global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments seg) {
+  typedef Kind<E> K;
+  typedef typename K::Frag Frag;
+  constexpr int C = K::C, NT = DV * 4, NW = NT / 64, NB = C / 16, NK = DK / 16;
+  __shared__ __align__(16) char q_tile[C * Tile<E, DK>::kRow], k_tile[C * Tile<E, DK>::kRow], v_tile[C * Tile<E, DV>::kRow];
+  __shared__ __align__(16) char score[K::kScores][C * Tile<E, C>::kRow];
+  __shared__ __align__(16) Decays<C> decays;
+  __shared__ uint32_t bad;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col0 = 16 * wave;
+  const int64_t heads = (int64_t)a.worlds * a.heads;
+  int64_t bh;
+  int segment;
+  place_of(heads, &bh, &segment);
+  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  const int64_t first = (int64_t)segment * seg.chunks * C;
+  const int64_t end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
+  const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv);
+  const float* gate = a.g + b * a.g_b + h * a.g_h;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  E* o = (E*)a.o.p + b * a.o.b + (int64_t)h * a.nv;
+
+  f32x4 s[NK];
+  if (segment == 0) {
+    read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, a.nk, a.nv, col0, s);
+  } else {
+    const f32x4* p = (const f32x4*)(seg.states + (segment * heads + bh) * (DK * DV)) + wave * NK * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < NK; i++) s[i] = p[i * 64];
+  }
+  // Tiles right of the diagonal that a pair of blocks takes in are 0 for good.
+  for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = f32x4{};
+  if (threadIdx.x == 0) bad = 0;
+  Load<E, DK, NT> lq, lk;
+  Load<E, DV, NT> lv;
+  Gate lg{};
+  auto fetch = [&](int64_t t) {
+    const int left = (int)min((int64_t)C, end - t);
+    lq.fetch(q + t * a.q.t, a.q.t, left, a.nk);
+    lk.fetch(k + t * a.k.t, a.k.t, left, a.nk);
+    lv.fetch(v + t * a.v.t, a.v.t, left, a.nv);
+    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
+  };
+  fetch(first);
+  float zeros = 0.0f;
+  for (int64_t t0 = first; t0 < end; t0 += C) {
+    __syncthreads();  // the last chunk's tiles are read
+    lq.stash(q_tile);
+    lk.stash(k_tile);
+    lv.stash(v_tile);
+    if (wave == 0) find_decays(lg, &decays);
+    __syncthreads();
+    if (t0 + C < end) fetch(t0 + C);
+    for (int n = wave; n < NB * (NB + 1) / 2; n += NW) {
+      int ta, tb;
+      tile_of(n, &ta, &tb);
+      Frag x[NK], y[NK];
+#pragma unroll
+      for (int i = 0; i < NK; i++) {
+        x[i] = Tile<E, DK>::along(k_tile, 16 * ta, i);
+        y[i] = Tile<E, DK>::along(q_tile, 16 * tb, i);
+      }
+      f32x4 p = mma<NK>(x, y, f32x4{});
+      const f32x4 l = decay_between(decays, ta, tb);
+#pragma unroll
+      for (int r = 0; r < 4; r++) p[r] = l[r] != 0.0f ? p[r] * l[r] * a.scale : 0.0f;
+      Frag z[K::kScores];
+      cut<K::kScores>(p, z, 1);
+#pragma unroll
+      for (int i = 0; i < K::kScores; i++)
+        *(Frag*)(score[i] + (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E)) = z[i];
+    }
+    // What the state from before the chunk answers: o^T = S^T Q^T.
+    Frag sp[K::kState][NK];
+#pragma unroll
+    for (int i = 0; i < NK; i++) cut<K::kState>(s[i], &sp[0][i], NK);
+    f32x4 acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      Frag y[NK];
+#pragma unroll
+      for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, j);
+      f32x4 x{};
+#pragma unroll
+      for (int p = K::kState - 1; p >= 0; p--) x = mma<NK>(sp[p], y, x);
+      acc[i] = scaled(x, decays.e[16 * i + c] * a.scale);
+    }
+    advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
+    Frag vf[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0);
+    __syncthreads();  // the scores are there
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
+      f32x4 x = acc[i];
+#pragma unroll
+      for (int p = K::kScores - 1; p >= 0; p--)
+#pragma unroll
+        for (int j = 0; j <= i; j += two) {
+          Frag y[two];
+#pragma unroll
+          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(score[p], 16 * i, j + n);
+          x = mma<two>(&vf[j], y, x);
+        }
+      zeros = zeros_of(x, zeros);
+      const int64_t t = t0 + 16 * i + c;
+      const int j0 = col0 + 4 * g;
+      if (t < end) {
+        E* p = o + t * a.o.t + j0;
+        if (j0 + 4 <= a.nv) {
+          Pack<E, 4> y;
+#pragma unroll
+          for (int r = 0; r < 4; r++) y.v[r] = from_f32<E>(x[r]);
+          *(Pack<E, 4>*)p = y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (j0 + r < a.nv) p[r] = from_f32<E>(x[r]);
+        }
+      }
+    }
+  }
+  if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nv, 1, a.nk, a.nv, col0, s);
+#pragma unroll
+  for (int i = 0; i < NK; i++) zeros = zeros_of(s[i], zeros);
+  if (not_finite(zeros)) bad = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) seg.flags[segment * heads + bh] = bad;
+}
+
+// What a segment adds to the state, and how much it leaves of it: the state behind
+// it, from 0. The last segment's is not needed.
+template <class E, int DR, int DC>
+__global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Rows rows, Rows cols, Segments seg) {
+  typedef Kind<E> K;
+  constexpr int C = K::C, NT = DC * 4, NR = DR / 16;
+  __shared__ __align__(16) char r_tile[C * Tile<E, DR>::kRow], c_tile[C * Tile<E, DC>::kRow];
+  __shared__ __align__(16) Decays<C> decays;
+  __shared__ uint32_t bad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col0 = 16 * wave;
+  const int64_t heads = (int64_t)a.worlds * a.heads;
+  int64_t bh;
+  int segment;
+  place_of(heads, &bh, &segment);
+  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  const int64_t first = (int64_t)segment * seg.chunks * C, end = first + (int64_t)seg.chunks * C;
+  const E *rp = row_of<E>(rows, b, h, a.nk), *cp = row_of<E>(cols, b, h, a.nv);
+  const float* gate = a.g + b * a.g_b + h * a.g_h;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  f32x4 s[NR];
+#pragma unroll
+  for (int i = 0; i < NR; i++) s[i] = f32x4{};
+  if (threadIdx.x == 0) bad = 0;
+  Load<E, DR, NT> lr;
+  Load<E, DC, NT> lc;
+  Gate lg{};
+  auto fetch = [&](int64_t t) {
+    lr.fetch(rp + t * rows.t, rows.t, C, a.nk);
+    lc.fetch(cp + t * cols.t, cols.t, C, a.nv);
+    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, C);
+  };
+  fetch(first);
+  double all = 0.0;
+  bool forgets = false;
+  for (int64_t t0 = first; t0 < end; t0 += C) {
+    __syncthreads();
+    lr.stash(r_tile);
+    lc.stash(c_tile);
+    if (wave == 0) find_decays(lg, &decays);
+    __syncthreads();
+    if (t0 + C < end) fetch(t0 + C);
+    advance_state<E, DR, DC>(r_tile, c_tile, decays.r, 1.0f, decays.f, col0, s);
+    all += decays.all;
+    forgets = forgets || decays.resets;
+  }
+  f32x4* p = (f32x4*)(seg.states + ((segment + 1) * heads + bh) * (DR * DC)) + wave * NR * 64 + lane;
+  float zeros = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    p[i * 64] = s[i];
+    zeros = zeros_of(s[i], zeros);
+  }
+  __syncthreads();
+  if (not_finite(zeros)) bad = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    seg.decay[segment * heads + bh] = forgets ? -1.0f : (float)exp2(all);
+    // Behind the segments' own marks.
+    seg.flags[(seg.count + segment) * heads + bh] = bad;
+  }
+}
+
+// The state before each segment, from what each adds: in place.
+template <int DR, int DC>
+__global__ __launch_bounds__(256) void join_segments(AttendArgs a, States first, Segments seg) {
+  const int64_t heads = (int64_t)a.worlds * a.heads, bh = blockIdx.x / (DR * DC / 256);
+  const int i = blockIdx.x % (DR * DC / 256) * 256 + threadIdx.x;
+  const int r = i & 3, lane = i >> 2 & 63, tile = i >> 8, row = tile % (DR / 16) * 16 + (lane >> 4) * 4 + r;
+  const int col = tile / (DR / 16) * 16 + (lane & 15), b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  float s = first.p && row < a.nk && col < a.nv ? first.p[b * first.b + h * first.h + (int64_t)row * a.nv + col] : 0.0f;
+  float* p = seg.states + bh * (DR * DC) + i;
+  const int64_t step = heads * (DR * DC);
+#pragma unroll 8
+  for (int n = 1; n < seg.count; n++) {
+    const float add = p[n * step], f = seg.decay[(n - 1) * heads + bh];
+    s = f < 0.0f ? add : fmaf(f, s, add);
+    p[n * step] = s;
+  }
+}
+
 // ── a single step ───────────────────────────────────────────────────────────
 //
 // A workgroup takes `width` columns of one head's state: a thread four
@@ -408,6 +930,58 @@ unsigned sequential_blocks(const phz_ops* o, const AttendArgs& a) {
   return (unsigned)std::min<int64_t>((int64_t)a.worlds * a.heads, 2 * o->cus);
 }
 
+// ── how the steps are spread ────────────────────────────────────────────────
+
+int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+// Few heads take their steps in segments, so that the chip is filled; each has
+// four chunks at least, since the segments' states are found in a pass of its own.
+Segments segments_of(const phz_ops* o, const AttendArgs& a, int chunk) {
+  const int64_t heads = (int64_t)a.worlds * a.heads, chunks = ceil_div(a.steps, chunk);
+  Segments s{};
+  const int64_t want = std::max<int64_t>(1, std::min(ceil_div(2 * o->cus, heads), chunks / 4));
+  s.chunks = (int32_t)ceil_div(chunks, want);
+  s.count = (int32_t)ceil_div(chunks, s.chunks);
+  return s;
+}
+
+// Calls f with the padded sizes as constants.
+template <class F>
+void with_size(int n, F&& f) {
+  if (n <= 32) f(std::integral_constant<int, 32>());
+  else if (n <= 64) f(std::integral_constant<int, 64>());
+  else f(std::integral_constant<int, 128>());
+}
+
+template <class E>
+int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
+  const int64_t heads = (int64_t)a.worlds * a.heads;
+  Segments seg = segments_of(o, a, Kind<E>::C);
+  if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
+  // Marks of the segments' results, and of their states.
+  const int64_t state = (int64_t)padded(a.nk) * padded(a.nv), flags = ceil_div(2 * seg.count * heads * 4, 256) * 256;
+  char* work = o->workspace(stream, (seg.count > 1 ? seg.count * heads * (state + 1) * 4 : 0) + flags);
+  if (!work) return 1;
+  seg.flags = (uint32_t*)work;
+  seg.states = (float*)(work + flags);
+  seg.decay = seg.states + seg.count * heads * state;
+  with_size(a.nk, [&](auto dk) {
+    with_size(a.nv, [&](auto dv) {
+      constexpr int DK = dk(), DV = dv();
+      if (seg.count > 1) {
+        hipLaunchKernelGGL((segment_states<E, DK, DV>), dim3((unsigned)(heads * (seg.count - 1))), dim3(DV * 4), 0, stream, a, a.k,
+                           a.v, seg);
+        hipLaunchKernelGGL((join_segments<DK, DV>), dim3((unsigned)(heads * (DK * DV / 256))), dim3(256), 0, stream, a, a.s0, seg);
+      }
+      hipLaunchKernelGGL((attend_chunks<E, DK, DV>), dim3((unsigned)(heads * seg.count)), dim3(DV * 4), 0, stream, a, seg);
+    });
+  });
+  AttendArgs again = a;
+  again.flags = seg.flags;
+  hipLaunchKernelGGL(attend_sequential<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again, 2 * seg.count - 1);
+  return launched(o, "linear attention") ? 0 : 1;
+}
+
 }  // namespace
 
 extern "C" {
@@ -435,10 +1009,7 @@ int phz_linear_attention(phz_ops* o, void* stream_, const phz_attention_cfg* cfg
         hipLaunchKernelGGL(copy_states, dim3(a.worlds * a.heads), dim3(256), 0, stream, a.s0, a.s1, a.heads, a.nk * a.nv);
       return launched(o, "linear attention") ? 0 : 1;
     }
-    const unsigned blocks = sequential_blocks(o, a);
-    if (q->dtype == PHZ_F32) hipLaunchKernelGGL(attend_sequential<float>, dim3(blocks), dim3(512), 0, stream, a, 0);
-    else hipLaunchKernelGGL(attend_sequential<bf16>, dim3(blocks), dim3(512), 0, stream, a, 0);
-    return launched(o, "linear attention") ? 0 : 1;
+    return q->dtype == PHZ_F32 ? forward<float>(o, stream, a) : forward<bf16>(o, stream, a);
   });
 }
 
