@@ -464,14 +464,15 @@ __device__ __forceinline__ void tile_of(int n, int* a, int* b) {
   *a = n - *b * (*b + 1) / 2;
 }
 
-// Segments: `chunks` chunks each, one a workgroup. States before them stand in
-// `states` [segments][heads of all worlds][kR * kC] as the waves hold them: of
-// rows x columns (kR x kC after padding), lane's four rows of a column together.
+// Segments: `chunks` chunks each, one a workgroup. The states between them stand in
+// `states` [count - 1][heads of all worlds][rows * columns, padded] as the waves
+// hold them, a lane's four rows of a column together.
 struct Segments {
   int32_t chunks, count;
   float* states;
-  float* decay;     // [segments][heads]: over a segment, negative where a reset is in it
-  uint32_t* flags;  // [segments][heads]: results that are not finite
+  float* decay;           // [count - 1][heads]: over a segment, negative where a reset is in it
+  uint32_t* flags;        // [count][heads]: results that are not finite
+  uint32_t* state_flags;  // [count - 1][heads]: states that are not
 };
 
 // A workgroup's head and segment. Neighbouring heads share lines of memory: they
@@ -575,7 +576,7 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
   if (segment == 0) {
     read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, a.nk, a.nv, col0, s);
   } else {
-    const f32x4* p = (const f32x4*)(seg.states + (segment * heads + bh) * (DK * DV)) + wave * NK * 64 + lane;
+    const f32x4* p = (const f32x4*)(seg.states + ((segment - 1) * heads + bh) * (DK * DV)) + wave * NK * 64 + lane;
 #pragma unroll
     for (int i = 0; i < NK; i++) s[i] = p[i * 64];
   }
@@ -680,10 +681,23 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
   if (threadIdx.x == 0) seg.flags[segment * heads + bh] = bad;
 }
 
-// What a segment adds to the state, and how much it leaves of it: the state behind
-// it, from 0. The last segment's is not needed.
-template <class E, int DR, int DC>
-__global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Rows rows, Rows cols, Segments seg) {
+// A state's rows and columns: what key and val are to it, and where an element of
+// it stands in the caller's.
+struct Roles {
+  Rows rows, cols;
+  int32_t nr, nc;
+  int64_t row_stride, col_stride;
+  States first;
+};
+
+// States alone, of one segment a workgroup:
+//   ADDS   what a segment but the last adds to the state, from 0, and how much it
+//          leaves of it
+//   BACK   the same of the gradient's, E, from the end, of a segment but the first
+//   EACH   the state before each chunk
+enum { ADDS, BACK, EACH };
+template <class E, int DR, int DC, int MODE>
+__global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Roles x, Segments seg, f32x4* each) {
   typedef Kind<E> K;
   constexpr int C = K::C, NT = DC * 4, NR = DR / 16;
   __shared__ __align__(16) char r_tile[C * Tile<E, DR>::kRow], c_tile[C * Tile<E, DC>::kRow];
@@ -692,40 +706,56 @@ __global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Rows rows
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col0 = 16 * wave;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
-  int segment;
-  place_of(heads, &bh, &segment);
+  int slot;
+  place_of(heads, &bh, &slot);
+  const int segment = MODE == BACK ? slot + 1 : slot;
   const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-  const int64_t first = (int64_t)segment * seg.chunks * C, end = first + (int64_t)seg.chunks * C;
-  const E *rp = row_of<E>(rows, b, h, a.nk), *cp = row_of<E>(cols, b, h, a.nv);
+  const int64_t first = (int64_t)segment * seg.chunks * C, end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
+  const E *rp = row_of<E>(x.rows, b, h, x.nr), *cp = row_of<E>(x.cols, b, h, x.nc);
   const float* gate = a.g + b * a.g_b + h * a.g_h;
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   f32x4 s[NR];
+  if (MODE == EACH && segment == 0) {
+    read_state(x.first.p ? x.first.p + b * x.first.b + h * x.first.h : nullptr, x.row_stride, x.col_stride, x.nr, x.nc, col0, s);
+  } else {
+    const f32x4* p = (const f32x4*)(seg.states + ((segment - 1) * heads + bh) * (DR * DC)) + wave * NR * 64 + lane;
 #pragma unroll
-  for (int i = 0; i < NR; i++) s[i] = f32x4{};
+    for (int i = 0; i < NR; i++) s[i] = MODE == EACH ? p[i * 64] : f32x4{};
+  }
   if (threadIdx.x == 0) bad = 0;
   Load<E, DR, NT> lr;
   Load<E, DC, NT> lc;
   Gate lg{};
   auto fetch = [&](int64_t t) {
-    lr.fetch(rp + t * rows.t, rows.t, C, a.nk);
-    lc.fetch(cp + t * cols.t, cols.t, C, a.nv);
-    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, C);
+    const int left = (int)min((int64_t)C, end - t);
+    lr.fetch(rp + t * x.rows.t, x.rows.t, left, x.nr);
+    lc.fetch(cp + t * x.cols.t, x.cols.t, left, x.nc);
+    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
   };
-  fetch(first);
+  const int64_t chunks = (end - first + C - 1) / C;
+  auto start = [&](int64_t n) { return first + (MODE == BACK ? chunks - 1 - n : n) * C; };
+  fetch(start(0));
   double all = 0.0;
   bool forgets = false;
-  for (int64_t t0 = first; t0 < end; t0 += C) {
+  for (int64_t n = 0; n < chunks; n++) {
+    if (MODE == EACH) {
+      f32x4* p = each + ((start(n) / C * heads + bh) * (DC / 16) + wave) * NR * 64 + lane;
+#pragma unroll
+      for (int i = 0; i < NR; i++) p[i * 64] = s[i];
+      if (n + 1 == chunks) break;
+    }
     __syncthreads();
     lr.stash(r_tile);
     lc.stash(c_tile);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
-    if (t0 + C < end) fetch(t0 + C);
-    advance_state<E, DR, DC>(r_tile, c_tile, decays.r, 1.0f, decays.f, col0, s);
+    if (n + 1 < chunks) fetch(start(n + 1));
+    advance_state<E, DR, DC>(r_tile, c_tile, MODE == BACK ? decays.e : decays.r, MODE == BACK ? a.scale : 1.0f, decays.f, col0, s);
     all += decays.all;
     forgets = forgets || decays.resets;
   }
-  f32x4* p = (f32x4*)(seg.states + ((segment + 1) * heads + bh) * (DR * DC)) + wave * NR * 64 + lane;
+  if (MODE == EACH) return;
+  f32x4* p = (f32x4*)(seg.states + (slot * heads + bh) * (DR * DC)) + wave * NR * 64 + lane;
   float zeros = 0.0f;
 #pragma unroll
   for (int i = 0; i < NR; i++) {
@@ -736,28 +766,341 @@ __global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Rows rows
   if (not_finite(zeros)) bad = 1;
   __syncthreads();
   if (threadIdx.x == 0) {
-    seg.decay[segment * heads + bh] = forgets ? -1.0f : (float)exp2(all);
-    // Behind the segments' own marks.
-    seg.flags[(seg.count + segment) * heads + bh] = bad;
+    seg.decay[slot * heads + bh] = forgets ? -1.0f : (float)exp2(all);
+    seg.state_flags[slot * heads + bh] = bad;
   }
 }
 
-// The state before each segment, from what each adds: in place.
+// The state before each segment but the first (the gradient behind each but the
+// last), from what each adds: in place.
 template <int DR, int DC>
-__global__ __launch_bounds__(256) void join_segments(AttendArgs a, States first, Segments seg) {
+__global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segments seg, bool back) {
   const int64_t heads = (int64_t)a.worlds * a.heads, bh = blockIdx.x / (DR * DC / 256);
   const int i = blockIdx.x % (DR * DC / 256) * 256 + threadIdx.x;
   const int r = i & 3, lane = i >> 2 & 63, tile = i >> 8, row = tile % (DR / 16) * 16 + (lane >> 4) * 4 + r;
   const int col = tile / (DR / 16) * 16 + (lane & 15), b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-  float s = first.p && row < a.nk && col < a.nv ? first.p[b * first.b + h * first.h + (int64_t)row * a.nv + col] : 0.0f;
-  float* p = seg.states + bh * (DR * DC) + i;
-  const int64_t step = heads * (DR * DC);
+  float s = x.first.p && row < x.nr && col < x.nc
+                ? x.first.p[b * x.first.b + h * x.first.h + row * x.row_stride + col * x.col_stride]
+                : 0.0f;
+  const int slots = seg.count - 1;
+  const int64_t step = (back ? -1 : 1) * heads * (DR * DC), from = back ? slots - 1 : 0;
+  float* p = seg.states + (from * heads + bh) * (DR * DC) + i;
+  const float* f = seg.decay + from * heads + bh;
 #pragma unroll 8
-  for (int n = 1; n < seg.count; n++) {
-    const float add = p[n * step], f = seg.decay[(n - 1) * heads + bh];
-    s = f < 0.0f ? add : fmaf(f, s, add);
-    p[n * step] = s;
+  for (int n = 0; n < slots; n++) {
+    const float add = *p, keep = *f;
+    s = keep < 0.0f ? add : fmaf(keep, s, add);
+    *p = s;
+    p += step;
+    f += back ? -heads : heads;
   }
+}
+
+// Four neighbouring elements of a row of an output. `wide`: f32 sums of each head's own.
+template <class E>
+__device__ __forceinline__ void put4(const Rows& r, int64_t t, int b, int h, int size, int at, f32x4 v, bool wide) {
+  auto go = [&](auto* base) {
+    typedef std::remove_reference_t<decltype(*base)> O;
+    O* p = base + t * r.t + b * r.b + (int64_t)h * size + at;
+    if (at + 4 <= size) {
+      Pack<O, 4> y;
+#pragma unroll
+      for (int i = 0; i < 4; i++) y.v[i] = from_f32<O>(v[i]);
+      *(Pack<O, 4>*)p = y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (at + i < size) p[i] = from_f32<O>(v[i]);
+    }
+  };
+  if (wide) go((float*)r.p);
+  else go((E*)r.p);
+}
+
+__device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
+  return fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], x[3] * y[3])));
+}
+
+// The gradients, chunks from the last to the first. Beside the forward pass's
+// products, with S the state before the chunk, E the loss's gradient for the one
+// behind it, and W = dO V^T, dA = scale W o L:
+//   dQ = dA K + scale e o (dO S^T),  dK = dA^T Q + r o (V E^T),  dV = A^T dO + r o (K E),
+//   E <- f E + scale (e o Q)^T dO.
+// E is held twice, as rows of keys (a wave's 16 columns of values) and as rows of
+// values (its 16 columns of keys), so that dV and dK each find it in registers.
+// A gate's gradient sums over all ways across it: from the state before to the
+// gradient behind, X = f <S, E>; from steps u >= t to the state before,
+// q_u . (the state's part of dq_u); from steps s < t to the gradient behind,
+// k_s . (its part of dk_s); and between steps of the chunk, M = A o W over u >= t >
+// s, R_{t+1} = R_t + sum_u M[u][t] - sum_s M[t][s].
+// No sum is taken over more than a chunk, so nothing large cancels.
+template <class E, int DK, int DV>
+__global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(AttendArgs a, Segments seg, const f32x4* each, int32_t wide) {
+  typedef Kind<E> K;
+  typedef typename K::Frag Frag;
+  constexpr int C = K::C, D = DK > DV ? DK : DV, NT = D * 4, NW = NT / 64, NB = C / 16, NK = DK / 16, NV = DV / 16;
+  constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
+  __shared__ __align__(16) char q_tile[C * Tile<E, DK>::kRow], k_tile[C * Tile<E, DK>::kRow];
+  __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow], o_tile[C * Tile<E, DV>::kRow];
+  __shared__ __align__(16) char score[K::kScores][C * Tile<E, C>::kRow], dscore[K::kScores][C * Tile<E, C>::kRow];
+  __shared__ __align__(16) Decays<C> decays;
+  __shared__ __align__(16) float row_sum[NB][C], col_sum[NB][C], q_dot[NK][C], k_dot[NK][C], x_dot[NK];
+  __shared__ uint32_t bad;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col0 = 16 * wave;
+  const int64_t heads = (int64_t)a.worlds * a.heads;
+  int64_t bh;
+  int segment;
+  place_of(heads, &bh, &segment);
+  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  const int64_t first = (int64_t)segment * seg.chunks * C;
+  const int64_t end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
+  const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv),
+          *d_o = row_of<E>(a.o, b, h, a.nv);
+  const float* gate = a.g + b * a.g_b + h * a.g_h;
+  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+  float* dg = a.dg ? a.dg + b * a.dg_b + h * a.dg_h : nullptr;
+
+  f32x4 ek[NK], ev[NV];  // rows of keys, rows of values
+  if (segment + 1 == seg.count) {
+    const float* ds = a.ds.p ? a.ds.p + b * a.ds.b + h * a.ds.h : nullptr;
+    read_state(ds, a.nv, 1, a.nk, a.nv, col0, ek);
+    read_state(ds, 1, a.nv, a.nv, a.nk, col0, ev);
+  } else {
+    const float* p = seg.states + (segment * heads + bh) * (DK * DV);
+#pragma unroll
+    for (int i = 0; i < NK; i++) ek[i] = wave < NV ? ((const f32x4*)p)[(wave * NK + i) * 64 + lane] : f32x4{};
+    // Element (row d, column j) stands at tile j / 16 * NK + d / 16, lane d % 16 / 4 * 16 + j % 16, row d % 4.
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        ev[i][r] = wave < NK ? p[(((i * NK + wave) * 64) + (c >> 2) * 16 + 4 * g + r) * 4 + (c & 3)] : 0.0f;
+  }
+  for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = ((f32x4*)dscore)[i] = f32x4{};
+  if (threadIdx.x == 0) bad = 0;
+  Load<E, DK, NT> lq, lk;
+  Load<E, DV, NT> lv, lo;
+  Gate lg{};
+  auto fetch = [&](int64_t t) {
+    const int left = (int)min((int64_t)C, end - t);
+    lq.fetch(q + t * a.q.t, a.q.t, left, a.nk);
+    lk.fetch(k + t * a.k.t, a.k.t, left, a.nk);
+    lv.fetch(v + t * a.v.t, a.v.t, left, a.nv);
+    lo.fetch(d_o + t * a.o.t, a.o.t, left, a.nv);
+    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
+  };
+  float zeros = 0.0f;
+  // The gates' gradients of the chunk at t0, by the last wave, a lane a step.
+  auto gates = [&](int64_t t0, float f, uint64_t resets) {
+    const int t = lane, tile = t / 16;
+    float x = 0.0f, qd = 0.0f, kd = 0.0f, m = 0.0f;
+    for (int w = 0; w < NK; w++) x += x_dot[w];
+    if (t < C) {
+      for (int w = 0; w < NK; w++) qd += q_dot[w][t], kd += k_dot[w][t];
+      for (int i = tile; i < NB; i++) m += col_sum[i][t];
+      for (int i = 0; i <= tile; i++) m -= row_sum[i][t];
+    }
+    const float kd1 = kd, m1 = m;
+#pragma unroll
+    for (int n = 1; n < C; n *= 2) {
+      const float y = __shfl_down(qd, n), z = __shfl_up(kd, n), u = __shfl_up(m, n);
+      if (lane + n < 64) qd += y;
+      if (lane >= n) kd += z, m += u;
+    }
+    const float sum = (f != 0.0f ? f * x : 0.0f) + qd + ((kd - kd1) + (m - m1));
+    const int64_t step = t0 + t;
+    if (t < C && step < end) {
+      const float out = resets >> t & 1 ? 0.0f : sum;
+      zeros = fmaf(out, 0.0f, zeros);
+      dg[step * a.dg_t] = out;
+    }
+  };
+  const int64_t chunks = (end - first + C - 1) / C;
+  fetch(first + (chunks - 1) * C);
+  float f_before = 0.0f;
+  uint64_t resets_before = 0;
+  for (int64_t n = chunks - 1; n >= 0; n--) {
+    const int64_t t0 = first + n * C;
+    __syncthreads();  // the chunk before is done with its tiles, and its sums are there
+    if (dg && n + 1 < chunks && wave == NW - 1) gates(t0 + C, f_before, resets_before);
+    lq.stash(q_tile);
+    lk.stash(k_tile);
+    lv.stash(v_tile);
+    lo.stash(o_tile);
+    if (wave == 0) find_decays(lg, &decays);
+    __syncthreads();
+    if (n > 0) fetch(t0 - C);
+    f32x4 s[NV];  // the state before the chunk: rows of values, the wave's 16 columns of keys
+    if (wave < NK) {
+      if (each) {
+        const f32x4* p = each + ((t0 / C * heads + bh) * NK + wave) * NV * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < NV; i++) s[i] = p[i * 64];
+      } else {
+        read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, 1, a.nv, a.nv, a.nk, col0, s);
+      }
+    }
+    for (int m = wave; m < NB * (NB + 1) / 2; m += NW) {
+      int ta, tb;
+      tile_of(m, &ta, &tb);
+      Frag x[NK > NV ? NK : NV], y[NK > NV ? NK : NV];
+#pragma unroll
+      for (int i = 0; i < NK; i++) {
+        x[i] = Tile<E, DK>::along(k_tile, 16 * ta, i);
+        y[i] = Tile<E, DK>::along(q_tile, 16 * tb, i);
+      }
+      f32x4 p = mma<NK>(x, y, f32x4{});
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        x[i] = Tile<E, DV>::along(v_tile, 16 * ta, i);
+        y[i] = Tile<E, DV>::along(o_tile, 16 * tb, i);
+      }
+      f32x4 w = mma<NV>(x, y, f32x4{});
+      const f32x4 l = decay_between(decays, ta, tb);
+      f32x4 ways;
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const bool there = l[r] != 0.0f;
+        p[r] = there ? p[r] * l[r] * a.scale : 0.0f;
+        ways[r] = there && (ta != tb || 4 * g + r != c) ? p[r] * w[r] : 0.0f;
+        w[r] = there ? w[r] * l[r] * a.scale : 0.0f;
+        sum += ways[r];
+      }
+      const int at = (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E);
+      Frag z[K::kScores];
+      cut<K::kScores>(p, z, 1);
+#pragma unroll
+      for (int i = 0; i < K::kScores; i++) *(Frag*)(score[i] + at) = z[i];
+      cut<K::kScores>(w, z, 1);
+#pragma unroll
+      for (int i = 0; i < K::kScores; i++) *(Frag*)(dscore[i] + at) = z[i];
+      if (dg) {
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (g == 0) row_sum[ta][16 * tb + c] = sum;
+#pragma unroll
+        for (int n = 1; n < 16; n *= 2)
+#pragma unroll
+          for (int r = 0; r < 4; r++) ways[r] += __shfl_xor(ways[r], n);
+        if (c == 0) *(f32x4*)&col_sum[tb][16 * ta + 4 * g] = ways;
+      }
+    }
+    __syncthreads();
+    f_before = decays.f;
+    resets_before = decays.resets;
+    // c + the intra-chunk product: A's fragments `x` (a block of steps each) with
+    // the scores' of tile i, along their rows or down their columns.
+    auto add = [&](const Frag* x, const char (&scores)[K::kScores][C * Tile<E, C>::kRow], int i, bool along, f32x4 acc) {
+#pragma unroll
+      for (int p = K::kScores - 1; p >= 0; p--)
+#pragma unroll
+        for (int j = 0; j < NB; j += two) {
+          if (along ? j > i : j + two <= i) continue;
+          Frag y[two];
+#pragma unroll
+          for (int m = 0; m < two; m++)
+            y[m] = along ? Tile<E, C>::along(scores[p], 16 * i, j + m) : Tile<E, C>::down(scores[p], j + m, 16 * i);
+          acc = mma<two>(x + j, y, acc);
+        }
+      zeros = zeros_of(acc, zeros);
+      return acc;
+    };
+    if (wave < NK) {
+      Frag x[NB], big[K::kState][NV];
+      // dQ
+#pragma unroll
+      for (int i = 0; i < NV; i++) cut<K::kState>(s[i], &big[0][i], NV);
+#pragma unroll
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(k_tile, i, col0);
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        Frag y[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(o_tile, 16 * i, j);
+        f32x4 acc{};
+#pragma unroll
+        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
+        acc = scaled(acc, decays.e[16 * i + c] * a.scale);
+        if (dg) {
+          float d = dot4(acc, widen(Tile<E, DK>::along(q_tile, 16 * i, wave)));
+          d += __shfl_xor(d, 16);
+          d += __shfl_xor(d, 32);
+          if (g == 0) q_dot[wave][16 * i + c] = d;
+        }
+        acc = add(x, dscore, i, true, acc);
+        const int64_t t = t0 + 16 * i + c;
+        if (t < end) put4<E>(a.dq, t, b, h, a.nk, col0 + 4 * g, acc, wide & 1);
+      }
+      // dK
+      if (dg) {
+        float d = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) d += dot4(s[i], ev[i]);
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) d += __shfl_xor(d, m);
+        if (lane == 0) x_dot[wave] = d;
+      }
+#pragma unroll
+      for (int i = 0; i < NV; i++) cut<K::kState>(ev[i], &big[0][i], NV);
+#pragma unroll
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0);
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        Frag y[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(v_tile, 16 * i, j);
+        f32x4 acc{};
+#pragma unroll
+        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
+        acc = scaled(acc, decays.r[16 * i + c]);
+        if (dg) {
+          float d = dot4(acc, widen(Tile<E, DK>::along(k_tile, 16 * i, wave)));
+          d += __shfl_xor(d, 16);
+          d += __shfl_xor(d, 32);
+          if (g == 0) k_dot[wave][16 * i + c] = d;
+        }
+        acc = add(x, dscore, i, false, acc);
+        const int64_t t = t0 + 16 * i + c;
+        if (t < end) put4<E>(a.dk, t, b, h, a.nk, col0 + 4 * g, acc, wide & 2);
+      }
+      advance_state<E, DV, DK>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, ev);
+    }
+    if (wave < NV) {
+      // dV
+      Frag x[NB], big[K::kState][NK];
+#pragma unroll
+      for (int i = 0; i < NK; i++) cut<K::kState>(ek[i], &big[0][i], NK);
+#pragma unroll
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DV>::down(o_tile, i, col0);
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        Frag y[NK];
+#pragma unroll
+        for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(k_tile, 16 * i, j);
+        f32x4 acc{};
+#pragma unroll
+        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NK>(big[p], y, acc);
+        acc = scaled(acc, decays.r[16 * i + c]);
+        acc = add(x, score, i, false, acc);
+        const int64_t t = t0 + 16 * i + c;
+        if (t < end) put4<E>(a.dv, t, b, h, a.nv, col0 + 4 * g, acc, wide & 4);
+      }
+      advance_state<E, DK, DV>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, ek);
+    }
+  }
+  __syncthreads();
+  if (dg && wave == NW - 1) gates(first, f_before, resets_before);
+  if (segment == 0 && a.ds0.p && wave < NV)
+    write_state(a.ds0.p + b * a.ds0.b + h * a.ds0.h, a.nv, 1, a.nk, a.nv, col0, ek);
+  if (wave < NV) {
+#pragma unroll
+    for (int i = 0; i < NK; i++) zeros = zeros_of(ek[i], zeros);
+  }
+  if (not_finite(zeros)) bad = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) seg.flags[segment * heads + bh] = bad;
 }
 
 // ── a single step ───────────────────────────────────────────────────────────
@@ -953,33 +1296,114 @@ void with_size(int n, F&& f) {
   else f(std::integral_constant<int, 128>());
 }
 
+// A call's pieces of workspace, each at a multiple of 256 bytes.
+struct Pieces {
+  int64_t size = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = size;
+    size += ceil_div(bytes, 256) * 256;
+    return at;
+  }
+};
+
 template <class E>
 int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
-  const int64_t heads = (int64_t)a.worlds * a.heads;
+  const int64_t heads = (int64_t)a.worlds * a.heads, state = (int64_t)padded(a.nk) * padded(a.nv) * 4;
   Segments seg = segments_of(o, a, Kind<E>::C);
   if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
-  // Marks of the segments' results, and of their states.
-  const int64_t state = (int64_t)padded(a.nk) * padded(a.nv), flags = ceil_div(2 * seg.count * heads * 4, 256) * 256;
-  char* work = o->workspace(stream, (seg.count > 1 ? seg.count * heads * (state + 1) * 4 : 0) + flags);
+  const int slots = seg.count - 1;
+  Pieces p;
+  const int64_t flags = p.take((seg.count + slots) * heads * 4), decay = p.take(slots * heads * 4), states = p.take(slots * heads * state);
+  char* work = o->workspace(stream, p.size);
   if (!work) return 1;
-  seg.flags = (uint32_t*)work;
-  seg.states = (float*)(work + flags);
-  seg.decay = seg.states + seg.count * heads * state;
+  seg.flags = (uint32_t*)(work + flags);
+  seg.state_flags = seg.flags + seg.count * heads;
+  seg.decay = (float*)(work + decay);
+  seg.states = (float*)(work + states);
   with_size(a.nk, [&](auto dk) {
     with_size(a.nv, [&](auto dv) {
       constexpr int DK = dk(), DV = dv();
-      if (seg.count > 1) {
-        hipLaunchKernelGGL((segment_states<E, DK, DV>), dim3((unsigned)(heads * (seg.count - 1))), dim3(DV * 4), 0, stream, a, a.k,
-                           a.v, seg);
-        hipLaunchKernelGGL((join_segments<DK, DV>), dim3((unsigned)(heads * (DK * DV / 256))), dim3(256), 0, stream, a, a.s0, seg);
+      if (slots) {
+        const Roles x{a.k, a.v, a.nk, a.nv, a.nv, 1, a.s0};
+        hipLaunchKernelGGL((segment_states<E, DK, DV, ADDS>), dim3((unsigned)(heads * slots)), dim3(DV * 4), 0, stream, a, x, seg,
+                           nullptr);
+        hipLaunchKernelGGL((join_segments<DK, DV>), dim3((unsigned)(heads * (DK * DV / 256))), dim3(256), 0, stream, a, x, seg, false);
       }
       hipLaunchKernelGGL((attend_chunks<E, DK, DV>), dim3((unsigned)(heads * seg.count)), dim3(DV * 4), 0, stream, a, seg);
     });
   });
   AttendArgs again = a;
   again.flags = seg.flags;
-  hipLaunchKernelGGL(attend_sequential<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again, 2 * seg.count - 1);
+  hipLaunchKernelGGL(attend_sequential<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again, seg.count + slots);
   return launched(o, "linear attention") ? 0 : 1;
+}
+
+// outs: dq, dk, dv; those of shared heads go through f32 sums of each head's own.
+template <class E>
+int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]) {
+  const int64_t T = a.steps, heads = (int64_t)a.worlds * a.heads, state = (int64_t)padded(a.nk) * padded(a.nv) * 4;
+  const int sizes[3] = {a.nk, a.nk, a.nv};
+  Segments seg = segments_of(o, a, Kind<E>::C);
+  const int64_t chunks = ceil_div(T, Kind<E>::C), slots = seg.count - 1;
+  if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
+  Pieces p;
+  int64_t own[3];
+  for (int i = 0; i < 3; i++) own[i] = outs[i].per > 1 ? p.take(T * heads * sizes[i] * 4) : -1;
+  const int64_t flags = p.take((seg.count + 2 * slots) * heads * 4), decay = p.take(slots * heads * 4);
+  const int64_t forth = p.take(slots * heads * state), back = p.take(slots * heads * state);
+  const int64_t each = p.take(chunks > 1 ? chunks * heads * state : 0);
+  char* work = o->workspace(stream, p.size);
+  if (!work) return 1;
+  int wide = 0;
+  Rows* to[3] = {&a.dq, &a.dk, &a.dv};
+  for (int i = 0; i < 3; i++) {
+    *to[i] = outs[i];
+    if (own[i] >= 0) {
+      wide |= 1 << i;
+      *to[i] = Rows{work + own[i], heads * sizes[i], (int64_t)a.heads * sizes[i], 1};
+    }
+  }
+  seg.flags = (uint32_t*)(work + flags);
+  seg.decay = (float*)(work + decay);
+  with_size(a.nk, [&](auto dk) {
+    with_size(a.nv, [&](auto dv) {
+      constexpr int DK = dk(), DV = dv(), D = DK > DV ? DK : DV;
+      const unsigned join = (unsigned)(heads * (DK * DV / 256)), most = (unsigned)(heads * seg.count);
+      // States have rows of values here, as dq reads them.
+      const Roles s{a.v, a.k, a.nv, a.nk, 1, a.nv, a.s0}, e{a.q, a.o, a.nk, a.nv, a.nv, 1, a.ds};
+      if (slots) {
+        seg.states = (float*)(work + forth);
+        seg.state_flags = seg.flags + seg.count * heads;
+        hipLaunchKernelGGL((segment_states<E, DV, DK, ADDS>), dim3((unsigned)(heads * slots)), dim3(DK * 4), 0, stream, a, s, seg,
+                           nullptr);
+        hipLaunchKernelGGL((join_segments<DV, DK>), dim3(join), dim3(256), 0, stream, a, s, seg, false);
+      }
+      if (chunks > 1) {
+        seg.states = (float*)(work + forth);
+        hipLaunchKernelGGL((segment_states<E, DV, DK, EACH>), dim3(most), dim3(DK * 4), 0, stream, a, s, seg, (f32x4*)(work + each));
+      }
+      if (slots) {
+        seg.states = (float*)(work + back);
+        seg.state_flags = seg.flags + (seg.count + slots) * heads;
+        hipLaunchKernelGGL((segment_states<E, DK, DV, BACK>), dim3((unsigned)(heads * slots)), dim3(DV * 4), 0, stream, a, e, seg,
+                           nullptr);
+        hipLaunchKernelGGL((join_segments<DK, DV>), dim3(join), dim3(256), 0, stream, a, e, seg, true);
+      }
+      hipLaunchKernelGGL((attend_gradients<E, DK, DV>), dim3(most), dim3(D * 4), 0, stream, a, seg,
+                         chunks > 1 ? (const f32x4*)(work + each) : nullptr, wide);
+    });
+  });
+  AttendArgs again = a;
+  again.flags = seg.flags;
+  hipLaunchKernelGGL(attend_sequential_backward<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again,
+                     (int32_t)(seg.count + 2 * slots), wide);
+  for (int i = 0; i < 3; i++) {
+    if (own[i] < 0) continue;
+    const unsigned n = (unsigned)std::min<int64_t>(ceil_div(T * heads / outs[i].per * sizes[i], 256), 16 * o->cus);
+    hipLaunchKernelGGL(join_heads<E>, dim3(n), dim3(256), 0, stream, (const float*)to[i]->p, outs[i], T * a.worlds, a.worlds, a.heads,
+                       sizes[i]);
+  }
+  return launched(o, "linear attention backward") ? 0 : 1;
 }
 
 }  // namespace
@@ -1043,40 +1467,10 @@ int phz_linear_attention_backward(phz_ops* o, void* stream_, const phz_attention
     }
     a.o = Rows{d_o->data, d_o->stride[0], d_o->stride[1], 1};
     if (dg) a.dg = (float*)dg->data, a.dg_t = dg->stride[0], a.dg_b = dg->stride[1], a.dg_h = dg->stride[2];
-    // Gradients of shared heads: each head's own in f32, then their sums.
-    struct { const phz_tensor* t; Rows* row; Rows to; int size; int64_t at; } outs[] = {
-        {dq, &a.dq, {dq->data, dq->stride[0], dq->stride[1], a.q.per}, a.nk, -1},
-        {dk, &a.dk, {dk->data, dk->stride[0], dk->stride[1], a.k.per}, a.nk, -1},
-        {dv, &a.dv, {dv->data, dv->stride[0], dv->stride[1], a.v.per}, a.nv, -1}};
-    int64_t need = 0;
-    for (auto& x : outs)
-      if (x.to.per > 1) x.at = need, need += T * B * H * x.size * 4;
-    char* work = nullptr;
-    if (need && !(work = o->workspace(stream, need))) return 1;
-    int wide = 0;
-    for (int i = 0; i < 3; i++) {
-      *outs[i].row = outs[i].to;
-      if (outs[i].at >= 0) {
-        wide |= 1 << i;
-        *outs[i].row = Rows{work + outs[i].at, B * H * outs[i].size, H * outs[i].size, 1};
-      }
-    }
-    const unsigned blocks = sequential_blocks(o, a);
-    if (q->dtype == PHZ_F32)
-      hipLaunchKernelGGL(attend_sequential_backward<float>, dim3(blocks), dim3(512), 0, stream, a, 0, wide);
-    else
-      hipLaunchKernelGGL(attend_sequential_backward<bf16>, dim3(blocks), dim3(512), 0, stream, a, 0, wide);
-    for (auto& x : outs) {
-      if (x.at < 0) continue;
-      const unsigned n = (unsigned)std::min<int64_t>(ceil_div(T * B * (H / x.to.per) * x.size, 256), 16 * o->cus);
-      if (q->dtype == PHZ_F32)
-        hipLaunchKernelGGL(join_heads<float>, dim3(n), dim3(256), 0, stream, (const float*)x.row->p, x.to, T * B, a.worlds,
-                           a.heads, x.size);
-      else
-        hipLaunchKernelGGL(join_heads<bf16>, dim3(n), dim3(256), 0, stream, (const float*)x.row->p, x.to, T * B, a.worlds,
-                           a.heads, x.size);
-    }
-    return launched(o, "linear attention backward") ? 0 : 1;
+    const Rows outs[3] = {{dq->data, dq->stride[0], dq->stride[1], a.q.per},
+                          {dk->data, dk->stride[0], dk->stride[1], a.k.per},
+                          {dv->data, dv->stride[0], dv->stride[1], a.v.per}};
+    return q->dtype == PHZ_F32 ? backward<float>(o, stream, a, outs) : backward<bf16>(o, stream, a, outs);
   });
 }
 
