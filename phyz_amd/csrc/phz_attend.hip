@@ -25,7 +25,10 @@ using namespace phzop;
 
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -293,6 +296,10 @@ __device__ __forceinline__ f32x4 mma(const s16x4* a, const s16x4* b, f32x4 c) {
   return c;
 }
 
+// The two bf16 of a word.
+__device__ __forceinline__ float low_half(uint32_t x) { return __builtin_bit_cast(float, x << 16); }
+__device__ __forceinline__ float high_half(uint32_t x) { return __builtin_bit_cast(float, x & 0xffff0000u); }
+
 // v in NP pieces, each `stride` fragments from the last.
 template <int NP>
 __device__ __forceinline__ void cut(f32x4 v, f32x4* out, int) {
@@ -303,22 +310,20 @@ template <int NP>
 __device__ __forceinline__ void cut(f32x4 v, s16x4* out, int stride) {
 #pragma unroll
   for (int p = 0; p < NP; p++) {
-    s16x4 x;
+    u32x2 x;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const bf16 h = from_f32<bf16>(v[i]);
-      x[i] = (short)h.bits;
-      if (p + 1 < NP) v[i] -= to_f32(h);
+    for (int i = 0; i < 2; i++) {
+      const f32x2 pair{v[2 * i], v[2 * i + 1]};
+      x[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2));
+      if (p + 1 < NP) v[2 * i] -= low_half(x[i]), v[2 * i + 1] -= high_half(x[i]);
     }
-    out[p * stride] = x;
+    out[p * stride] = __builtin_bit_cast(s16x4, x);
   }
 }
 __device__ __forceinline__ f32x4 widen(f32x4 v) { return v; }
 __device__ __forceinline__ f32x4 widen(s16x4 v) {
-  f32x4 x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = to_f32(bf16{(uint16_t)v[i]});
-  return x;
+  const u32x2 x = __builtin_bit_cast(u32x2, v);
+  return f32x4{low_half(x[0]), high_half(x[0]), low_half(x[1]), high_half(x[1])};
 }
 // a where it is kept, 0 (whatever x is) where nothing is left of it.
 __device__ __forceinline__ f32x4 scaled(f32x4 x, float by) {
@@ -354,32 +359,58 @@ struct Tile {
 };
 
 // A chunk's rows of one tensor on their way from memory to LDS through registers,
-// NT threads; rows and columns that do not exist are 0.
+// NT threads, each a column of 16 bytes. Rows behind the last step are that step's
+// again: what they come to is not stored, and adds nothing to the state (their
+// weights are 0). Columns that do not exist are 0; a column that ends within the
+// 16 bytes goes to LDS an element at a time, when the others leave registers.
+// What follows from these is found where it is used, and not kept in registers
+// through the loop over chunks (which it would fill).
+__device__ __forceinline__ void again(int& x, int& y) { asm volatile("" : "+v"(x), "+v"(y)); }
+
 template <class E, int D, int NT>
 struct Load {
   static constexpr int C = Kind<E>::C, EL = 16 / sizeof(E), kPer = D / EL, kStep = NT / kPer;
   static constexpr int N = (C + kStep - 1) / kStep;
   Pack<E, EL> x[N];
   __device__ __forceinline__ void fetch(const E* base, int64_t stride, int left, int d) {
-    const int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+    int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+    again(col, row0);
+    // (Also says that what the registers held before is not needed any more.)
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int row = row0 + i * kStep;
-      const E* p = base + row * stride + col;
-      if (row < left && col + EL <= d) {
-        x[i] = *(const Pack<E, EL>*)p;
-      } else {
+    for (int i = 0; i < N; i++) x[i] = Pack<E, EL>{};
+    if (col + EL > d || left <= 0) return;
+    const E* p = base + col;
+    if (left == C) {
+      p += row0 * stride;
 #pragma unroll
-        for (int e = 0; e < EL; e++) x[i].v[e] = row < left && col + e < d ? p[e] : E{};
-      }
+      for (int i = 0; i < N; i++, p += kStep * stride)
+        if (C % kStep == 0 || row0 < C) x[i] = *(const Pack<E, EL>*)p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = *(const Pack<E, EL>*)(p + min(row0 + i * kStep, left - 1) * stride);
     }
   }
-  __device__ __forceinline__ void stash(char* l) const {
-    const int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+  // The same base, stride and d as fetch had.
+  __device__ __forceinline__ void stash(char* l, const E* base, int64_t stride, int left, int d) const {
+    int col = threadIdx.x % kPer * EL, row0 = threadIdx.x / kPer;
+    again(col, row0);
+    l += row0 * Tile<E, D>::kRow + col * (int)sizeof(E);
+    if (col + EL <= d || col >= d) {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (C % kStep == 0 || row0 + i * kStep < C)
+          *(f32x4*)(l + i * kStep * Tile<E, D>::kRow) = __builtin_bit_cast(f32x4, x[i]);
+      return;
+    }
+    const int n = d - col;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int row = row0 + i * kStep;
-      if (C % kStep == 0 || row < C) *(f32x4*)(l + row * Tile<E, D>::kRow + col * (int)sizeof(E)) = __builtin_bit_cast(f32x4, x[i]);
+      if (C % kStep != 0 && row0 + i * kStep >= C) continue;
+      const E* p = base + min(row0 + i * kStep, left - 1) * stride + col;
+      Pack<E, EL> y;
+#pragma unroll
+      for (int e = 0; e < EL; e++) y.v[e] = e < n ? p[e] : E{};
+      *(f32x4*)(l + i * kStep * Tile<E, D>::kRow) = __builtin_bit_cast(f32x4, y);
     }
   }
 };
@@ -390,24 +421,37 @@ struct Decays {
   double sum[C];            // of log2 of the gates up to t
   float e[C], r[C];         // from the start to t, from t to the end; 0 behind or before a reset
   float u[C], w[C];         // from the end of the tile of 16 before to t, from t to the end of its tile
-  int32_t since[C];         // the last step up to t at which an episode begins, or 0
+  int32_t since[C];         // the last step up to t at which an episode begins, or 0; C behind the last step
   float f;                  // over all of it, or 0
   double all;               // log2 of it without resets
   uint64_t resets;
 };
 struct Gate {
   float x;
-  bool reset;
+  bool reset, live;
 };
 // A lane a step; by one wave.
 __device__ __forceinline__ Gate fetch_gate(const float* g, int64_t g_t, const uint8_t* reset, int64_t r_t, int left) {
   const int lane = threadIdx.x & 63;
-  Gate v{0.0f, false};
+  Gate v{0.0f, false, lane < left};
   if (lane < left) {
     v.x = g[lane * g_t];
     v.reset = reset && reset[lane * r_t];
   }
   return v;
+}
+// x moved between lanes by a DPP control; 0 where there is no such lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double x) {
+  const u32x2 v = __builtin_bit_cast(u32x2, x);
+  const u32x2 y{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[0], CTRL, ROWS, 0xf, false),
+                (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[1], CTRL, ROWS, 0xf, false)};
+  return __builtin_bit_cast(double, y);
+}
+__device__ __forceinline__ double of_lane(double x, int lane) {
+  const u32x2 v = __builtin_bit_cast(u32x2, x);
+  const u32x2 y{(uint32_t)__builtin_amdgcn_readlane((int)v[0], lane), (uint32_t)__builtin_amdgcn_readlane((int)v[1], lane)};
+  return __builtin_bit_cast(double, y);
 }
 template <int C>
 __device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
@@ -415,23 +459,24 @@ __device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
   const bool reset = v.reset || v.x < kForgets;
   // A reset's own gate does not count: what is left of before is nothing.
   double x = reset ? 0.0 : (double)v.x * 1.4426950408889634074;
-#pragma unroll
-  for (int m = 1; m < C; m *= 2) {
-    const double y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
+  x += moved<0x111, 0xf>(x);  // row_shr by 1, 2, 4, 8: sums within rows of 16 lanes
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  const double mine = x, row = moved<0x15f, 0xf>(x);  // the row's last lane's
+  x += moved<0x142, 0xa>(x);  // lane 15 to the row behind it, in rows 1 and 3
+  x += moved<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
   const uint64_t resets = __ballot(reset);
-  const double all = __shfl(x, C - 1);
-  const double before = __shfl(x, max((lane & ~15) - 1, 0)), last = __shfl(x, lane | 15);
+  const double all = of_lane(x, C - 1);
   if (lane >= C) return;
   const uint64_t upto = resets & (2ull << lane) - 1ull;
   const int at = resets ? 63 - __builtin_clzll(resets) : 0;
   d->sum[lane] = x;
-  d->e[lane] = upto ? 0.0f : __builtin_amdgcn_exp2f((float)x);
-  d->r[lane] = lane >= at ? __builtin_amdgcn_exp2f((float)(all - x)) : 0.0f;
-  d->u[lane] = __builtin_amdgcn_exp2f((float)(lane < 16 ? x : x - before));
-  d->w[lane] = __builtin_amdgcn_exp2f((float)(last - x));
-  d->since[lane] = upto ? 63 - __builtin_clzll(upto) : 0;
+  d->e[lane] = upto || !v.live ? 0.0f : __builtin_amdgcn_exp2f((float)x);
+  d->r[lane] = v.live && lane >= at ? __builtin_amdgcn_exp2f((float)(all - x)) : 0.0f;
+  d->u[lane] = __builtin_amdgcn_exp2f((float)mine);
+  d->w[lane] = __builtin_amdgcn_exp2f((float)(row - mine));
+  d->since[lane] = !v.live ? C : upto ? 63 - __builtin_clzll(upto) : 0;
   if (lane == 0) {
     d->f = resets ? 0.0f : __builtin_amdgcn_exp2f((float)all);
     d->all = all;
@@ -477,11 +522,14 @@ struct Segments {
 
 // A workgroup's head and segment. Neighbouring heads share lines of memory: they
 // go to one XCD.
-__device__ __forceinline__ void place_of(int64_t heads, int64_t* bh, int* segment) {
-  const uint32_t n = gridDim.x, per = n / 8, i = blockIdx.x;
+__device__ __forceinline__ void place_of(const AttendArgs& a, int64_t* bh, int* segment, int* b, int* h) {
+  const uint32_t n = gridDim.x, per = n / 8, i = blockIdx.x, heads = (uint32_t)(a.worlds * a.heads);
   const uint32_t id = i < per * 8 ? i % 8 * per + i / 8 : i;
-  *bh = id % heads;
-  *segment = (int)(id / heads);
+  const uint32_t s = id / heads, at = id - s * heads;
+  *segment = (int)s;
+  *bh = at;
+  *b = (int)(at / (uint32_t)a.heads);
+  *h = (int)(at % (uint32_t)a.heads);
 }
 
 __device__ __forceinline__ bool not_finite(float sum_of_zeros) { return sum_of_zeros != 0.0f || sum_of_zeros != sum_of_zeros; }
@@ -496,26 +544,57 @@ __device__ __forceinline__ float zeros_of(f32x4 x, float z) {
 template <int NB>
 __device__ __forceinline__ void read_state(const float* p, int64_t row_stride, int64_t col_stride, int rows, int cols, int col0,
                                            f32x4 (&s)[NB]) {
-  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), g = lane >> 4;
+  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), row0 = (lane >> 4) * 4;
 #pragma unroll
-  for (int i = 0; i < NB; i++)
+  for (int i = 0; i < NB; i++) s[i] = f32x4{};
+  if (!p || col >= cols) return;
+  p += row0 * row_stride + col * col_stride;
+  if (rows == 16 * NB) {
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = 16 * i + 4 * g + r;
-      s[i][r] = p && row < rows && col < cols ? p[row * row_stride + col * col_stride] : 0.0f;
-    }
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[i][r] = p[(16 * i + r) * row_stride];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (row0 + 16 * i + r < rows) s[i][r] = p[(16 * i + r) * row_stride];
+  }
 }
 template <int NB>
-__device__ __forceinline__ void write_state(float* p, int64_t row_stride, int64_t col_stride, int rows, int cols, int col0,
-                                            const f32x4 (&s)[NB]) {
-  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), g = lane >> 4;
+__device__ __forceinline__ void write_state(float* p, int64_t row_stride, int rows, int cols, int col0, const f32x4 (&s)[NB]) {
+  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), row0 = (lane >> 4) * 4;
+  if (col >= cols) return;
+  p += row0 * row_stride + col;
+  if (rows == 16 * NB) {
 #pragma unroll
-  for (int i = 0; i < NB; i++)
+    for (int i = 0; i < NB; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = 16 * i + 4 * g + r;
-      if (row < rows && col < cols) p[row * row_stride + col * col_stride] = s[i][r];
-    }
+      for (int r = 0; r < 4; r++) p[(16 * i + r) * row_stride] = s[i][r];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (row0 + 16 * i + r < rows) p[(16 * i + r) * row_stride] = s[i][r];
+  }
+}
+
+// Four neighbouring elements, from `at` on, of an output's row of `size`.
+template <class E>
+__device__ __forceinline__ void put4(E* row, int size, int at, f32x4 v) {
+  E* p = row + at;
+  if (at + 4 <= size) {
+    Pack<E, 4> y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y.v[i] = from_f32<E>(v[i]);
+    *(Pack<E, 4>*)p = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (at + i < size) p[i] = from_f32<E>(v[i]);
+  }
 }
 
 // s <- f s + rows^T (weight o cols) of one chunk: the wave's 16 columns.
@@ -544,27 +623,32 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
 #pragma unroll
     for (int p = K::kExact - 1; p >= 0; p--) x = mma<NB>(k, v[p], x);
     s[i] = x;
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 // The forward pass. Wave w has columns 16 w .. 16 w + 15 of the state and of o.
-// Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS.
+// Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS, where
+// q and k were: half the LDS again would be two workgroups a compute unit less.
 template <class E, int DK, int DV>
-__global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments seg) {
+__global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendArgs a, Segments seg) {
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
   constexpr int C = K::C, NT = DV * 4, NW = NT / 64, NB = C / 16, NK = DK / 16;
-  __shared__ __align__(16) char q_tile[C * Tile<E, DK>::kRow], k_tile[C * Tile<E, DK>::kRow], v_tile[C * Tile<E, DV>::kRow];
-  __shared__ __align__(16) char score[K::kScores][C * Tile<E, C>::kRow];
+  constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
+  constexpr int kTiles = NB * (NB + 1) / 2, kMine = (kTiles + NW - 1) / NW;
+  constexpr int kTile = C * Tile<E, DK>::kRow, kScore = C * Tile<E, C>::kRow;
+  __shared__ __align__(16) char shared[2 * kTile > K::kScores * kScore ? 2 * kTile : K::kScores * kScore];
+  __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow];
   __shared__ __align__(16) Decays<C> decays;
   __shared__ uint32_t bad;
+  char *q_tile = shared, *k_tile = shared + kTile;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col0 = 16 * wave;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
-  int segment;
-  place_of(heads, &bh, &segment);
-  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  int segment, b, h;
+  place_of(a, &bh, &segment, &b, &h);
   const int64_t first = (int64_t)segment * seg.chunks * C;
   const int64_t end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
   const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv);
@@ -572,6 +656,17 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   E* o = (E*)a.o.p + b * a.o.b + (int64_t)h * a.nv;
 
+  Load<E, DK, NT> lq, lk;
+  Load<E, DV, NT> lv;
+  Gate lg{};
+  auto fetch = [&](int64_t t) {
+    const int left = (int)max((int64_t)0, min((int64_t)C, end - t));
+    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
+    lq.fetch(q + t * a.q.t, a.q.t, left, a.nk);
+    lk.fetch(k + t * a.k.t, a.k.t, left, a.nk);
+    lv.fetch(v + t * a.v.t, a.v.t, left, a.nv);
+  };
+  fetch(first);
   f32x4 s[NK];
   if (segment == 0) {
     read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, a.nk, a.nv, col0, s);
@@ -580,30 +675,21 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
 #pragma unroll
     for (int i = 0; i < NK; i++) s[i] = p[i * 64];
   }
-  // Tiles right of the diagonal that a pair of blocks takes in are 0 for good.
-  for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = f32x4{};
   if (threadIdx.x == 0) bad = 0;
-  Load<E, DK, NT> lq, lk;
-  Load<E, DV, NT> lv;
-  Gate lg{};
-  auto fetch = [&](int64_t t) {
-    const int left = (int)min((int64_t)C, end - t);
-    lq.fetch(q + t * a.q.t, a.q.t, left, a.nk);
-    lk.fetch(k + t * a.k.t, a.k.t, left, a.nk);
-    lv.fetch(v + t * a.v.t, a.v.t, left, a.nv);
-    if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
-  };
-  fetch(first);
   float zeros = 0.0f;
   for (int64_t t0 = first; t0 < end; t0 += C) {
     __syncthreads();  // the last chunk's tiles are read
-    lq.stash(q_tile);
-    lk.stash(k_tile);
-    lv.stash(v_tile);
+    const int left = (int)min((int64_t)C, end - t0);
+    lq.stash(q_tile, q + t0 * a.q.t, a.q.t, left, a.nk);
+    lk.stash(k_tile, k + t0 * a.k.t, a.k.t, left, a.nk);
+    lv.stash(v_tile, v + t0 * a.v.t, a.v.t, left, a.nv);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
-    if (t0 + C < end) fetch(t0 + C);
-    for (int n = wave; n < NB * (NB + 1) / 2; n += NW) {
+    Frag mine[kMine][K::kScores];
+#pragma unroll
+    for (int m = 0; m < kMine; m++) {
+      const int n = wave + m * NW;
+      if (n >= kTiles) break;
       int ta, tb;
       tile_of(n, &ta, &tb);
       Frag x[NK], y[NK];
@@ -616,35 +702,50 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
       const f32x4 l = decay_between(decays, ta, tb);
 #pragma unroll
       for (int r = 0; r < 4; r++) p[r] = l[r] != 0.0f ? p[r] * l[r] * a.scale : 0.0f;
-      Frag z[K::kScores];
-      cut<K::kScores>(p, z, 1);
-#pragma unroll
-      for (int i = 0; i < K::kScores; i++)
-        *(Frag*)(score[i] + (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E)) = z[i];
+      cut<K::kScores>(p, mine[m], 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
     // What the state from before the chunk answers: o^T = S^T Q^T.
-    Frag sp[K::kState][NK];
-#pragma unroll
-    for (int i = 0; i < NK; i++) cut<K::kState>(s[i], &sp[0][i], NK);
     f32x4 acc[NB];
+    {
+      Frag sp[K::kState][NK];
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-      Frag y[NK];
+      for (int i = 0; i < NK; i++) cut<K::kState>(s[i], &sp[0][i], NK);
 #pragma unroll
-      for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, j);
-      f32x4 x{};
+      for (int i = 0; i < NB; i++) {
+        Frag y[NK];
 #pragma unroll
-      for (int p = K::kState - 1; p >= 0; p--) x = mma<NK>(sp[p], y, x);
-      acc[i] = scaled(x, decays.e[16 * i + c] * a.scale);
+        for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, j);
+        f32x4 x{};
+#pragma unroll
+        for (int p = K::kState - 1; p >= 0; p--) x = mma<NK>(sp[p], y, x);
+        acc[i] = scaled(x, decays.e[16 * i + c] * a.scale);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
+    __syncthreads();  // q and k are read
+    fetch(t0 + C);  // nothing where that is the end
+#pragma unroll
+    for (int m = 0; m < kMine; m++) {
+      const int n = wave + m * NW;
+      if (n >= kTiles) break;
+      int ta, tb;
+      tile_of(n, &ta, &tb);
+      char* at = shared + (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E);
+#pragma unroll
+      for (int i = 0; i < K::kScores; i++) {
+        *(Frag*)(at + i * kScore) = mine[m][i];
+        // The tile right of the diagonal that a pair of blocks takes in.
+        if (two == 2 && ta == tb && tb % 2 == 0) *(Frag*)(at + i * kScore + 16 * sizeof(E)) = Frag{};
+      }
+    }
     Frag vf[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0);
     __syncthreads();  // the scores are there
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
       f32x4 x = acc[i];
 #pragma unroll
       for (int p = K::kScores - 1; p >= 0; p--)
@@ -652,28 +753,16 @@ __global__ __launch_bounds__(DV * 4) void attend_chunks(AttendArgs a, Segments s
         for (int j = 0; j <= i; j += two) {
           Frag y[two];
 #pragma unroll
-          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(score[p], 16 * i, j + n);
+          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(shared + p * kScore, 16 * i, j + n);
           x = mma<two>(&vf[j], y, x);
         }
       zeros = zeros_of(x, zeros);
       const int64_t t = t0 + 16 * i + c;
-      const int j0 = col0 + 4 * g;
-      if (t < end) {
-        E* p = o + t * a.o.t + j0;
-        if (j0 + 4 <= a.nv) {
-          Pack<E, 4> y;
-#pragma unroll
-          for (int r = 0; r < 4; r++) y.v[r] = from_f32<E>(x[r]);
-          *(Pack<E, 4>*)p = y;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (j0 + r < a.nv) p[r] = from_f32<E>(x[r]);
-        }
-      }
+      if (t < end) put4<E>(o + t * a.o.t, a.nv, col0 + 4 * g, x);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nv, 1, a.nk, a.nv, col0, s);
+  if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nv, a.nk, a.nv, col0, s);
 #pragma unroll
   for (int i = 0; i < NK; i++) zeros = zeros_of(s[i], zeros);
   if (not_finite(zeros)) bad = 1;
@@ -697,7 +786,7 @@ struct Roles {
 //   EACH   the state before each chunk
 enum { ADDS, BACK, EACH };
 template <class E, int DR, int DC, int MODE>
-__global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Roles x, Segments seg, f32x4* each) {
+__global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(AttendArgs a, Roles x, Segments seg, f32x4* each) {
   typedef Kind<E> K;
   constexpr int C = K::C, NT = DC * 4, NR = DR / 16;
   __shared__ __align__(16) char r_tile[C * Tile<E, DR>::kRow], c_tile[C * Tile<E, DC>::kRow];
@@ -706,10 +795,9 @@ __global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Roles x, 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col0 = 16 * wave;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
-  int slot;
-  place_of(heads, &bh, &slot);
+  int slot, b, h;
+  place_of(a, &bh, &slot, &b, &h);
   const int segment = MODE == BACK ? slot + 1 : slot;
-  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
   const int64_t first = (int64_t)segment * seg.chunks * C, end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
   const E *rp = row_of<E>(x.rows, b, h, x.nr), *cp = row_of<E>(x.cols, b, h, x.nc);
   const float* gate = a.g + b * a.g_b + h * a.g_h;
@@ -727,7 +815,7 @@ __global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Roles x, 
   Load<E, DC, NT> lc;
   Gate lg{};
   auto fetch = [&](int64_t t) {
-    const int left = (int)min((int64_t)C, end - t);
+    const int left = (int)max((int64_t)0, min((int64_t)C, end - t));
     lr.fetch(rp + t * x.rows.t, x.rows.t, left, x.nr);
     lc.fetch(cp + t * x.cols.t, x.cols.t, left, x.nc);
     if (wave == 0) lg = fetch_gate(gate + t * a.g_t, a.g_t, reset ? reset + t * a.r_t : nullptr, a.r_t, left);
@@ -745,8 +833,10 @@ __global__ __launch_bounds__(DC * 4) void segment_states(AttendArgs a, Roles x, 
       if (n + 1 == chunks) break;
     }
     __syncthreads();
-    lr.stash(r_tile);
-    lc.stash(c_tile);
+    const int64_t t0 = start(n);
+    const int left = (int)min((int64_t)C, end - t0);
+    lr.stash(r_tile, rp + t0 * x.rows.t, x.rows.t, left, x.nr);
+    lc.stash(c_tile, cp + t0 * x.cols.t, x.cols.t, left, x.nc);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
     if (n + 1 < chunks) fetch(start(n + 1));
@@ -796,25 +886,12 @@ __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segm
   }
 }
 
-// Four neighbouring elements of a row of an output. `wide`: f32 sums of each head's own.
+// A gradient's row of one head; `wide`: f32 sums of each head's own.
 template <class E>
 __device__ __forceinline__ void put4(const Rows& r, int64_t t, int b, int h, int size, int at, f32x4 v, bool wide) {
-  auto go = [&](auto* base) {
-    typedef std::remove_reference_t<decltype(*base)> O;
-    O* p = base + t * r.t + b * r.b + (int64_t)h * size + at;
-    if (at + 4 <= size) {
-      Pack<O, 4> y;
-#pragma unroll
-      for (int i = 0; i < 4; i++) y.v[i] = from_f32<O>(v[i]);
-      *(Pack<O, 4>*)p = y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (at + i < size) p[i] = from_f32<O>(v[i]);
-    }
-  };
-  if (wide) go((float*)r.p);
-  else go((E*)r.p);
+  const int64_t row = t * r.t + b * r.b + (int64_t)h * size;
+  if (wide) put4((float*)r.p + row, size, at, v);
+  else put4((E*)r.p + row, size, at, v);
 }
 
 __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
@@ -850,9 +927,8 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
   const int col0 = 16 * wave;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
-  int segment;
-  place_of(heads, &bh, &segment);
-  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+  int segment, b, h;
+  place_of(a, &bh, &segment, &b, &h);
   const int64_t first = (int64_t)segment * seg.chunks * C;
   const int64_t end = min((int64_t)a.steps, first + (int64_t)seg.chunks * C);
   const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv),
@@ -883,7 +959,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
   Load<E, DV, NT> lv, lo;
   Gate lg{};
   auto fetch = [&](int64_t t) {
-    const int left = (int)min((int64_t)C, end - t);
+    const int left = (int)max((int64_t)0, min((int64_t)C, end - t));
     lq.fetch(q + t * a.q.t, a.q.t, left, a.nk);
     lk.fetch(k + t * a.k.t, a.k.t, left, a.nk);
     lv.fetch(v + t * a.v.t, a.v.t, left, a.nv);
@@ -924,10 +1000,11 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
     const int64_t t0 = first + n * C;
     __syncthreads();  // the chunk before is done with its tiles, and its sums are there
     if (dg && n + 1 < chunks && wave == NW - 1) gates(t0 + C, f_before, resets_before);
-    lq.stash(q_tile);
-    lk.stash(k_tile);
-    lv.stash(v_tile);
-    lo.stash(o_tile);
+    const int left = (int)min((int64_t)C, end - t0);
+    lq.stash(q_tile, q + t0 * a.q.t, a.q.t, left, a.nk);
+    lk.stash(k_tile, k + t0 * a.k.t, a.k.t, left, a.nk);
+    lv.stash(v_tile, v + t0 * a.v.t, a.v.t, left, a.nv);
+    lo.stash(o_tile, d_o + t0 * a.o.t, a.o.t, left, a.nv);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
     if (n > 0) fetch(t0 - C);
@@ -1008,10 +1085,11 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
       return acc;
     };
     if (wave < NK) {
-      Frag x[NB], big[K::kState][NV];
+      // In three pieces: the gates' gradients, which are f32, follow from these.
+      Frag x[NB], big[K::kExact][NV];
       // dQ
 #pragma unroll
-      for (int i = 0; i < NV; i++) cut<K::kState>(s[i], &big[0][i], NV);
+      for (int i = 0; i < NV; i++) cut<K::kExact>(s[i], &big[0][i], NV);
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(k_tile, i, col0);
 #pragma unroll
@@ -1021,7 +1099,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
         for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(o_tile, 16 * i, j);
         f32x4 acc{};
 #pragma unroll
-        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
+        for (int p = K::kExact - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
         acc = scaled(acc, decays.e[16 * i + c] * a.scale);
         if (dg) {
           float d = dot4(acc, widen(Tile<E, DK>::along(q_tile, 16 * i, wave)));
@@ -1043,7 +1121,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
         if (lane == 0) x_dot[wave] = d;
       }
 #pragma unroll
-      for (int i = 0; i < NV; i++) cut<K::kState>(ev[i], &big[0][i], NV);
+      for (int i = 0; i < NV; i++) cut<K::kExact>(ev[i], &big[0][i], NV);
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0);
 #pragma unroll
@@ -1053,7 +1131,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
         for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(v_tile, 16 * i, j);
         f32x4 acc{};
 #pragma unroll
-        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
+        for (int p = K::kExact - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
         acc = scaled(acc, decays.r[16 * i + c]);
         if (dg) {
           float d = dot4(acc, widen(Tile<E, DK>::along(k_tile, 16 * i, wave)));
@@ -1093,7 +1171,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
   __syncthreads();
   if (dg && wave == NW - 1) gates(first, f_before, resets_before);
   if (segment == 0 && a.ds0.p && wave < NV)
-    write_state(a.ds0.p + b * a.ds0.b + h * a.ds0.h, a.nv, 1, a.nk, a.nv, col0, ek);
+    write_state(a.ds0.p + b * a.ds0.b + h * a.ds0.h, a.nv, a.nk, a.nv, col0, ek);
   if (wave < NV) {
 #pragma unroll
     for (int i = 0; i < NK; i++) zeros = zeros_of(ek[i], zeros);
