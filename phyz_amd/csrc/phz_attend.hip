@@ -149,19 +149,42 @@ __device__ __forceinline__ void each_element(int rows, int col, bool live, float
 
 // A head whose steps are taken one after the other: what the chunks' products
 // cannot do is right here, infinities and NaN that a reset cuts off from the
-// steps behind it. Workgroups look through the heads' flags. 2 waves a SIMD.
+// steps behind it. A workgroup looks through its heads' flags, a thread a head at a
+// time (one wave's look at each in turn took 17 us for 16384 heads, this 6). 2 waves a SIMD.
+struct Flagged {
+  const AttendArgs& a;
+  int32_t marks;
+  uint64_t* mask;  // of 8, in LDS
+  int64_t all;
+  // Calls f(head) for each of the workgroup's heads that is marked, or for all.
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    for (int64_t bh0 = blockIdx.x; bh0 < all; bh0 += 512 * (int64_t)gridDim.x) {
+      const int64_t mine = bh0 + threadIdx.x * (int64_t)gridDim.x;
+      uint32_t any = 0;
+      if (mine < all) {
+        any = !a.flags;
+        #pragma unroll 16
+        for (int m = 0; m < marks; m++) any |= a.flags[m * all + mine];
+      }
+      const uint64_t marked = __ballot(any != 0);
+      if (!__syncthreads_or(any)) continue;
+      if ((threadIdx.x & 63) == 0) mask[threadIdx.x >> 6] = marked;
+      __syncthreads();
+      for (int i = 0; i < 512; i++)
+        if (mask[i >> 6] >> (i & 63) & 1) f(bh0 + i * (int64_t)gridDim.x);
+      __syncthreads();
+    }
+  }
+};
 template <class E>
 __global__ __launch_bounds__(512) void attend_sequential(AttendArgs a, int32_t marks) {
   const int wave = threadIdx.x >> 6, c = threadIdx.x & 15, col0 = 16 * wave;
   const int64_t all = (int64_t)a.worlds * a.heads;
-  for (int64_t bh = blockIdx.x; bh < all; bh += gridDim.x) {
-    if (a.flags) {
-      uint32_t any = 0;
-      for (int m = 0; m < marks; m++) any |= a.flags[m * all + bh];
-      if (!any) continue;
-    }
+  __shared__ uint64_t mask[8];
+  Flagged{a, marks, mask, all}.each([&](int64_t bh) {
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-    if (col0 >= a.nv) continue;
+    if (col0 >= a.nv) return;
     Sweep w{row_of<E>(a.q, b, h, a.nk), row_of<E>(a.k, b, h, a.nk), row_of<E>(a.v, b, h, a.nv), a.q.t, a.k.t, a.v.t, a.nk, a.nv,
             1.0f, a.scale, a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, false};
     float s[8][4];
@@ -173,7 +196,7 @@ __global__ __launch_bounds__(512) void attend_sequential(AttendArgs a, int32_t m
       const int col = col0 + c;
       each_element(a.nk, col, col < a.nv, s, [&](int d, float v) { last[(int64_t)d * a.nv + col] = v; });
     }
-  }
+  });
 }
 
 // Its gradients. dg by <E_t, S_t> = q_t dq_t + dg_{t+1} = dg_t + k_t dk_t, in f64.
@@ -194,12 +217,8 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
     __syncthreads();
     return sum;
   };
-  for (int64_t bh = blockIdx.x; bh < all; bh += gridDim.x) {
-    if (a.flags) {
-      uint32_t any = 0;
-      for (int m = 0; m < marks; m++) any |= a.flags[m * all + bh];
-      if (!any) continue;
-    }
+  __shared__ uint64_t mask[8];
+  Flagged{a, marks, mask, all}.each([&](int64_t bh) {
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
     const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv),
             *d_o = row_of<E>(a.o, b, h, a.nv);
@@ -252,7 +271,7 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
       const int col = col0 + c;
       each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = forget ? 0.0f : keep * x; });
     }
-  }
+  });
 }
 
 // ── chunks: products of tiles of 16 ─────────────────────────────────────────
@@ -332,19 +351,26 @@ __device__ __forceinline__ f32x4 scaled(f32x4 x, float by) {
   return x;
 }
 
+// The lane, as a value that the compiler finds anew: the addresses that follow from
+// it are then not all kept in registers through the loop over chunks.
+__device__ __forceinline__ int fresh_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // A tile of ROWS x D in LDS, rows 16 bytes apart from whole banks: fragments along
 // a row and down a column fall into all banks.
 template <class E, int D>
 struct Tile {
   typedef typename Kind<E>::Frag Frag;
   static constexpr int kRow = D * sizeof(E) + 16;
-  static __device__ __forceinline__ Frag along(const char* l, int row, int block) {
-    const int lane = threadIdx.x & 63;
+  static __device__ __forceinline__ Frag along(const char* l, int row, int block, int lane) {
     return *(const Frag*)(l + (row + (lane & 15)) * kRow + (16 * block + (lane >> 4) * 4) * (int)sizeof(E));
   }
   // Rows 16 block + 4 g .. + 3 of column col + c.
-  static __device__ __forceinline__ Frag down(const char* l, int block, int col) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  static __device__ __forceinline__ Frag down(const char* l, int block, int col, int lane) {
+    const int c = lane & 15, g = lane >> 4;
     if constexpr (sizeof(E) == 4) {
       f32x4 v;
 #pragma unroll
@@ -384,7 +410,7 @@ struct Load {
       p += row0 * stride;
 #pragma unroll
       for (int i = 0; i < N; i++, p += kStep * stride)
-        if (C % kStep == 0 || row0 < C) x[i] = *(const Pack<E, EL>*)p;
+        if (C % kStep == 0 || row0 + i * kStep < C) x[i] = *(const Pack<E, EL>*)p;
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++) x[i] = *(const Pack<E, EL>*)(p + min(row0 + i * kStep, left - 1) * stride);
@@ -486,8 +512,8 @@ __device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
 // L[t][s] for the lane's t = 16 b + c and s = 16 a + 4 g .. + 3: between tiles the
 // product of the way from s to its tile's end, from there to t's tile, and on to t.
 template <int C>
-__device__ __forceinline__ f32x4 decay_between(const Decays<C>& d, int a, int b) {
-  const int lane = threadIdx.x & 63, t = 16 * b + (lane & 15), s = 16 * a + (lane >> 4) * 4, since = d.since[t];
+__device__ __forceinline__ f32x4 decay_between(const Decays<C>& d, int a, int b, int lane) {
+  const int t = 16 * b + (lane & 15), s = 16 * a + (lane >> 4) * 4, since = d.since[t];
   f32x4 x;
   if (a == b) {
     const double at = d.sum[t];
@@ -539,45 +565,49 @@ __device__ __forceinline__ float zeros_of(f32x4 x, float z) {
   return z;
 }
 
-// The wave's 16 columns of a state in the caller's layout (element (row, col) at
-// row * row_stride + col * col_stride).
-template <int NB>
-__device__ __forceinline__ void read_state(const float* p, int64_t row_stride, int64_t col_stride, int rows, int cols, int col0,
-                                           f32x4 (&s)[NB]) {
-  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), row0 = (lane >> 4) * 4;
+// NB blocks, from `block` on, of 16 columns of a state in the caller's layout, as rows of keys or of
+// values (TURNED): a lane's four neighbouring rows are nv, or one, element apart.
+template <bool TURNED, int NB>
+__device__ __forceinline__ void read_state(const float* p, int nk, int nv, int col0, int block, f32x4 (&s)[NB]) {
+  const int lane = fresh_lane(), col = col0 + (lane & 15), row0 = (lane >> 4) * 4 + 16 * block;
+  const int rows = TURNED ? nv : nk, cols = TURNED ? nk : nv;
 #pragma unroll
   for (int i = 0; i < NB; i++) s[i] = f32x4{};
   if (!p || col >= cols) return;
-  p += row0 * row_stride + col * col_stride;
-  if (rows == 16 * NB) {
+  p += TURNED ? row0 + col * nv : row0 * nv + col;
+  if (TURNED) {
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+    for (int i = 0; i < NB; i++) {
+      if (row0 + 16 * i + 4 <= rows) {
+        s[i] = __builtin_bit_cast(f32x4, *(const Pack<float, 4>*)(p + 16 * i));
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; r++) s[i][r] = p[(16 * i + r) * row_stride];
+        for (int r = 0; r < 4; r++)
+          if (row0 + 16 * i + r < rows) s[i][r] = p[16 * i + r];
+      }
+    }
   } else {
+    // One pointer that moves on: 4 NB of them would fill the registers.
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+    for (int i = 0; i < NB; i++, p += 16 * nv) {
+      const float* at = p;
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (row0 + 16 * i + r < rows) s[i][r] = p[(16 * i + r) * row_stride];
+      for (int r = 0; r < 4; r++, at += nv)
+        if (row0 + 16 * i + r < rows) s[i][r] = *at;
+    }
   }
 }
 template <int NB>
-__device__ __forceinline__ void write_state(float* p, int64_t row_stride, int rows, int cols, int col0, const f32x4 (&s)[NB]) {
-  const int lane = threadIdx.x & 63, col = col0 + (lane & 15), row0 = (lane >> 4) * 4;
-  if (col >= cols) return;
-  p += row0 * row_stride + col;
-  if (rows == 16 * NB) {
+__device__ __forceinline__ void write_state(float* p, int nk, int nv, int col0, const f32x4 (&s)[NB]) {
+  const int lane = fresh_lane(), col = col0 + (lane & 15), row0 = (lane >> 4) * 4;
+  if (col >= nv) return;
+  p += row0 * nv + col;
 #pragma unroll
-    for (int i = 0; i < NB; i++)
+  for (int i = 0; i < NB; i++, p += 16 * nv) {
+    float* at = p;
 #pragma unroll
-      for (int r = 0; r < 4; r++) p[(16 * i + r) * row_stride] = s[i][r];
-  } else {
-#pragma unroll
-    for (int i = 0; i < NB; i++)
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (row0 + 16 * i + r < rows) p[(16 * i + r) * row_stride] = s[i][r];
+    for (int r = 0; r < 4; r++, at += nv)
+      if (row0 + 16 * i + r < nk) *at = s[i][r];
   }
 }
 
@@ -604,11 +634,11 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
   constexpr int NB = K::C / 16;
-  const int g = (threadIdx.x & 63) >> 4;
+  const int lane = fresh_lane(), g = lane >> 4;
   Frag v[K::kExact][NB];
 #pragma unroll
   for (int i = 0; i < NB; i++) {
-    f32x4 x = widen(Tile<E, DC>::down(cols, i, col0));
+    f32x4 x = widen(Tile<E, DC>::down(cols, i, col0, lane));
     const f32x4 w = *(const f32x4*)(weight + 16 * i + 4 * g);
 #pragma unroll
     for (int r = 0; r < 4; r++) x[r] *= w[r] * scale;
@@ -618,7 +648,7 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
   for (int i = 0; i < DR / 16; i++) {
     Frag k[NB];
 #pragma unroll
-    for (int j = 0; j < NB; j++) k[j] = Tile<E, DR>::down(rows, j, 16 * i);
+    for (int j = 0; j < NB; j++) k[j] = Tile<E, DR>::down(rows, j, 16 * i, lane);
     f32x4 x = scaled(s[i], f);
 #pragma unroll
     for (int p = K::kExact - 1; p >= 0; p--) x = mma<NB>(k, v[p], x);
@@ -631,19 +661,19 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
 // Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS, where
 // q and k were: half the LDS again would be two workgroups a compute unit less.
 template <class E, int DK, int DV>
-__global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendArgs a, Segments seg) {
+__global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void attend_chunks(AttendArgs a, Segments seg) {
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
   constexpr int C = K::C, NT = DV * 4, NW = NT / 64, NB = C / 16, NK = DK / 16;
   constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
-  constexpr int kTiles = NB * (NB + 1) / 2, kMine = (kTiles + NW - 1) / NW;
+  constexpr int kTiles = NB * (NB + 1) / 2, kMine = (kTiles + NW - 1) / NW, NH = 2;
   constexpr int kTile = C * Tile<E, DK>::kRow, kScore = C * Tile<E, C>::kRow;
   __shared__ __align__(16) char shared[2 * kTile > K::kScores * kScore ? 2 * kTile : K::kScores * kScore];
   __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow];
   __shared__ __align__(16) Decays<C> decays;
   __shared__ uint32_t bad;
   char *q_tile = shared, *k_tile = shared + kTile;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col0 = 16 * wave;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
@@ -669,9 +699,9 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
   fetch(first);
   f32x4 s[NK];
   if (segment == 0) {
-    read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, a.nk, a.nv, col0, s);
+    read_state<false>(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nk, a.nv, col0, 0, s);
   } else {
-    const f32x4* p = (const f32x4*)(seg.states + ((segment - 1) * heads + bh) * (DK * DV)) + wave * NK * 64 + lane;
+    const f32x4* p = (const f32x4*)(seg.states + ((segment - 1) * heads + bh) * (DK * DV)) + wave * NK * 64 + fresh_lane();
 #pragma unroll
     for (int i = 0; i < NK; i++) s[i] = p[i * 64];
   }
@@ -688,6 +718,7 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
     Frag mine[kMine][K::kScores];
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
+      const int lane = fresh_lane();
       const int n = wave + m * NW;
       if (n >= kTiles) break;
       int ta, tb;
@@ -695,37 +726,40 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
       Frag x[NK], y[NK];
 #pragma unroll
       for (int i = 0; i < NK; i++) {
-        x[i] = Tile<E, DK>::along(k_tile, 16 * ta, i);
-        y[i] = Tile<E, DK>::along(q_tile, 16 * tb, i);
+        x[i] = Tile<E, DK>::along(k_tile, 16 * ta, i, lane);
+        y[i] = Tile<E, DK>::along(q_tile, 16 * tb, i, lane);
       }
       f32x4 p = mma<NK>(x, y, f32x4{});
-      const f32x4 l = decay_between(decays, ta, tb);
+      const f32x4 l = decay_between(decays, ta, tb, lane);
 #pragma unroll
       for (int r = 0; r < 4; r++) p[r] = l[r] != 0.0f ? p[r] * l[r] * a.scale : 0.0f;
       cut<K::kScores>(p, mine[m], 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     // What the state from before the chunk answers: o^T = S^T Q^T.
-    f32x4 acc[NB];
-    {
-      Frag sp[K::kState][NK];
+    // Some of the state's rows at a time: all its pieces would fill the registers.
+    f32x4 acc[NB] = {};
+    const int at = fresh_lane();
 #pragma unroll
-      for (int i = 0; i < NK; i++) cut<K::kState>(s[i], &sp[0][i], NK);
+    for (int half = 0; half < NK; half += NH) {
+      Frag sp[K::kState][NH];
+#pragma unroll
+      for (int i = 0; i < NH; i++) cut<K::kState>(s[half + i], &sp[0][i], NH);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        Frag y[NK];
+        Frag y[NH];
 #pragma unroll
-        for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, j);
-        f32x4 x{};
+        for (int j = 0; j < NH; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, half + j, at);
 #pragma unroll
-        for (int p = K::kState - 1; p >= 0; p--) x = mma<NK>(sp[p], y, x);
-        acc[i] = scaled(x, decays.e[16 * i + c] * a.scale);
+        for (int p = K::kState - 1; p >= 0; p--) acc[i] = mma<NH>(sp[p], y, acc[i]);
+        if (half + NH == NK) acc[i] = scaled(acc[i], decays.e[16 * i + (at & 15)] * a.scale);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
     __syncthreads();  // q and k are read
     fetch(t0 + C);  // nothing where that is the end
+    const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
       const int n = wave + m * NW;
@@ -742,7 +776,7 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
     }
     Frag vf[NB];
 #pragma unroll
-    for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0);
+    for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0, lane);
     __syncthreads();  // the scores are there
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -753,7 +787,7 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
         for (int j = 0; j <= i; j += two) {
           Frag y[two];
 #pragma unroll
-          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(shared + p * kScore, 16 * i, j + n);
+          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(shared + p * kScore, 16 * i, j + n, lane);
           x = mma<two>(&vf[j], y, x);
         }
       zeros = zeros_of(x, zeros);
@@ -762,7 +796,7 @@ __global__ __launch_bounds__(DV * 4, DK > DV ? 2 : 3) void attend_chunks(AttendA
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nv, a.nk, a.nv, col0, s);
+  if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nk, a.nv, col0, s);
 #pragma unroll
   for (int i = 0; i < NK; i++) zeros = zeros_of(s[i], zeros);
   if (not_finite(zeros)) bad = 1;
@@ -783,7 +817,7 @@ struct Roles {
 //   ADDS   what a segment but the last adds to the state, from 0, and how much it
 //          leaves of it
 //   BACK   the same of the gradient's, E, from the end, of a segment but the first
-//   EACH   the state before each chunk
+//   EACH   the state before each chunk but the first, which stands elsewhere
 enum { ADDS, BACK, EACH };
 template <class E, int DR, int DC, int MODE>
 __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(AttendArgs a, Roles x, Segments seg, f32x4* each) {
@@ -804,7 +838,7 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   f32x4 s[NR];
   if (MODE == EACH && segment == 0) {
-    read_state(x.first.p ? x.first.p + b * x.first.b + h * x.first.h : nullptr, x.row_stride, x.col_stride, x.nr, x.nc, col0, s);
+    read_state<true>(x.first.p ? x.first.p + b * x.first.b + h * x.first.h : nullptr, x.nc, x.nr, col0, 0, s);
   } else {
     const f32x4* p = (const f32x4*)(seg.states + ((segment - 1) * heads + bh) * (DR * DC)) + wave * NR * 64 + lane;
 #pragma unroll
@@ -826,12 +860,12 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
   double all = 0.0;
   bool forgets = false;
   for (int64_t n = 0; n < chunks; n++) {
-    if (MODE == EACH) {
+    if (MODE == EACH && n > 0) {
       f32x4* p = each + ((start(n) / C * heads + bh) * (DC / 16) + wave) * NR * 64 + lane;
 #pragma unroll
       for (int i = 0; i < NR; i++) p[i * 64] = s[i];
-      if (n + 1 == chunks) break;
     }
+    if (MODE == EACH && n + 1 == chunks) break;
     __syncthreads();
     const int64_t t0 = start(n);
     const int left = (int)min((int64_t)C, end - t0);
@@ -876,13 +910,22 @@ __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segm
   const int64_t step = (back ? -1 : 1) * heads * (DR * DC), from = back ? slots - 1 : 0;
   float* p = seg.states + (from * heads + bh) * (DR * DC) + i;
   const float* f = seg.decay + from * heads + bh;
-#pragma unroll 8
-  for (int n = 0; n < slots; n++) {
-    const float add = *p, keep = *f;
-    s = keep < 0.0f ? add : fmaf(keep, s, add);
-    *p = s;
-    p += step;
-    f += back ? -heads : heads;
+  const int64_t f_step = back ? -heads : heads;
+  // Sixteen at a time: their loads wait together.
+  constexpr int N = 16;
+  for (int n = 0; n < slots; n += N) {
+    float add[N], keep[N];
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (n + j < slots) add[j] = p[j * step], keep[j] = f[j * f_step];
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (n + j < slots) {
+        s = keep[j] < 0.0f ? add[j] : fmaf(keep[j], s, add[j]);
+        p[j * step] = s;
+      }
+    p += N * step;
+    f += N * f_step;
   }
 }
 
@@ -903,28 +946,40 @@ __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
 // behind it, and W = dO V^T, dA = scale W o L:
 //   dQ = dA K + scale e o (dO S^T),  dK = dA^T Q + r o (V E^T),  dV = A^T dO + r o (K E),
 //   E <- f E + scale (e o Q)^T dO.
-// E is held twice, as rows of keys (a wave's 16 columns of values) and as rows of
-// values (its 16 columns of keys), so that dV and dK each find it in registers.
+// E is held twice: as rows of values by the first NK waves, 16 columns of keys each,
+// which find dK, and as rows of keys by the NV others, which find dV. dQ's tiles are
+// dealt out to all. (One wave for a column of each takes twice the registers: 458 us
+// against 254 at 256 steps of 2048 heads of 64 in bf16, the same in f32.)
 // A gate's gradient sums over all ways across it: from the state before to the
 // gradient behind, X = f <S, E>; from steps u >= t to the state before,
 // q_u . (the state's part of dq_u); from steps s < t to the gradient behind,
 // k_s . (its part of dk_s); and between steps of the chunk, M = A o W over u >= t >
 // s, R_{t+1} = R_t + sum_u M[u][t] - sum_s M[t][s].
 // No sum is taken over more than a chunk, so nothing large cancels.
+template <int DK, int DV>
+constexpr int kGradientThreads = (DK + DV) * 4;
+
 template <class E, int DK, int DV>
-__global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(AttendArgs a, Segments seg, const f32x4* each, int32_t wide) {
+__global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradients(AttendArgs a, Segments seg, const float* forth,
+                                                                                  const f32x4* each, int32_t wide) {
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
-  constexpr int C = K::C, D = DK > DV ? DK : DV, NT = D * 4, NW = NT / 64, NB = C / 16, NK = DK / 16, NV = DV / 16;
+  constexpr int C = K::C, NT = kGradientThreads<DK, DV>, NW = NT / 64, NB = C / 16, NK = DK / 16, NV = DV / 16;
   constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
+  // dQ's tiles: each in kParts parts of kPer blocks of steps, by a wave of the first
+  // and some of the second kind.
+  constexpr int kParts = 1 + NV / NK < NB ? 1 + NV / NK : NB, kPer = (NB + kParts - 1) / kParts;
   __shared__ __align__(16) char q_tile[C * Tile<E, DK>::kRow], k_tile[C * Tile<E, DK>::kRow];
   __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow], o_tile[C * Tile<E, DV>::kRow];
   __shared__ __align__(16) char score[K::kScores][C * Tile<E, C>::kRow], dscore[K::kScores][C * Tile<E, C>::kRow];
   __shared__ __align__(16) Decays<C> decays;
   __shared__ __align__(16) float row_sum[NB][C], col_sum[NB][C], q_dot[NK][C], k_dot[NK][C], x_dot[NK];
   __shared__ uint32_t bad;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col0 = 16 * wave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool keys = wave < NK;  // else values
+  const int col0 = 16 * (keys ? wave : wave - NK);
+  const int tile = wave % NK, part = wave / NK;  // of dQ
+  const bool asks = part < kParts && part * kPer < NB;
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
   int segment, b, h;
@@ -937,21 +992,27 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
   float* dg = a.dg ? a.dg + b * a.dg_b + h * a.dg_h : nullptr;
 
-  f32x4 ek[NK], ev[NV];  // rows of keys, rows of values
-  if (segment + 1 == seg.count) {
-    const float* ds = a.ds.p ? a.ds.p + b * a.ds.b + h * a.ds.h : nullptr;
-    read_state(ds, a.nv, 1, a.nk, a.nv, col0, ek);
-    read_state(ds, 1, a.nv, a.nv, a.nk, col0, ev);
-  } else {
-    const float* p = seg.states + (segment * heads + bh) * (DK * DV);
+  constexpr int NE = NK > NV ? NK : NV;
+  f32x4 e[NE] = {};  // rows of values (NV blocks), or of keys (NK)
+  {
+    const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+    if (segment + 1 == seg.count) {
+      const float* ds = a.ds.p ? a.ds.p + b * a.ds.b + h * a.ds.h : nullptr;
+      if (keys) read_state<true>(ds, a.nk, a.nv, col0, 0, *(f32x4(*)[NV])e);
+      else read_state<false>(ds, a.nk, a.nv, col0, 0, *(f32x4(*)[NK])e);
+    } else {
+      const float* p = seg.states + (segment * heads + bh) * (DK * DV);
+      if (keys) {
+        // Element (row d, column j) stands at tile j / 16 * NK + d / 16, lane d % 16 / 4 * 16 + j % 16, row d % 4.
 #pragma unroll
-    for (int i = 0; i < NK; i++) ek[i] = wave < NV ? ((const f32x4*)p)[(wave * NK + i) * 64 + lane] : f32x4{};
-    // Element (row d, column j) stands at tile j / 16 * NK + d / 16, lane d % 16 / 4 * 16 + j % 16, row d % 4.
+        for (int i = 0; i < NV; i++)
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+          for (int r = 0; r < 4; r++) e[i][r] = p[(((i * NK + wave) * 64) + (c >> 2) * 16 + 4 * g + r) * 4 + (c & 3)];
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        ev[i][r] = wave < NK ? p[(((i * NK + wave) * 64) + (c >> 2) * 16 + 4 * g + r) * 4 + (c & 3)] : 0.0f;
+        for (int i = 0; i < NK; i++) e[i] = ((const f32x4*)p)[((wave - NK) * NK + i) * 64 + lane];
+      }
+    }
   }
   for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = ((f32x4*)dscore)[i] = f32x4{};
   if (threadIdx.x == 0) bad = 0;
@@ -969,7 +1030,7 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
   float zeros = 0.0f;
   // The gates' gradients of the chunk at t0, by the last wave, a lane a step.
   auto gates = [&](int64_t t0, float f, uint64_t resets) {
-    const int t = lane, tile = t / 16;
+    const int lane = fresh_lane(), t = lane, tile = t / 16;
     float x = 0.0f, qd = 0.0f, kd = 0.0f, m = 0.0f;
     for (int w = 0; w < NK; w++) x += x_dot[w];
     if (t < C) {
@@ -992,6 +1053,23 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
       dg[step * a.dg_t] = out;
     }
   };
+  // acc + the intra-chunk product: A's fragments `x` (a block of steps each) with
+  // the scores' of tile i, along their rows or down their columns.
+  auto add = [&](const Frag* x, const char (&scores)[K::kScores][C * Tile<E, C>::kRow], int i, bool along, f32x4 acc, int lane) {
+#pragma unroll
+    for (int p = K::kScores - 1; p >= 0; p--)
+#pragma unroll
+      for (int j = 0; j < NB; j += two) {
+        if (along ? j > i : j + two <= i) continue;
+        Frag y[two];
+#pragma unroll
+        for (int m = 0; m < two; m++)
+          y[m] = along ? Tile<E, C>::along(scores[p], 16 * i, j + m, lane) : Tile<E, C>::down(scores[p], j + m, 16 * i, lane);
+        acc = mma<two>(x + j, y, acc);
+      }
+    zeros = zeros_of(acc, zeros);
+    return acc;
+  };
   const int64_t chunks = (end - first + C - 1) / C;
   fetch(first + (chunks - 1) * C);
   float f_before = 0.0f;
@@ -1007,34 +1085,43 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
     lo.stash(o_tile, d_o + t0 * a.o.t, a.o.t, left, a.nv);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
-    if (n > 0) fetch(t0 - C);
-    f32x4 s[NV];  // the state before the chunk: rows of values, the wave's 16 columns of keys
-    if (wave < NK) {
-      if (each) {
-        const f32x4* p = each + ((t0 / C * heads + bh) * NK + wave) * NV * 64 + lane;
-#pragma unroll
-        for (int i = 0; i < NV; i++) s[i] = p[i * 64];
+    // Blocks of the state before the chunk: rows of values, the tile's columns of keys.
+    constexpr int NS = NV < 4 ? NV : 4;
+    auto state_before = [&](int block, f32x4 (&s)[NS]) {
+      if (n == 0 && segment == 0) {
+        read_state<true>(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nk, a.nv, 16 * tile, block, s);
       } else {
-        read_state(a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, 1, a.nv, a.nv, a.nk, col0, s);
+        const f32x4* p = n == 0 ? (const f32x4*)forth + ((segment - 1) * heads + bh) * (NK * NV * 64) : each + (t0 / C * heads + bh) * (NK * NV * 64);
+        p += (tile * NV + block) * 64 + fresh_lane();
+#pragma unroll
+        for (int i = 0; i < NS; i++) s[i] = p[i * 64];
       }
-    }
+    };
+    f32x4 s[NS];
+    if (asks) state_before(0, s);
     for (int m = wave; m < NB * (NB + 1) / 2; m += NW) {
+      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
       int ta, tb;
       tile_of(m, &ta, &tb);
-      Frag x[NK > NV ? NK : NV], y[NK > NV ? NK : NV];
+      // c + the tile's products, four blocks at a time.
+      auto score_of = [&](auto tag, const char* left, const char* right) {
+        constexpr int D = decltype(tag)::value, N = D / 16 < 4 ? D / 16 : 4;
+        f32x4 p{};
 #pragma unroll
-      for (int i = 0; i < NK; i++) {
-        x[i] = Tile<E, DK>::along(k_tile, 16 * ta, i);
-        y[i] = Tile<E, DK>::along(q_tile, 16 * tb, i);
-      }
-      f32x4 p = mma<NK>(x, y, f32x4{});
+        for (int i = 0; i < D / 16; i += N) {
+          Frag x[N], y[N];
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        x[i] = Tile<E, DV>::along(v_tile, 16 * ta, i);
-        y[i] = Tile<E, DV>::along(o_tile, 16 * tb, i);
-      }
-      f32x4 w = mma<NV>(x, y, f32x4{});
-      const f32x4 l = decay_between(decays, ta, tb);
+          for (int j = 0; j < N; j++) {
+            x[j] = Tile<E, D>::along(left, 16 * ta, i + j, lane);
+            y[j] = Tile<E, D>::along(right, 16 * tb, i + j, lane);
+          }
+          p = mma<N>(x, y, p);
+        }
+        return p;
+      };
+      f32x4 p = score_of(std::integral_constant<int, DK>(), k_tile, q_tile);
+      f32x4 w = score_of(std::integral_constant<int, DV>(), v_tile, o_tile);
+      const f32x4 l = decay_between(decays, ta, tb, lane);
       f32x4 ways;
       float sum = 0.0f;
 #pragma unroll
@@ -1067,114 +1154,114 @@ __global__ __launch_bounds__((DK > DV ? DK : DV) * 4) void attend_gradients(Atte
     __syncthreads();
     f_before = decays.f;
     resets_before = decays.resets;
-    // c + the intra-chunk product: A's fragments `x` (a block of steps each) with
-    // the scores' of tile i, along their rows or down their columns.
-    auto add = [&](const Frag* x, const char (&scores)[K::kScores][C * Tile<E, C>::kRow], int i, bool along, f32x4 acc) {
+    // acc[i] += (state's columns)^T (rows of `with`, of steps' blocks from i0 on) over
+    // up to four blocks of the contraction, from `block` on, the state in NP pieces.
+    auto far = [&](auto pieces, auto rows, const f32x4* state, const char* with, int block, int i0, auto& acc, int lane) {
+      constexpr int NP = decltype(pieces)::value, D = decltype(rows)::value, N = D / 16 < 4 ? D / 16 : 4;
+      Frag big[NP][N];
 #pragma unroll
-      for (int p = K::kScores - 1; p >= 0; p--)
+      for (int i = 0; i < N; i++) cut<NP>(state[i], &big[0][i], N);
 #pragma unroll
-        for (int j = 0; j < NB; j += two) {
-          if (along ? j > i : j + two <= i) continue;
-          Frag y[two];
+      for (int i = 0; i < (int)(sizeof acc / sizeof acc[0]); i++) {
+        Frag y[N];
 #pragma unroll
-          for (int m = 0; m < two; m++)
-            y[m] = along ? Tile<E, C>::along(scores[p], 16 * i, j + m) : Tile<E, C>::down(scores[p], j + m, 16 * i);
-          acc = mma<two>(x + j, y, acc);
-        }
-      zeros = zeros_of(acc, zeros);
-      return acc;
-    };
-    if (wave < NK) {
-      // In three pieces: the gates' gradients, which are f32, follow from these.
-      Frag x[NB], big[K::kExact][NV];
-      // dQ
+        for (int j = 0; j < N; j++) y[j] = Tile<E, D>::along(with, 16 * (i0 + i), block + j, lane);
 #pragma unroll
-      for (int i = 0; i < NV; i++) cut<K::kExact>(s[i], &big[0][i], NV);
-#pragma unroll
-      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(k_tile, i, col0);
-#pragma unroll
-      for (int i = 0; i < NB; i++) {
-        Frag y[NV];
-#pragma unroll
-        for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(o_tile, 16 * i, j);
-        f32x4 acc{};
-#pragma unroll
-        for (int p = K::kExact - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
-        acc = scaled(acc, decays.e[16 * i + c] * a.scale);
-        if (dg) {
-          float d = dot4(acc, widen(Tile<E, DK>::along(q_tile, 16 * i, wave)));
-          d += __shfl_xor(d, 16);
-          d += __shfl_xor(d, 32);
-          if (g == 0) q_dot[wave][16 * i + c] = d;
-        }
-        acc = add(x, dscore, i, true, acc);
-        const int64_t t = t0 + 16 * i + c;
-        if (t < end) put4<E>(a.dq, t, b, h, a.nk, col0 + 4 * g, acc, wide & 1);
+        for (int p = NP - 1; p >= 0; p--) acc[i] = mma<N>(big[p], y, acc[i]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // dK
-      if (dg) {
-        float d = 0.0f;
+    };
+    // In three pieces where the gates' gradients, which are f32, follow; else as the
+    // results, which are rounded, need.
+    constexpr std::integral_constant<int, K::kExact> exact{};
+    constexpr std::integral_constant<int, K::kState> rounded{};
+    constexpr std::integral_constant<int, DK> dk{};
+    constexpr std::integral_constant<int, DV> dv{};
+    // A dot product with a row of q or k, over the tile's 16 columns.
+    auto dot = [&](f32x4 x, const char* rows, int i, int column, float* to, int lane) {
+      float d = dot4(x, widen(Tile<E, DK>::along(rows, 16 * i, column, lane)));
+      d += __shfl_xor(d, 16);
+      d += __shfl_xor(d, 32);
+      if (lane < 16) to[16 * i + lane] = d;
+    };
+    if (asks) {
+      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+      f32x4 acc[kPer] = {};
+      float d = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++) d += dot4(s[i], ev[i]);
+      for (int block = 0; block < NV; block += NS) {
+        if (block) state_before(block, s);
+        if (dg && keys) {
+#pragma unroll
+          for (int i = 0; i < NS; i++) d += dot4(s[i], e[block + i]);
+        }
+        far(exact, dv, s, o_tile, block, part * kPer, acc, lane);
+      }
+      if (dg && keys) {
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) d += __shfl_xor(d, m);
         if (lane == 0) x_dot[wave] = d;
       }
+      Frag x[NB];
 #pragma unroll
-      for (int i = 0; i < NV; i++) cut<K::kExact>(ev[i], &big[0][i], NV);
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(k_tile, i, 16 * tile, lane);
 #pragma unroll
-      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0);
+      for (int m = 0; m < kParts; m++)
+        if (m == part) {
 #pragma unroll
-      for (int i = 0; i < NB; i++) {
-        Frag y[NV];
-#pragma unroll
-        for (int j = 0; j < NV; j++) y[j] = Tile<E, DV>::along(v_tile, 16 * i, j);
-        f32x4 acc{};
-#pragma unroll
-        for (int p = K::kExact - 1; p >= 0; p--) acc = mma<NV>(big[p], y, acc);
-        acc = scaled(acc, decays.r[16 * i + c]);
-        if (dg) {
-          float d = dot4(acc, widen(Tile<E, DK>::along(k_tile, 16 * i, wave)));
-          d += __shfl_xor(d, 16);
-          d += __shfl_xor(d, 32);
-          if (g == 0) k_dot[wave][16 * i + c] = d;
+          for (int n = 0; n < kPer; n++) {
+            const int i = m * kPer + n;
+            if (i >= NB) break;
+            f32x4 y = scaled(acc[n], decays.e[16 * i + c] * a.scale);
+            if (dg) dot(y, q_tile, i, tile, q_dot[tile], lane);
+            y = add(x, dscore, i, true, y, lane);
+            const int64_t t = t0 + 16 * i + c;
+            if (t < end) put4<E>(a.dq, t, b, h, a.nk, 16 * tile + 4 * g, y, wide & 1);
+          }
         }
-        acc = add(x, dscore, i, false, acc);
-        const int64_t t = t0 + 16 * i + c;
-        if (t < end) put4<E>(a.dk, t, b, h, a.nk, col0 + 4 * g, acc, wide & 2);
-      }
-      advance_state<E, DV, DK>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, ev);
     }
-    if (wave < NV) {
-      // dV
-      Frag x[NB], big[K::kState][NK];
+    if (n > 0) fetch(t0 - C);
+    if (keys) {
+      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+      f32x4 acc[NB] = {};
 #pragma unroll
-      for (int i = 0; i < NK; i++) cut<K::kState>(ek[i], &big[0][i], NK);
+      for (int block = 0; block < NV; block += NS) far(exact, dv, e + block, v_tile, block, 0, acc, lane);
+      Frag x[NB];
 #pragma unroll
-      for (int i = 0; i < NB; i++) x[i] = Tile<E, DV>::down(o_tile, i, col0);
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0, lane);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        Frag y[NK];
-#pragma unroll
-        for (int j = 0; j < NK; j++) y[j] = Tile<E, DK>::along(k_tile, 16 * i, j);
-        f32x4 acc{};
-#pragma unroll
-        for (int p = K::kState - 1; p >= 0; p--) acc = mma<NK>(big[p], y, acc);
-        acc = scaled(acc, decays.r[16 * i + c]);
-        acc = add(x, score, i, false, acc);
+        f32x4 y = scaled(acc[i], decays.r[16 * i + c]);
+        if (dg) dot(y, k_tile, i, wave, k_dot[wave], lane);
+        y = add(x, dscore, i, false, y, lane);
         const int64_t t = t0 + 16 * i + c;
-        if (t < end) put4<E>(a.dv, t, b, h, a.nv, col0 + 4 * g, acc, wide & 4);
+        if (t < end) put4<E>(a.dk, t, b, h, a.nk, col0 + 4 * g, y, wide & 2);
       }
-      advance_state<E, DK, DV>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, ek);
+      advance_state<E, DV, DK>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NV])e);
+    } else {
+      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+      f32x4 acc[NB] = {};
+#pragma unroll
+      for (int block = 0; block < NK; block += 4) far(rounded, dk, e + block, k_tile, block, 0, acc, lane);
+      Frag x[NB];
+#pragma unroll
+      for (int i = 0; i < NB; i++) x[i] = Tile<E, DV>::down(o_tile, i, col0, lane);
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        const f32x4 y = add(x, score, i, false, scaled(acc[i], decays.r[16 * i + c]), lane);
+        const int64_t t = t0 + 16 * i + c;
+        if (t < end) put4<E>(a.dv, t, b, h, a.nv, col0 + 4 * g, y, wide & 4);
+      }
+      advance_state<E, DK, DV>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NK])e);
     }
   }
   __syncthreads();
   if (dg && wave == NW - 1) gates(first, f_before, resets_before);
-  if (segment == 0 && a.ds0.p && wave < NV)
-    write_state(a.ds0.p + b * a.ds0.b + h * a.ds0.h, a.nv, a.nk, a.nv, col0, ek);
-  if (wave < NV) {
+  if (!keys) {
+    if (segment == 0 && a.ds0.p)
+      write_state(a.ds0.p + b * a.ds0.b + h * a.ds0.h, a.nk, a.nv, col0, *(f32x4(*)[NK])e);
 #pragma unroll
-    for (int i = 0; i < NK; i++) zeros = zeros_of(ek[i], zeros);
+    for (int i = 0; i < NK; i++) zeros = zeros_of(e[i], zeros);
   }
   if (not_finite(zeros)) bad = 1;
   __syncthreads();
@@ -1429,7 +1516,7 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
   for (int i = 0; i < 3; i++) own[i] = outs[i].per > 1 ? p.take(T * heads * sizes[i] * 4) : -1;
   const int64_t flags = p.take((seg.count + 2 * slots) * heads * 4), decay = p.take(slots * heads * 4);
   const int64_t forth = p.take(slots * heads * state), back = p.take(slots * heads * state);
-  const int64_t each = p.take(chunks > 1 ? chunks * heads * state : 0);
+  const int64_t each = p.take(seg.chunks > 1 ? chunks * heads * state : 0);
   char* work = o->workspace(stream, p.size);
   if (!work) return 1;
   int wide = 0;
@@ -1445,7 +1532,7 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
   seg.decay = (float*)(work + decay);
   with_size(a.nk, [&](auto dk) {
     with_size(a.nv, [&](auto dv) {
-      constexpr int DK = dk(), DV = dv(), D = DK > DV ? DK : DV;
+      constexpr int DK = dk(), DV = dv();
       const unsigned join = (unsigned)(heads * (DK * DV / 256)), most = (unsigned)(heads * seg.count);
       // States have rows of values here, as dq reads them.
       const Roles s{a.v, a.k, a.nv, a.nk, 1, a.nv, a.s0}, e{a.q, a.o, a.nk, a.nv, a.nv, 1, a.ds};
@@ -1456,7 +1543,7 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
                            nullptr);
         hipLaunchKernelGGL((join_segments<DV, DK>), dim3(join), dim3(256), 0, stream, a, s, seg, false);
       }
-      if (chunks > 1) {
+      if (seg.chunks > 1) {
         seg.states = (float*)(work + forth);
         hipLaunchKernelGGL((segment_states<E, DV, DK, EACH>), dim3(most), dim3(DK * 4), 0, stream, a, s, seg, (f32x4*)(work + each));
       }
@@ -1467,8 +1554,8 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
                            nullptr);
         hipLaunchKernelGGL((join_segments<DK, DV>), dim3(join), dim3(256), 0, stream, a, e, seg, true);
       }
-      hipLaunchKernelGGL((attend_gradients<E, DK, DV>), dim3(most), dim3(D * 4), 0, stream, a, seg,
-                         chunks > 1 ? (const f32x4*)(work + each) : nullptr, wide);
+      hipLaunchKernelGGL((attend_gradients<E, DK, DV>), dim3(most), dim3(kGradientThreads<DK, DV>), 0, stream, a, seg,
+                         (const float*)(work + forth), (const f32x4*)(work + each), wide);
     });
   });
   AttendArgs again = a;
