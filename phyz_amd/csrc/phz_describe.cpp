@@ -42,7 +42,8 @@ const int kTensors[kPlain] = {6, 10, 4, 6, 7, 2, 3, 8, 13, 7, 4};
 // operators and the update's.
 const bool kForward[kPlain] = {true, false, true, true, false, true, false, true, false, true, true};
 
-PyObject *g_dtypes[kDtypes], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device, *g_requires_grad;
+PyObject *g_dtypes[kDtypes], *g_data_ptr, *g_shape, *g_stride, *g_dtype, *g_get_device, *g_requires_grad,
+    *g_is_contiguous, *g_numel;
 const int kCodes[kDtypes] = {PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_U8, PHZ_I32, PHZ_I64};
 
 // False, with no Python error left, where `o` is no tensor that can be
@@ -67,29 +68,36 @@ bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false) {
     if (ok) t->data = PyLong_AsVoidPtr(v);
     Py_XDECREF(v);
   }
+  if (flat) {
+    // Two calls that make no tuples; strides do not matter then.
+    v = ok ? PyObject_CallMethodNoArgs(o, g_is_contiguous) : nullptr;
+    ok = v == Py_True;
+    Py_XDECREF(v);
+    v = ok ? PyObject_CallMethodNoArgs(o, g_numel) : nullptr;
+    ok = v != nullptr;
+    if (ok) {
+      t->size[0] = PyLong_AsLongLong(v);
+      t->stride[0] = 1;
+      t->ndim = 1;
+    }
+    Py_XDECREF(v);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      ok = false;
+    }
+    return ok;
+  }
   PyObject* shape = ok ? PyObject_GetAttr(o, g_shape) : nullptr;
   PyObject* stride = shape ? PyObject_CallMethodNoArgs(o, g_stride) : nullptr;
   ok = ok && shape && stride && PyTuple_Check(shape) && PyTuple_Check(stride);
   if (ok) {
     const Py_ssize_t n = PyTuple_GET_SIZE(shape);
-    ok = PyTuple_GET_SIZE(stride) == n && (flat || (n >= 1 && n <= 3));
-    if (flat) {
-      int64_t all = 1;
-      for (Py_ssize_t i = n; ok && i-- > 0;) {
-        const int64_t size = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
-        ok = size <= 1 || PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i)) == all || all == 0;
-        all *= size;
-      }
-      t->size[0] = all;
-      t->stride[0] = 1;
-      t->ndim = 1;
-    } else {
-      for (Py_ssize_t i = 0; ok && i < n; i++) {
-        t->size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
-        t->stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i));
-      }
-      t->ndim = (int32_t)n;
+    ok = PyTuple_GET_SIZE(stride) == n && n >= 1 && n <= 3;
+    for (Py_ssize_t i = 0; ok && i < n; i++) {
+      t->size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+      t->stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride, i));
     }
+    t->ndim = (int32_t)n;
   }
   Py_XDECREF(shape);
   Py_XDECREF(stride);
@@ -233,7 +241,7 @@ PyMODINIT_FUNC PyInit__describe() {
   static_assert(sizeof(phz_tensor) == 64, "phz_tensor");
   const struct { PyObject** at; const char* name; } names[] = {
       {&g_data_ptr, "data_ptr"}, {&g_shape, "shape"}, {&g_stride, "stride"}, {&g_dtype, "dtype"}, {&g_get_device, "get_device"},
-      {&g_requires_grad, "requires_grad"}};
+      {&g_requires_grad, "requires_grad"}, {&g_is_contiguous, "is_contiguous"}, {&g_numel, "numel"}};
   for (auto& s : names)
     if (!(*s.at = PyUnicode_InternFromString(s.name))) return nullptr;
   return PyModule_Create(&g_module);
