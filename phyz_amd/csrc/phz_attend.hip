@@ -27,6 +27,7 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_of_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -281,17 +282,18 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
 // column) c. The matrix instructions' result has that form too, its rows along the
 // contraction: a state that one product leaves in registers is the next one's
 // operand as it is.
+// kSide: chains of products side by side (f32's take as long to issue as to end).
 template <class E> struct Kind;
 template <> struct Kind<float> {
   typedef f32x4 Frag;
-  static constexpr int C = 32, kScores = 1, kState = 1, kExact = 1;
+  static constexpr int C = 32, kScores = 1, kState = 1, kExact = 1, kSide = 1;
 };
 // bf16: operands that are f32 go in pieces, each the rounding of what the ones
 // before leave: scores and the state as it is read in two (2^-17 of them: the
 // results are rounded to 2^-9), what is added to the state in three, as f32 holds it.
 template <> struct Kind<bf16> {
   typedef s16x4 Frag;
-  static constexpr int C = 64, kScores = 2, kState = 2, kExact = 3;
+  static constexpr int C = 64, kScores = 2, kState = 2, kExact = 3, kSide = 2;
 };
 
 // c + A B over N blocks of 16.
@@ -313,6 +315,25 @@ __device__ __forceinline__ f32x4 mma(const s16x4* a, const s16x4* b, f32x4 c) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
   }
   return c;
+}
+
+// U of them side by side, chains that do not wait for each other: c[u] + A B with
+// the operands' fragments sa and sb apart.
+template <int N, int U>
+__device__ __forceinline__ void mma_side(const f32x4* a, int sa, const f32x4* b, int sb, f32x4* c) {
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int u = 0; u < U; u++) c[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u * sa + i][r], b[u * sb + i][r], c[u], 0, 0, 0);
+}
+template <int N, int U>
+__device__ __forceinline__ void mma_side(const s16x4* a, int sa, const s16x4* b, int sb, f32x4* c) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+#pragma unroll
+    for (int u = 0; u < U; u++) c[u] = mma<2>(a + u * sa + i, b + u * sb + i, c[u]);
 }
 
 // The two bf16 of a word.
@@ -407,10 +428,15 @@ struct Load {
     if (col + EL > d || left <= 0) return;
     const E* p = base + col;
     if (left == C) {
-      p += row0 * stride;
+      p += (uint32_t)row0 * (uint64_t)stride;
 #pragma unroll
       for (int i = 0; i < N; i++, p += kStep * stride)
-        if (C % kStep == 0 || row0 + i * kStep < C) x[i] = *(const Pack<E, EL>*)p;
+        if (C % kStep == 0 || row0 + i * kStep < C) {
+          // f32 past the caches (401 us against 420 for 64 steps of 16384 heads); lines
+          // of bf16 are shared by heads.
+          if constexpr (sizeof(E) == 4) x[i] = __builtin_bit_cast(std::remove_reference_t<decltype(x[i])>, __builtin_nontemporal_load((const f32x4_of_4*)p));
+          else x[i] = *(const Pack<E, EL>*)p;
+        }
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++) x[i] = *(const Pack<E, EL>*)(p + min(row0 + i * kStep, left - 1) * stride);
@@ -452,17 +478,19 @@ struct Decays {
   double all;               // log2 of it without resets
   uint64_t resets;
 };
+// As it was read: a comparison would wait for the loads.
 struct Gate {
   float x;
-  bool reset, live;
+  uint32_t reset;
+  bool live;
 };
 // A lane a step; by one wave.
 __device__ __forceinline__ Gate fetch_gate(const float* g, int64_t g_t, const uint8_t* reset, int64_t r_t, int left) {
   const int lane = threadIdx.x & 63;
-  Gate v{0.0f, false, lane < left};
+  Gate v{0.0f, 0, lane < left};
   if (lane < left) {
     v.x = g[lane * g_t];
-    v.reset = reset && reset[lane * r_t];
+    if (reset) v.reset = reset[lane * r_t];
   }
   return v;
 }
@@ -482,7 +510,7 @@ __device__ __forceinline__ double of_lane(double x, int lane) {
 template <int C>
 __device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
   const int lane = threadIdx.x & 63;
-  const bool reset = v.reset || v.x < kForgets;
+  const bool reset = v.reset != 0 || v.x < kForgets;
   // A reset's own gate does not count: what is left of before is nothing.
   double x = reset ? 0.0 : (double)v.x * 1.4426950408889634074;
   x += moved<0x111, 0xf>(x);  // row_shr by 1, 2, 4, 8: sums within rows of 16 lanes
@@ -546,11 +574,13 @@ struct Segments {
   uint32_t* state_flags;  // [count - 1][heads]: states that are not
 };
 
-// A workgroup's head and segment. Neighbouring heads share lines of memory: they
-// go to one XCD.
+// A workgroup's head and segment. Neighbouring heads share lines of memory: 16 of
+// them go to one XCD. (More, and the XCDs are far apart in each row: 64 steps of 8192
+// heads' gradients 646 us with an eighth of all a XCD, 623 so; one, and lines are
+// read twice: 777 steps of 222 heads 302 us against 292.)
 __device__ __forceinline__ void place_of(const AttendArgs& a, int64_t* bh, int* segment, int* b, int* h) {
-  const uint32_t n = gridDim.x, per = n / 8, i = blockIdx.x, heads = (uint32_t)(a.worlds * a.heads);
-  const uint32_t id = i < per * 8 ? i % 8 * per + i / 8 : i;
+  const uint32_t n = gridDim.x, i = blockIdx.x, heads = (uint32_t)(a.worlds * a.heads);
+  const uint32_t id = i < n / 128 * 128 ? i / 128 * 128 + i % 8 * 16 + i % 128 / 8 : i;
   const uint32_t s = id / heads, at = id - s * heads;
   *segment = (int)s;
   *bh = at;
@@ -611,11 +641,14 @@ __device__ __forceinline__ void write_state(float* p, int nk, int nv, int col0, 
   }
 }
 
-// Four neighbouring elements, from `at` on, of an output's row of `size`.
+// Four neighbouring elements of an output's row, of which it has `left` more.
+// (f32 is not read again here: past the caches, 418 us against 442 for 64 steps of
+// 16384 heads; the half lines of bf16 have to meet there.)
 template <class E>
-__device__ __forceinline__ void put4(E* row, int size, int at, f32x4 v) {
-  E* p = row + at;
-  if (at + 4 <= size) {
+__device__ __forceinline__ void put4(E* p, int left, f32x4 v) {
+  if (sizeof(E) == 4 && left >= 4) {
+    __builtin_nontemporal_store(v, (f32x4_of_4*)p);
+  } else if (left >= 4) {
     Pack<E, 4> y;
 #pragma unroll
     for (int i = 0; i < 4; i++) y.v[i] = from_f32<E>(v[i]);
@@ -623,17 +656,42 @@ __device__ __forceinline__ void put4(E* row, int size, int at, f32x4 v) {
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (at + i < size) p[i] = from_f32<E>(v[i]);
+      if (i < left) p[i] = from_f32<E>(v[i]);
   }
 }
+// A wave's 16 columns, from col0 on, of a chunk's rows of one head: a lane's four of
+// row 16 i + c. `wide`: f32 sums of each head's own. Whole tiles need no questions.
+template <class E, int C>
+struct Put {
+  char* p;
+  int64_t step;  // bytes to 16 rows further
+  int rows, cols;
+  bool whole, wide;
+  __device__ __forceinline__ Put(const Rows& r, int64_t t0, int left, int b, int h, int size, int col0, int lane, bool wide_) : wide(wide_) {
+    const uint32_t c = lane & 15, g = lane >> 4;
+    const int e = wide ? 4 : (int)sizeof(E);
+    p = (char*)r.p + (t0 * r.t + b * r.b + (int64_t)h * size + col0) * e + (c * (uint64_t)r.t + 4 * g) * e;
+    step = 16 * r.t * e;
+    rows = left - (int)c, cols = size - col0 - 4 * (int)g;
+    whole = left == C && col0 + 16 <= size;
+  }
+  __device__ __forceinline__ void operator()(int i, f32x4 v) const {
+    char* at = p + i * step;
+    if (!whole && 16 * i >= rows) return;
+    const int left = whole ? 4 : cols;
+    if (wide) put4((float*)at, left, v);
+    else put4((E*)at, left, v);
+  }
+};
 
-// s <- f s + rows^T (weight o cols) of one chunk: the wave's 16 columns.
-template <class E, int DR, int DC>
+// s <- f s + rows^T (weight o cols) of one chunk: the wave's 16 columns, SIDE blocks
+// of rows at a time (one where registers are short).
+template <class E, int DR, int DC, int SIDE = Kind<E>::kSide>
 __device__ __forceinline__ void advance_state(const char* rows, const char* cols, const float* weight, float scale, float f, int col0,
                                               f32x4 (&s)[DR / 16]) {
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
-  constexpr int NB = K::C / 16;
+  constexpr int NB = K::C / 16, U = SIDE;
   const int lane = fresh_lane(), g = lane >> 4;
   Frag v[K::kExact][NB];
 #pragma unroll
@@ -645,14 +703,19 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
     cut<K::kExact>(x, &v[0][i], NB);
   }
 #pragma unroll
-  for (int i = 0; i < DR / 16; i++) {
-    Frag k[NB];
+  for (int i = 0; i < DR / 16; i += U) {
+    Frag k[U][NB];
+    f32x4 x[U];
 #pragma unroll
-    for (int j = 0; j < NB; j++) k[j] = Tile<E, DR>::down(rows, j, 16 * i, lane);
-    f32x4 x = scaled(s[i], f);
+    for (int u = 0; u < U; u++) {
 #pragma unroll
-    for (int p = K::kExact - 1; p >= 0; p--) x = mma<NB>(k, v[p], x);
-    s[i] = x;
+      for (int j = 0; j < NB; j++) k[u][j] = Tile<E, DR>::down(rows, j, 16 * (i + u), lane);
+      x[u] = scaled(s[i + u], f);
+    }
+#pragma unroll
+    for (int p = K::kExact - 1; p >= 0; p--) mma_side<NB, U>(k[0], NB, v[p], 0, x);
+#pragma unroll
+    for (int u = 0; u < U; u++) s[i + u] = x[u];
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -665,8 +728,12 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
   constexpr int C = K::C, NT = DV * 4, NW = NT / 64, NB = C / 16, NK = DK / 16;
-  constexpr int two = sizeof(E) == 2 ? 2 : 1;  // blocks of an instruction
+  constexpr int two = sizeof(E) == 2 ? 2 : 1, U = K::kSide;  // blocks of an instruction, chains
   constexpr int kTiles = NB * (NB + 1) / 2, kMine = (kTiles + NW - 1) / NW, NH = 2;
+  // The next chunk's loads go out before this one's products where registers allow
+  // it (1024 steps of 512 heads of 64 bf16: 104 us against 113), in f32 behind them,
+  // which is bound by memory anyway (64 of 16384: 442 against 455).
+  constexpr bool kEarly = sizeof(E) == 2 && DK <= 64;
   constexpr int kTile = C * Tile<E, DK>::kRow, kScore = C * Tile<E, C>::kRow;
   __shared__ __align__(16) char shared[2 * kTile > K::kScores * kScore ? 2 * kTile : K::kScores * kScore];
   __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow];
@@ -675,6 +742,7 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
   char *q_tile = shared, *k_tile = shared + kTile;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col0 = 16 * wave;
+  const bool live = col0 < a.nv;  // else the wave helps with loads and scores alone
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
   int segment, b, h;
@@ -684,7 +752,6 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
   const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv);
   const float* gate = a.g + b * a.g_b + h * a.g_h;
   const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
-  E* o = (E*)a.o.p + b * a.o.b + (int64_t)h * a.nv;
 
   Load<E, DK, NT> lq, lk;
   Load<E, DV, NT> lv;
@@ -715,6 +782,7 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
     lv.stash(v_tile, v + t0 * a.v.t, a.v.t, left, a.nv);
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
+    if (kEarly) fetch(t0 + C);
     Frag mine[kMine][K::kScores];
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
@@ -740,25 +808,30 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
     // Some of the state's rows at a time: all its pieces would fill the registers.
     f32x4 acc[NB] = {};
     const int at = fresh_lane();
+    if (live) {
 #pragma unroll
-    for (int half = 0; half < NK; half += NH) {
-      Frag sp[K::kState][NH];
+      for (int half = 0; half < NK; half += NH) {
+        Frag sp[K::kState][NH];
 #pragma unroll
-      for (int i = 0; i < NH; i++) cut<K::kState>(s[half + i], &sp[0][i], NH);
+        for (int i = 0; i < NH; i++) cut<K::kState>(s[half + i], &sp[0][i], NH);
 #pragma unroll
-      for (int i = 0; i < NB; i++) {
-        Frag y[NH];
+        for (int i = 0; i < NB; i += U) {
+          Frag y[U][NH];
 #pragma unroll
-        for (int j = 0; j < NH; j++) y[j] = Tile<E, DK>::along(q_tile, 16 * i, half + j, at);
+          for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int p = K::kState - 1; p >= 0; p--) acc[i] = mma<NH>(sp[p], y, acc[i]);
-        if (half + NH == NK) acc[i] = scaled(acc[i], decays.e[16 * i + (at & 15)] * a.scale);
-        __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < NH; j++) y[u][j] = Tile<E, DK>::along(q_tile, 16 * (i + u), half + j, at);
+#pragma unroll
+          for (int p = K::kState - 1; p >= 0; p--) mma_side<NH, U>(sp[p], 0, y[0], NH, &acc[i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < NB; i++) acc[i] = scaled(acc[i], decays.e[16 * i + (at & 15)] * a.scale);
+      advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
     }
-    advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
     __syncthreads();  // q and k are read
-    fetch(t0 + C);  // nothing where that is the end
+    if (!kEarly) fetch(t0 + C);  // nothing where that is the end
     const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
@@ -775,25 +848,33 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
       }
     }
     Frag vf[NB];
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0, lane);
+      for (int i = 0; i < NB; i++) vf[i] = Tile<E, DV>::down(v_tile, i, col0, lane);
+    }
     __syncthreads();  // the scores are there
+    if (live) {
+      const Put<E, C> put(a.o, t0, left, b, h, a.nv, col0, lane, false);
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-      f32x4 x = acc[i];
+      for (int i = 0; i < NB; i += two) {
+        // In bf16 two tiles of rows take the same pairs of blocks.
 #pragma unroll
-      for (int p = K::kScores - 1; p >= 0; p--)
+        for (int p = K::kScores - 1; p >= 0; p--) {
+          Frag y[two][NB];
 #pragma unroll
-        for (int j = 0; j <= i; j += two) {
-          Frag y[two];
+          for (int u = 0; u < two; u++)
 #pragma unroll
-          for (int n = 0; n < two; n++) y[n] = Tile<E, C>::along(shared + p * kScore, 16 * i, j + n, lane);
-          x = mma<two>(&vf[j], y, x);
+            for (int j = 0; j < i + two; j++) y[u][j] = Tile<E, C>::along(shared + p * kScore, 16 * (i + u), j, lane);
+#pragma unroll
+          for (int j = 0; j < i + two; j += two) mma_side<two, two>(&vf[j], 0, &y[0][j], NB, &acc[i]);
         }
-      zeros = zeros_of(x, zeros);
-      const int64_t t = t0 + 16 * i + c;
-      if (t < end) put4<E>(o + t * a.o.t, a.nv, col0 + 4 * g, x);
-      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < two; u++) {
+          zeros = zeros_of(acc[i + u], zeros);
+          put(i + u, acc[i + u]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   if (end == a.steps && a.s1.p) write_state(a.s1.p + b * a.s1.b + h * a.s1.h, a.nk, a.nv, col0, s);
@@ -874,7 +955,8 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
     if (n + 1 < chunks) fetch(start(n + 1));
-    advance_state<E, DR, DC>(r_tile, c_tile, MODE == BACK ? decays.e : decays.r, MODE == BACK ? a.scale : 1.0f, decays.f, col0, s);
+    if (col0 < x.nc)
+      advance_state<E, DR, DC>(r_tile, c_tile, MODE == BACK ? decays.e : decays.r, MODE == BACK ? a.scale : 1.0f, decays.f, col0, s);
     all += decays.all;
     forgets = forgets || decays.resets;
   }
@@ -929,14 +1011,6 @@ __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segm
   }
 }
 
-// A gradient's row of one head; `wide`: f32 sums of each head's own.
-template <class E>
-__device__ __forceinline__ void put4(const Rows& r, int64_t t, int b, int h, int size, int at, f32x4 v, bool wide) {
-  const int64_t row = t * r.t + b * r.b + (int64_t)h * size;
-  if (wide) put4((float*)r.p + row, size, at, v);
-  else put4((E*)r.p + row, size, at, v);
-}
-
 __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
   return fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], x[3] * y[3])));
 }
@@ -979,7 +1053,8 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
   const bool keys = wave < NK;  // else values
   const int col0 = 16 * (keys ? wave : wave - NK);
   const int tile = wave % NK, part = wave / NK;  // of dQ
-  const bool asks = part < kParts && part * kPer < NB;
+  const bool asks = part < kParts && part * kPer < NB && 16 * tile < a.nk;
+  const bool live = col0 < (keys ? a.nk : a.nv);  // else the wave helps with loads and scores alone
   const int64_t heads = (int64_t)a.worlds * a.heads;
   int64_t bh;
   int segment, b, h;
@@ -1015,6 +1090,9 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
     }
   }
   for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = ((f32x4*)dscore)[i] = f32x4{};
+  // (Tiles of columns that do not exist leave theirs so.)
+  for (int i = threadIdx.x; i < NK * C; i += NT) (&q_dot[0][0])[i] = (&k_dot[0][0])[i] = 0.0f;
+  if (threadIdx.x < NK) x_dot[threadIdx.x] = 0.0f;
   if (threadIdx.x == 0) bad = 0;
   Load<E, DK, NT> lq, lk;
   Load<E, DV, NT> lv, lo;
@@ -1158,11 +1236,12 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
     // up to four blocks of the contraction, from `block` on, the state in NP pieces.
     auto far = [&](auto pieces, auto rows, const f32x4* state, const char* with, int block, int i0, auto& acc, int lane) {
       constexpr int NP = decltype(pieces)::value, D = decltype(rows)::value, N = D / 16 < 4 ? D / 16 : 4;
+      constexpr int M = sizeof acc / sizeof acc[0];
       Frag big[NP][N];
 #pragma unroll
       for (int i = 0; i < N; i++) cut<NP>(state[i], &big[0][i], N);
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof acc / sizeof acc[0]); i++) {
+      for (int i = 0; i < M; i++) {
         Frag y[N];
 #pragma unroll
         for (int j = 0; j < N; j++) y[j] = Tile<E, D>::along(with, 16 * (i0 + i), block + j, lane);
@@ -1185,7 +1264,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       if (lane < 16) to[16 * i + lane] = d;
     };
     if (asks) {
-      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+      const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[kPer] = {};
       float d = 0.0f;
 #pragma unroll
@@ -1205,6 +1284,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       Frag x[NB];
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(k_tile, i, 16 * tile, lane);
+      const Put<E, C> put(a.dq, t0, left, b, h, a.nk, 16 * tile, lane, wide & 1);
 #pragma unroll
       for (int m = 0; m < kParts; m++)
         if (m == part) {
@@ -1215,44 +1295,44 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
             f32x4 y = scaled(acc[n], decays.e[16 * i + c] * a.scale);
             if (dg) dot(y, q_tile, i, tile, q_dot[tile], lane);
             y = add(x, dscore, i, true, y, lane);
-            const int64_t t = t0 + 16 * i + c;
-            if (t < end) put4<E>(a.dq, t, b, h, a.nk, 16 * tile + 4 * g, y, wide & 1);
+            put(i, y);
           }
         }
     }
     if (n > 0) fetch(t0 - C);
-    if (keys) {
-      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+    if (!live) {
+    } else if (keys) {
+      const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[NB] = {};
 #pragma unroll
       for (int block = 0; block < NV; block += NS) far(exact, dv, e + block, v_tile, block, 0, acc, lane);
       Frag x[NB];
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0, lane);
+      const Put<E, C> put(a.dk, t0, left, b, h, a.nk, col0, lane, wide & 2);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
         f32x4 y = scaled(acc[i], decays.r[16 * i + c]);
         if (dg) dot(y, k_tile, i, wave, k_dot[wave], lane);
         y = add(x, dscore, i, false, y, lane);
-        const int64_t t = t0 + 16 * i + c;
-        if (t < end) put4<E>(a.dk, t, b, h, a.nk, col0 + 4 * g, y, wide & 2);
+        put(i, y);
       }
-      advance_state<E, DV, DK>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NV])e);
+      advance_state<E, DV, DK, 1>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NV])e);
     } else {
-      const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+      const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[NB] = {};
 #pragma unroll
       for (int block = 0; block < NK; block += 4) far(rounded, dk, e + block, k_tile, block, 0, acc, lane);
       Frag x[NB];
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DV>::down(o_tile, i, col0, lane);
+      const Put<E, C> put(a.dv, t0, left, b, h, a.nv, col0, lane, wide & 4);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
         const f32x4 y = add(x, score, i, false, scaled(acc[i], decays.r[16 * i + c]), lane);
-        const int64_t t = t0 + 16 * i + c;
-        if (t < end) put4<E>(a.dv, t, b, h, a.nv, col0 + 4 * g, y, wide & 4);
+        put(i, y);
       }
-      advance_state<E, DK, DV>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NK])e);
+      advance_state<E, DK, DV, 1>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NK])e);
     }
   }
   __syncthreads();
@@ -1442,15 +1522,28 @@ unsigned sequential_blocks(const phz_ops* o, const AttendArgs& a) {
 
 int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
 
-// Few heads take their steps in segments, so that the chip is filled; each has
-// four chunks at least, since the segments' states are found in a pass of its own.
-Segments segments_of(const phz_ops* o, const AttendArgs& a, int chunk) {
+// Few heads take their steps in segments, as many as the chip holds workgroups at a
+// time (`resident` a compute unit); each has four chunks at least, since the segments'
+// states are found in a pass of its own. Heads that fill more than half of it do not:
+// 1023 steps of 305 heads in one 106 us, in two 139.
+Segments segments_of(const phz_ops* o, const AttendArgs& a, int chunk, int resident) {
   const int64_t heads = (int64_t)a.worlds * a.heads, chunks = ceil_div(a.steps, chunk);
   Segments s{};
-  const int64_t want = std::max<int64_t>(1, std::min(ceil_div(2 * o->cus, heads), chunks / 4));
+  const int64_t want = std::max<int64_t>(1, std::min((int64_t)resident * o->cus / heads, chunks / 4));
   s.chunks = (int32_t)ceil_div(chunks, want);
   s.count = (int32_t)ceil_div(chunks, s.chunks);
   return s;
+}
+
+// Workgroups of a kernel that a compute unit holds.
+template <class Kernel>
+int resident_of(Kernel kernel, int threads) {
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void*)kernel, threads, 0) != hipSuccess) {
+    (void)hipGetLastError();
+    return 1;
+  }
+  return std::max(n, 1);
 }
 
 // Calls f with the padded sizes as constants.
@@ -1474,7 +1567,14 @@ struct Pieces {
 template <class E>
 int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
   const int64_t heads = (int64_t)a.worlds * a.heads, state = (int64_t)padded(a.nk) * padded(a.nv) * 4;
-  Segments seg = segments_of(o, a, Kind<E>::C);
+  int resident = 1;
+  with_size(a.nk, [&](auto dk) {
+    with_size(a.nv, [&](auto dv) {
+      static const int n = resident_of(attend_chunks<E, dk(), dv()>, dv() * 4);
+      resident = n;
+    });
+  });
+  Segments seg = segments_of(o, a, Kind<E>::C, resident);
   if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
   const int slots = seg.count - 1;
   Pieces p;
@@ -1508,7 +1608,14 @@ template <class E>
 int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]) {
   const int64_t T = a.steps, heads = (int64_t)a.worlds * a.heads, state = (int64_t)padded(a.nk) * padded(a.nv) * 4;
   const int sizes[3] = {a.nk, a.nk, a.nv};
-  Segments seg = segments_of(o, a, Kind<E>::C);
+  int resident = 1;
+  with_size(a.nk, [&](auto dk) {
+    with_size(a.nv, [&](auto dv) {
+      static const int n = resident_of(attend_gradients<E, dk(), dv()>, kGradientThreads<dk(), dv()>);
+      resident = n;
+    });
+  });
+  Segments seg = segments_of(o, a, Kind<E>::C, resident);
   const int64_t chunks = ceil_div(T, Kind<E>::C), slots = seg.count - 1;
   if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
   Pieces p;
