@@ -1011,6 +1011,40 @@ __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segm
   }
 }
 
+// Sums over lanes, in each of them, that stay in registers: over a row of 16, and of
+// the four rows' values of a lane.
+template <int N>
+__device__ __forceinline__ float rotated(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum_of_row(float x) {
+  x += rotated<8>(x);
+  x += rotated<4>(x);
+  x += rotated<2>(x);
+  return x + rotated<1>(x);
+}
+__device__ __forceinline__ float sum_of_rows(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto y = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, (uint32_t)y[0]) + __builtin_bit_cast(float, (uint32_t)y[1]));
+  const auto z = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_bit_cast(float, (uint32_t)z[0]) + __builtin_bit_cast(float, (uint32_t)z[1]);
+}
+
+// Sums over the lanes up to each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float sums_up_to(float x) {
+  x += moved<0x111, 0xf>(x);
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);
+  return x + moved<0x143, 0xc>(x);
+}
+
 __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
   return fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], x[3] * y[3])));
 }
@@ -1112,18 +1146,13 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
     float x = 0.0f, qd = 0.0f, kd = 0.0f, m = 0.0f;
     for (int w = 0; w < NK; w++) x += x_dot[w];
     if (t < C) {
-      for (int w = 0; w < NK; w++) qd += q_dot[w][t], kd += k_dot[w][t];
+      // (q's from the last step on.)
+      for (int w = 0; w < NK; w++) qd += q_dot[w][C - 1 - t], kd += k_dot[w][t];
       for (int i = tile; i < NB; i++) m += col_sum[i][t];
       for (int i = 0; i <= tile; i++) m -= row_sum[i][t];
     }
-    const float kd1 = kd, m1 = m;
-#pragma unroll
-    for (int n = 1; n < C; n *= 2) {
-      const float y = __shfl_down(qd, n), z = __shfl_up(kd, n), u = __shfl_up(m, n);
-      if (lane + n < 64) qd += y;
-      if (lane >= n) kd += z, m += u;
-    }
-    const float sum = (f != 0.0f ? f * x : 0.0f) + qd + ((kd - kd1) + (m - m1));
+    const float before = sums_up_to(kd) - kd + (sums_up_to(m) - m);
+    const float sum = (f != 0.0f ? f * x : 0.0f) + __shfl(sums_up_to(qd), (C - 1 - t) & 63) + before;
     const int64_t step = t0 + t;
     if (t < C && step < end) {
       const float out = resets >> t & 1 ? 0.0f : sum;
@@ -1219,13 +1248,10 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
 #pragma unroll
       for (int i = 0; i < K::kScores; i++) *(Frag*)(dscore[i] + at) = z[i];
       if (dg) {
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
+        sum = sum_of_rows(sum);
         if (g == 0) row_sum[ta][16 * tb + c] = sum;
 #pragma unroll
-        for (int n = 1; n < 16; n *= 2)
-#pragma unroll
-          for (int r = 0; r < 4; r++) ways[r] += __shfl_xor(ways[r], n);
+        for (int r = 0; r < 4; r++) ways[r] = sum_of_row(ways[r]);
         if (c == 0) *(f32x4*)&col_sum[tb][16 * ta + 4 * g] = ways;
       }
     }
@@ -1258,9 +1284,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
     constexpr std::integral_constant<int, DV> dv{};
     // A dot product with a row of q or k, over the tile's 16 columns.
     auto dot = [&](f32x4 x, const char* rows, int i, int column, float* to, int lane) {
-      float d = dot4(x, widen(Tile<E, DK>::along(rows, 16 * i, column, lane)));
-      d += __shfl_xor(d, 16);
-      d += __shfl_xor(d, 32);
+      const float d = sum_of_rows(dot4(x, widen(Tile<E, DK>::along(rows, 16 * i, column, lane))));
       if (lane < 16) to[16 * i + lane] = d;
     };
     if (asks) {
@@ -1277,8 +1301,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
         far(exact, dv, s, o_tile, block, part * kPer, acc, lane);
       }
       if (dg && keys) {
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) d += __shfl_xor(d, m);
+        d = sum_of_rows(sum_of_row(d));
         if (lane == 0) x_dot[wave] = d;
       }
       Frag x[NB];
