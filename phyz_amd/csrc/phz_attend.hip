@@ -723,6 +723,10 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
 // The forward pass. Wave w has columns 16 w .. 16 w + 15 of the state and of o.
 // Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS, where
 // q and k were: half the LDS again would be two workgroups a compute unit less.
+// Long rollouts of many heads are bound by memory (64 steps of 16384 heads of 64 f32:
+// 382 us, 4.2 TB/s); in bf16, and where heads are few, by the chain of a chunk's
+// phases: 32768 steps of 8 heads of 128 take 95 us here, two workgroups a compute
+// unit, of which LDS is busy about 40%, the vector units 35%, the matrix units 20%.
 template <class E, int DK, int DV>
 __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void attend_chunks(AttendArgs a, Segments seg) {
   typedef Kind<E> K;
@@ -978,7 +982,8 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
 }
 
 // The state before each segment but the first (the gradient behind each but the
-// last), from what each adds: in place.
+// last), from what each adds: in place. 63 segments of 8 heads of 128: 12 us for 66 MB
+// both ways (22 with one load after the other).
 template <int DR, int DC>
 __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segments seg, bool back) {
   const int64_t heads = (int64_t)a.worlds * a.heads, bh = blockIdx.x / (DR * DC / 256);
@@ -1064,6 +1069,9 @@ __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
 // k_s . (its part of dk_s); and between steps of the chunk, M = A o W over u >= t >
 // s, R_{t+1} = R_t + sum_u M[u][t] - sum_s M[t][s].
 // No sum is taken over more than a chunk, so nothing large cancels.
+// 64 steps of 8192 heads of 64 f32: 490 us at 3.0 TB/s, of whose time the matrix
+// units are busy 37% and the vector units a third; 777 steps of 222 heads of 48 and
+// 80 in bf16: 150 us, one workgroup of twelve waves a compute unit, phases again.
 template <int DK, int DV>
 constexpr int kGradientThreads = (DK + DV) * 4;
 
@@ -1375,7 +1383,9 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
 //
 // A workgroup takes `width` columns of one head's state: a thread four
 // neighbouring columns of every RP-th row, read, replaced and read by q; the
-// rows' sums meet in LDS.
+// rows' sums meet in LDS. One pass over the states: 1024 worlds x 4 heads of 64 in 24
+// us, 5.5 TB/s (a part of them from the memory-side cache); 8 x 8 heads of 128 in 8 us,
+// which is two trips to memory and the launch.
 constexpr int kStepThreads = 256;
 
 template <class E>
