@@ -1384,8 +1384,8 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
 //
 // A workgroup takes `width` columns of one head's state: a thread four
 // neighbouring columns of every RP-th row, read, replaced and read by q; the
-// rows' sums meet in LDS. One pass over the states: 1024 worlds x 4 heads of 64 in 24
-// us, 5.5 TB/s (a part of them from the memory-side cache); 8 x 8 heads of 128 in 8 us,
+// rows' sums meet in LDS. One pass over the states: 1024 worlds x 4 heads of 64 in 23
+// us, 6.0 TB/s (a part of them from the memory-side cache); 8 x 8 heads of 128 in 8 us,
 // which is two trips to memory and the launch.
 constexpr int kStepThreads = 256;
 
@@ -1411,17 +1411,27 @@ __global__ __launch_bounds__(kStepThreads) void attend_step(AttendArgs a, int32_
 #pragma unroll
     for (int i = 0; i < 4; i++) val[i] = i < n ? to_f32(v[j + i]) : 0.0f;
     if (n == 4) {
-#pragma unroll 8
-      for (int d = rr; d < a.nk; d += rows) {
-        auto* at = (Pack<float, 4>*)(s + (int64_t)d * a.nv + j);
-        Pack<float, 4> w = *at;
-        const float kd = to_f32(k[d]), qd = to_f32(q[d]);
+      // Four rows at a time: their loads wait together.
+      constexpr int R = 4;
+      for (int d0 = rr; d0 < a.nk; d0 += R * rows) {
+        Pack<float, 4> w[R];
+        E kd[R], qd[R];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          w.v[i] = fmaf(kd, val[i], forget ? 0.0f : keep * w.v[i]);
-          acc[i] = fmaf(qd, w.v[i], acc[i]);
+        for (int r = 0; r < R; r++) {
+          const int d = d0 + r * rows;
+          if (d < a.nk) w[r] = *(const Pack<float, 4>*)(s + d * a.nv + j), kd[r] = k[d], qd[r] = q[d];
         }
-        *at = w;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          const int d = d0 + r * rows;
+          if (d >= a.nk) break;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            w[r].v[i] = fmaf(to_f32(kd[r]), val[i], forget ? 0.0f : keep * w[r].v[i]);
+            acc[i] = fmaf(to_f32(qd[r]), w[r].v[i], acc[i]);
+          }
+          *(Pack<float, 4>*)(s + d * a.nv + j) = w[r];
+        }
       }
     } else {
       for (int d = rr; d < a.nk; d += rows) {
