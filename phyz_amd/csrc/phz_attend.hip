@@ -286,14 +286,15 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
 template <class E> struct Kind;
 template <> struct Kind<float> {
   typedef f32x4 Frag;
-  static constexpr int C = 32, kScores = 1, kState = 1, kExact = 1, kSide = 1;
+  static constexpr int C = 32, kPieces = 1, kSide = 1;
 };
-// bf16: operands that are f32 go in pieces, each the rounding of what the ones
-// before leave: scores and the state as it is read in two (2^-17 of them: the
-// results are rounded to 2^-9), what is added to the state in three, as f32 holds it.
+// bf16: operands that are f32 (scores, states, what is added to a state) go in
+// three pieces, each the rounding of what the ones before leave, which hold what f32
+// does. (Two leave 2^-17 of each: bf16 results were then 8e-5 to 1.1e-4 of their norm
+// from the rounding of 64 bits', now at most 4e-5, for 2 to 9% of the time.)
 template <> struct Kind<bf16> {
   typedef s16x4 Frag;
-  static constexpr int C = 64, kScores = 2, kState = 2, kExact = 3, kSide = 2;
+  static constexpr int C = 64, kPieces = 3, kSide = 2;
 };
 
 // c + A B over N blocks of 16.
@@ -401,6 +402,41 @@ struct Tile {
       // The transposing read hands each lane of 16 a column of a 4 x 16 block.
       typedef __attribute__((address_space(3))) s16x4 lds4;
       return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(l + (16 * block + 4 * g + (c >> 2)) * kRow + col * 2 + (c & 3) * 8));
+    }
+  }
+};
+
+// A chunk's scores in LDS: the tiles on and below the diagonal alone, so that three
+// pieces are smaller than two whole squares. Block b's b + 1 tiles stand beside those
+// of the block as far from the other end: rows of one length, 16 bytes apart from
+// whole banks.
+template <class E>
+struct Scores {
+  typedef typename Kind<E>::Frag Frag;
+  static constexpr int NB = Kind<E>::C / 16, kTileRow = 16 * sizeof(E), kRow = kTileRow * (NB + 1) + 16, kSize = NB / 2 * 16 * kRow;
+  static __device__ __forceinline__ constexpr int at(int a, int b) {
+    return b >= NB / 2 ? (NB - 1 - b) * 16 * kRow + kTileRow * a : b * 16 * kRow + kTileRow * (NB - b + a);
+  }
+  // Row c of block b, columns 16 a + 4 g .. + 3, for a <= b.
+  static __device__ __forceinline__ int place(int a, int b, int lane) {
+    return at(a, b) + (lane & 15) * kRow + (lane >> 4) * 4 * (int)sizeof(E);
+  }
+  // Fragments of the tile of rows b and columns a: along its rows, and down its
+  // columns; nothing above the diagonal.
+  static __device__ __forceinline__ Frag along(const char* l, int b, int a, int lane) {
+    return a <= b ? *(const Frag*)(l + place(a, b, lane)) : Frag{};
+  }
+  static __device__ __forceinline__ Frag down(const char* l, int b, int a, int lane) {
+    if (a > b) return Frag{};
+    const int c = lane & 15, g = lane >> 4;
+    if constexpr (sizeof(E) == 4) {
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; r++) v[r] = *(const float*)(l + at(a, b) + (4 * g + r) * kRow + 4 * c);
+      return v;
+    } else {
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(l + at(a, b) + (4 * g + (c >> 2)) * kRow + (c & 3) * 8));
     }
   }
 };
@@ -694,14 +730,14 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
   typedef typename K::Frag Frag;
   constexpr int NB = K::C / 16, U = SIDE;
   const int lane = fresh_lane(), g = lane >> 4;
-  Frag v[K::kExact][NB];
+  Frag v[K::kPieces][NB];
 #pragma unroll
   for (int i = 0; i < NB; i++) {
     f32x4 x = widen(Tile<E, DC>::down(cols, i, col0, lane));
     const f32x4 w = *(const f32x4*)(weight + 16 * i + 4 * g);
 #pragma unroll
     for (int r = 0; r < 4; r++) x[r] *= w[r] * scale;
-    cut<K::kExact>(x, &v[0][i], NB);
+    cut<K::kPieces>(x, &v[0][i], NB);
   }
 #pragma unroll
   for (int i = 0; i < DR / 16; i += U) {
@@ -714,7 +750,7 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
       x[u] = scaled(s[i + u], f);
     }
 #pragma unroll
-    for (int p = K::kExact - 1; p >= 0; p--) mma_side<NB, U>(k[0], NB, v[p], 0, x);
+    for (int p = K::kPieces - 1; p >= 0; p--) mma_side<NB, U>(k[0], NB, v[p], 0, x);
 #pragma unroll
     for (int u = 0; u < U; u++) s[i + u] = x[u];
     __builtin_amdgcn_sched_barrier(0);
@@ -739,8 +775,8 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
   // it (1024 steps of 512 heads of 64 bf16: 104 us against 113), in f32 behind them,
   // which is bound by memory anyway (64 of 16384: 442 against 455).
   constexpr bool kEarly = sizeof(E) == 2 && DK <= 64;
-  constexpr int kTile = C * Tile<E, DK>::kRow, kScore = C * Tile<E, C>::kRow;
-  __shared__ __align__(16) char shared[2 * kTile > K::kScores * kScore ? 2 * kTile : K::kScores * kScore];
+  constexpr int kTile = C * Tile<E, DK>::kRow, kScore = Scores<E>::kSize;
+  __shared__ __align__(16) char shared[2 * kTile > K::kPieces * kScore ? 2 * kTile : K::kPieces * kScore];
   __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow];
   __shared__ __align__(16) Decays<C> decays;
   __shared__ uint32_t bad;
@@ -788,7 +824,7 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
     if (wave == 0) find_decays(lg, &decays);
     __syncthreads();
     if (kEarly) fetch(t0 + C);
-    Frag mine[kMine][K::kScores];
+    Frag mine[kMine][K::kPieces];
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
       const int lane = fresh_lane();
@@ -806,7 +842,7 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
       const f32x4 l = decay_between(decays, ta, tb, lane);
 #pragma unroll
       for (int r = 0; r < 4; r++) p[r] = l[r] != 0.0f ? p[r] * l[r] * a.scale : 0.0f;
-      cut<K::kScores>(p, mine[m], 1);
+      cut<K::kPieces>(p, mine[m], 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     // What the state from before the chunk answers: o^T = S^T Q^T.
@@ -816,9 +852,9 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
     if (live) {
 #pragma unroll
       for (int half = 0; half < NK; half += NH) {
-        Frag sp[K::kState][NH];
+        Frag sp[K::kPieces][NH];
 #pragma unroll
-        for (int i = 0; i < NH; i++) cut<K::kState>(s[half + i], &sp[0][i], NH);
+        for (int i = 0; i < NH; i++) cut<K::kPieces>(s[half + i], &sp[0][i], NH);
 #pragma unroll
         for (int i = 0; i < NB; i += U) {
           Frag y[U][NH];
@@ -827,7 +863,7 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
 #pragma unroll
             for (int j = 0; j < NH; j++) y[u][j] = Tile<E, DK>::along(q_tile, 16 * (i + u), half + j, at);
 #pragma unroll
-          for (int p = K::kState - 1; p >= 0; p--) mma_side<NH, U>(sp[p], 0, y[0], NH, &acc[i]);
+          for (int p = K::kPieces - 1; p >= 0; p--) mma_side<NH, U>(sp[p], 0, y[0], NH, &acc[i]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -837,20 +873,16 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
     }
     __syncthreads();  // q and k are read
     if (!kEarly) fetch(t0 + C);  // nothing where that is the end
-    const int lane = fresh_lane(), c = lane & 15, g = lane >> 4;
+    const int lane = fresh_lane();
 #pragma unroll
     for (int m = 0; m < kMine; m++) {
       const int n = wave + m * NW;
       if (n >= kTiles) break;
       int ta, tb;
       tile_of(n, &ta, &tb);
-      char* at = shared + (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E);
+      char* at = shared + Scores<E>::place(ta, tb, lane);
 #pragma unroll
-      for (int i = 0; i < K::kScores; i++) {
-        *(Frag*)(at + i * kScore) = mine[m][i];
-        // The tile right of the diagonal that a pair of blocks takes in.
-        if (two == 2 && ta == tb && tb % 2 == 0) *(Frag*)(at + i * kScore + 16 * sizeof(E)) = Frag{};
-      }
+      for (int i = 0; i < K::kPieces; i++) *(Frag*)(at + i * kScore) = mine[m][i];
     }
     Frag vf[NB];
     if (live) {
@@ -864,12 +896,12 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
       for (int i = 0; i < NB; i += two) {
         // In bf16 two tiles of rows take the same pairs of blocks.
 #pragma unroll
-        for (int p = K::kScores - 1; p >= 0; p--) {
+        for (int p = K::kPieces - 1; p >= 0; p--) {
           Frag y[two][NB];
 #pragma unroll
           for (int u = 0; u < two; u++)
 #pragma unroll
-            for (int j = 0; j < i + two; j++) y[u][j] = Tile<E, C>::along(shared + p * kScore, 16 * (i + u), j, lane);
+            for (int j = 0; j < i + two; j++) y[u][j] = Scores<E>::along(shared + p * kScore, i + u, j, lane);
 #pragma unroll
           for (int j = 0; j < i + two; j += two) mma_side<two, two>(&vf[j], 0, &y[0][j], NB, &acc[i]);
         }
@@ -1088,7 +1120,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
   constexpr int kParts = 1 + NV / NK < NB ? 1 + NV / NK : NB, kPer = (NB + kParts - 1) / kParts;
   __shared__ __align__(16) char q_tile[C * Tile<E, DK>::kRow], k_tile[C * Tile<E, DK>::kRow];
   __shared__ __align__(16) char v_tile[C * Tile<E, DV>::kRow], o_tile[C * Tile<E, DV>::kRow];
-  __shared__ __align__(16) char score[K::kScores][C * Tile<E, C>::kRow], dscore[K::kScores][C * Tile<E, C>::kRow];
+  __shared__ __align__(16) char score[K::kPieces][Scores<E>::kSize], dscore[K::kPieces][Scores<E>::kSize];
   __shared__ __align__(16) Decays<C> decays;
   __shared__ __align__(16) float row_sum[NB][C], col_sum[NB][C], q_dot[NK][C], k_dot[NK][C], x_dot[NK];
   __shared__ uint32_t bad;
@@ -1132,7 +1164,6 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       }
     }
   }
-  for (int i = threadIdx.x; i < (int)sizeof score / 16; i += NT) ((f32x4*)score)[i] = ((f32x4*)dscore)[i] = f32x4{};
   // (Tiles of columns that do not exist leave theirs so.)
   for (int i = threadIdx.x; i < NK * C; i += NT) (&q_dot[0][0])[i] = (&k_dot[0][0])[i] = 0.0f;
   if (threadIdx.x < NK) x_dot[threadIdx.x] = 0.0f;
@@ -1171,16 +1202,16 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
   };
   // acc + the intra-chunk product: A's fragments `x` (a block of steps each) with
   // the scores' of tile i, along their rows or down their columns.
-  auto add = [&](const Frag* x, const char (&scores)[K::kScores][C * Tile<E, C>::kRow], int i, bool along, f32x4 acc, int lane) {
+  auto add = [&](const Frag* x, const char (&scores)[K::kPieces][Scores<E>::kSize], int i, bool along, f32x4 acc, int lane) {
 #pragma unroll
-    for (int p = K::kScores - 1; p >= 0; p--)
+    for (int p = K::kPieces - 1; p >= 0; p--)
 #pragma unroll
       for (int j = 0; j < NB; j += two) {
         if (along ? j > i : j + two <= i) continue;
         Frag y[two];
 #pragma unroll
         for (int m = 0; m < two; m++)
-          y[m] = along ? Tile<E, C>::along(scores[p], 16 * i, j + m, lane) : Tile<E, C>::down(scores[p], j + m, 16 * i, lane);
+          y[m] = along ? Scores<E>::along(scores[p], i, j + m, lane) : Scores<E>::down(scores[p], j + m, i, lane);
         acc = mma<two>(x + j, y, acc);
       }
     zeros = zeros_of(acc, zeros);
@@ -1248,14 +1279,14 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
         w[r] = there ? w[r] * l[r] * a.scale : 0.0f;
         sum += ways[r];
       }
-      const int at = (16 * tb + c) * Tile<E, C>::kRow + (16 * ta + 4 * g) * (int)sizeof(E);
-      Frag z[K::kScores];
-      cut<K::kScores>(p, z, 1);
+      const int at = Scores<E>::place(ta, tb, lane);
+      Frag z[K::kPieces];
+      cut<K::kPieces>(p, z, 1);
 #pragma unroll
-      for (int i = 0; i < K::kScores; i++) *(Frag*)(score[i] + at) = z[i];
-      cut<K::kScores>(w, z, 1);
+      for (int i = 0; i < K::kPieces; i++) *(Frag*)(score[i] + at) = z[i];
+      cut<K::kPieces>(w, z, 1);
 #pragma unroll
-      for (int i = 0; i < K::kScores; i++) *(Frag*)(dscore[i] + at) = z[i];
+      for (int i = 0; i < K::kPieces; i++) *(Frag*)(dscore[i] + at) = z[i];
       if (dg) {
         sum = sum_of_rows(sum);
         if (g == 0) row_sum[ta][16 * tb + c] = sum;
@@ -1268,27 +1299,28 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
     f_before = decays.f;
     resets_before = decays.resets;
     // acc[i] += (state's columns)^T (rows of `with`, of steps' blocks from i0 on) over
-    // up to four blocks of the contraction, from `block` on, the state in NP pieces.
-    auto far = [&](auto pieces, auto rows, const f32x4* state, const char* with, int block, int i0, auto& acc, int lane) {
-      constexpr int NP = decltype(pieces)::value, D = decltype(rows)::value, N = D / 16 < 4 ? D / 16 : 4;
-      constexpr int M = sizeof acc / sizeof acc[0];
-      Frag big[NP][N];
+    // up to four blocks of the contraction, from `block` on.
+    auto far = [&](auto rows, const f32x4* state, const char* with, int block, int i0, auto& acc, int lane) {
+      constexpr int NP = K::kPieces, D = decltype(rows)::value, NF = D / 16 < 4 ? D / 16 : 4;
+      constexpr int M = sizeof acc / sizeof acc[0], N = 2;
+      // Two blocks' pieces at a time: four fill the registers (684 us against 606 for
+      // 4096 steps of 64 heads of 128 and 128 in bf16).
 #pragma unroll
-      for (int i = 0; i < N; i++) cut<NP>(state[i], &big[0][i], N);
+      for (int k = 0; k < NF; k += N) {
+        Frag big[NP][N];
 #pragma unroll
-      for (int i = 0; i < M; i++) {
-        Frag y[N];
+        for (int i = 0; i < N; i++) cut<NP>(state[k + i], &big[0][i], N);
 #pragma unroll
-        for (int j = 0; j < N; j++) y[j] = Tile<E, D>::along(with, 16 * (i0 + i), block + j, lane);
+        for (int i = 0; i < M; i++) {
+          Frag y[N];
 #pragma unroll
-        for (int p = NP - 1; p >= 0; p--) acc[i] = mma<N>(big[p], y, acc[i]);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int j = 0; j < N; j++) y[j] = Tile<E, D>::along(with, 16 * (i0 + i), block + k + j, lane);
+#pragma unroll
+          for (int p = NP - 1; p >= 0; p--) acc[i] = mma<N>(big[p], y, acc[i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     };
-    // In three pieces where the gates' gradients, which are f32, follow; else as the
-    // results, which are rounded, need.
-    constexpr std::integral_constant<int, K::kExact> exact{};
-    constexpr std::integral_constant<int, K::kState> rounded{};
     constexpr std::integral_constant<int, DK> dk{};
     constexpr std::integral_constant<int, DV> dv{};
     // A dot product with a row of q or k, over the tile's 16 columns.
@@ -1307,7 +1339,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
 #pragma unroll
           for (int i = 0; i < NS; i++) d += dot4(s[i], e[block + i]);
         }
-        far(exact, dv, s, o_tile, block, part * kPer, acc, lane);
+        far(dv, s, o_tile, block, part * kPer, acc, lane);
       }
       if (dg && keys) {
         d = sum_of_rows(sum_of_row(d));
@@ -1337,7 +1369,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[NB] = {};
 #pragma unroll
-      for (int block = 0; block < NV; block += NS) far(exact, dv, e + block, v_tile, block, 0, acc, lane);
+      for (int block = 0; block < NV; block += NS) far(dv, e + block, v_tile, block, 0, acc, lane);
       Frag x[NB];
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DK>::down(q_tile, i, col0, lane);
@@ -1354,7 +1386,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[NB] = {};
 #pragma unroll
-      for (int block = 0; block < NK; block += 4) far(rounded, dk, e + block, k_tile, block, 0, acc, lane);
+      for (int block = 0; block < NK; block += 4) far(dk, e + block, k_tile, block, 0, acc, lane);
       Frag x[NB];
 #pragma unroll
       for (int i = 0; i < NB; i++) x[i] = Tile<E, DV>::down(o_tile, i, col0, lane);
