@@ -66,6 +66,14 @@ __device__ __forceinline__ const E* row_of(const Rows& r, int b, int h, int size
   return (const E*)r.p + b * r.b + (int64_t)(h / r.per) * size;
 }
 
+// The lane, as a value that the compiler finds anew: the addresses that follow from
+// it are then not all kept in registers through a loop over steps or chunks.
+__device__ __forceinline__ int fresh_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // ── one step after another ──────────────────────────────────────────────────
 //
 // A wave holds 16 columns of one head's state: lane (c, g) = (lane % 16, lane /
@@ -83,48 +91,66 @@ struct Sweep {
   bool back;
 };
 
-template <class E, class Out>
-__device__ __forceinline__ void sweep(const AttendArgs& a, const Sweep& w, int b, int h, int col0, float (&s)[8][4], Out&& out) {
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int col = col0 + c;
-  const bool live = col < w.cols;
+// What is left of the state that comes into step t: exp(g), or 0 where an episode
+// begins.
+struct Keep {
+  float by;
+  bool forget;
+};
+__device__ __forceinline__ Keep keep_of(const AttendArgs& a, int b, int h, int64_t t) {
+  if (t >= a.steps) return Keep{1.0f, false};
+  const float x = a.g[b * a.g_b + h * a.g_h + t * a.g_t];
+  return Keep{expf(x), x < kForgets || (a.reset && a.reset[b * a.r_b + t * a.r_t])};
+}
+__device__ __forceinline__ void first_state(const Sweep& w, int col0, float (&s)[8][4]) {
+  const int lane = fresh_lane(), col = col0 + (lane & 15), g = lane >> 4;
 #pragma unroll
   for (int i = 0; i < 8; i++)
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const int d = 16 * i + 4 * g + r;
-      s[i][r] = w.first && live && d < w.rows ? w.first[d * w.f_row + col * w.f_col] : 0.0f;
+      s[i][r] = w.first && col < w.cols && d < w.rows ? w.first[d * w.f_row + col * w.f_col] : 0.0f;
     }
-  const float* gate = a.g + b * a.g_b + h * a.g_h;
-  const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+}
+// Step t, and the column's sum over the lane's rows of read. (Rows that do not exist
+// are left alone: a value that is not finite times their 0 is not 0.)
+template <class E>
+__device__ __forceinline__ float take_step(const AttendArgs& a, const Sweep& w, int b, int h, int64_t t, int col0, float (&s)[8][4]) {
+  const int lane = fresh_lane(), col = col0 + (lane & 15), g = lane >> 4;
+  // Backwards the state of step t + 1 comes in by that step's gate.
+  const Keep keep = keep_of(a, b, h, w.back ? t + 1 : t);
+  const E* key = (const E*)w.key + t * w.key_t;
+  const E* read = (const E*)w.read + t * w.read_t;
+  const float val = col < w.cols ? to_f32(((const E*)w.val)[t * w.val_t + col]) * w.key_scale : 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    if (16 * i >= w.rows) break;
+    const int d = 16 * i + 4 * g;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const uint32_t at = (uint32_t)min(d + r, w.rows - 1);
+      const bool there = d + r < w.rows;
+      const float kept = keep.forget ? 0.0f : keep.by * s[i][r], x = fmaf(to_f32(key[at]), val, kept);
+      s[i][r] = there ? x : s[i][r];
+      sum = there ? fmaf(to_f32(read[at]), x, sum) : sum;
+    }
+  }
+  return sum;
+}
+template <class E, class Before, class Out>
+__device__ __forceinline__ void sweep(const AttendArgs& a, const Sweep& w, int b, int h, int col0, float (&s)[8][4], Before&& before,
+                                      Out&& out) {
+  const int col = col0 + (threadIdx.x & 15);
+  first_state(w, col0, s);
+#pragma unroll 1
   for (int n = 0; n < a.steps; n++) {
     const int64_t t = w.back ? a.steps - 1 - n : n;
-    // Backwards the state of step t + 1 comes in by that step's gate.
-    const int64_t tg = w.back ? t + 1 : t;
-    float x = 0.0f;
-    bool forget = false;
-    if (tg < a.steps) {
-      x = gate[tg * a.g_t];
-      forget = x < kForgets || (reset && reset[tg * a.r_t]);
-    }
-    const float keep = expf(x);
-    const E* key = (const E*)w.key + t * w.key_t;
-    const E* read = (const E*)w.read + t * w.read_t;
-    const float val = live ? to_f32(((const E*)w.val)[t * w.val_t + col]) * w.key_scale : 0.0f;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int d = 16 * i + 4 * g + r;
-        if (d >= w.rows) continue;
-        const float kept = forget ? 0.0f : keep * s[i][r];
-        s[i][r] = fmaf(to_f32(key[d]), val, kept);
-        sum = fmaf(to_f32(read[d]), s[i][r], sum);
-      }
+    before(t);
+    float sum = take_step<E>(a, w, b, h, t, col0, s);
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    out(t, col, live, sum * w.out_scale);
+    out(t, col, col < w.cols, sum * w.out_scale);
   }
 }
 
@@ -189,7 +215,7 @@ __global__ __launch_bounds__(512) void attend_sequential(AttendArgs a, int32_t m
     Sweep w{row_of<E>(a.q, b, h, a.nk), row_of<E>(a.k, b, h, a.nk), row_of<E>(a.v, b, h, a.nv), a.q.t, a.k.t, a.v.t, a.nk, a.nv,
             1.0f, a.scale, a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr, a.nv, 1, false};
     float s[8][4];
-    sweep<E>(a, w, b, h, col0, s, [&](int64_t t, int col, bool live, float v) {
+    sweep<E>(a, w, b, h, col0, s, [](int64_t) {}, [&](int64_t t, int col, bool live, float v) {
       if (live && (threadIdx.x & 63) < 16) put<E>(a.o, t, b, h, a.nv, col, v, false);
     });
     if (a.s1.p) {
@@ -200,17 +226,31 @@ __global__ __launch_bounds__(512) void attend_sequential(AttendArgs a, int32_t m
   });
 }
 
-// Its gradients. dg by <E_t, S_t> = q_t dq_t + dg_{t+1} = dg_t + k_t dk_t, in f64.
-// `wide`: which of dq, dk, dv are sums of each head's own (1, 2, 4).
+// Its gradients. `wide`: which of dq, dk, dv are sums of each head's own (1, 2, 4).
+// dg = exp(g_t) <E_t, S_{t-1}> by that formula: what is not finite reaches the steps
+// that the formula says, and no others, and no sum is taken over steps. E goes back
+// from the last step; the states that it meets, as many steps' at a time as LDS holds,
+// are found again from the one before their `chunk` steps, which the first pass leaves
+// in `kept`, one a chunk from chunk `from` on (blocks: 16 rows each of a padded state):
+// the passes over the products are done with that memory. A head of 4000 steps of 64 and
+// 64 f32 takes 61 ms, 0.1 where all is finite.
+struct Kept {
+  float* p;
+  int64_t step;  // elements to the next chunk's
+  int32_t size, blocks, from, chunk;
+};
 template <class E>
-__global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, int32_t marks, int32_t wide) {
+__global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, int32_t marks, int32_t wide, Kept kept) {
+  // 16 blocks of 16 rows of states, beside one in registers.
+  __shared__ float met[16 * 4][512];
+  const int most = 16 / kept.blocks + 1;
   __shared__ float part[8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, col0 = 16 * wave;
   const int64_t all = (int64_t)a.worlds * a.heads;
-  // The sum of one value of each column over the workgroup, in thread 0.
+  // The sum of one value of each lane over the workgroup, in every thread.
   auto total = [&](float v) {
 #pragma unroll
-    for (int m = 1; m < 16; m *= 2) v += __shfl_xor(v, m);
+    for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
     if (lane == 0) part[wave] = v;
     __syncthreads();
     float sum = 0.0f;
@@ -225,52 +265,87 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
             *d_o = row_of<E>(a.o, b, h, a.nv);
     const float* s0 = a.s0.p ? a.s0.p + b * a.s0.b + h * a.s0.h : nullptr;
     const float* ds = a.ds.p ? a.ds.p + b * a.ds.b + h * a.ds.h : nullptr;
-    float* dg = a.dg ? a.dg + b * a.dg_b + h * a.dg_h : nullptr;
-    const float* gate = a.g + b * a.g_b + h * a.g_h;
-    const uint8_t* reset = a.reset ? a.reset + b * a.r_b : nullptr;
+    // The states' transposes: dq reads S, dk and dg E, by their columns d.
+    const Sweep of_s{d_o, v, k, a.o.t, a.v.t, a.k.t, a.nv, a.nk, 1.0f, a.scale, s0, 1, a.nv, false};
+    const Sweep of_e{v, d_o, q, a.v.t, a.o.t, a.q.t, a.nv, a.nk, a.scale, 1.0f, ds, 1, a.nv, true};
+    auto slot = [&](int64_t t) {
+      return kept.p + (t / kept.chunk - kept.from) * kept.step + bh * kept.size + wave * kept.blocks * 256 + lane;
+    };
+    const bool holds = a.dg && col0 < a.nk;
     float s[8][4];
-    // dq: the state's transpose, over its columns d.
-    sweep<E>(a, Sweep{d_o, v, k, a.o.t, a.v.t, a.k.t, a.nv, a.nk, 1.0f, a.scale, s0, 1, a.nv, false}, b, h, col0, s,
+    sweep<E>(a, of_s, b, h, col0, s,
+             [&](int64_t t) {
+               if (!holds || t == 0 || t % kept.chunk) return;
+               float* p = slot(t);
+#pragma unroll
+               for (int i = 0; i < 8; i++)
+                 if (i < kept.blocks)
+#pragma unroll
+                   for (int r = 0; r < 4; r++) p[(i * 4 + r) * 64] = s[i][r];
+             },
              [&](int64_t t, int col, bool live, float x) {
                if (live && lane < 16) put<E>(a.dq, t, b, h, a.nk, col, x, wide & 1);
-               if (dg) {
-                 const float sum = total(live ? to_f32(q[t * a.q.t + col]) * x : 0.0f);
-                 if (threadIdx.x == 0) dg[t * a.dg_t] = sum;
-               }
              });
-    double later = 0.0;
-    if (dg) {
-      float mine = 0.0f;
-      const int col = col0 + c;
-      if (ds)
-        each_element(a.nv, col, col < a.nk, s, [&](int j, float x) { mine = fmaf(ds[(int64_t)col * a.nv + j], x, mine); });
-      mine += __shfl_xor(mine, 16);
-      mine += __shfl_xor(mine, 32);
-      later = total(mine);
-    }
-    sweep<E>(a, Sweep{v, d_o, q, a.v.t, a.o.t, a.q.t, a.nv, a.nk, a.scale, 1.0f, ds, 1, a.nv, true}, b, h, col0, s,
-             [&](int64_t t, int col, bool live, float x) {
-               if (live && lane < 16) put<E>(a.dk, t, b, h, a.nk, col, x, wide & 2);
-               if (dg) {
-                 const float sum = total(live ? to_f32(k[t * a.k.t + col]) * x : 0.0f);
-                 if (threadIdx.x == 0) {
-                   later += (double)dg[t * a.dg_t] - (double)sum;
-                   const float y = gate[t * a.g_t];
-                   if (y < kForgets || (reset && reset[t * a.r_t])) later = 0.0;
-                   dg[t * a.dg_t] = (float)later;
-                 }
-               }
-             });
-    sweep<E>(a, Sweep{k, q, d_o, a.k.t, a.q.t, a.o.t, a.nk, a.nv, a.scale, 1.0f, ds, a.nv, 1, true}, b, h, col0, s,
+    sweep<E>(a, of_e, b, h, col0, s, [](int64_t) {}, [&](int64_t t, int col, bool live, float x) {
+      if (live && lane < 16) put<E>(a.dk, t, b, h, a.nk, col, x, wide & 2);
+    });
+    sweep<E>(a, Sweep{k, q, d_o, a.k.t, a.q.t, a.o.t, a.nk, a.nv, a.scale, 1.0f, ds, a.nv, 1, true}, b, h, col0, s, [](int64_t) {},
              [&](int64_t t, int col, bool live, float x) {
                if (live && lane < 16) put<E>(a.dv, t, b, h, a.nv, col, x, wide & 4);
              });
     if (a.ds0.p) {
       float* out = a.ds0.p + b * a.ds0.b + h * a.ds0.h;
-      const float y = gate[0], keep = expf(y);
-      const bool forget = y < kForgets || (reset && reset[0]);
+      const Keep keep = keep_of(a, b, h, 0);
       const int col = col0 + c;
-      each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = forget ? 0.0f : keep * x; });
+      each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = keep.forget ? 0.0f : keep.by * x; });
+    }
+    if (!a.dg) return;
+    float* dg = a.dg + b * a.dg_b + h * a.dg_h;
+    float e[8][4];
+    first_state(of_e, col0, e);
+    for (int64_t t1 = a.steps; t1 > 0;) {
+      // Steps from t1 - n to t1 - 1, of the chunk that begins at t0.
+      const int64_t t0 = (t1 - 1) / kept.chunk * kept.chunk;
+      const int n = (int)min((int64_t)most, t1 - t0);
+      if (t0 == 0) {
+        first_state(of_s, col0, s);
+      } else if (holds) {
+        const float* p = slot(t0);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[i][r] = i < kept.blocks ? p[(i * 4 + r) * 64] : 0.0f;
+      }
+#pragma unroll 1
+      for (int64_t t = t0; t < t1 - 1; t++) {
+        const int m = (int)(t - (t1 - n));
+        if (m >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (i < kept.blocks)
+#pragma unroll
+              for (int r = 0; r < 4; r++) met[(m * kept.blocks + i) * 4 + r][threadIdx.x] = s[i][r];
+        }
+        (void)take_step<E>(a, of_s, b, h, t, col0, s);
+      }
+#pragma unroll 1
+      for (int m = n - 1; m >= 0; m--) {
+        const int64_t t = t1 - n + m;
+        (void)take_step<E>(a, of_e, b, h, t, col0, e);
+        float mine = 0.0f;
+        if (col0 + c < a.nk) {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (i < kept.blocks)
+#pragma unroll
+              for (int r = 0; r < 4; r++)
+                mine = fmaf(e[i][r], m + 1 < n ? met[(m * kept.blocks + i) * 4 + r][threadIdx.x] : s[i][r], mine);
+        }
+        const float sum = total(mine);
+        const Keep keep = keep_of(a, b, h, t);
+        if (threadIdx.x == 0) dg[t * a.dg_t] = keep.forget ? 0.0f : keep.by * sum;
+      }
+      t1 -= n;
     }
   });
 }
@@ -371,14 +446,6 @@ __device__ __forceinline__ f32x4 scaled(f32x4 x, float by) {
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = by != 0.0f ? x[i] * by : 0.0f;
   return x;
-}
-
-// The lane, as a value that the compiler finds anew: the addresses that follow from
-// it are then not all kept in registers through the loop over chunks.
-__device__ __forceinline__ int fresh_lane() {
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));
-  return lane;
 }
 
 // A tile of ROWS x D in LDS, rows 16 bytes apart from whole banks: fragments along
@@ -1601,10 +1668,6 @@ bool all_apart(phz_ops* o, std::initializer_list<Named> outs, std::initializer_l
   return true;
 }
 
-unsigned sequential_blocks(const phz_ops* o, const AttendArgs& a) {
-  return (unsigned)std::min<int64_t>((int64_t)a.worlds * a.heads, 2 * o->cus);
-}
-
 // ── how the steps are spread ────────────────────────────────────────────────
 
 int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
@@ -1686,7 +1749,8 @@ int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
   });
   AttendArgs again = a;
   again.flags = seg.flags;
-  hipLaunchKernelGGL(attend_sequential<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again, seg.count + slots);
+  hipLaunchKernelGGL(attend_sequential<E>, dim3((unsigned)std::min<int64_t>(heads, 2 * o->cus)), dim3(512), 0, stream, again,
+                     seg.count + slots);
   return launched(o, "linear attention") ? 0 : 1;
 }
 
@@ -1754,8 +1818,11 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
   });
   AttendArgs again = a;
   again.flags = seg.flags;
-  hipLaunchKernelGGL(attend_sequential_backward<E>, dim3(sequential_blocks(o, a)), dim3(512), 0, stream, again,
-                     (int32_t)(seg.count + 2 * slots), wide);
+  // (A compute unit holds one workgroup of it.)
+  const Kept kept{(float*)(work + (seg.chunks > 1 ? each : forth)), heads * (state / 4), (int32_t)(state / 4), padded(a.nv) / 16,
+                  seg.chunks > 1 ? 0 : 1, Kind<E>::C};
+  hipLaunchKernelGGL(attend_sequential_backward<E>, dim3((unsigned)std::min<int64_t>(heads, o->cus)), dim3(512), 0, stream, again,
+                     (int32_t)(seg.count + 2 * slots), wide, kept);
   for (int i = 0; i < 3; i++) {
     if (own[i] < 0) continue;
     const bool four = sizes[i] % 4 == 0;
