@@ -480,8 +480,11 @@ typedef struct {
  * zeros). Where reset [steps][worlds] u8 is nonzero, or g below -104 (exp(g) is 0
  * in f32), S_{t-1} counts as 0, whatever it holds. o [steps][worlds][heads *
  * size_v] in q's type; s_last like s0 (or NULL) receives the state after the last
- * step. States are held in f32, sums in f32. g is at most 0 where gates decay;
- * above, states grow as the recurrence does, up to exp(g) of 2^32 in 16 steps. */
+ * step. States are held in f32, sums in f32; o is rounded to q's type once. What
+ * gates leave of a state counts down to f32's least normal number, whatever its
+ * size; of a step's own k v^T less than 2^-126 may count as 0. g is at most 0 where
+ * gates decay; above, states grow as the recurrence does, up to exp(g) of 2^32 in 16
+ * steps. */
 int phz_linear_attention(phz_ops* ops, void* stream, const phz_attention_cfg* cfg, const phz_tensor* q,
                          const phz_tensor* k, const phz_tensor* v, const phz_tensor* g, const phz_tensor* s0,
                          const phz_tensor* reset, const phz_tensor* o, const phz_tensor* s_last);

@@ -91,16 +91,22 @@ struct Sweep {
   bool back;
 };
 
-// What is left of the state that comes into step t: exp(g), or 0 where an episode
-// begins.
+// What is left of the state that comes into a step: exp(g) of it, or 0 where an
+// episode begins. Below f32's normal numbers exp(g) is a product of two, since the
+// state may be large enough to need its digits.
 struct Keep {
-  float by;
+  float by, rest;
   bool forget;
+  __device__ __forceinline__ Keep(float x, bool reset) : forget(reset || x < kForgets) {
+    const bool small = x < -87.0f;
+    by = expf(small ? 0.5f * x : x);
+    rest = small ? by : 1.0f;
+  }
+  __device__ __forceinline__ float of(float s) const { return forget ? 0.0f : s * by * rest; }
 };
 __device__ __forceinline__ Keep keep_of(const AttendArgs& a, int b, int h, int64_t t) {
-  if (t >= a.steps) return Keep{1.0f, false};
-  const float x = a.g[b * a.g_b + h * a.g_h + t * a.g_t];
-  return Keep{expf(x), x < kForgets || (a.reset && a.reset[b * a.r_b + t * a.r_t])};
+  if (t >= a.steps) return Keep(0.0f, false);
+  return Keep(a.g[b * a.g_b + h * a.g_h + t * a.g_t], a.reset && a.reset[b * a.r_b + t * a.r_t]);
 }
 __device__ __forceinline__ void first_state(const Sweep& w, int col0, float (&s)[8][4]) {
   const int lane = fresh_lane(), col = col0 + (lane & 15), g = lane >> 4;
@@ -131,7 +137,7 @@ __device__ __forceinline__ float take_step(const AttendArgs& a, const Sweep& w, 
     for (int r = 0; r < 4; r++) {
       const uint32_t at = (uint32_t)min(d + r, w.rows - 1);
       const bool there = d + r < w.rows;
-      const float kept = keep.forget ? 0.0f : keep.by * s[i][r], x = fmaf(to_f32(key[at]), val, kept);
+      const float x = fmaf(to_f32(key[at]), val, keep.of(s[i][r]));
       s[i][r] = there ? x : s[i][r];
       sum = there ? fmaf(to_f32(read[at]), x, sum) : sum;
     }
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
       float* out = a.ds0.p + b * a.ds0.b + h * a.ds0.h;
       const Keep keep = keep_of(a, b, h, 0);
       const int col = col0 + c;
-      each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = keep.forget ? 0.0f : keep.by * x; });
+      each_element(a.nk, col, col < a.nv, s, [&](int d, float x) { out[(int64_t)d * a.nv + col] = keep.of(x); });
     }
     if (!a.dg) return;
     float* dg = a.dg + b * a.dg_b + h * a.dg_h;
@@ -332,6 +338,8 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
       for (int m = n - 1; m >= 0; m--) {
         const int64_t t = t1 - n + m;
         (void)take_step<E>(a, of_e, b, h, t, col0, e);
+        // The gate before the sum, which may pass f32's range without it.
+        const Keep keep = keep_of(a, b, h, t);
         float mine = 0.0f;
         if (col0 + c < a.nk) {
 #pragma unroll
@@ -339,11 +347,10 @@ __global__ __launch_bounds__(512) void attend_sequential_backward(AttendArgs a, 
             if (i < kept.blocks)
 #pragma unroll
               for (int r = 0; r < 4; r++)
-                mine = fmaf(e[i][r], m + 1 < n ? met[(m * kept.blocks + i) * 4 + r][threadIdx.x] : s[i][r], mine);
+                mine = fmaf(keep.of(e[i][r]), m + 1 < n ? met[(m * kept.blocks + i) * 4 + r][threadIdx.x] : s[i][r], mine);
         }
         const float sum = total(mine);
-        const Keep keep = keep_of(a, b, h, t);
-        if (threadIdx.x == 0) dg[t * a.dg_t] = keep.forget ? 0.0f : keep.by * sum;
+        if (threadIdx.x == 0) dg[t * a.dg_t] = keep.forget ? 0.0f : sum;
       }
       t1 -= n;
     }
@@ -441,10 +448,14 @@ __device__ __forceinline__ f32x4 widen(s16x4 v) {
   const u32x2 x = __builtin_bit_cast(u32x2, v);
   return f32x4{low_half(x[0]), high_half(x[0]), low_half(x[1]), high_half(x[1])};
 }
-// a where it is kept, 0 (whatever x is) where nothing is left of it.
-__device__ __forceinline__ f32x4 scaled(f32x4 x, float by) {
+// What decays leave of a state, times `by`: 0, whatever x is, where an episode begins
+// between; else x times the square of their root, which f32 holds down to 2^-252 of
+// it (an infinity stays one, or becomes a NaN, which sends the head to the steps one
+// after the other).
+__device__ __forceinline__ f32x4 left_of(f32x4 x, float root, float by) {
+  const float f = root * by;
 #pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = by != 0.0f ? x[i] * by : 0.0f;
+  for (int i = 0; i < 4; i++) x[i] = root < 0.0f ? 0.0f : x[i] * root * f;
   return x;
 }
 
@@ -575,9 +586,10 @@ template <int C>
 struct Decays {
   double sum[C];            // of log2 of the gates up to t
   float e[C], r[C];         // from the start to t, from t to the end; 0 behind or before a reset
+  float e_root[C], r_root[C];  // their roots, negative there
   float u[C], w[C];         // from the end of the tile of 16 before to t, from t to the end of its tile
   int32_t since[C];         // the last step up to t at which an episode begins, or 0; C behind the last step
-  float f;                  // over all of it, or 0
+  float f_root;             // of that over all of it, negative where a reset is in it
   double all;               // log2 of it without resets
   uint64_t resets;
 };
@@ -629,13 +641,17 @@ __device__ __forceinline__ void find_decays(Gate v, Decays<C>* d) {
   const uint64_t upto = resets & (2ull << lane) - 1ull;
   const int at = resets ? 63 - __builtin_clzll(resets) : 0;
   d->sum[lane] = x;
-  d->e[lane] = upto || !v.live ? 0.0f : __builtin_amdgcn_exp2f((float)x);
-  d->r[lane] = v.live && lane >= at ? __builtin_amdgcn_exp2f((float)(all - x)) : 0.0f;
+  const bool from_start = v.live && !upto, to_end = v.live && lane >= at;
+  const float e_root = __builtin_amdgcn_exp2f(0.5f * (float)x), r_root = __builtin_amdgcn_exp2f(0.5f * (float)(all - x));
+  d->e[lane] = from_start ? e_root * e_root : 0.0f;
+  d->r[lane] = to_end ? r_root * r_root : 0.0f;
+  d->e_root[lane] = from_start ? e_root : -1.0f;
+  d->r_root[lane] = to_end ? r_root : -1.0f;
   d->u[lane] = __builtin_amdgcn_exp2f((float)mine);
   d->w[lane] = __builtin_amdgcn_exp2f((float)(row - mine));
   d->since[lane] = !v.live ? C : upto ? 63 - __builtin_clzll(upto) : 0;
   if (lane == 0) {
-    d->f = resets ? 0.0f : __builtin_amdgcn_exp2f((float)all);
+    d->f_root = resets ? -1.0f : __builtin_amdgcn_exp2f(0.5f * (float)all);
     d->all = all;
     d->resets = resets;
   }
@@ -672,7 +688,7 @@ __device__ __forceinline__ void tile_of(int n, int* a, int* b) {
 struct Segments {
   int32_t chunks, count;
   float* states;
-  float* decay;           // [count - 1][heads]: over a segment, negative where a reset is in it
+  float* decay;           // [count - 1][heads]: root of that over a segment, negative where a reset is in it
   uint32_t* flags;        // [count][heads]: results that are not finite
   uint32_t* state_flags;  // [count - 1][heads]: states that are not
 };
@@ -788,39 +804,44 @@ struct Put {
   }
 };
 
-// s <- f s + rows^T (weight o cols) of one chunk: the wave's 16 columns, SIDE blocks
+// s <- f s + rows^T (weight o cols) of one chunk, f by its root: the wave's 16 columns, SIDE blocks
 // of rows at a time (one where registers are short).
 template <class E, int DR, int DC, int SIDE = Kind<E>::kSide>
-__device__ __forceinline__ void advance_state(const char* rows, const char* cols, const float* weight, float scale, float f, int col0,
+__device__ __forceinline__ void advance_state(const char* rows, const char* cols, const float* weight, float scale, float f_root, int col0,
                                               f32x4 (&s)[DR / 16]) {
   typedef Kind<E> K;
   typedef typename K::Frag Frag;
-  constexpr int NB = K::C / 16, U = SIDE;
+  // (Few registers: two blocks of steps at a time as well, 308 us against 342 for 256
+  // steps of 2048 heads of 64 backwards in bf16, 553 against 610 for 4096 of 64 of 128.)
+  constexpr int NB = K::C / 16, U = SIDE, NJ = SIDE == 1 ? 2 : NB;
   const int lane = fresh_lane(), g = lane >> 4;
-  Frag v[K::kPieces][NB];
 #pragma unroll
-  for (int i = 0; i < NB; i++) {
-    f32x4 x = widen(Tile<E, DC>::down(cols, i, col0, lane));
-    const f32x4 w = *(const f32x4*)(weight + 16 * i + 4 * g);
+  for (int j0 = 0; j0 < NB; j0 += NJ) {
+    Frag v[K::kPieces][NJ];
 #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] *= w[r] * scale;
-    cut<K::kPieces>(x, &v[0][i], NB);
-  }
+    for (int i = 0; i < NJ; i++) {
+      f32x4 x = widen(Tile<E, DC>::down(cols, j0 + i, col0, lane));
+      const f32x4 w = *(const f32x4*)(weight + 16 * (j0 + i) + 4 * g);
 #pragma unroll
-  for (int i = 0; i < DR / 16; i += U) {
-    Frag k[U][NB];
-    f32x4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-#pragma unroll
-      for (int j = 0; j < NB; j++) k[u][j] = Tile<E, DR>::down(rows, j, 16 * (i + u), lane);
-      x[u] = scaled(s[i + u], f);
+      for (int r = 0; r < 4; r++) x[r] *= w[r] * scale;
+      cut<K::kPieces>(x, &v[0][i], NJ);
     }
 #pragma unroll
-    for (int p = K::kPieces - 1; p >= 0; p--) mma_side<NB, U>(k[0], NB, v[p], 0, x);
+    for (int i = 0; i < DR / 16; i += U) {
+      Frag k[U][NJ];
+      f32x4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) s[i + u] = x[u];
-    __builtin_amdgcn_sched_barrier(0);
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) k[u][j] = Tile<E, DR>::down(rows, j0 + j, 16 * (i + u), lane);
+        x[u] = j0 ? s[i + u] : left_of(s[i + u], f_root, 1.0f);
+      }
+#pragma unroll
+      for (int p = K::kPieces - 1; p >= 0; p--) mma_side<NJ, U>(k[0], NJ, v[p], 0, x);
+#pragma unroll
+      for (int u = 0; u < U; u++) s[i + u] = x[u];
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -935,8 +956,8 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
         }
       }
 #pragma unroll
-      for (int i = 0; i < NB; i++) acc[i] = scaled(acc[i], decays.e[16 * i + (at & 15)] * a.scale);
-      advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f, col0, s);
+      for (int i = 0; i < NB; i++) acc[i] = left_of(acc[i], decays.e_root[16 * i + (at & 15)], a.scale);
+      advance_state<E, DK, DV>(k_tile, v_tile, decays.r, 1.0f, decays.f_root, col0, s);
     }
     __syncthreads();  // q and k are read
     if (!kEarly) fetch(t0 + C);  // nothing where that is the end
@@ -1060,7 +1081,7 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
     __syncthreads();
     if (n + 1 < chunks) fetch(start(n + 1));
     if (col0 < x.nc)
-      advance_state<E, DR, DC>(r_tile, c_tile, MODE == BACK ? decays.e : decays.r, MODE == BACK ? a.scale : 1.0f, decays.f, col0, s);
+      advance_state<E, DR, DC>(r_tile, c_tile, MODE == BACK ? decays.e : decays.r, MODE == BACK ? a.scale : 1.0f, decays.f_root, col0, s);
     all += decays.all;
     forgets = forgets || decays.resets;
   }
@@ -1076,7 +1097,7 @@ __global__ __launch_bounds__(DC * 4, DR > 2 * DC ? 2 : 4) void segment_states(At
   if (not_finite(zeros)) bad = 1;
   __syncthreads();
   if (threadIdx.x == 0) {
-    seg.decay[slot * heads + bh] = forgets ? -1.0f : (float)exp2(all);
+    seg.decay[slot * heads + bh] = forgets ? -1.0f : (float)exp2(0.5 * all);
     seg.state_flags[slot * heads + bh] = bad;
   }
 }
@@ -1108,7 +1129,7 @@ __global__ __launch_bounds__(256) void join_segments(AttendArgs a, Roles x, Segm
 #pragma unroll
     for (int j = 0; j < N; j++)
       if (n + j < slots) {
-        s = keep[j] < 0.0f ? add[j] : fmaf(keep[j], s, add[j]);
+        s = keep[j] < 0.0f ? add[j] : fmaf(keep[j] * s, keep[j], add[j]);
         p[j * step] = s;
       }
     p += N * step;
@@ -1248,7 +1269,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
   };
   float zeros = 0.0f;
   // The gates' gradients of the chunk at t0, by the last wave, a lane a step.
-  auto gates = [&](int64_t t0, float f, uint64_t resets) {
+  auto gates = [&](int64_t t0, float f_root, uint64_t resets) {
     const int lane = fresh_lane(), t = lane, tile = t / 16;
     float x = 0.0f, qd = 0.0f, kd = 0.0f, m = 0.0f;
     for (int w = 0; w < NK; w++) x += x_dot[w];
@@ -1259,7 +1280,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       for (int i = 0; i <= tile; i++) m -= row_sum[i][t];
     }
     const float before = sums_up_to(kd) - kd + (sums_up_to(m) - m);
-    const float sum = (f != 0.0f ? f * x : 0.0f) + __shfl(sums_up_to(qd), (C - 1 - t) & 63) + before;
+    const float sum = (f_root < 0.0f ? 0.0f : x * f_root * f_root) + __shfl(sums_up_to(qd), (C - 1 - t) & 63) + before;
     const int64_t step = t0 + t;
     if (t < C && step < end) {
       const float out = resets >> t & 1 ? 0.0f : sum;
@@ -1363,7 +1384,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       }
     }
     __syncthreads();
-    f_before = decays.f;
+    f_before = decays.f_root;
     resets_before = decays.resets;
     // acc[i] += (state's columns)^T (rows of `with`, of steps' blocks from i0 on) over
     // up to four blocks of the contraction, from `block` on.
@@ -1423,7 +1444,7 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
           for (int n = 0; n < kPer; n++) {
             const int i = m * kPer + n;
             if (i >= NB) break;
-            f32x4 y = scaled(acc[n], decays.e[16 * i + c] * a.scale);
+            f32x4 y = left_of(acc[n], decays.e_root[16 * i + c], a.scale);
             if (dg) dot(y, q_tile, i, tile, q_dot[tile], lane);
             y = add(x, dscore, i, true, y, lane);
             put(i, y);
@@ -1443,12 +1464,12 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       const Put<E, C> put(a.dk, t0, left, b, h, a.nk, col0, lane, wide & 2);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        f32x4 y = scaled(acc[i], decays.r[16 * i + c]);
+        f32x4 y = left_of(acc[i], decays.r_root[16 * i + c], 1.0f);
         if (dg) dot(y, k_tile, i, wave, k_dot[wave], lane);
         y = add(x, dscore, i, false, y, lane);
         put(i, y);
       }
-      advance_state<E, DV, DK, 1>(o_tile, q_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NV])e);
+      advance_state<E, DV, DK, 1>(o_tile, q_tile, decays.e, a.scale, decays.f_root, col0, *(f32x4(*)[NV])e);
     } else {
       const int lane = fresh_lane(), c = lane & 15;
       f32x4 acc[NB] = {};
@@ -1460,10 +1481,10 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       const Put<E, C> put(a.dv, t0, left, b, h, a.nv, col0, lane, wide & 4);
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        const f32x4 y = add(x, score, i, false, scaled(acc[i], decays.r[16 * i + c]), lane);
+        const f32x4 y = add(x, score, i, false, left_of(acc[i], decays.r_root[16 * i + c], 1.0f), lane);
         put(i, y);
       }
-      advance_state<E, DK, DV, 1>(q_tile, o_tile, decays.e, a.scale, decays.f, col0, *(f32x4(*)[NK])e);
+      advance_state<E, DK, DV, 1>(q_tile, o_tile, decays.e, a.scale, decays.f_root, col0, *(f32x4(*)[NK])e);
     }
   }
   __syncthreads();
@@ -1498,9 +1519,7 @@ __global__ __launch_bounds__(kStepThreads) void attend_step(AttendArgs a, int32_
   const int j0 = part * width, cols = min(width, a.nv - j0);
   const int groups = (cols + 3) / 4, rows = kStepThreads / groups;
   const int jj = threadIdx.x % groups, rr = threadIdx.x / groups;
-  const float x = a.g[b * a.g_b + h * a.g_h];
-  const bool forget = x < kForgets || (a.reset && a.reset[b * a.r_b]);
-  const float keep = expf(x);
+  const Keep keep(a.g[b * a.g_b + h * a.g_h], a.reset && a.reset[b * a.r_b]);
   float* s = a.s1.p + b * a.s1.b + h * a.s1.h + j0;
   const E *q = row_of<E>(a.q, b, h, a.nk), *k = row_of<E>(a.k, b, h, a.nk), *v = row_of<E>(a.v, b, h, a.nv) + j0;
   float acc[4] = {};
@@ -1526,7 +1545,7 @@ __global__ __launch_bounds__(kStepThreads) void attend_step(AttendArgs a, int32_
           if (d >= a.nk) break;
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            w[r].v[i] = fmaf(to_f32(kd[r]), val[i], forget ? 0.0f : keep * w[r].v[i]);
+            w[r].v[i] = fmaf(to_f32(kd[r]), val[i], keep.of(w[r].v[i]));
             acc[i] = fmaf(to_f32(qd[r]), w[r].v[i], acc[i]);
           }
           *(Pack<float, 4>*)(s + d * a.nv + j) = w[r];
@@ -1539,7 +1558,7 @@ __global__ __launch_bounds__(kStepThreads) void attend_step(AttendArgs a, int32_
         for (int i = 0; i < 4; i++)
           if (i < n) {
             float& w = s[(int64_t)d * a.nv + j + i];
-            w = fmaf(kd, val[i], forget ? 0.0f : keep * w);
+            w = fmaf(kd, val[i], keep.of(w));
             acc[i] = fmaf(qd, w, acc[i]);
           }
       }
