@@ -1279,7 +1279,9 @@ __global__ __launch_bounds__((kGradientThreads<DK, DV>), 4) void attend_gradient
       for (int i = tile; i < NB; i++) m += col_sum[i][t];
       for (int i = 0; i <= tile; i++) m -= row_sum[i][t];
     }
-    const float before = sums_up_to(kd) - kd + (sums_up_to(m) - m);
+    // Of the steps before: not with t's own taken off again, which a gate that closes
+    // leaves far larger than the others.
+    const float up = __shfl_up(sums_up_to(kd + m), 1), before = lane ? up : 0.0f;
     const float sum = (f_root < 0.0f ? 0.0f : x * f_root * f_root) + __shfl(sums_up_to(qd), (C - 1 - t) & 63) + before;
     const int64_t step = t0 + t;
     if (t < C && step < end) {

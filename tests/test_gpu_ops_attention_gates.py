@@ -69,3 +69,14 @@ def test_shared_heads_and_several_bad_steps(ops):
     R.within(dg[..., 1:], grads[3][..., 1:], bounds[3][..., 1:], "dg of other heads")
     R.within(ds0[:, 1:], grads[4][:, 1:], bounds[4][:, 1:], "ds0 of other heads")
     assert torch.isnan(dg[:41, 0, 0]).all() and torch.isnan(dg[51:, 0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [A.F32, A.BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T", [2, 33, 100, 1500])
+def test_gates_that_close(ops, T, dtype):
+    """Gates that leave little have gradients as little, also beside keys and values
+    whose own weight in the last state's gradient is not."""
+    x = A.inputs(T, 2, 2, 24, 32, dtype, 14, reset=0)
+    x["g"].fill_(-12.0)
+    want, bound = R.attention_backward(x["do"], x["q"], x["k"], x["v"], x["g"], x["s0"], None, x["ds"], 24, 32, 24 ** -0.5)
+    R.within(A.backward(ops, x, 24, 32)[3], want[3], bound[3], "dg")
