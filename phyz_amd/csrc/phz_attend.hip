@@ -1689,6 +1689,27 @@ bool all_apart(phz_ops* o, std::initializer_list<Named> outs, std::initializer_l
   return true;
 }
 
+// A launch has fewer than 2^32 threads, a workgroup up to 1024 of them: calls of more
+// heads of all worlds take some worlds at a time, one after the other in the stream.
+constexpr int64_t kMostHeads = (1 << 22) - 1;
+template <class F>
+int by_worlds(const AttendArgs& a, int64_t elem, F&& f) {
+  const int64_t most = kMostHeads / a.heads;
+  for (int64_t b = 0; b < a.worlds; b += most) {
+    AttendArgs x = a;
+    x.worlds = (int32_t)std::min(most, a.worlds - b);
+    for (Rows* r : {&x.q, &x.k, &x.v, &x.o, &x.dq, &x.dk, &x.dv})
+      if (r->p) r->p = (char*)r->p + b * r->b * elem;
+    for (States* s : {&x.s0, &x.s1, &x.ds, &x.ds0})
+      if (s->p) s->p += b * s->b;
+    if (x.g) x.g += b * x.g_b;
+    if (x.dg) x.dg += b * x.dg_b;
+    if (x.reset) x.reset += b * x.r_b;
+    if (f(x)) return 1;
+  }
+  return 0;
+}
+
 // ── how the steps are spread ────────────────────────────────────────────────
 
 int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
@@ -1746,7 +1767,6 @@ int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
     });
   });
   Segments seg = segments_of(o, a, Kind<E>::C, resident);
-  if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
   const int slots = seg.count - 1;
   Pieces p;
   const int64_t flags = p.take((seg.count + slots) * heads * 4), decay = p.take(slots * heads * 4), states = p.take(slots * heads * state);
@@ -1768,6 +1788,7 @@ int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
       hipLaunchKernelGGL((attend_chunks<E, DK, DV>), dim3((unsigned)(heads * seg.count)), dim3(DV * 4), 0, stream, a, seg);
     });
   });
+  if (!launched(o, "linear attention")) return 1;
   AttendArgs again = a;
   again.flags = seg.flags;
   hipLaunchKernelGGL(attend_sequential<E>, dim3((unsigned)std::min<int64_t>(heads, 2 * o->cus)), dim3(512), 0, stream, again,
@@ -1775,9 +1796,10 @@ int forward(phz_ops* o, hipStream_t stream, const AttendArgs& a) {
   return launched(o, "linear attention") ? 0 : 1;
 }
 
-// outs: dq, dk, dv; those of shared heads go through f32 sums of each head's own.
+// dq, dk and dv of shared heads go through f32 sums of each head's own.
 template <class E>
-int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]) {
+int backward(phz_ops* o, hipStream_t stream, AttendArgs a) {
+  const Rows outs[3] = {a.dq, a.dk, a.dv};
   const int64_t T = a.steps, heads = (int64_t)a.worlds * a.heads, state = (int64_t)padded(a.nk) * padded(a.nv) * 4;
   const int sizes[3] = {a.nk, a.nk, a.nv};
   int resident = 1;
@@ -1789,7 +1811,6 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
   });
   Segments seg = segments_of(o, a, Kind<E>::C, resident);
   const int64_t chunks = ceil_div(T, Kind<E>::C), slots = seg.count - 1;
-  if (heads * seg.count > 0x7fffffffll) return o->fail("too many heads of all worlds");
   Pieces p;
   int64_t own[3];
   for (int i = 0; i < 3; i++) own[i] = outs[i].per > 1 ? p.take(T * heads * sizes[i] * 4) : -1;
@@ -1837,6 +1858,7 @@ int backward(phz_ops* o, hipStream_t stream, AttendArgs a, const Rows (&outs)[3]
                          (const float*)(work + forth), (const f32x4*)(work + each), wide);
     });
   });
+  if (!launched(o, "linear attention backward")) return 1;
   AttendArgs again = a;
   again.flags = seg.flags;
   // (A compute unit holds one workgroup of it.)
@@ -1876,12 +1898,14 @@ int phz_linear_attention(phz_ops* o, void* stream_, const phz_attention_cfg* cfg
     auto stream = (hipStream_t)stream_;
     DeviceGuard guard(o);
     if (!guard.ok) return 1;
-    if (a.steps == 0) {
-      if (a.s1.p)
-        hipLaunchKernelGGL(copy_states, dim3(a.worlds * a.heads), dim3(256), 0, stream, a.s0, a.s1, a.heads, a.nk * a.nv);
-      return launched(o, "linear attention") ? 0 : 1;
-    }
-    return q->dtype == PHZ_F32 ? forward<float>(o, stream, a) : forward<bf16>(o, stream, a);
+    return by_worlds(a, elem_bytes(q->dtype), [&](const AttendArgs& x) {
+      if (x.steps == 0) {
+        if (x.s1.p)
+          hipLaunchKernelGGL(copy_states, dim3(x.worlds * x.heads), dim3(256), 0, stream, x.s0, x.s1, x.heads, x.nk * x.nv);
+        return launched(o, "linear attention") ? 0 : 1;
+      }
+      return q->dtype == PHZ_F32 ? forward<float>(o, stream, x) : forward<bf16>(o, stream, x);
+    });
   });
 }
 
@@ -1908,17 +1932,19 @@ int phz_linear_attention_backward(phz_ops* o, void* stream_, const phz_attention
     auto stream = (hipStream_t)stream_;
     DeviceGuard guard(o);
     if (!guard.ok) return 1;
-    if (T == 0) {
-      if (a.ds0.p)
-        hipLaunchKernelGGL(copy_states, dim3((unsigned)(B * H)), dim3(256), 0, stream, a.ds, a.ds0, a.heads, a.nk * a.nv);
-      return launched(o, "linear attention backward") ? 0 : 1;
-    }
     a.o = Rows{d_o->data, d_o->stride[0], d_o->stride[1], 1};
     if (dg) a.dg = (float*)dg->data, a.dg_t = dg->stride[0], a.dg_b = dg->stride[1], a.dg_h = dg->stride[2];
-    const Rows outs[3] = {{dq->data, dq->stride[0], dq->stride[1], a.q.per},
-                          {dk->data, dk->stride[0], dk->stride[1], a.k.per},
-                          {dv->data, dv->stride[0], dv->stride[1], a.v.per}};
-    return q->dtype == PHZ_F32 ? backward<float>(o, stream, a, outs) : backward<bf16>(o, stream, a, outs);
+    a.dq = Rows{dq->data, dq->stride[0], dq->stride[1], a.q.per};
+    a.dk = Rows{dk->data, dk->stride[0], dk->stride[1], a.k.per};
+    a.dv = Rows{dv->data, dv->stride[0], dv->stride[1], a.v.per};
+    return by_worlds(a, elem_bytes(q->dtype), [&](const AttendArgs& x) {
+      if (x.steps == 0) {
+        if (x.ds0.p)
+          hipLaunchKernelGGL(copy_states, dim3(x.worlds * x.heads), dim3(256), 0, stream, x.ds, x.ds0, x.heads, x.nk * x.nv);
+        return launched(o, "linear attention backward") ? 0 : 1;
+      }
+      return q->dtype == PHZ_F32 ? backward<float>(o, stream, x) : backward<bf16>(o, stream, x);
+    });
   });
 }
 
@@ -1938,19 +1964,16 @@ int phz_linear_attention_step(phz_ops* o, void* stream_, const phz_attention_cfg
     a.o = Rows{out->data, 0, out->stride[0], 1};
     DeviceGuard guard(o);
     if (!guard.ok) return 1;
-    const int64_t all = (int64_t)a.worlds * a.heads;
-    // Few heads: several workgroups to one, of 16 columns at least.
-    int width = (a.nv + 3) / 4 * 4;
-    while (all * ceil_div(a.nv, width) < 2 * o->cus && width % 32 == 0) width /= 2;
-    const int parts = (int)ceil_div(a.nv, width);
-    if (all * parts > 0x7fffffffll) return o->fail("too many heads of all worlds");
-    if (q->dtype == PHZ_F32)
-      hipLaunchKernelGGL(attend_step<float>, dim3((unsigned)(all * parts)), dim3(kStepThreads), 0, (hipStream_t)stream_, a, parts,
-                         width);
-    else
-      hipLaunchKernelGGL(attend_step<bf16>, dim3((unsigned)(all * parts)), dim3(kStepThreads), 0, (hipStream_t)stream_, a, parts,
-                         width);
-    return launched(o, "linear attention step") ? 0 : 1;
+    return by_worlds(a, elem_bytes(q->dtype), [&](const AttendArgs& x) {
+      const int64_t all = (int64_t)x.worlds * x.heads;
+      // Few heads: several workgroups to one, of 16 columns at least.
+      int width = (x.nv + 3) / 4 * 4;
+      while (all * ceil_div(x.nv, width) < 2 * o->cus && width % 32 == 0) width /= 2;
+      const int parts = (int)ceil_div(x.nv, width);
+      hipLaunchKernelGGL((q->dtype == PHZ_F32 ? attend_step<float> : attend_step<bf16>), dim3((unsigned)(all * parts)),
+                         dim3(kStepThreads), 0, (hipStream_t)stream_, x, parts, width);
+      return launched(o, "linear attention step") ? 0 : 1;
+    });
   });
 }
 
