@@ -314,7 +314,8 @@ struct Spans {
   }
 };
 
-// Launches over the entries, kTensors and 2^31 workgroups at a time.
+// Launches over the entries, kTensors and fewer than 2^32 threads at a time.
+constexpr uint64_t kMostGroups = (1ull << 32) / kThreads - 1;
 template <class F>
 void in_launches(const phz_ops* o, const std::vector<One>& all, AdamWArgs a, F&& launch) {
   int64_t wide = 0;
@@ -326,7 +327,7 @@ void in_launches(const phz_ops* o, const std::vector<One>& all, AdamWArgs a, F&&
     uint64_t groups = 0;
     while (i < all.size() && a.count < kTensors) {
       const uint64_t more = (uint64_t)ceil_div(all[i].n, a.span);
-      if (a.count && groups + more > 0x7fffffffull) break;
+      if (a.count && groups + more > kMostGroups) break;
       a.t[a.count] = all[i++];
       a.t[a.count++].first = (uint32_t)groups;
       groups += more;
@@ -335,7 +336,7 @@ void in_launches(const phz_ops* o, const std::vector<One>& all, AdamWArgs a, F&&
   }
 }
 
-constexpr int64_t kMostElements = 1ll << 40;  // of a tensor: its workgroups fit a launch
+constexpr int64_t kMostElements = (int64_t)kMostGroups * kSpan;  // of a tensor: its workgroups fit a launch
 
 bool check_exponents(phz_ops* o, int64_t i, const phz_tensor* e, int64_t n) {
   return vectors(o, "exponents", i, e, 2 * ceil_div(n, kBlock), PHZ_U8, true);
