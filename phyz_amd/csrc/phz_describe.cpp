@@ -48,8 +48,9 @@ const int kCodes[kDtypes] = {PHZ_F32, PHZ_F64, PHZ_BF16, PHZ_U8, PHZ_U8, PHZ_I32
 
 // False, with no Python error left, where `o` is no tensor that can be
 // described (the caller finds out why and says so). `flat`: as a vector, which a
-// contiguous tensor of any number of axes is.
-bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false) {
+// contiguous tensor of any number of axes is; its shape goes to `shape`, where that is
+// asked for.
+bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false, PyObject** of_shape = nullptr) {
   PyObject* v = PyObject_CallMethodNoArgs(o, g_get_device);
   bool ok = v && PyLong_AsLong(v) == device;
   Py_XDECREF(v);
@@ -73,14 +74,20 @@ bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false) {
     v = ok ? PyObject_CallMethodNoArgs(o, g_is_contiguous) : nullptr;
     ok = v == Py_True;
     Py_XDECREF(v);
-    v = ok ? PyObject_CallMethodNoArgs(o, g_numel) : nullptr;
-    ok = v != nullptr;
-    if (ok) {
-      t->size[0] = PyLong_AsLongLong(v);
-      t->stride[0] = 1;
-      t->ndim = 1;
+    t->stride[0] = 1;
+    t->ndim = 1;
+    if (of_shape) {
+      v = ok ? PyObject_GetAttr(o, g_shape) : nullptr;
+      ok = v && PyTuple_Check(v);
+      t->size[0] = 1;
+      for (Py_ssize_t i = 0; ok && i < PyTuple_GET_SIZE(v); i++) t->size[0] *= PyLong_AsLongLong(PyTuple_GET_ITEM(v, i));
+      *of_shape = v;
+    } else {
+      v = ok ? PyObject_CallMethodNoArgs(o, g_numel) : nullptr;
+      ok = v != nullptr;
+      if (ok) t->size[0] = PyLong_AsLongLong(v);
+      Py_XDECREF(v);
     }
-    Py_XDECREF(v);
     if (PyErr_Occurred()) {
       PyErr_Clear();
       ok = false;
@@ -106,6 +113,24 @@ bool describe(PyObject* o, long device, phz_tensor* t, bool flat = false) {
     ok = false;
   }
   return ok;
+}
+
+// Whether elements of two shapes with as many of them, one after the other, are at
+// the same places: axes of one element aside the shapes are one, or either is a vector.
+bool same_places(PyObject* a, PyObject* b) {
+  const Py_ssize_t na = PyTuple_GET_SIZE(a), nb = PyTuple_GET_SIZE(b);
+  Py_ssize_t i = 0, j = 0, axes[2] = {};
+  bool same = true;
+  for (;;) {
+    long long x = 1, y = 1;
+    while (i < na && (x = PyLong_AsLongLong(PyTuple_GET_ITEM(a, i))) == 1) i++;
+    while (j < nb && (y = PyLong_AsLongLong(PyTuple_GET_ITEM(b, j))) == 1) j++;
+    if (i >= na && j >= nb) break;
+    same = same && i < na && j < nb && x == y;
+    if (i < na) axes[0]++, i++;
+    if (j < nb) axes[1]++, j++;
+  }
+  return same || axes[0] < 2 || axes[1] < 2;
 }
 
 // call(op, handle, stream, device, head, tensors, unrecorded): the entry point's
@@ -167,7 +192,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // call_lists(op, handle, stream, device, head, lists, single): an entry point of
 // lists of tensors, each a vector. Lists are tuples of one length, or None;
 // `single` is a tensor or None. The result as in call(), -1 - (5 i + l) for tensor
-// i of list l (l = 0 .. 4) and -1 - 5 n for the single one.
+// i of list l (l = 0 .. 4) and -1 - 5 n for the single one, -2^40 - i where the
+// update's gradient i has another shape than its weights.
 PyObject* call_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 7 || !PyTuple_Check(args[5]) || PyTuple_GET_SIZE(args[5]) != 5) {
     PyErr_SetString(PyExc_TypeError, "call_lists(op, handle, stream, device, head, five lists, single)");
@@ -197,9 +223,22 @@ PyObject* call_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return PyErr_NoMemory();
   }
   T t[6] = {};
-  for (int l = 0; l < 5; l++) {
-    if (lists[l] == Py_None) continue;
-    t[l] = d.data() + n * l;
+  for (int l = 0; l < 5; l++)
+    if (lists[l] != Py_None) t[l] = d.data() + n * l;
+  const bool pairs = op == kPlain && t[0] && t[1];  // weights and their gradients
+  for (Py_ssize_t i = 0; pairs && i < n; i++) {
+    PyObject *a = nullptr, *b = nullptr;
+    const bool wa = describe(PyTuple_GET_ITEM(lists[0], i), device, &d[i], true, &a);
+    // (A vector's gradient is not asked: a shape is an object made.)
+    const bool wb = wa && describe(PyTuple_GET_ITEM(lists[1], i), device, &d[n + i], true, PyTuple_GET_SIZE(a) > 1 ? &b : nullptr);
+    const bool apart = wb && b && d[i].size[0] == d[n + i].size[0] && d[i].size[0] > 1 && !same_places(a, b);
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    if (!wb) return PyLong_FromSsize_t(-1 - (5 * i + wa));
+    if (apart) return PyLong_FromLongLong(-(1ll << 40) - i);
+  }
+  for (int l = pairs ? 2 : 0; l < 5; l++) {
+    if (!t[l]) continue;
     for (Py_ssize_t i = 0; i < n; i++)
       if (!describe(PyTuple_GET_ITEM(lists[l], i), device, &d[n * l + i], true)) return PyLong_FromSsize_t(-1 - (5 * i + l));
   }

@@ -179,6 +179,9 @@ class Ops:
                               tuple(lists), single)
         if rc > 0:
             raise OpsError(self._L.phz_ops_last_error(self._h).decode())
+        if rc <= -(1 << 40):
+            i = -(1 << 40) - rc
+            raise OpsError(f"{names[1]}[{i}] has the shape {tuple(lists[1][i].shape)}, {names[0]}[{i}] {tuple(lists[0][i].shape)}")
         if rc < 0:
             i, l = divmod(-1 - rc, 5)
             name, t = (names[5], single) if i == n else (f"{names[l]}[{i}]", lists[l][i])
@@ -458,7 +461,7 @@ class Ops:
     def adamw_step(self, w, g, m, v, step, exponents=None, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                    weight_decay: float = 0.01, seed: int = 0):
         """One AdamW step of the tensors w (float32 or bfloat16, in place) for the
-        gradients g (either), with the moments m and v (in place; float32, or uint8
+        gradients g (either; of w's shapes, or vectors), with the moments m and v (in place; float32, or uint8
         with their exponents): lists of one length, of contiguous tensors of any
         shapes, best made by adamw_state. step, an int64 tensor of one element, counts
         the steps, also in replays of a captured graph. Moments of 8 bits are rounded
