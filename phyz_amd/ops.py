@@ -168,7 +168,7 @@ class Ops:
         """One entry point of lists of tensors on the current stream."""
         names = names.split()
         for name, x in zip(names, lists):
-            if x is not None and not isinstance(x, (list, tuple)):
+            if not isinstance(x, (list, tuple)) and (x is not None or name == names[0]):
                 raise OpsError(f"{name} has to be a list of tensors, not {type(x).__name__}")
         lists = [None if x is None else tuple(x) for x in lists]
         n = len(lists[0])
@@ -201,6 +201,23 @@ class Ops:
         if not isinstance(t, torch.Tensor):
             raise OpsError(f"{name} has to be a torch tensor, not {type(t).__name__}")
         return t
+
+    @staticmethod
+    def _whole(x, name: str) -> int:
+        try:
+            n = int(x)
+            if n == x and -1 << 31 <= n < 1 << 31:
+                return n
+        except (TypeError, ValueError, OverflowError):
+            pass
+        raise OpsError(f"{name} has to be a whole number, not {x!r}")
+
+    @staticmethod
+    def _number(x, name: str) -> float:
+        try:
+            return float(x)
+        except (TypeError, ValueError, OverflowError):
+            raise OpsError(f"{name} has to be a number, not {x!r}") from None
 
     @staticmethod
     def _choice(table, key, what):
@@ -327,14 +344,17 @@ class Ops:
     @staticmethod
     def _heads(q, v, g, size_k, size_v, scale):
         """(heads, the head sizes and scale as the library takes them)."""
+        for t, name in ((v, "v"), (g, "g")):
+            if t.dim() < 1:
+                raise OpsError(f"{name} has 0 dimensions, expected {q.dim()}")
         heads = g.shape[-1]
         if heads < 1:
             raise OpsError("g has no heads")
-        size_k = q.shape[-1] // heads if size_k is None else int(size_k)
-        size_v = v.shape[-1] // heads if size_v is None else int(size_v)
+        size_k = q.shape[-1] // heads if size_k is None else Ops._whole(size_k, "size_k")
+        size_v = v.shape[-1] // heads if size_v is None else Ops._whole(size_v, "size_v")
         if not (1 <= size_k <= 128 and 1 <= size_v <= 128):
             raise OpsError(f"size_k and size_v have to be 1 to 128, not {size_k} and {size_v}")
-        return heads, _lib.AttentionCfg(size_k ** -0.5 if scale is None else float(scale), size_k, size_v)
+        return heads, _lib.AttentionCfg(size_k ** -0.5 if scale is None else Ops._number(scale, "scale"), size_k, size_v)
 
     @staticmethod
     def _matrices(s, name: str, cfg):
@@ -433,7 +453,7 @@ class Ops:
         freq is float64 (rotary_frequencies). inverse turns back: the gradient for x is
         rotary(dy, ..., inverse=True). `out` may be x."""
         p = self._choice(PAIRS, layout, "layout")
-        cfg = _lib.RotaryCfg(float(scale), int(heads), p, int(bool(inverse)))
+        cfg = _lib.RotaryCfg(self._number(scale, "scale"), self._whole(heads, "heads"), p, int(bool(inverse)))
         y = out if out is not None else torch.empty_like(self._tensor(x, "x"))
         x3, p2, y3 = x, positions, y
         if isinstance(x, torch.Tensor) and x.dim() == 2:
@@ -449,7 +469,7 @@ class Ops:
         """(m, v, exponents, step) of adamw_step for tensors like params, before the
         first step: moments in 32 bits (exponents None), or in 8 with an exponent for
         each 256 elements."""
-        params = list(params)
+        params = [Ops._tensor(p, "params") for p in params]
         if bits not in (32, 8):
             raise OpsError(f"moments have 32 or 8 bits, not {bits}")
         dt = torch.float32 if bits == 32 else torch.uint8
@@ -466,7 +486,16 @@ class Ops:
         shapes, best made by adamw_state. step, an int64 tensor of one element, counts
         the steps, also in replays of a captured graph. Moments of 8 bits are rounded
         by random bits that follow from seed and step."""
-        cfg = _lib.AdamWCfg(lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xffffffff)
+        try:
+            b1, b2 = betas
+        except (TypeError, ValueError):
+            raise OpsError(f"betas have to be two numbers, not {betas!r}") from None
+        try:
+            seed = int(seed) & 0xffffffff
+        except (TypeError, ValueError, OverflowError):
+            raise OpsError(f"seed has to be a whole number, not {seed!r}") from None
+        cfg = _lib.AdamWCfg(*(self._number(x, n) for x, n in ((lr, "lr"), (b1, "betas"), (b2, "betas"), (eps, "eps"),
+                                                              (weight_decay, "weight_decay"))), seed)
         self._run_lists(_ADAMW, C.addressof(cfg), "w g m v exponents step", (w, g, m, v, exponents), self._tensor(step, "step"))
         _written([*w, *m, *v, *(exponents or ()), step])
 
