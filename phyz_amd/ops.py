@@ -34,7 +34,8 @@ and then raises.
 
 Autograd records none of this: gradients come from the _backward calls. The
 forward operators refuse tensors that require gradients while it is recording
-(call them under torch.no_grad(), or on detached tensors); the _backward calls
+(call them under torch.no_grad(), or on detached tensors), and tensors that carry
+tangents of forward-mode differentiation; the _backward calls
 and muon_step take them as they are. What a call writes in place or into `out`
 counts as changed for graphs that saved it.
 """
@@ -45,6 +46,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -63,6 +65,8 @@ _ENTRIES = ("phz_gated_scan", "phz_gated_scan_backward", "phz_gated_step", "phz_
             "phz_linear_attention_step", "phz_rotary", "phz_adamw_step", "phz_adamw_values")
 (_SCAN, _SCAN_BACKWARD, _STEP, _LINEAR, _LINEAR_BACKWARD, _ORTHOGONALIZE, _MUON, _ATTENTION, _ATTENTION_BACKWARD,
  _ATTENTION_STEP, _ROTARY, _ADAMW, _ADAMW_VALUES) = range(13)
+# Whose results a user may expect autograd to know.
+_FORWARD = {_SCAN, _STEP, _LINEAR, _ORTHOGONALIZE, _ATTENTION, _ATTENTION_STEP, _ROTARY}
 _describe = None
 
 
@@ -140,6 +144,10 @@ class Ops:
     # ── calls ──
     def _run(self, op: int, head: int, names: str, *tensors):
         """One entry point on the current stream; `names` are the tensors'."""
+        if getattr(forward_ad, "_current_level", 0) >= 0 and op in _FORWARD:
+            for name, t in zip(names.split(), tensors):
+                if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                    raise OpsError(f"{name} carries a tangent, which these operators do not record: call on detached tensors")
         stream = _raw_stream(self.device) if self.device >= 0 else 0
         rc = self._call(op, self._h, stream, self.device, head, tensors, False)
         if rc < -100:
