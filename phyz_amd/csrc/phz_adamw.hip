@@ -394,7 +394,8 @@ int phz_adamw_step(phz_ops* o, void* stream_, const phz_adamw_cfg* cfg, int64_t 
     a.fix = fix;
     a.b1 = (float)cfg->beta1, a.b2 = (float)cfg->beta2;
     a.c1 = (float)(1.0 - cfg->beta1), a.c2 = (float)(1.0 - cfg->beta2);
-    a.keep = (float)(1.0 - cfg->lr * cfg->weight_decay), a.eps = (float)cfg->eps;
+    // (An eps that is not 0 keeps 0 / (0 + eps) at 0, also where f32 has no such number.)
+    a.keep = (float)(1.0 - cfg->lr * cfg->weight_decay), a.eps = cfg->eps > 0 ? (float)fmax(cfg->eps, 0x1p-126) : 0.0f;
     hipLaunchKernelGGL(advance, dim3(1), dim3(1), 0, stream, (int64_t*)step->data, cfg->lr, cfg->beta1, cfg->beta2, cfg->seed, fix);
     for (int k = 0; k < 4; k++) {
       auto go = [&](auto kernel) {
