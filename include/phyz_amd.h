@@ -538,7 +538,8 @@ typedef struct {
  *         below the block's: m's code c (a sign and 7 bits) is
  *         (8 + c % 8) 2^(E - 144 + c / 8), or c % 8 times 2^(E - 143) where c / 8 is
  *         0, v's (8 bits) the same with 160 and 159; E is the biased exponent of the
- *         block's largest element, at least 40. What is not finite is 0x80 or 0xff.
+ *         block's largest element, at least 40. What is not finite is 0x80 or 0xff
+ *         (a finite value within a sixteenth of f32's end may round to an infinity).
  *         Values are rounded up with the probability that makes them right on
  *         average (to nearest, v would stand still where g^2 changes it by less than
  *         a sixteenth a step), by bits that depend on seed, t, the tensor's place in

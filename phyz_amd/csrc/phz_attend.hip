@@ -183,7 +183,7 @@ __device__ __forceinline__ void each_element(int rows, int col, bool live, float
 // A head whose steps are taken one after the other: what the chunks' products
 // cannot do is right here, infinities and NaN that a reset cuts off from the
 // steps behind it. A workgroup looks through its heads' flags, a thread a head at a
-// time (one wave's look at each in turn took 17 us for 16384 heads, this 6). 2 waves a SIMD.
+// time (one wave's look at each in turn took 17 us for 16384 heads, this 6).
 struct Flagged {
   const AttendArgs& a;
   int32_t marks;
@@ -546,7 +546,7 @@ struct Load {
 #pragma unroll
       for (int i = 0; i < N; i++, p += kStep * stride)
         if (C % kStep == 0 || row0 + i * kStep < C) {
-          // f32 past the caches (401 us against 420 for 64 steps of 16384 heads); lines
+          // f32 past the caches (404 us against 421 for 64 steps of 16384 heads); lines
           // of bf16 are shared by heads.
           if constexpr (sizeof(E) == 4) x[i] = __builtin_bit_cast(std::remove_reference_t<decltype(x[i])>, __builtin_nontemporal_load((const f32x4_of_4*)p));
           else x[i] = *(const Pack<E, EL>*)p;
@@ -695,8 +695,9 @@ struct Segments {
 
 // A workgroup's head and segment. Neighbouring heads share lines of memory: 16 of
 // them go to one XCD. (More, and the XCDs are far apart in each row: 64 steps of 8192
-// heads' gradients 646 us with an eighth of all a XCD, 623 so; one, and lines are
-// read twice: 777 steps of 222 heads 302 us against 292.)
+// heads' gradients 593 us with an eighth of all a XCD, 568 so; one, and lines are
+// read twice: 777 steps of 222 heads 220 us against 218, 1023 of 305 forward 110
+// against 108; 64 steps of 16384 in bf16 lose 2% so.)
 __device__ __forceinline__ void place_of(const AttendArgs& a, int64_t* bh, int* segment, int* b, int* h) {
   const uint32_t n = gridDim.x, i = blockIdx.x, heads = (uint32_t)(a.worlds * a.heads);
   const uint32_t id = i < n / 128 * 128 ? i / 128 * 128 + i % 8 * 16 + i % 128 / 8 : i;
@@ -762,7 +763,7 @@ __device__ __forceinline__ void write_state(float* p, int nk, int nv, int col0, 
 }
 
 // Four neighbouring elements of an output's row, of which it has `left` more.
-// LAST: f32 that is not read again here goes past the caches (418 us against 442 for
+// LAST: f32 that is not read again here goes past the caches (404 us against 425 for
 // 64 steps of 16384 heads); the half lines of bf16 have to meet there.
 template <bool LAST, class E>
 __device__ __forceinline__ void put4(E* p, int left, f32x4 v) {
@@ -849,9 +850,9 @@ __device__ __forceinline__ void advance_state(const char* rows, const char* cols
 // Scores are found a tile of 16 x 16 at a time by all waves, and meet in LDS, where
 // q and k were: half the LDS again would be two workgroups a compute unit less.
 // Long rollouts of many heads are bound by memory (64 steps of 16384 heads of 64 f32:
-// 382 us, 4.2 TB/s); in bf16, and where heads are few, by the chain of a chunk's
-// phases: 32768 steps of 8 heads of 128 take 95 us here, two workgroups a compute
-// unit, of which LDS is busy about 40%, the vector units 35%, the matrix units 20%.
+// 377 us, 4.3 TB/s); in bf16, and where heads are few, by the chain of a chunk's
+// phases: 32768 steps of 8 heads of 128 take 107 us here, two workgroups a compute
+// unit, of which the matrix units are busy 24% and the vector units issue 47%.
 template <class E, int DK, int DV>
 __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void attend_chunks(AttendArgs a, Segments seg) {
   typedef Kind<E> K;
@@ -860,8 +861,8 @@ __global__ __launch_bounds__(DV * 4, DV == 128 ? 4 : DK > DV ? 2 : 3) void atten
   constexpr int two = sizeof(E) == 2 ? 2 : 1, U = K::kSide;  // blocks of an instruction, chains
   constexpr int kTiles = NB * (NB + 1) / 2, kMine = (kTiles + NW - 1) / NW, NH = 2;
   // The next chunk's loads go out before this one's products where registers allow
-  // it (1024 steps of 512 heads of 64 bf16: 104 us against 113), in f32 behind them,
-  // which is bound by memory anyway (64 of 16384: 442 against 455).
+  // it (1024 steps of 512 heads of 64 bf16: 112 us against 133), in f32 behind them,
+  // which is bound by memory anyway (64 of 16384: 404 against 426).
   constexpr bool kEarly = sizeof(E) == 2 && DK <= 64;
   constexpr int kTile = C * Tile<E, DK>::kRow, kScore = Scores<E>::kSize;
   __shared__ __align__(16) char shared[2 * kTile > K::kPieces * kScore ? 2 * kTile : K::kPieces * kScore];
@@ -1182,8 +1183,9 @@ __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
 //   E <- f E + scale (e o Q)^T dO.
 // E is held twice: as rows of values by the first NK waves, 16 columns of keys each,
 // which find dK, and as rows of keys by the NV others, which find dV. dQ's tiles are
-// dealt out to all. (One wave for a column of each takes twice the registers: 458 us
-// against 254 at 256 steps of 2048 heads of 64 in bf16, the same in f32.)
+// dealt out to all. (One wave for a column of each takes twice the registers: when the
+// roles were dealt, 458 us against 254 at 256 steps of 2048 heads of 64 in bf16, the
+// same in f32.)
 // A gate's gradient sums over all ways across it: from the state before to the
 // gradient behind, X = f <S, E>; from steps u >= t to the state before,
 // q_u . (the state's part of dq_u); from steps s < t to the gradient behind,
@@ -1192,7 +1194,7 @@ __device__ __forceinline__ float dot4(f32x4 x, f32x4 y) {
 // No sum is taken over more than a chunk, so nothing large cancels.
 // 64 steps of 8192 heads of 64 f32: 490 us at 3.0 TB/s, of whose time the matrix
 // units are busy 37% and the vector units a third; 777 steps of 222 heads of 48 and
-// 80 in bf16: 150 us, one workgroup of twelve waves a compute unit, phases again.
+// 80 in bf16: 159 us, one workgroup of twelve waves a compute unit, phases again.
 template <int DK, int DV>
 constexpr int kGradientThreads = (DK + DV) * 4;
 
@@ -1717,7 +1719,7 @@ int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
 // Few heads take their steps in segments, as many as the chip holds workgroups at a
 // time (`resident` a compute unit); each has four chunks at least, since the segments'
 // states are found in a pass of its own. Heads that fill more than half of it do not:
-// 1023 steps of 305 heads in one 106 us, in two 139.
+// 1023 steps of 305 heads in one 108 us, in two 138.
 Segments segments_of(const phz_ops* o, const AttendArgs& a, int chunk, int resident) {
   const int64_t heads = (int64_t)a.worlds * a.heads, chunks = ceil_div(a.steps, chunk);
   Segments s{};

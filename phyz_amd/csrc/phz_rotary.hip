@@ -2,7 +2,7 @@
 // angle that is the position times the pair's frequency.
 //
 // A turn is taken in three steps: position * freq / 2 pi in f64, less its nearest
-// whole number (a position of 2^40 still leaves 12 bits of f32's fraction below),
+// whole number (at freq 1 a position of 2^40 still leaves some 15 bits of a turn),
 // the rest in f32, and sine and cosine by their series on a quarter turn. A
 // lane takes one pair of a row, or four neighbours where rows are many, and turns
 // them in every head, so the angles are found once a row. Bound by memory: 262144 rows
@@ -19,8 +19,9 @@ namespace {
 constexpr double kTurn = 0.15915494309189533577;  // 1 / 2 pi
 
 // (cos, sin) of 2 pi u for |u| <= 1/2. On |r| <= pi/4 the series to r^8 and r^9
-// leave less than 2^-26 of 1: the terms after them are (pi/4)^10 / 10! and
-// (pi/4)^11 / 11!.
+// leave at most the terms after them, (pi/4)^10 / 10! = 2^-25.3 and (pi/4)^11 / 11! =
+// 2^-29.1; with the roundings of the series both are within 1.2 * 2^-24, and u's own,
+// up to 2^-26 of a turn, is 2^-23.3 of an angle.
 __device__ __forceinline__ void turn(float u, float* c, float* s) {
   const float quarter = rintf(4.0f * u);
   const float r = 6.2831853071795865f * fmaf(-0.25f, quarter, u), x = r * r;
