@@ -20,7 +20,7 @@ constexpr double kTurn = 0.15915494309189533577;  // 1 / 2 pi
 
 // (cos, sin) of 2 pi u for |u| <= 1/2. On |r| <= pi/4 the series to r^8 and r^9
 // leave at most the terms after them, (pi/4)^10 / 10! = 2^-25.3 and (pi/4)^11 / 11! =
-// 2^-29.1; with the roundings of the series both are within 1.2 * 2^-24, and u's own,
+// 2^-29.1; with the roundings on the way cos is within 1.3 and sin 1.6 of 2^-24, and u's own,
 // up to 2^-26 of a turn, is 2^-23.3 of an angle.
 __device__ __forceinline__ void turn(float u, float* c, float* s) {
   const float quarter = rintf(4.0f * u);
